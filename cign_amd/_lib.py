@@ -72,6 +72,11 @@ _SIGNATURES = {
     "cign_gamma_residual_bwd": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _F32, _P, _P, _P, _I64]),
     "cign_add_ln_cat_fwd": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _F32, _P, _P, _P, _P]),
     "cign_add_ln_cat_bwd": (C.c_int, [_P, _I64, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64]),
+    # LayerNorm of any width (layernorm.hip)
+    "cign_layernorm_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _I64, _P, _P, _F32, _P, _P, _P]),
+    "cign_layernorm_bwd_workspace_bytes": (_I64, [_I64, _I32]),
+    "cign_layernorm_bwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P,
+                                     _I64]),
     # hop gate (gate.hip)
     "cign_hop_gate_bwd_workspace_bytes": (_I64, [_I64, _I32, _I32]),
     "cign_hop_gate_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),

@@ -1,0 +1,406 @@
+// LayerNorm of rows of 1 <= D <= 16384 values, float32 or bf16, forward and
+// backward: the model's output norm (width hidden * (layers + 1)) and any other
+// norm beyond the 256 values of the block ops (nodeops.hip).
+//
+// Row x, xh = (x - mean) rstd, y = xh w + b. Backward, with d = g w:
+//   grad_x = rstd (d - mean(d) - xh mean(d xh)),
+//   grad_w = sum over rows of g xh, grad_b = sum over rows of g.
+//
+// Both passes are streams: the forward reads a row once and writes it once, the
+// backward reads x and g once and writes grad_x; a row stays in registers
+// between its sums and its results (the variance is that of the centred
+// values), and the next row's loads are issued before the current row's sums.
+// NT threads own a row: lanes of a wavefront while the registers of 64 lanes
+// hold it, a workgroup beyond. The parameter gradients are added up per thread
+// over the rows of its workgroup, one partial row a workgroup, which
+// param_kernel adds in a fixed order (no atomics).
+#include "rowops.h"
+#include "rowvec.h"
+
+namespace cign {
+namespace layernorm {
+using namespace rowvec;
+
+constexpr int kMaxWidth = 16384;
+
+template <int N>
+using IC = std::integral_constant<int, N>;
+
+template <int NT>
+struct Shape {
+  static constexpr int kThreads = NT < kBlock ? kBlock : NT;
+  static constexpr int kRows = kThreads / NT;                          // rows of a workgroup at a time
+  static constexpr int kSlots = NT > kWave ? 2 * (NT / kWave) : 1;     // LDS slots of its reductions
+};
+
+template <typename T, typename TW, int W, int NT, int V>
+__global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int D, const T* x, int64_t ldx,
+                                                                  const TW* weight, const TW* bias, float eps, T* y,
+                                                                  float* mean, float* rstd) {
+  using X = RowChunk<T, W>;
+  using P = RowChunk<TW, W>;
+  __shared__ float slots[Shape<NT>::kSlots][1];
+  GroupReduce<NT, 1> reduce(slots);
+  const int q = threadIdx.x & (NT - 1);
+  int at[V], own[V];
+  typename P::Raw wr[V], br[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = q + v * NT;
+    at[v] = chunk_start<W>(c, D);
+    own[v] = c * W - at[v];
+    if (weight) wr[v] = P::load(weight + at[v]);
+    if (bias) br[v] = P::load(bias + at[v]);
+  }
+  const float inv = 1.0f / static_cast<float>(D);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * Shape<NT>::kRows;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * Shape<NT>::kRows + threadIdx.x / NT;
+  typename X::Raw next[V];
+  if (r < n)
+#pragma unroll
+    for (int v = 0; v < V; ++v) next[v] = X::load(x + r * ldx + at[v]);
+  for (; r < n; r += step) {
+    float xv[V][W];
+#pragma unroll
+    for (int v = 0; v < V; ++v) X::unpack(next[v], xv[v]);
+    const int64_t rn = r + step < n ? r + step : r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) next[v] = X::load(x + rn * ldx + at[v]);
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int w = 0; w < W; ++w) s[0] += w >= own[v] ? xv[v][w] : 0.0f;
+    reduce.template run<AddOp>(s);
+    const float mu = s[0] * inv;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        xv[v][w] -= mu;
+        s[0] += w >= own[v] ? xv[v][w] * xv[v][w] : 0.0f;
+      }
+    reduce.template run<AddOp>(s);
+    const float rs = 1.0f / sqrtf(s[0] * inv + eps);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (own[v] >= W) continue;
+      float o[W], p[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) o[w] = xv[v][w] * rs;
+      if (weight) {
+        P::unpack(wr[v], p);
+#pragma unroll
+        for (int w = 0; w < W; ++w) o[w] *= p[w];
+      }
+      if (bias) {
+        P::unpack(br[v], p);
+#pragma unroll
+        for (int w = 0; w < W; ++w) o[w] += p[w];
+      }
+      X::store(y + r * D + at[v], o);
+    }
+    if (q == 0 && mean) {
+      mean[r] = mu;
+      rstd[r] = rs;
+    }
+  }
+}
+
+// Rows [r0, r1) of workgroup b; part [2][nb][D] (weight, bias).
+template <typename T, typename TW, int W, int NT, int V>
+__global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int D, const T* gy, int64_t ldg,
+                                                                  const T* x, int64_t ldx, const TW* weight,
+                                                                  const float* mean, const float* rstd, T* gx,
+                                                                  float* part, int nb) {
+  using X = RowChunk<T, W>;
+  using P = RowChunk<TW, W>;
+  constexpr int kRows = Shape<NT>::kRows;
+  __shared__ float slots[Shape<NT>::kSlots][2];
+  GroupReduce<NT, 2> reduce(slots);
+  const int q = threadIdx.x & (NT - 1);
+  const int slot = threadIdx.x / NT;
+  int at[V], own[V];
+  typename P::Raw wr[V];
+  float aw[V][W], ab[V][W];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = q + v * NT;
+    at[v] = chunk_start<W>(c, D);
+    own[v] = c * W - at[v];
+    if (weight) wr[v] = P::load(weight + at[v]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) aw[v][w] = ab[v][w] = 0.0f;
+  }
+  const float inv = 1.0f / static_cast<float>(D);
+  int64_t r0, r1;
+  rowops::block_rows(n, nb, blockIdx.x, r0, r1);
+  int64_t r = r0 + slot;
+  typename X::Raw xn[V], gn[V];
+  float mun = 0.0f, rsn = 0.0f;
+  if (r < r1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      xn[v] = X::load(x + r * ldx + at[v]);
+      gn[v] = X::load(gy + r * ldg + at[v]);
+    }
+    mun = mean[r];
+    rsn = rstd[r];
+  }
+  for (; r < r1; r += kRows) {
+    float xh[V][W], g[V][W];
+    const float mu = mun, rs = rsn;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      X::unpack(xn[v], xh[v]);
+      X::unpack(gn[v], g[v]);
+    }
+    const int64_t rn = r + kRows < r1 ? r + kRows : r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      xn[v] = X::load(x + rn * ldx + at[v]);
+      gn[v] = X::load(gy + rn * ldg + at[v]);
+    }
+    mun = mean[rn];
+    rsn = rstd[rn];
+    float s[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float p[W];
+      if (weight) {
+        P::unpack(wr[v], p);
+      } else {
+#pragma unroll
+        for (int w = 0; w < W; ++w) p[w] = 1.0f;
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        xh[v][w] = (xh[v][w] - mu) * rs;
+        aw[v][w] = fmaf(g[v][w], xh[v][w], aw[v][w]);
+        ab[v][w] += g[v][w];
+        g[v][w] *= p[w];
+        s[0] += w >= own[v] ? g[v][w] : 0.0f;
+        s[1] += w >= own[v] ? g[v][w] * xh[v][w] : 0.0f;
+      }
+    }
+    if (!gx) continue;  // only the parameters' gradients are asked for
+    reduce.template run<AddOp>(s);
+    const float c1 = s[0] * inv, c2 = s[1] * inv;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (own[v] >= W) continue;
+      float o[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) o[w] = rs * (g[v][w] - c1 - xh[v][w] * c2);
+      X::store(gx + r * D + at[v], o);
+    }
+  }
+  if (!part) return;
+  if constexpr (kRows == 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (own[v] >= W) continue;
+      RowChunk<float, W>::store(part + static_cast<int64_t>(blockIdx.x) * D + at[v], aw[v]);
+      RowChunk<float, W>::store(part + (static_cast<int64_t>(nb) + blockIdx.x) * D + at[v], ab[v]);
+    }
+  } else {
+    // the workgroup's row slots, added in order
+    constexpr int kCells = NT * V * W;
+    __shared__ float lds[kRows * kCells];
+    for (int k = 0; k < 2; ++k) {
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int w = 0; w < W; ++w) lds[slot * kCells + (q + v * NT) * W + w] = k ? ab[v][w] : aw[v][w];
+      __syncthreads();
+      float* dst = part + (static_cast<int64_t>(k) * nb + blockIdx.x) * D;
+      for (int i = threadIdx.x; i < kCells; i += kBlock) {
+        const int c = i / W;
+        const int col = chunk_start<W>(c, D) + i % W;
+        if (c * W >= D || col < c * W) continue;  // past the row, or another chunk's
+        float s = 0.0f;
+        for (int j = 0; j < kRows; ++j) s += lds[j * kCells + i];
+        dst[col] = s;
+      }
+    }
+  }
+}
+
+// grad_w and grad_b from the nb partial rows of each: a workgroup adds 32
+// columns, 32 slices of the partial rows at a time, then the slices in an LDS
+// tree; a fixed order.
+constexpr int kParamCols = 32, kParamThreads = 1024;
+
+template <typename TW>
+__global__ __launch_bounds__(kParamThreads) void param_kernel(const float* part, int nb, int D, TW* gw, TW* gb) {
+  constexpr int kSlices = kParamThreads / kParamCols;
+  __shared__ float red[kParamThreads];
+  TW* out = blockIdx.y == 0 ? gw : gb;
+  if (!out) return;
+  const float* src = part + static_cast<int64_t>(blockIdx.y) * nb * D;
+  const int c = blockIdx.x * kParamCols + threadIdx.x % kParamCols;
+  const int s = threadIdx.x / kParamCols;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < D) {
+    int b = s;
+    for (; b + 3 * kSlices < nb; b += 4 * kSlices)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) acc[u] += src[static_cast<int64_t>(b + u * kSlices) * D + c];
+    for (; b < nb; b += kSlices) acc[0] += src[static_cast<int64_t>(b) * D + c];
+  }
+  red[threadIdx.x] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  __syncthreads();
+  for (int h = kSlices / 2; h > 0; h >>= 1) {
+    if (s < h) red[threadIdx.x] += red[threadIdx.x + h * kParamCols];
+    __syncthreads();
+  }
+  if (s == 0 && c < D) out[c] = from_f32<TW>(red[threadIdx.x]);
+}
+
+// f(IC<W>, IC<NT>, IC<V>) for rows of D values of T with at most VMAX chunks a
+// lane of a wavefront row: the lanes of a row are the next power of two of its
+// chunks, 64 lanes hold up to VMAX chunks each, wider rows take a workgroup of
+// 256, 512 or 1024 threads.
+template <typename T, int VMAX, class F>
+int with_shape(int D, F&& f) {
+  constexpr int W = kChunk<T>;
+  if (D < W) {
+    if (D <= 1) return f(IC<1>(), IC<1>(), IC<1>());
+    if (D <= 2) return f(IC<1>(), IC<2>(), IC<1>());
+    if (D <= 4) return f(IC<1>(), IC<4>(), IC<1>());
+    return f(IC<1>(), IC<8>(), IC<1>());
+  }
+  const int nc = (D + W - 1) / W;
+  if (nc <= 1) return f(IC<W>(), IC<1>(), IC<1>());
+  if (nc <= 2) return f(IC<W>(), IC<2>(), IC<1>());
+  if (nc <= 4) return f(IC<W>(), IC<4>(), IC<1>());
+  if (nc <= 8) return f(IC<W>(), IC<8>(), IC<1>());
+  if (nc <= 16) return f(IC<W>(), IC<16>(), IC<1>());
+  if (nc <= 32) return f(IC<W>(), IC<32>(), IC<1>());
+  if (nc <= 64) return f(IC<W>(), IC<64>(), IC<1>());
+  if (nc <= 128) return f(IC<W>(), IC<64>(), IC<2>());
+  if constexpr (VMAX >= 3)
+    if (nc <= 192) return f(IC<W>(), IC<64>(), IC<3>());
+  if constexpr (VMAX >= 4)
+    if (nc <= 256) return f(IC<W>(), IC<64>(), IC<4>());
+  if constexpr (VMAX >= 5)
+    if (nc <= 320) return f(IC<W>(), IC<64>(), IC<5>());
+  if (nc <= 256) return f(IC<W>(), IC<256>(), IC<1>());
+  if (nc <= 512) return f(IC<W>(), IC<256>(), IC<2>());
+  if constexpr (W == 4) {
+    if (nc <= 768) return f(IC<W>(), IC<256>(), IC<3>());
+    if (nc <= 1024) return f(IC<W>(), IC<256>(), IC<4>());
+    if (nc <= 2048) return f(IC<W>(), IC<512>(), IC<4>());
+    return f(IC<W>(), IC<1024>(), IC<4>());
+  } else {
+    if (nc <= 1024) return f(IC<W>(), IC<512>(), IC<2>());
+    return f(IC<W>(), IC<1024>(), IC<2>());
+  }
+}
+
+// f(T, TW) for the storage codes of rows and parameters.
+template <class F>
+int with_types(int x_dtype, int w_dtype, F&& f) {
+  if (x_dtype == kF32) return f(float(), float());
+  if (w_dtype == kF32) return f(bf16(), float());
+  return f(bf16(), bf16());
+}
+
+int check_args(const char* who, int64_t n, int D, int x_dtype, int w_dtype) {
+  if (n < 0) return set_error(kInvalid, "%s: negative row count", who);
+  if (D < 1 || D > kMaxWidth) return set_error(kInvalid, "%s: requires 1<=D<=%d, got %d", who, kMaxWidth, D);
+  if ((x_dtype != kF32 && x_dtype != kBF16) || (w_dtype != kF32 && w_dtype != x_dtype))
+    return set_error(kInvalid, "%s: dtypes are 0 or 1, the parameters' 0 or the rows'", who);
+  return kOk;
+}
+
+// Workgroups of the backward: its partial rows.
+int bwd_blocks(int64_t n, int rows) {
+  const int64_t groups = (n + rows - 1) / rows;
+  return static_cast<int>(groups < 512 ? groups : 512);
+}
+
+template <typename T>
+constexpr int kFwdV = sizeof(T) == 4 ? 5 : 4;
+template <typename T>
+constexpr int kBwdV = sizeof(T) == 4 ? 5 : 2;
+
+}  // namespace layernorm
+}  // namespace cign
+
+using namespace cign;
+using namespace cign::layernorm;
+
+extern "C" {
+
+int cign_layernorm_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, const void* x,
+                       int64_t x_stride, const void* weight, const void* bias, float eps, void* y, float* mean,
+                       float* rstd) {
+  const char* who = "cign_layernorm_fwd";
+  const int rc = check_args(who, n, D, x_dtype, w_dtype);
+  if (rc) return rc;
+  if (n == 0) return kOk;
+  if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return set_error(kInvalid, "%s: null argument", who);
+  if (x_stride < 0) return set_error(kInvalid, "%s: negative row stride", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return with_types(x_dtype, w_dtype, [&](auto t, auto tw) {
+    using T = decltype(t);
+    using TW = decltype(tw);
+    return with_shape<T, kFwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
+      constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
+      const int64_t groups = (n + Shape<NT>::kRows - 1) / Shape<NT>::kRows;
+      const int grid = static_cast<int>(groups < 4096 ? groups : 4096);
+      hipLaunchKernelGGL((fwd_kernel<T, TW, W, NT, V>), dim3(grid), dim3(Shape<NT>::kThreads), 0, st, n, D,
+                         static_cast<const T*>(x), x_stride, static_cast<const TW*>(weight),
+                         static_cast<const TW*>(bias), eps, static_cast<T*>(y), mean, rstd);
+      return check_launch(who);
+    });
+  });
+}
+
+int64_t cign_layernorm_bwd_workspace_bytes(int64_t n, int32_t D) {
+  if (n < 0 || D < 1 || D > kMaxWidth) return 0;
+  return 2 * static_cast<int64_t>(sizeof(float)) * bwd_blocks(n, 1) * D;
+}
+
+int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, const void* grad_y,
+                       int64_t grad_y_stride, const void* x, int64_t x_stride, const void* weight, const float* mean,
+                       const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                       int64_t workspace_bytes) {
+  const char* who = "cign_layernorm_bwd";
+  const int rc = check_args(who, n, D, x_dtype, w_dtype);
+  if (rc) return rc;
+  if (n > 0 && (!grad_y || !x || !mean || !rstd)) return set_error(kInvalid, "%s: null argument", who);
+  if (x_stride < 0 || grad_y_stride < 0) return set_error(kInvalid, "%s: negative row stride", who);
+  const bool params = grad_weight || grad_bias;
+  if (!params && (!grad_x || n == 0)) return kOk;
+  if (params && (!workspace || workspace_bytes < cign_layernorm_bwd_workspace_bytes(n, D)))
+    if (n > 0) return set_error(kInvalid, "%s: workspace too small", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return with_types(x_dtype, w_dtype, [&](auto t, auto tw) {
+    using T = decltype(t);
+    using TW = decltype(tw);
+    float* part = params ? static_cast<float*>(workspace) : nullptr;
+    int nb = 0;
+    if (n > 0) {
+      const int err = with_shape<T, kBwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
+        constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
+        nb = bwd_blocks(n, Shape<NT>::kRows);
+        hipLaunchKernelGGL((bwd_kernel<T, TW, W, NT, V>), dim3(nb), dim3(Shape<NT>::kThreads), 0, st, n, D,
+                           static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(x), x_stride,
+                           static_cast<const TW*>(weight), mean, rstd, static_cast<T*>(grad_x), part, nb);
+        return check_launch(who);
+      });
+      if (err) return err;
+    }
+    if (!params) return static_cast<int>(kOk);
+    // no rows: nb = 0 and the sums are zero
+    hipLaunchKernelGGL((param_kernel<TW>), dim3((D + kParamCols - 1) / kParamCols, 2), dim3(kParamThreads), 0, st, part,
+                       nb, D, static_cast<TW*>(grad_weight), static_cast<TW*>(grad_bias));
+    return check_launch(who);
+  });
+}
+
+}  // extern "C"

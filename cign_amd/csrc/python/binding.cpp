@@ -94,6 +94,9 @@ PyMethodDef methods[] = {
     CIGN_ENTRY(cign_gamma_residual_bwd),
     CIGN_ENTRY(cign_add_ln_cat_fwd),
     CIGN_ENTRY(cign_add_ln_cat_bwd),
+    CIGN_ENTRY(cign_layernorm_fwd),
+    CIGN_ENTRY(cign_layernorm_bwd_workspace_bytes),
+    CIGN_ENTRY(cign_layernorm_bwd),
     CIGN_ENTRY(cign_hop_gate_bwd_workspace_bytes),
     CIGN_ENTRY(cign_hop_gate_fwd),
     CIGN_ENTRY(cign_hop_gate_bwd),

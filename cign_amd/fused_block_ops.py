@@ -6,7 +6,9 @@ The three fused ops are:
 - add + LayerNorm;
 - dropout-gamma-residual.
 
-Each has a backward, for rows of 1 <= D <= 256 in float32. The extension object has
+Each has a backward, for rows of 1 <= D <= 256 in float32. ``fused_layernorm``
+(no counterpart in the reference, whose output LayerNorm is torch's) is the
+LayerNorm alone, for rows of up to 16384 values in float32 or bfloat16. The extension object has
 the reference binding's six entry points (fused_block_ops.py:15 inline
 binding; fused_block_ops_ext/fused_block_ops.cpp:39-98), over the C-ABI
 entry points cign_dropout_ln_*, cign_add_ln_* and cign_gamma_residual_*.
@@ -17,11 +19,14 @@ Dropout keep bits are splitmix64(seed ^ (idx * 0xD2B74407B1CE6E93)) >> 11 as a
 from __future__ import annotations
 
 import itertools
+import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check, check_input
+from ._rows import as_rows, check_rows, on_device_of
 
 _EXT = None
 _EXT_ERROR = None
@@ -348,3 +353,90 @@ def fused_dropout_gamma_residual(h, g, gamma, dropout_p):
     if gamma.dim() != 1 or gamma.numel() != D:
         raise ValueError(f"vector gamma must have shape [{D}]")
     return _DropoutGammaResidualFn.apply(h, g, gamma, float(dropout_p), _next_seed(2, dropout_p))
+
+
+MAX_LAYERNORM_WIDTH = 16384
+
+
+def _layernorm_forward(x, weight, bias, eps, with_stats):
+    """(y, mean, rstd) of cign_layernorm_fwd; mean and rstd ([rows]) are None
+    unless with_stats."""
+    lib = _lib.load_library()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows, stride = as_rows(x)
+    n, D = rows.shape
+    mean = rstd = None
+    if with_stats:
+        mean = torch.empty((n,), dtype=torch.float32, device=x.device)
+        rstd = torch.empty((n,), dtype=torch.float32, device=x.device)
+    param = weight if weight is not None else bias
+    code = _lib.DTYPE_CODE[x.dtype if param is None else param.dtype]
+    with on_device_of(x):
+        lib.call("cign_layernorm_fwd", _lib.stream_ptr(x.device), n, D, _lib.DTYPE_CODE[x.dtype], code,
+                 rows.data_ptr(), stride, _lib.ptr(weight), _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(mean),
+                 _lib.ptr(rstd))
+    return y, mean, rstd
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """cign_layernorm_fwd / cign_layernorm_bwd."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _layernorm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, mean, rstd = ctx.saved_tensors
+        lib = _lib.load_library()
+        rows, stride = as_rows(x)
+        grads, grad_stride = as_rows(grad_y)
+        n, D = rows.shape
+        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device)
+        gx = new(x.shape, x.dtype) if ctx.needs_input_grad[0] else None
+        gw = new((D,), weight.dtype) if ctx.needs_input_grad[1] else None
+        gb = new((D,), ctx.bias_dtype) if ctx.needs_input_grad[2] else None
+        dtype = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
+        ws_bytes = 0 if gw is None and gb is None else int(lib.cign_layernorm_bwd_workspace_bytes(n, D))
+        ws = _lib.workspace(ws_bytes, x.device) if ws_bytes else None
+        with on_device_of(x):
+            lib.call("cign_layernorm_bwd", _lib.stream_ptr(x.device), n, D, _lib.DTYPE_CODE[x.dtype],
+                     _lib.DTYPE_CODE[dtype], grads.data_ptr(), grad_stride, rows.data_ptr(), stride,
+                     _lib.ptr(weight), mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb),
+                     _lib.ptr(ws), ws_bytes)
+        return gx, gw, gb, None
+
+
+def fused_layernorm(x, weight=None, bias=None, eps=1e-5):
+    """LayerNorm over the last axis: (x - mean) / sqrt(var + eps) * weight +
+    bias, var the biased variance, all sums in float32, the result in x's type.
+
+    x: [..., D], float32 or bfloat16, 1 <= D <= 16384; row-strided views are
+    read in place. weight, bias: [D], float32 or x's type (both the same), or
+    None for ones and zeros. Gradients of all three, once differentiable;
+    those of weight and bias are summed over the rows in float32, in an order
+    that depends on the shape alone."""
+    D = check_rows(x, "x", MAX_LAYERNORM_WIDTH)
+    dtype = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, x.dtype) or dtype not in (None, t.dtype):
+            raise TypeError("LayerNorm weight/bias must both be float32 or both of x's type")
+        if t.shape != (D,):
+            raise ValueError(f"LayerNorm {name} must have shape [{D}], got {tuple(t.shape)}")
+        if t.device != x.device:
+            raise ValueError(f"LayerNorm {name} must be on {x.device}, got {t.device}")
+        dtype = t.dtype
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias))):
+        return _LayerNormFn.apply(x, weight, bias, eps)
+    return _layernorm_forward(x, weight, bias, eps, False)[0]

@@ -340,6 +340,33 @@ int cign_gamma_residual_bwd(void* stream, int64_t n, int32_t D, const float* gra
                             const float* gamma, const uint8_t* mask, float dropout_p, float* grad_g, float* grad_gamma,
                             void* workspace, int64_t workspace_bytes);
 
+/* ---- LayerNorm of any width (float32 or bfloat16, 1 <= D <= 16384) --------- */
+
+/* y[r] = (x[r] - mean) * rstd * weight + bias over rows of D values, rstd =
+ * 1 / sqrt(var + eps), var the biased variance; sums in float32, y in x's
+ * type. x_dtype 0 or 1; w_dtype, of weight and bias, 0 or x_dtype. weight or
+ * bias may be NULL (ones, zeros). Row r of x starts at r * x_stride values
+ * (x_stride may be 0 or below D: x is only read); y is [n, D]. mean and rstd
+ * [n] float32, both or neither (NULL: an evaluation that keeps neither). No
+ * alignment beyond the type's own. No counterpart in the reference: its
+ * output LayerNorm is torch's (generic_engine/model_cign.py:1195-1199). */
+int cign_layernorm_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, const void* x,
+                       int64_t x_stride, const void* weight, const void* bias, float eps, void* y, float* mean,
+                       float* rstd);
+
+/* Workspace bytes of cign_layernorm_bwd with grad_weight or grad_bias. */
+int64_t cign_layernorm_bwd_workspace_bytes(int64_t n, int32_t D);
+
+/* Gradients of the above given grad_y (x's type, rows grad_y_stride values
+ * apart): grad_x [n, D], grad_weight and grad_bias [D] (w_dtype), each may be
+ * NULL. The parameters' gradients are float32 sums over the rows in an order
+ * that depends on (n, D) alone, rounded once; without them the workspace may
+ * be NULL. */
+int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, const void* grad_y,
+                       int64_t grad_y_stride, const void* x, int64_t x_stride, const void* weight, const float* mean,
+                       const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
+                       int64_t workspace_bytes);
+
 /* ---- hop gate (float32) ------------------------------------------------- */
 
 /* Node-mode hop gate: alpha [n,K] = softmax_k(score @ weight^T + bias), score
