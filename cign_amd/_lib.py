@@ -77,6 +77,11 @@ _SIGNATURES = {
     "cign_layernorm_bwd_workspace_bytes": (_I64, [_I64, _I32]),
     "cign_layernorm_bwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P,
                                      _I64]),
+    # rows of logits (class_logprobs.hip)
+    "cign_class_logprobs_workspace_bytes": (_I64, [_I32, _I64, _I32, _I32]),
+    "cign_class_logprobs_fwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _P, _I64, _I32, _P, _P, _P, _P, _P, _P,
+                                          _I64]),
+    "cign_class_logprobs_bwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _P, _I64, _P, _P, _P, _P]),
     # hop gate (gate.hip)
     "cign_hop_gate_bwd_workspace_bytes": (_I64, [_I64, _I32, _I32]),
     "cign_hop_gate_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),

@@ -1,0 +1,497 @@
+// Log probabilities of given classes, entropy and the top classes of rows of
+// logits, and the gradient of the first two.
+//
+// With l = x / T, lse = log sum e^l and p = e^(l - lse):
+//   logprob = l[label] - lse, entropy = -sum p (l - lse) = ln2 (log2 s - t / s)
+//   (m, s, t: rowsoftmax.h), top classes by x, the lowest index first among
+//   equals;
+//   grad_x[j] = (g ([j = label] - p_j) - h p_j (log p_j + entropy)) / T for the
+//   gradients g of logprob and h of entropy.
+// The forward reads the logits once, the backward reads them once and writes
+// their gradient; nothing of the row's length is kept between the two, only
+// (m, log2 s, entropy) of each row.
+//
+// Top classes are ordered by a 64-bit key, the value's order-preserving bits
+// above the complement of the index, so that every key of a row is different
+// and the order never depends on which thread finds a class.
+#include "rowsoftmax.h"
+
+namespace cign {
+namespace class_logprobs {
+using namespace rowsoftmax;
+
+constexpr int kCandidates = 1024;    // keys a slice's selection keeps in LDS
+constexpr int kShortTopRow = 512;    // longest row whose top classes lane groups pick
+
+// NaN counts as -inf, -0 as +0.
+__device__ __forceinline__ float ranked(float x) { return fmaxf(x, -kInf) + 0.0f; }
+__device__ __forceinline__ uint64_t key_of(float x, int index) {
+  const uint32_t b = __float_as_uint(ranked(x));
+  const uint32_t u = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+  return static_cast<uint64_t>(u) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+
+// A row's outputs, written by one thread.
+struct Out {
+  const int64_t* label;  // NULL: none asked for
+  int64_t ignore;
+  float* logprob;
+  float* entropy;
+  float* stats;  // [n, 4]: m, log2 s (inf: no class left), entropy, unused; NULL: not kept
+  int K;
+  float* top_logprob;
+  int64_t* top_index;
+};
+
+template <typename T>
+struct In {
+  int64_t n;
+  int V;
+  const T* x;
+  int64_t ld;
+  float c, inv_t;  // log2(e) / T, 1 / T
+};
+
+__device__ __forceinline__ float logprob_of(float x, float m, float l2s, float inv_t) {
+  return (x - m) * inv_t - l2s * kLn2;
+}
+
+// Label, entropy and statistics of row r from its joined (m, s, t); l2s is
+// what logprob_of takes, 0 for a row without a class (-inf then comes out).
+template <typename T>
+__device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t, float& l2s) {
+  const bool none = s == 0.0f;
+  l2s = none ? 0.0f : log2f(s);
+  const float H = none ? 0.0f : kLn2 * (l2s - t / s);
+  o.entropy[r] = H;
+  if (o.label) {
+    const int64_t y = o.label[r];
+    float lp = 0.0f;
+    if (y != o.ignore)
+      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), m, l2s, in.inv_t) : __builtin_nanf("");
+    o.logprob[r] = lp;
+  }
+  if (o.stats) {
+    float* p = o.stats + 4 * r;
+    p[0] = m;
+    p[1] = none ? kInf : l2s;
+    p[2] = H;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void put_top(const In<T>& in, const Out& o, int64_t r, int rank, uint64_t key, float m,
+                                        float l2s) {
+  const int i = key_index(key);
+  o.top_index[r * o.K + rank] = i;
+  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), m, l2s, in.inv_t);
+}
+
+// The largest key below `below` of a share's own values.
+template <typename T, int W, int U>
+__device__ __forceinline__ uint64_t best_below(const Share<T, W, U>& sh, uint64_t below) {
+  uint64_t best = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[W];
+    RowChunk<T, W>::unpack(sh.raw[u], v);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const uint64_t k = key_of(v[w], sh.at[u] + w);
+      if (w >= sh.own[u] && k < below && k > best) best = k;
+    }
+  }
+  return best;
+}
+
+template <int LPR>
+__device__ __forceinline__ uint64_t group_max(uint64_t k) {
+  for_offsets<1, LPR>([&](auto OC) {
+    constexpr int o = decltype(OC)::value;
+    const uint32_t lo = __float_as_uint(xor_shfl<o>(__uint_as_float(static_cast<uint32_t>(k))));
+    const uint32_t hi = __float_as_uint(xor_shfl<o>(__uint_as_float(static_cast<uint32_t>(k >> 32))));
+    const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
+    if (other > k) k = other;
+  });
+  return k;
+}
+
+// Rows that LPR lanes hold.
+template <typename T, int W, int LPR, int U, bool TOP>
+__global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
+  constexpr int kRows = kBlock / LPR;
+  const int q = threadIdx.x & (LPR - 1);
+  const int nc = (in.V + W - 1) / W;
+  Share<T, W, U> sh;
+  sh.place(q, LPR, nc, in.V);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / LPR; r < in.n; r += step) {
+    sh.load(in.x + r * in.ld);
+    sh.mask_foreign();
+    float m = sh.largest(), s = 0.0f, t = 0.0f;
+    sh.template sums<true>(shift_of(m), in.c, s, t);
+    join<LPR>(m, s, t, in.c);
+    float l2s = s == 0.0f ? 0.0f : log2f(s);
+    if (q == 0) finish(in, o, r, m, s, t, l2s);
+    if constexpr (TOP) {
+      uint64_t mine = best_below(sh, ~0ull);
+      for (int k = 0; k < o.K; ++k) {
+        const uint64_t best = group_max<LPR>(mine);
+        if (mine == best) {  // one lane: keys differ
+          put_top(in, o, r, k, best, m, l2s);
+          mine = best_below(sh, best);
+        }
+      }
+    }
+  }
+}
+
+// Slices of long rows: (m, s, t) to part[(r * S + slice)] (a float4), the K
+// largest keys, in falling order, to keys[(r * S + slice) * K ...] (0: the
+// slice has no more). With S = 1 the row's outputs are written at once.
+template <typename T, int U, bool TOP>
+__global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float4* part, uint64_t* keys) {
+  constexpr int W = kChunk<T>;
+  __shared__ float slots[2 * kWavesPerBlock][3];
+  __shared__ uint64_t sample[TOP ? kBlock : 1];
+  __shared__ uint64_t cand[TOP ? kCandidates : 1];
+  __shared__ uint64_t threshold;
+  __shared__ int found;
+  const int nc = (in.V + W - 1) / W;
+  const int64_t items = in.n * sl.S;
+  const int lane = lane_id();
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t r = item / sl.S;
+    const int slice = static_cast<int>(item - r * sl.S);
+    const int end = min((slice + 1) * sl.cps, nc);
+    Share<T, W, U> sh;
+    sh.place(slice * sl.cps + threadIdx.x, kBlock, end, in.V);
+    sh.load(in.x + r * in.ld);
+    sh.mask_foreign();
+    float m = sh.largest(), s = 0.0f, t = 0.0f;
+    sh.template sums<true>(shift_of(m), in.c, s, t);
+    join<kWave>(m, s, t, in.c);
+    // the wavefronts' results; a wavefront's shift is its largest value, or 0 with s = 0
+    float(*sl_slots)[3] = slots + turn * kWavesPerBlock;
+    turn ^= 1;
+    if (lane == 0) {
+      float* p = sl_slots[wave_id()];
+      p[0] = s == 0.0f ? -kInf : m;
+      p[1] = s;
+      p[2] = t;
+    }
+    if (TOP && threadIdx.x == 0) {
+      threshold = 1;
+      found = 0;
+    }
+    uint64_t mine = 0;
+    if constexpr (TOP) {
+      mine = best_below(sh, ~0ull);
+      sample[threadIdx.x] = mine;
+    }
+    __syncthreads();
+    const bool has = lane < kWavesPerBlock;
+    m = has ? sl_slots[lane & 3][0] : -kInf;
+    s = has ? sl_slots[lane & 3][1] : 0.0f;
+    t = has ? sl_slots[lane & 3][2] : 0.0f;
+    join<kWavesPerBlock>(m, s, t, in.c);  // lanes 0..3 of each wavefront
+    m = shfl(m, 0);
+    s = shfl(s, 0);
+    t = shfl(t, 0);
+    float l2s = s == 0.0f ? 0.0f : log2f(s);
+    if (threadIdx.x == 0) {
+      if (sl.S == 1)
+        finish(in, o, r, m, s, t, l2s);
+      else
+        part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
+    }
+    if constexpr (TOP) {
+      // The K-th largest of the threads' best keys bounds the slice's K-th
+      // key from below; every key at or above it is a candidate.
+      const int K = o.K;
+      int above = 0;
+      for (int i = 0; i < kBlock; ++i) above += sample[i] > mine;
+      if (mine != 0 && above == K - 1) threshold = mine;
+      __syncthreads();
+      const uint64_t bar = threshold;
+      if (mine >= bar) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float v[W];
+          RowChunk<T, W>::unpack(sh.raw[u], v);
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const uint64_t k = key_of(v[w], sh.at[u] + w);
+            if (w >= sh.own[u] && k >= bar) {
+              const int at = atomicAdd(&found, 1);
+              if (at < kCandidates) cand[at] = k;
+            }
+          }
+        }
+      }
+      __syncthreads();
+      const int count = found;
+      uint64_t* list = keys + item * K;
+      if (count <= kCandidates) {
+        for (int i = threadIdx.x; i < count; i += kBlock) {
+          const uint64_t k = cand[i];
+          int rank = 0;
+          for (int j = 0; j < count; ++j) rank += cand[j] > k;
+          if (rank < K) {
+            if (sl.S == 1)
+              put_top(in, o, r, rank, k, m, l2s);
+            else
+              list[rank] = k;
+          }
+        }
+        if (sl.S > 1)
+          for (int i = count + threadIdx.x; i < K; i += kBlock) list[i] = 0;
+      } else {
+        // More candidates than the buffer holds (many large values in few
+        // threads' chunks): K rounds over the registers.
+        uint64_t below = ~0ull;
+        for (int k = 0; k < K; ++k) {
+          const uint64_t w = group_max<kWave>(best_below(sh, below));
+          __syncthreads();
+          if (lane == 0) sample[wave_id()] = w;
+          __syncthreads();
+          uint64_t best = sample[0];
+          for (int i = 1; i < kWavesPerBlock; ++i) best = sample[i] > best ? sample[i] : best;
+          if (threadIdx.x == 0) {
+            if (sl.S == 1)
+              put_top(in, o, r, k, best, m, l2s);
+            else
+              list[k] = best;
+          }
+          below = best;
+        }
+      }
+      __syncthreads();  // the next item's samples and candidates
+    }
+  }
+}
+
+// Rows from their slices: a wavefront a row; lane i holds slice i. The top
+// classes are merged from the slices' falling lists, kept in LDS.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kWave) void join_kernel(In<T> in, Out o, int S, const float4* part, const uint64_t* keys) {
+  extern __shared__ uint64_t lists[];
+  const int lane = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < in.n; r += gridDim.x) {
+    const bool has = lane < S;
+    const float4 p = has ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
+    float m = p.x, s = p.y, t = p.z;
+    if constexpr (TOP) {
+      __syncthreads();
+      for (int i = lane; i < S * o.K; i += kWave) lists[i] = keys[r * S * o.K + i];
+      __syncthreads();
+    }
+    join<kWave>(m, s, t, in.c);
+    float l2s = s == 0.0f ? 0.0f : log2f(s);
+    if (lane == 0) finish(in, o, r, m, s, t, l2s);
+    if constexpr (TOP) {
+      int next = 0;
+      uint64_t mine = has ? lists[lane * o.K] : 0;
+      for (int k = 0; k < o.K; ++k) {
+        const uint64_t best = group_max<kWave>(mine);
+        if (has && mine == best) {
+          put_top(in, o, r, k, best, m, l2s);
+          ++next;
+          mine = next < o.K ? lists[lane * o.K + next] : 0;
+        }
+      }
+    }
+  }
+}
+
+// grad_x of rows held by LPR threads (lanes, or LPR = 256: the slices of a
+// long row). Rows whose gradients are both zero (an ignored label) are zeros,
+// whatever their logits hold.
+template <typename T, int W, int LPR, int U, bool ENT>
+__global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, const int64_t* label, int64_t ignore,
+                                                      const float* stats, const float* g_lp, const float* g_ent,
+                                                      T* gx) {
+  using X = RowChunk<T, W>;
+  constexpr int kRows = kBlock / LPR;
+  const int q = threadIdx.x & (LPR - 1);
+  const int nc = (in.V + W - 1) / W;
+  const int64_t items = in.n * S;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / LPR; item < items; item += step) {
+    const int64_t r = S == 1 ? item : item / S;
+    const int slice = S == 1 ? 0 : static_cast<int>(item - r * S);
+    const float m = stats[4 * r], l2s = stats[4 * r + 1];
+    const int64_t y = label ? label[r] : ignore;
+    float g = 0.0f, h = 0.0f;
+    if (g_lp && y != ignore) g = y >= 0 && y < in.V ? g_lp[r] : __builtin_nanf("");
+    if (ENT) h = g_ent[r];
+    if (l2s == kInf) g = h = 0.0f;  // no class left
+    // p_j (a + b log2 p_j), and g at the label
+    const float a = -(g + h * stats[4 * r + 2]) * in.inv_t, b = -h * kLn2 * in.inv_t;
+    const float gl = g * in.inv_t;
+    const bool zero = g == 0.0f && h == 0.0f;
+    Share<T, W, U> sh;
+    sh.place(slice * cps + q, LPR, min((slice + 1) * cps, nc), in.V);
+    if (!zero) sh.load(in.x + r * in.ld);
+    T* row = gx + r * in.V;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[W];
+      if (zero) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[w] = 0.0f;
+      } else {
+        X::unpack(sh.raw[u], v);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float d = fmaf(v[w] - m, in.c, -l2s);
+          const float p = __builtin_amdgcn_exp2f(d);
+          v[w] = p * (ENT ? fmaf(b, fmaxf(d, -1e30f), a) : a);
+        }
+        const int64_t at = y - sh.at[u];
+        if (at >= 0 && at < W)
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (w == at) v[w] += gl;
+      }
+      Share<T, W, U>::store(row, sh.at[u], sh.own[u], v);
+    }
+  }
+}
+
+int check_args(const char* who, int dtype, int64_t n, int V, int64_t ld, float temperature) {
+  if (dtype != kF32 && dtype != kBF16) return set_error(kInvalid, "%s: dtype must be 0 or 1", who);
+  if (n < 0) return set_error(kInvalid, "%s: negative row count", who);
+  if (V < 1 || V > kMaxClasses) return set_error(kInvalid, "%s: requires 1<=V<=%d, got %d", who, kMaxClasses, V);
+  if (ld < 0) return set_error(kInvalid, "%s: negative row stride", who);
+  if (!(temperature > 0.0f && temperature < kInf)) return set_error(kInvalid, "%s: temperature must be positive", who);
+  return kOk;
+}
+
+// Whether slices take the row: longer than a wavefront holds, or than its
+// lanes' rounds pick top classes from.
+template <typename T>
+bool sliced(int V, int K) {
+  return !wavefront_row<T>(V) || (K > 0 && V > kShortTopRow);
+}
+
+template <typename F>
+int with_type(int dtype, F&& f) {
+  return dtype == kF32 ? f(float()) : f(bf16());
+}
+
+template <typename T>
+int64_t workspace_bytes(int64_t n, int V, int K) {
+  if (!sliced<T>(V, K)) return 0;
+  const Slicing sl = slicing<T>(V, n);
+  return sl.S == 1 ? 0 : n * sl.S * (static_cast<int64_t>(sizeof(float4)) + 8 * K);
+}
+
+template <typename T>
+int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void* workspace, int64_t bytes) {
+  if (bytes < workspace_bytes<T>(in.n, in.V, o.K)) return set_error(kInvalid, "%s: workspace too small", who);
+  if (!sliced<T>(in.V, o.K))
+    return with_lanes<T>(in.V, [&](auto WC, auto LC, auto UC) {
+      constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;
+      constexpr int kRows = kBlock / LPR;
+      const int grid = grid_of((in.n + kRows - 1) / kRows);
+      if (o.K > 0) {
+        if constexpr (W * LPR * U <= kShortTopRow)
+          hipLaunchKernelGGL((lanes_kernel<T, W, LPR, U, true>), dim3(grid), dim3(kBlock), 0, st, in, o);
+      } else {
+        hipLaunchKernelGGL((lanes_kernel<T, W, LPR, U, false>), dim3(grid), dim3(kBlock), 0, st, in, o);
+      }
+      return check_launch(who);
+    });
+  const Slicing sl = slicing<T>(in.V, in.n);
+  float4* part = static_cast<float4*>(workspace);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(part + (sl.S == 1 ? 0 : in.n * sl.S));
+  const int rc = with_chunks<T>(sl.U, [&](auto UC) {
+    constexpr int U = decltype(UC)::value;
+    const int grid = grid_of(in.n * sl.S);
+    if (o.K > 0)
+      hipLaunchKernelGGL((slice_kernel<T, U, true>), dim3(grid), dim3(kBlock), 0, st, in, o, sl, part, keys);
+    else
+      hipLaunchKernelGGL((slice_kernel<T, U, false>), dim3(grid), dim3(kBlock), 0, st, in, o, sl, part, keys);
+    return check_launch(who);
+  });
+  if (rc || sl.S == 1) return rc;
+  const int grid = grid_of(in.n);
+  if (o.K > 0)
+    hipLaunchKernelGGL((join_kernel<T, true>), dim3(grid), dim3(kWave), sizeof(uint64_t) * sl.S * o.K, st, in, o, sl.S,
+                       part, keys);
+  else
+    hipLaunchKernelGGL((join_kernel<T, false>), dim3(grid), dim3(kWave), 0, st, in, o, sl.S, part, keys);
+  return check_launch(who);
+}
+
+}  // namespace class_logprobs
+}  // namespace cign
+
+using namespace cign;
+using namespace cign::class_logprobs;
+
+extern "C" {
+
+int64_t cign_class_logprobs_workspace_bytes(int32_t dtype, int64_t n, int32_t V, int32_t top_k) {
+  if (n < 1 || V < 1 || V > kMaxClasses || top_k < 0 || top_k > kMaxList) return 0;
+  return with_type(dtype, [&](auto t) { return workspace_bytes<decltype(t)>(n, V, top_k); });
+}
+
+int cign_class_logprobs_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                            float temperature, const int64_t* label, int64_t ignore_index, int32_t top_k,
+                            float* logprob, float* entropy, float* top_logprob, int64_t* top_index, float* stats,
+                            void* workspace, int64_t workspace_bytes) {
+  const char* who = "cign_class_logprobs_fwd";
+  const int rc = check_args(who, dtype, n, V, x_stride, temperature);
+  if (rc) return rc;
+  if (top_k < 0 || top_k > kMaxList || top_k > V)
+    return set_error(kInvalid, "%s: requires 0<=top_k<=min(V, %d), got %d", who, kMaxList, top_k);
+  if (n == 0) return kOk;
+  if (!x || !entropy || (label && !logprob) || (top_k > 0 && (!top_logprob || !top_index)))
+    return set_error(kInvalid, "%s: null argument", who);
+  const Out o{label, ignore_index, logprob, entropy, stats, top_k, top_logprob, top_index};
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const In<T> in{n, V, static_cast<const T*>(x), x_stride, kLog2e / temperature, 1.0f / temperature};
+    return forward(who, static_cast<hipStream_t>(stream), in, o, workspace, workspace_bytes);
+  });
+}
+
+int cign_class_logprobs_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                            float temperature, const int64_t* label, int64_t ignore_index, const float* stats,
+                            const float* grad_logprob, const float* grad_entropy, void* grad_x) {
+  const char* who = "cign_class_logprobs_bwd";
+  const int rc = check_args(who, dtype, n, V, x_stride, temperature);
+  if (rc) return rc;
+  if (n == 0) return kOk;
+  if (!x || !stats || !grad_x || (grad_logprob && !label)) return set_error(kInvalid, "%s: null argument", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    const In<T> in{n, V, static_cast<const T*>(x), x_stride, kLog2e / temperature, 1.0f / temperature};
+    const auto launch = [&](auto WC, auto LC, auto UC, int S, int cps) {
+      constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;
+      constexpr int kRows = kBlock / LPR;
+      const int grid = grid_of((n * S + kRows - 1) / kRows);
+      if (grad_entropy)
+        hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, true>), dim3(grid), dim3(kBlock), 0, st, in, S, cps, label,
+                           ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
+      else
+        hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, false>), dim3(grid), dim3(kBlock), 0, st, in, S, cps, label,
+                           ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
+      return check_launch(who);
+    };
+    constexpr int kW = kChunk<T>;
+    const int nc = (V + kW - 1) / kW;
+    if (wavefront_row<T>(V))
+      return with_lanes<T>(V, [&](auto WC, auto LC, auto UC) { return launch(WC, LC, UC, 1, V); });
+    constexpr int U = 16 / kW * 2;  // 32 values a thread
+    const int S = (nc + kBlock * U - 1) / (kBlock * U);
+    return launch(IC<kW>(), IC<kBlock>(), IC<U>(), S, (nc + S - 1) / S);
+  });
+}
+
+}  // extern "C"

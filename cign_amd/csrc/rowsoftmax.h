@@ -1,0 +1,203 @@
+// What the operators over rows of logits share (class_logprobs.hip,
+// distill.hip): how a row is laid over threads, and its softmax statistics.
+//
+// l = x / T is the row's logits at temperature T and c = log2(e) / T, so that
+// exp(l - l_max) = 2^((x - m) c) with m the largest x: the shift is taken from
+// x itself, before any rounding of a product, and one hardware exponential
+// (v_exp_f32) makes each term. A row's statistics are (m, s, t):
+//   s = sum 2^((x - m) c), t = sum 2^((x - m) c) (x - m) c,
+// in float32; a masked class (-inf) adds nothing to either. A row of masked
+// classes alone has s = 0.
+//
+// Rows of up to 64 lanes x 8 chunks belong to lanes of one wavefront (the
+// next power of two of the row's chunks); longer rows are cut into slices, a
+// workgroup each, whose statistics a second kernel joins. Either way the
+// values stay in registers between the largest value and the sums, so the
+// logits are read once.
+#pragma once
+
+#include "rowvec.h"
+
+namespace cign {
+namespace rowsoftmax {
+using namespace rowvec;
+
+constexpr int kMaxClasses = 1 << 20;
+constexpr int kMaxList = 128;   // entries of a row's list of classes
+constexpr int kMaxSlices = 64;  // one lane of the joining wavefront each
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr float kInf = __builtin_huge_valf();
+
+template <int N>
+using IC = std::integral_constant<int, N>;
+
+// Workgroups of a launch that strides over its items.
+constexpr int64_t kMaxGrid = 1 << 20;
+inline int grid_of(int64_t items) { return static_cast<int>(items < kMaxGrid ? items : kMaxGrid); }
+
+// f(IC<W>, IC<LPR>, IC<U>) for rows of V values of T that a wavefront holds,
+// -1 for longer ones.
+template <typename T, class F>
+int with_lanes(int V, F&& f) {
+  constexpr int W = kChunk<T>;
+  if (V < W) {
+    if (V <= 1) return f(IC<1>(), IC<1>(), IC<1>());
+    if (V <= 2) return f(IC<1>(), IC<2>(), IC<1>());
+    if (V <= 4) return f(IC<1>(), IC<4>(), IC<1>());
+    return f(IC<1>(), IC<8>(), IC<1>());
+  }
+  const int nc = (V + W - 1) / W;
+  if (nc <= 1) return f(IC<W>(), IC<1>(), IC<1>());
+  if (nc <= 2) return f(IC<W>(), IC<2>(), IC<1>());
+  if (nc <= 4) return f(IC<W>(), IC<4>(), IC<1>());
+  if (nc <= 8) return f(IC<W>(), IC<8>(), IC<1>());
+  if (nc <= 16) return f(IC<W>(), IC<16>(), IC<1>());
+  if (nc <= 32) return f(IC<W>(), IC<32>(), IC<1>());
+  if (nc <= 64) return f(IC<W>(), IC<64>(), IC<1>());
+  if (nc <= 128) return f(IC<W>(), IC<64>(), IC<2>());
+  if (nc <= 256) return f(IC<W>(), IC<64>(), IC<4>());
+  if (nc <= 512) return f(IC<W>(), IC<64>(), IC<8>());
+  return -1;
+}
+
+template <typename T>
+bool wavefront_row(int V) {
+  return V <= 512 * kChunk<T>;
+}
+
+// The slices of long rows: S a row, of cps chunks each, U chunks a thread
+// (256 U >= cps; U W <= 64 values). The longest that leave at least 1024
+// workgroups, so that few rows still spread over the card.
+struct Slicing {
+  int U, S, cps;
+};
+template <typename T>
+Slicing slicing(int V, int64_t n) {
+  constexpr int W = kChunk<T>;
+  const int nc = (V + W - 1) / W;
+  int U = 64 / W;
+  auto slices = [&](int u) { return (nc + kBlock * u - 1) / (kBlock * u); };
+  while (U > 1 && n * slices(U) < 1024 && slices(U / 2) <= kMaxSlices) U /= 2;
+  const int S = slices(U), cps = (nc + S - 1) / S;
+  while (U > 1 && kBlock * (U / 2) >= cps) U /= 2;
+  return Slicing{U, S, cps};
+}
+
+template <typename T, class F>
+int with_chunks(int U, F&& f) {
+  if (U <= 1) return f(IC<1>());
+  if (U <= 2) return f(IC<2>());
+  if (U <= 4) return f(IC<4>());
+  if (U <= 8) return f(IC<8>());
+  if constexpr (sizeof(T) == 4) return f(IC<16>());
+  return -1;
+}
+
+// The values of a raw chunk whose bit of `kill` is set become -inf. Chunks
+// that keep all of theirs (nearly every one) skip the work together.
+template <typename T, int W>
+__device__ __forceinline__ void mask_out(typename RowChunk<T, W>::Raw& q, uint32_t kill) {
+  if (kill == 0) return;
+  if constexpr (W == 1) {
+    q = from_f32<T>(-kInf);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (kill >> w & 1) q[w] = -kInf;
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (kill >> w & 1) q[w / 2] = w & 1 ? (q[w / 2] & 0xffffu) | 0xff800000u : (q[w / 2] & 0xffff0000u) | 0xff80u;
+  }
+}
+
+// A thread's share of a row: U chunks at positions first, first + stride, ...
+// below `end` (chunk numbers); places past the end repeat the last chunk and
+// own nothing.
+template <typename T, int W, int U>
+struct Share {
+  using X = RowChunk<T, W>;
+  typename X::Raw raw[U];
+  int at[U];   // first value of the chunk
+  int own[U];  // its own values start here (W: none)
+
+  __device__ __forceinline__ void place(int first, int stride, int end, int V) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = first + u * stride;
+      at[u] = chunk_start<W>(c < end ? c : end - 1, V);
+      own[u] = c < end ? c * W - at[u] : W;
+    }
+  }
+  __device__ __forceinline__ void load(const T* row) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = X::load(row + at[u]);
+  }
+  __device__ __forceinline__ void mask_foreign() {
+#pragma unroll
+    for (int u = 0; u < U; ++u) mask_out<T, W>(raw[u], (1u << own[u]) - 1u);
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = -kInf;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[W];
+      X::unpack(raw[u], v);
+#pragma unroll
+      for (int w = 0; w < W; ++w) m = fmaxf(m, v[w]);
+    }
+    return m;
+  }
+  // Adds the share's s (and t) relative to m.
+  template <bool WITH_T>
+  __device__ __forceinline__ void sums(float m, float c, float& s, float& t) const {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[W];
+      X::unpack(raw[u], v);
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float d = (v[w] - m) * c;
+        const float e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        if constexpr (WITH_T) t = fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf counts nothing
+      }
+    }
+  }
+  // Stores chunk u's own values of a result.
+  static __device__ __forceinline__ void store(T* row, int at, int own, const float (&v)[W]) {
+    if (own == 0) {
+      X::store(row + at, v);
+    } else if (own < W) {
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (w >= own) row[at + w] = from_f32<T>(v[w]);
+    }
+  }
+};
+
+// The shift of a row whose largest value is m: 0 for a row without any.
+__device__ __forceinline__ float shift_of(float m) { return m == -kInf ? 0.0f : m; }
+
+// Joins statistics over the LPR lanes of a group (one (m, s, t) a lane; m as
+// largest() gave it, s and t relative to shift_of(m)). m becomes the shift.
+template <int LPR>
+__device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
+  float top = m;
+  for_offsets<1, LPR>([&](auto OC) { top = fmaxf(top, xor_shfl<decltype(OC)::value>(top)); });
+  top = shift_of(top);
+  const float d = (shift_of(m) - top) * c;
+  const float e = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(d);
+  t = s == 0.0f ? 0.0f : e * fmaf(s, fmaxf(d, -1e30f), t);
+  s *= e;
+  for_offsets<1, LPR>([&](auto OC) {
+    constexpr int o = decltype(OC)::value;
+    s += xor_shfl<o>(s);
+    t += xor_shfl<o>(t);
+  });
+  m = top;
+}
+
+}  // namespace rowsoftmax
+}  // namespace cign

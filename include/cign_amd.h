@@ -367,6 +367,35 @@ int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
                        const float* rstd, void* grad_x, void* grad_weight, void* grad_bias, void* workspace,
                        int64_t workspace_bytes);
 
+/* ---- rows of logits (float32 or bfloat16, 1 <= V <= 1048576) --------------- */
+
+/* Workspace bytes of cign_class_logprobs_fwd. */
+int64_t cign_class_logprobs_workspace_bytes(int32_t dtype, int64_t n, int32_t V, int32_t top_k);
+
+/* For the logits x of n rows (row r at r * x_stride values), l = x /
+ * temperature and lse = log sum_j e^l: logprob[r] = l[label[r]] - lse (0
+ * where label[r] is ignore_index, NaN where it is another value outside
+ * [0, V); label NULL: no logprob), entropy[r] = -sum p log p, and the top_k
+ * classes (0..128, at most V) in falling order, the lowest index first among
+ * equals (NaN counts as -inf): top_logprob, top_index [n, top_k]. -inf
+ * masks a class; a row without any class left has logprob -inf, entropy 0.
+ * stats [n, 4] float32 is what cign_class_logprobs_bwd reads (NULL: not
+ * kept). No alignment beyond the type's own. No counterpart in the reference:
+ * it takes torch's cross-entropy, argmax and softmax of its logits
+ * (generic_engine/train_cign.py:2123, :1774-1817). */
+int cign_class_logprobs_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                            float temperature, const int64_t* label, int64_t ignore_index, int32_t top_k,
+                            float* logprob, float* entropy, float* top_logprob, int64_t* top_index, float* stats,
+                            void* workspace, int64_t workspace_bytes);
+
+/* grad_x [n, V] (x's type) for the gradients of logprob and entropy (each may
+ * be NULL). Rows whose gradients are both zero, an ignored label's among
+ * them, are zeros whatever their logits hold, and so are rows without any
+ * class left. */
+int cign_class_logprobs_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                            float temperature, const int64_t* label, int64_t ignore_index, const float* stats,
+                            const float* grad_logprob, const float* grad_entropy, void* grad_x);
+
 /* ---- hop gate (float32) ------------------------------------------------- */
 
 /* Node-mode hop gate: alpha [n,K] = softmax_k(score @ weight^T + bias), score

@@ -236,7 +236,12 @@ def test_layernorm_on_a_side_stream_and_in_a_graph():
     x, w, b, g = _inputs(513, 1281, BF16, F32, 2)
     for t in (x, w, b):
         t.requires_grad_()
-    step = lambda: (fused_layernorm(x, w, b), *torch.autograd.grad(fused_layernorm(x, w, b), (x, w, b), g))
+
+    def step():
+        y = fused_layernorm(x, w, b)
+        # detached: no eager graph of the leaves lives on while a step is captured
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b), g)]
+
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
