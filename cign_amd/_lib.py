@@ -82,6 +82,10 @@ _SIGNATURES = {
     "cign_class_logprobs_fwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _P, _I64, _I32, _P, _P, _P, _P, _P, _P,
                                           _I64]),
     "cign_class_logprobs_bwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _P, _I64, _P, _P, _P, _P]),
+    # loss against a teacher's top classes (distill.hip)
+    "cign_distill_topk_workspace_bytes": (_I64, [_I32, _I64, _I32]),
+    "cign_distill_topk_fwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _I32, _I32, _P, _P, _P, _P, _P, _P, _I64]),
+    "cign_distill_topk_bwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _I32, _P, _P, _P, _P, _P]),
     # hop gate (gate.hip)
     "cign_hop_gate_bwd_workspace_bytes": (_I64, [_I64, _I32, _I32]),
     "cign_hop_gate_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),

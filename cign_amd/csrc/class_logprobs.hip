@@ -161,7 +161,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
   const int nc = (in.V + W - 1) / W;
   const int64_t items = in.n * sl.S;
   const int lane = lane_id();
-  int turn = 0;
+  BlockJoin across(slots);
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int64_t r = item / sl.S;
     const int slice = static_cast<int>(item - r * sl.S);
@@ -173,15 +173,6 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     float m = sh.largest(), s = 0.0f, t = 0.0f;
     sh.template sums<true>(shift_of(m), in.c, s, t);
     join<kWave>(m, s, t, in.c);
-    // the wavefronts' results; a wavefront's shift is its largest value, or 0 with s = 0
-    float(*sl_slots)[3] = slots + turn * kWavesPerBlock;
-    turn ^= 1;
-    if (lane == 0) {
-      float* p = sl_slots[wave_id()];
-      p[0] = s == 0.0f ? -kInf : m;
-      p[1] = s;
-      p[2] = t;
-    }
     if (TOP && threadIdx.x == 0) {
       threshold = 1;
       found = 0;
@@ -191,15 +182,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
       mine = best_below(sh, ~0ull);
       sample[threadIdx.x] = mine;
     }
-    __syncthreads();
-    const bool has = lane < kWavesPerBlock;
-    m = has ? sl_slots[lane & 3][0] : -kInf;
-    s = has ? sl_slots[lane & 3][1] : 0.0f;
-    t = has ? sl_slots[lane & 3][2] : 0.0f;
-    join<kWavesPerBlock>(m, s, t, in.c);  // lanes 0..3 of each wavefront
-    m = shfl(m, 0);
-    s = shfl(s, 0);
-    t = shfl(t, 0);
+    across.run(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
     if (threadIdx.x == 0) {
       if (sl.S == 1)

@@ -100,6 +100,9 @@ PyMethodDef methods[] = {
     CIGN_ENTRY(cign_class_logprobs_workspace_bytes),
     CIGN_ENTRY(cign_class_logprobs_fwd),
     CIGN_ENTRY(cign_class_logprobs_bwd),
+    CIGN_ENTRY(cign_distill_topk_workspace_bytes),
+    CIGN_ENTRY(cign_distill_topk_fwd),
+    CIGN_ENTRY(cign_distill_topk_bwd),
     CIGN_ENTRY(cign_hop_gate_bwd_workspace_bytes),
     CIGN_ENTRY(cign_hop_gate_fwd),
     CIGN_ENTRY(cign_hop_gate_bwd),

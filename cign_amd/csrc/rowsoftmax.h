@@ -182,8 +182,11 @@ __device__ __forceinline__ float shift_of(float m) { return m == -kInf ? 0.0f : 
 
 // Joins statistics over the LPR lanes of a group (one (m, s, t) a lane; m as
 // largest() gave it, s and t relative to shift_of(m)). m becomes the shift.
+// Every lane gets the same bits: a lane that contracted its own product into
+// the first addition would round differently from its partner.
 template <int LPR>
 __device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
+#pragma clang fp contract(off)
   float top = m;
   for_offsets<1, LPR>([&](auto OC) { top = fmaxf(top, xor_shfl<decltype(OC)::value>(top)); });
   top = shift_of(top);
@@ -198,6 +201,32 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
   });
   m = top;
 }
+
+// The same over a workgroup of kBlock threads whose wavefronts have joined
+// theirs: every thread gets the result. The slots alternate (GroupReduce), so
+// this is the call's only barrier.
+struct BlockJoin {
+  float (*slots)[3];  // [2 * kWavesPerBlock]
+  int turn = 0;
+  __device__ explicit BlockJoin(float (*p)[3]) : slots(p) {}
+
+  __device__ __forceinline__ void run(float& m, float& s, float& t, float c) {
+    static_assert(kWavesPerBlock == 4, "one quad joins the wavefronts");
+    float(*p)[3] = slots + turn * kWavesPerBlock;
+    turn ^= 1;
+    if (lane_id() == 0) {
+      p[wave_id()][0] = s == 0.0f ? -kInf : m;
+      p[wave_id()][1] = s;
+      p[wave_id()][2] = t;
+    }
+    __syncthreads();
+    const int k = lane_id() & 3;
+    m = p[k][0];
+    s = p[k][1];
+    t = p[k][2];
+    join<4>(m, s, t, c);  // the same in every quad
+  }
+};
 
 }  // namespace rowsoftmax
 }  // namespace cign

@@ -396,6 +396,31 @@ int cign_class_logprobs_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, c
                             float temperature, const int64_t* label, int64_t ignore_index, const float* stats,
                             const float* grad_logprob, const float* grad_entropy, void* grad_x);
 
+/* Workspace bytes of cign_distill_topk_fwd. */
+int64_t cign_distill_topk_workspace_bytes(int32_t dtype, int64_t n, int32_t V);
+
+/* loss[r] = temperature^2 KL(p || q) of the student's q = softmax(x /
+ * temperature) over V classes against a teacher's list of K places a row
+ * (1..128): teacher_index [n, K] (negative: an empty place; V or more: the
+ * loss is NaN) and teacher_logprob [n, K] float32, its log probabilities at
+ * the same temperature. tail 0: p is the list renormalised; 1: the mass the
+ * list leaves, max(0, 1 - sum e^teacher_logprob), is one more class, all
+ * classes outside the list together (none where the list names every class).
+ * A row without a listed class has loss 0. stats [n, 8] and teacher_mass
+ * [n, K], float32, both or neither, are what the backward reads. No
+ * counterpart in the reference, which trains on labels alone
+ * (generic_engine/train_cign.py:2123). */
+int cign_distill_topk_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                          float temperature, int32_t tail, int32_t K, const float* teacher_logprob,
+                          const int64_t* teacher_index, float* loss, float* stats, float* teacher_mass,
+                          void* workspace, int64_t workspace_bytes);
+
+/* grad_x [n, V] (x's type) for grad_loss [n]. Rows without a listed class, or
+ * whose grad_loss is zero, are zeros whatever their logits hold. */
+int cign_distill_topk_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, const void* x, int64_t x_stride,
+                          float temperature, int32_t K, const int64_t* teacher_index, const float* stats,
+                          const float* teacher_mass, const float* grad_loss, void* grad_x);
+
 /* ---- hop gate (float32) ------------------------------------------------- */
 
 /* Node-mode hop gate: alpha [n,K] = softmax_k(score @ weight^T + bias), score
