@@ -30,6 +30,11 @@ __device__ __forceinline__ uint64_t key_of(float x, int index) {
   const uint32_t u = b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
   return static_cast<uint64_t>(u) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
 }
+// The value of a key, -inf for the bar below every key.
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  return u == 0 ? -kInf : __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
 __device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
 
 // A row's outputs, written by one thread.
@@ -53,8 +58,10 @@ struct In {
   float c, inv_t;  // log2(e) / T, 1 / T
 };
 
-__device__ __forceinline__ float logprob_of(float x, float m, float l2s, float inv_t) {
-  return (x - m) * inv_t - l2s * kLn2;
+__device__ __forceinline__ float logprob_of(float x, const Shift& sf, float l2s, float inv_t) {
+  const float d = sf.d(x);
+  // a class at the type's lowest value: log2 p overflows, log p may not
+  return d == -kInf ? (x - sf.m) * inv_t - l2s * kLn2 : (d - l2s) * kLn2;
 }
 
 // Label, entropy and statistics of row r from its joined (m, s, t); l2s is
@@ -69,7 +76,7 @@ __device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r,
     const int64_t y = o.label[r];
     float lp = 0.0f;
     if (y != o.ignore)
-      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), m, l2s, in.inv_t) : __builtin_nanf("");
+      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), Shift(m, in.c), l2s, in.inv_t) : __builtin_nanf("");
     o.logprob[r] = lp;
   }
   if (o.stats) {
@@ -85,7 +92,7 @@ __device__ __forceinline__ void put_top(const In<T>& in, const Out& o, int64_t r
                                         float l2s) {
   const int i = key_index(key);
   o.top_index[r * o.K + rank] = i;
-  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), m, l2s, in.inv_t);
+  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), Shift(m, in.c), l2s, in.inv_t);
 }
 
 // The largest key below `below` of a share's own values.
@@ -105,8 +112,45 @@ __device__ __forceinline__ uint64_t best_below(const Share<T, W, U>& sh, uint64_
   return best;
 }
 
+// The key of the share's largest value m (Share::largest), best_below(~0)
+// without making every value's key: the first own value equal to m. A share
+// whose m is -inf or NaN takes the long way.
+template <typename T, int W, int U>
+__device__ __forceinline__ uint64_t best_key(const Share<T, W, U>& sh, float m) {
+  if (!(m > -kInf)) return best_below(sh, ~0ull);
+  int index = 0;
+#pragma unroll
+  for (int u = U - 1; u >= 0; --u) {
+    float v[W];
+    RowChunk<T, W>::unpack(sh.raw[u], v);
+#pragma unroll
+    for (int w = W - 1; w >= 0; --w) index = v[w] == m ? sh.at[u] + w : index;
+  }
+  return key_of(m, index);
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  const auto step = [&](auto CTRL) {
+    const uint32_t o = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(CTRL)::value, 0xF, 0xF, true);
+    v = o > v ? o : v;
+  };
+  step(IC<0xB1>());   // quad_perm [1,0,3,2]
+  step(IC<0x4E>());   // quad_perm [2,3,0,1]
+  step(IC<0x141>());  // row_half_mirror: the other quad of 8 (quads are uniform by now)
+  step(IC<0x128>());  // row_ror:8
+  step(IC<0x142>());  // row_bcast:15, a row's result to the next row
+  step(IC<0x143>());  // row_bcast:31, rows 0 and 1 to rows 2 and 3
+  return __builtin_amdgcn_readlane(v, kWave - 1);
+}
+
+// The largest key of LPR lanes, on all of them.
 template <int LPR>
 __device__ __forceinline__ uint64_t group_max(uint64_t k) {
+  if constexpr (LPR == kWave) {
+    const uint32_t hi = wave_max(static_cast<uint32_t>(k >> 32));
+    const uint32_t lo = wave_max(static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+  }
   for_offsets<1, LPR>([&](auto OC) {
     constexpr int o = decltype(OC)::value;
     const uint32_t lo = __float_as_uint(xor_shfl<o>(__uint_as_float(static_cast<uint32_t>(k))));
@@ -130,7 +174,7 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     sh.load(in.x + r * in.ld);
     sh.mask_foreign();
     float m = sh.largest(), s = 0.0f, t = 0.0f;
-    sh.template sums<true>(shift_of(m), in.c, s, t);
+    sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<LPR>(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
     if (q == 0) finish(in, o, r, m, s, t, l2s);
@@ -150,7 +194,7 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
 // Slices of long rows: (m, s, t) to part[(r * S + slice)] (a float4), the K
 // largest keys, in falling order, to keys[(r * S + slice) * K ...] (0: the
 // slice has no more). With S = 1 the row's outputs are written at once.
-template <typename T, int U, bool TOP>
+template <typename T, int U, bool TOP, bool PAST>
 __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float4* part, uint64_t* keys) {
   constexpr int W = kChunk<T>;
   __shared__ float slots[2 * kWavesPerBlock][3];
@@ -168,19 +212,27 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     const int end = min((slice + 1) * sl.cps, nc);
     Share<T, W, U> sh;
     sh.place(slice * sl.cps + threadIdx.x, kBlock, end, in.V);
-    sh.load(in.x + r * in.ld);
+    sh.template load<PAST>(in.x + r * in.ld);
     sh.mask_foreign();
-    float m = sh.largest(), s = 0.0f, t = 0.0f;
-    sh.template sums<true>(shift_of(m), in.c, s, t);
+    const float top = sh.largest();
+    float m = top, s = 0.0f, t = 0.0f;
+    sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<kWave>(m, s, t, in.c);
     if (TOP && threadIdx.x == 0) {
       threshold = 1;
       found = 0;
     }
     uint64_t mine = 0;
+    const bool quads = TOP && o.K <= kBlock / 4;
     if constexpr (TOP) {
-      mine = best_below(sh, ~0ull);
-      sample[threadIdx.x] = mine;
+      mine = best_key(sh, top);
+      uint64_t best = mine;
+      if (quads) {
+        best = group_max<4>(mine);
+        if ((threadIdx.x & 3) == 0) sample[threadIdx.x >> 2] = best;
+      } else {
+        sample[threadIdx.x] = best;
+      }
     }
     across.run(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
@@ -191,21 +243,34 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
     }
     if constexpr (TOP) {
-      // The K-th largest of the threads' best keys bounds the slice's K-th
-      // key from below; every key at or above it is a candidate.
+      // The K-th largest of the best keys of quads (K <= 64) or threads bounds
+      // the slice's K-th key from below; every key at or above it is a
+      // candidate. Each quad counts the keys above its own, a quarter a lane.
       const int K = o.K;
-      int above = 0;
-      for (int i = 0; i < kBlock; ++i) above += sample[i] > mine;
-      if (mine != 0 && above == K - 1) threshold = mine;
+      if (quads) {
+        const uint64_t own = sample[threadIdx.x >> 2];
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < kBlock / 16; ++i) above += sample[(threadIdx.x & 3) * (kBlock / 16) + i] > own;
+        above += __float_as_int(xor_shfl<1>(__int_as_float(above)));
+        above += __float_as_int(xor_shfl<2>(__int_as_float(above)));
+        if (own != 0 && above == K - 1) threshold = own;  // one quad: keys differ
+      } else {
+        int above = 0;
+        for (int i = 0; i < kBlock; ++i) above += sample[i] > mine;
+        if (mine != 0 && above == K - 1) threshold = mine;
+      }
       __syncthreads();
       const uint64_t bar = threshold;
       if (mine >= bar) {
+        const float low = key_value(bar);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float v[W];
           RowChunk<T, W>::unpack(sh.raw[u], v);
 #pragma unroll
           for (int w = 0; w < W; ++w) {
+            if (!(ranked(v[w]) >= low)) continue;
             const uint64_t k = key_of(v[w], sh.at[u] + w);
             if (w >= sh.own[u] && k >= bar) {
               const int at = atomicAdd(&found, 1);
@@ -275,16 +340,26 @@ __global__ __launch_bounds__(kWave) void join_kernel(In<T> in, Out o, int S, con
     float l2s = s == 0.0f ? 0.0f : log2f(s);
     if (lane == 0) finish(in, o, r, m, s, t, l2s);
     if constexpr (TOP) {
-      int next = 0;
+      // the heads of the lists against each other; the winner's next comes in
+      // while the following round runs
+      int next = 1;
       uint64_t mine = has ? lists[lane * o.K] : 0;
+      uint64_t then = has && o.K > 1 ? lists[lane * o.K + 1] : 0;
+      uint64_t won[kMaxList / kWave] = {};  // places lane, lane + 64
       for (int k = 0; k < o.K; ++k) {
         const uint64_t best = group_max<kWave>(mine);
-        if (has && mine == best) {
-          put_top(in, o, r, k, best, m, l2s);
+        if (mine == best) {  // one lane: keys differ
+          mine = then;
           ++next;
-          mine = next < o.K ? lists[lane * o.K + next] : 0;
+          then = next < o.K ? lists[lane * o.K + next] : 0;
         }
+#pragma unroll
+        for (int i = 0; i < kMaxList / kWave; ++i)
+          if (k == lane + i * kWave) won[i] = best;
       }
+#pragma unroll
+      for (int i = 0; i < kMaxList / kWave; ++i)
+        if (lane + i * kWave < o.K) put_top(in, o, r, lane + i * kWave, won[i], m, l2s);
     }
   }
 }
@@ -292,7 +367,7 @@ __global__ __launch_bounds__(kWave) void join_kernel(In<T> in, Out o, int S, con
 // grad_x of rows held by LPR threads (lanes, or LPR = 256: the slices of a
 // long row). Rows whose gradients are both zero (an ignored label) are zeros,
 // whatever their logits hold.
-template <typename T, int W, int LPR, int U, bool ENT>
+template <typename T, int W, int LPR, int U, bool ENT, int PASS>
 __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, const int64_t* label, int64_t ignore,
                                                       const float* stats, const float* g_lp, const float* g_ent,
                                                       T* gx) {
@@ -315,9 +390,10 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
     const float a = -(g + h * stats[4 * r + 2]) * in.inv_t, b = -h * kLn2 * in.inv_t;
     const float gl = g * in.inv_t;
     const bool zero = g == 0.0f && h == 0.0f;
+    const Shift sf(m, in.c);
     Share<T, W, U> sh;
     sh.place(slice * cps + q, LPR, min((slice + 1) * cps, nc), in.V);
-    if (!zero) sh.load(in.x + r * in.ld);
+    if (!zero) sh.template load<PASS == kPast>(in.x + r * in.ld);
     T* row = gx + r * in.V;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -327,19 +403,25 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
         for (int w = 0; w < W; ++w) v[w] = 0.0f;
       } else {
         X::unpack(sh.raw[u], v);
+        const auto turn = [&](auto of) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float d = fmaf(v[w] - m, in.c, -l2s);
-          const float p = __builtin_amdgcn_exp2f(d);
-          v[w] = p * (ENT ? fmaf(b, fmaxf(d, -1e30f), a) : a);
-        }
+          for (int w = 0; w < W; ++w) {
+            const float d = of(v[w]) - l2s;  // log2 p
+            const float p = __builtin_amdgcn_exp2f(d);
+            v[w] = p * (ENT ? fmaf(b, fmaxf(d, -1e30f), a) : a);
+          }
+        };
+        if (sf.far)
+          turn([&](float x) { return sf.far_d(x); });
+        else
+          turn([&](float x) { return sf.near_d(x); });
         const int64_t at = y - sh.at[u];
         if (at >= 0 && at < W)
 #pragma unroll
           for (int w = 0; w < W; ++w)
             if (w == at) v[w] += gl;
       }
-      Share<T, W, U>::store(row, sh.at[u], sh.own[u], v);
+      Share<T, W, U>::template store<PASS != kThrough>(row, sh.at[u], sh.own[u], v);
     }
   }
 }
@@ -394,10 +476,15 @@ int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void
   const int rc = with_chunks<T>(sl.U, [&](auto UC) {
     constexpr int U = decltype(UC)::value;
     const int grid = grid_of(in.n * sl.S);
+    const auto launch = [&](auto TC, auto SC) {
+      hipLaunchKernelGGL((slice_kernel<T, U, decltype(TC)::value, decltype(SC)::value>), dim3(grid), dim3(kBlock), 0, st,
+                         in, o, sl, part, keys);
+    };
+    const bool past = pass_of<T>(in.n, in.V) == kPast;
     if (o.K > 0)
-      hipLaunchKernelGGL((slice_kernel<T, U, true>), dim3(grid), dim3(kBlock), 0, st, in, o, sl, part, keys);
+      past ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
     else
-      hipLaunchKernelGGL((slice_kernel<T, U, false>), dim3(grid), dim3(kBlock), 0, st, in, o, sl, part, keys);
+      past ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
     return check_launch(who);
   });
   if (rc || sl.S == 1) return rc;
@@ -459,12 +546,16 @@ int cign_class_logprobs_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, c
       constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;
       constexpr int kRows = kBlock / LPR;
       const int grid = grid_of((n * S + kRows - 1) / kRows);
-      if (grad_entropy)
-        hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, true>), dim3(grid), dim3(kBlock), 0, st, in, S, cps, label,
-                           ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
-      else
-        hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, false>), dim3(grid), dim3(kBlock), 0, st, in, S, cps, label,
-                           ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
+      // lane groups narrower than a wavefront: rows of a few classes, never that many bytes in earnest
+      with_pass(LPR < kWave ? kThrough : pass_of<T>(n, V), [&](auto PC) {
+        constexpr int PASS = LPR < kWave ? kThrough : decltype(PC)::value;
+        if (grad_entropy)
+          hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, true, PASS>), dim3(grid), dim3(kBlock), 0, st, in, S, cps, label,
+                             ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
+        else
+          hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, false, PASS>), dim3(grid), dim3(kBlock), 0, st, in, S, cps,
+                             label, ignore_index, stats, grad_logprob, grad_entropy, static_cast<T*>(grad_x));
+      });
       return check_launch(who);
     };
     constexpr int kW = kChunk<T>;

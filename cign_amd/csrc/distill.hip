@@ -43,8 +43,8 @@ struct In {
 
 // What the backward takes of a row.
 struct Stats {
-  float mb, l2b, cb;  // gradient of a class outside the list: cb 2^((x - mb) c - l2b)
-  float m, l2s, a;    // of a listed class: a 2^((x - m) c - l2s) - p
+  float mb, l2b, cb;  // gradient of a class outside the list: cb 2^(d - l2b), d by Shift(mb)
+  float m, l2s, a;    // of a listed class: a 2^(d - l2s) - p, d by Shift(m)
   float pad[2];
 };
 
@@ -54,10 +54,17 @@ struct Out {
   float* p;      // [n, K]: the teacher's mass at the place's class, over all places that name it
 };
 
+constexpr double kLn2d = 0.6931471805599453, kInfd = __builtin_huge_val();
+
 template <int LPR>
 __device__ __forceinline__ double lanes_sum(double v) {
-#pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) v += __shfl_xor(v, o, kWave);
+  for_offsets<1, LPR>([&](auto OC) {
+    constexpr int o = decltype(OC)::value;
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __float_as_uint(xor_shfl<o>(__uint_as_float(static_cast<uint32_t>(b))));
+    const uint32_t hi = __float_as_uint(xor_shfl<o>(__uint_as_float(static_cast<uint32_t>(b >> 32))));
+    v += __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+  });
   return v;
 }
 
@@ -67,14 +74,62 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-// Row r by LPR lanes (lane q), from the joined statistics (m, s) of the
-// classes outside the list (TAIL) or of all classes.
+// Shift::d in float64 (relative to the same rounded product).
+__device__ __forceinline__ double wide_d(const Shift& sf, float x) {
+  const double xd = x;
+  return sf.far ? (xd - sf.m) * sf.c : xd * sf.c - sf.mc;
+}
+
+// What is known of a row's list once its lanes have been through it once.
+struct ListSummary {
+  float top, top_x;    // the teacher's largest value, the student's largest logit (of a listed class)
+  bool any, bad;       // a place that names a class; one that names none of the V
+};
+
+// The student over all classes, from its statistics (m, s) outside the list
+// (TAIL; over all classes otherwise) and the listed logits' sum.
+struct Student {
+  Shift rest, all;
+  float s;    // relative to `rest`
+  double lz;  // log of the sum over all classes, relative to `all`
+  bool none;  // no class left
+  __device__ __forceinline__ Student(float m, float s_, float mt, float c) : rest(m, c), all(mt, c), s(s_) {}
+  __device__ __forceinline__ void total(double listed) {
+    const double st = listed + (s == 0.0f ? 0.0 : static_cast<double>(s) * exp2f(all.d_of(rest.m)));
+    none = st == 0.0;
+    lz = none ? 0.0 : log(st);
+  }
+  __device__ __forceinline__ double logq(float x) const { return none ? -kInfd : wide_d(all, x) * kLn2d - lz; }
+};
+
+// The row's loss and statistics from the sums over its list, by one lane.
+template <typename T, bool TAIL>
+__device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t r, const Student& q,
+                                         const ListSummary& list, double members, double loss, double mass) {
+  double a = mass, cb = mass;
+  if constexpr (TAIL) {
+    const double left = list.any && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
+    const double lrest =
+        q.s == 0.0f ? -kInfd : static_cast<double>(q.all.d_of(q.rest.m)) * kLn2d + log(static_cast<double>(q.s)) - q.lz;
+    if (left > 0.0) loss += left * (log(left) - lrest);
+    a = mass + left;
+    cb = a * exp(lrest) - left;
+  }
+  if (list.bad) loss = a = cb = __builtin_nan("");
+  o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
+  if (o.stats)
+    o.stats[r] = Stats{q.rest.m, q.s == 0.0f ? kInf : log2f(q.s), static_cast<float>(cb), q.all.m,
+                       q.none ? kInf : static_cast<float>(q.lz * (1.0 / kLn2d)), static_cast<float>(a), {0.0f, 0.0f}};
+}
+
+// Row r by LPR < 64 lanes (lane q), from the joined statistics (m, s) of the
+// classes outside the list (TAIL) or of all classes. Rows this short have short
+// lists: each lane goes through its places once for every step.
 template <typename T, int LPR, bool TAIL>
 __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m, float s) {
   const int64_t* index = in.index + r * in.K;
   const float* t = in.t + r * in.K;
   const T* row = in.x + r * in.ld;
-  const double inv_t = 1.0 / in.temperature;
   float top = -kInf, top_x = -kInf, any = 0.0f, bad = 0.0f;
   for (int i = q; i < in.K; i += LPR) {
     const int64_t j = index[i];
@@ -87,43 +142,27 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
     top = fmaxf(top, t[i]);
     top_x = fmaxf(top_x, to_f32(row[j]));
   }
-  top = lanes_max<LPR>(top);
-  top_x = lanes_max<LPR>(top_x);
-  any = lanes_max<LPR>(any);
-  bad = lanes_max<LPR>(bad);
-
-  // the student over all classes: (mt, st)
-  double st = s;
-  float mt = m;
-  double members = 0.0;
-  if constexpr (TAIL) {
-    mt = shift_of(fmaxf(s == 0.0f ? -kInf : m, top_x));
-    double listed = 0.0;
-    for (int i = q; i < in.K; i += LPR) {
-      const int64_t j = index[i];
-      if (j < 0 || j >= in.V) continue;
+  const ListSummary list{lanes_max<LPR>(top), lanes_max<LPR>(top_x), lanes_max<LPR>(any) != 0.0f,
+                         lanes_max<LPR>(bad) != 0.0f};
+  Student st(m, s, TAIL ? shift_of(fmaxf(s == 0.0f ? -kInf : m, list.top_x)) : m, in.c);
+  double members = 0.0, listed = 0.0, total = 0.0;
+  for (int i = q; i < in.K; i += LPR) {
+    const int64_t j = index[i];
+    if (j < 0 || j >= in.V) continue;
+    if constexpr (TAIL) {
       bool first = true;
       for (int k = 0; k < i; ++k) first = first && index[k] != j;
       if (!first) continue;
       members += 1.0;
-      listed += exp2f((to_f32(row[j]) - mt) * in.c);
+      listed += exp2f(st.all.d(to_f32(row[j])));
+    } else {
+      total += exp(static_cast<double>(t[i]) - shift_of(list.top));
     }
-    members = lanes_sum<LPR>(members);
-    st = (s == 0.0f ? 0.0 : static_cast<double>(s) * exp2(static_cast<double>((m - mt) * in.c))) +
-         lanes_sum<LPR>(listed);
   }
-  const bool none = st == 0.0;
-  const double lz = none ? 0.0 : log(st);
-
-  // the teacher
-  double shift = 0.0;  // log p = t - shift
-  if constexpr (!TAIL) {
-    double total = 0.0;
-    for (int i = q; i < in.K; i += LPR)
-      if (index[i] >= 0 && index[i] < in.V) total += exp(static_cast<double>(t[i]) - shift_of(top));
-    total = lanes_sum<LPR>(total);
-    shift = total == 0.0 ? 0.0 : shift_of(top) + log(total);
-  }
+  st.total(lanes_sum<LPR>(listed));
+  members = lanes_sum<LPR>(members);
+  total = lanes_sum<LPR>(total);
+  const double shift = total == 0.0 ? 0.0 : shift_of(list.top) + log(total);  // log p = t - shift
   double loss = 0.0, mass = 0.0;
   for (int i = q; i < in.K; i += LPR) {
     const int64_t j = index[i];
@@ -132,9 +171,7 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
       const double lp = static_cast<double>(t[i]) - shift;
       const double p = exp(lp);
       if (p != 0.0) {
-        const float x = to_f32(row[j]);
-        const double lq = none ? -static_cast<double>(kInf) : (static_cast<double>(x) - mt) * inv_t - lz;
-        loss += p * (lp - lq);
+        loss += p * (lp - st.logq(to_f32(row[j])));
         mass += p;
       }
       if (o.p) {
@@ -147,23 +184,130 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
   }
   loss = lanes_sum<LPR>(loss);
   mass = lanes_sum<LPR>(mass);
+  if (q == 0) conclude<T, TAIL>(in, o, r, st, list, members, loss, mass);
+}
 
-  double a = mass, cb = mass, lrest = 0.0;
-  if constexpr (TAIL) {
-    const double left = any != 0.0f && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
-    lrest = s == 0.0f ? -static_cast<double>(kInf)
-                      : (static_cast<double>(m) - mt) * inv_t + log(static_cast<double>(s)) - lz;
-    if (left > 0.0) loss += left * (log(left) - lrest);
-    a = mass + left;
-    cb = a * exp(lrest) - left;
+// The same by a whole wavefront: up to two places a lane in registers, the
+// list's classes and masses in the wavefront's part of LDS, where a place finds
+// the others that name its class.
+struct WaveList {
+  int index[kMaxList];  // -1: names no class
+  float p[kMaxList];
+};
+
+__device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
+template <typename T, bool TAIL, int E>
+__device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int64_t r, int lane, float m, float s,
+                                              WaveList& lds) {
+  int at[E];
+  float t[E], x[E];
+  float top = -kInf, top_x = -kInf;
+  bool any = false, bad = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = lane + e * kWave;
+    const bool in_list = i < in.K;
+    const int64_t j = in_list ? in.index[r * in.K + i] : -1;
+    t[e] = in_list ? in.t[r * in.K + i] : 0.0f;
+    any = any || j >= 0;
+    bad = bad || j >= in.V;
+    at[e] = j >= 0 && j < in.V ? static_cast<int>(j) : -1;
   }
-  if (bad != 0.0f) loss = a = cb = __builtin_nan("");
-  if (q != 0) return;
-  o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
-  if (o.stats)
-    o.stats[r] = Stats{m, s == 0.0f ? kInf : log2f(s), static_cast<float>(cb), mt,
-                       none ? kInf : static_cast<float>(lz * 1.4426950408889634), static_cast<float>(a),
-                       {0.0f, 0.0f}};
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] = at[e] >= 0 ? to_f32(in.x[r * in.ld + at[e]]) : 0.0f;
+  wave_lds_fence();  // the former row's list has been read
+#pragma unroll
+  for (int e = 0; e < E; ++e) lds.index[lane + e * kWave] = at[e];
+  wave_lds_fence();
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (at[e] >= 0) {
+      top = fmaxf(top, t[e]);
+      top_x = fmaxf(top_x, x[e]);
+    }
+  const ListSummary list{lanes_max<kWave>(top), lanes_max<kWave>(top_x), __any(any) != 0, __any(bad) != 0};
+  // the places that name the same class
+  bool first[E], again = false;
+#pragma unroll
+  for (int e = 0; e < E; ++e) first[e] = at[e] >= 0;
+  for (int k = 0; k < in.K; k += 4) {
+    const int4 j = *reinterpret_cast<const int4*>(&lds.index[k]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = lane + e * kWave;
+      const bool b0 = j.x == at[e] && k != i, b1 = j.y == at[e] && k + 1 != i;
+      const bool b2 = j.z == at[e] && k + 2 != i, b3 = j.w == at[e] && k + 3 != i;
+      const bool same = at[e] >= 0 && (b0 || b1 || b2 || b3);
+      again = again || same;
+      if (same && ((b0 && k < i) || (b1 && k + 1 < i) || (b2 && k + 2 < i) || (b3 && k + 3 < i))) first[e] = false;
+    }
+  }
+  Student st(m, s, TAIL ? shift_of(fmaxf(s == 0.0f ? -kInf : m, list.top_x)) : m, in.c);
+  double members = 0.0, listed = 0.0, total = 0.0;
+  const double top64 = shift_of(list.top);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (at[e] < 0) continue;
+    if constexpr (TAIL) {
+      members += first[e] ? 1.0 : 0.0;
+      listed += first[e] ? exp2f(st.all.d(x[e])) : 0.0f;
+    } else {
+      total += exp(static_cast<double>(t[e]) - top64);
+    }
+  }
+  if constexpr (TAIL) {
+    listed = lanes_sum<kWave>(listed);
+    members = lanes_sum<kWave>(members);
+  } else {
+    total = lanes_sum<kWave>(total);
+  }
+  st.total(listed);
+  const double shift = total == 0.0 ? 0.0 : top64 + log(total);  // log p = t - shift
+  double loss = 0.0, mass = 0.0;
+  float at_class[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    at_class[e] = 0.0f;
+    if (at[e] < 0) continue;
+    const double lp = static_cast<double>(t[e]) - shift;
+    const double p = exp(lp);
+    at_class[e] = static_cast<float>(p);
+    if (p != 0.0) {
+      loss += p * (lp - st.logq(x[e]));
+      mass += p;
+    }
+  }
+  if (o.p) {
+    if (__any(again)) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) lds.p[lane + e * kWave] = at_class[e];
+      wave_lds_fence();
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (at[e] < 0) continue;
+        double sum = 0.0;
+        for (int k = 0; k < in.K; ++k) sum += lds.index[k] == at[e] ? lds.p[k] : 0.0f;
+        at_class[e] = static_cast<float>(sum);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (lane + e * kWave < in.K) o.p[r * in.K + lane + e * kWave] = at_class[e];
+  }
+  loss = lanes_sum<kWave>(loss);
+  mass = lanes_sum<kWave>(mass);
+  if (lane == 0) conclude<T, TAIL>(in, o, r, st, list, members, loss, mass);
+}
+
+template <typename T, bool TAIL>
+__device__ __forceinline__ void finish_wave(const In<T>& in, const Out& o, int64_t r, int lane, float m, float s,
+                                            WaveList& lds) {
+  static_assert(kMaxList == 2 * kWave, "one or two places a lane");
+  if (in.K <= kWave)
+    finish_places<T, TAIL, 1>(in, o, r, lane, m, s, lds);
+  else
+    finish_places<T, TAIL, 2>(in, o, r, lane, m, s, lds);
 }
 
 // The bits of a share's chunk c (W places from column c W of the bitmap's
@@ -180,6 +324,7 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
   constexpr int kRows = kBlock / LPR;
   constexpr int kWords = (LPR * U * W + 31) / 32;
   __shared__ uint32_t bitmap[TAIL ? kRows * kWords : 1];
+  __shared__ WaveList lists[LPR == kWave ? kWavesPerBlock : 1];
   const int q = threadIdx.x & (LPR - 1);
   const int slot = threadIdx.x / LPR;
   uint32_t* bits = bitmap + (TAIL ? slot * kWords : 0);
@@ -207,19 +352,25 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     for (int u = 0; u < U; ++u)
       mask_out<T, W>(sh.raw[u], TAIL ? kill_bits<W>(bits, q + u * LPR, sh.own[u]) : (1u << sh.own[u]) - 1u);
     float m = sh.largest(), s = 0.0f, t = 0.0f;
-    sh.template sums<false>(shift_of(m), in.c, s, t);
+    sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
     join<LPR>(m, s, t, in.c);
-    finish<T, LPR, TAIL>(in, o, r, q, m, s);
+    if constexpr (LPR == kWave)
+      finish_wave<T, TAIL>(in, o, r, q, m, s, lists[wave_id()]);
+    else
+      finish<T, LPR, TAIL>(in, o, r, q, m, s);
   }
 }
 
-// Slices of long rows: (m, s) to part[r * S + slice], or, with S = 1, the row.
-template <typename T, int U, bool TAIL>
+// Slices of long rows: (m, s) to part[r * S + slice]; ONE: a row's only slice,
+// which finishes it (apart, since its registers would cost the others a
+// wavefront a SIMD).
+template <typename T, int U, bool TAIL, bool ONE, bool PAST>
 __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float2* part) {
   constexpr int W = kChunk<T>;
   constexpr int kWords = kBlock * U * W / 32;
   __shared__ float slots[2 * kWavesPerBlock][3];
   __shared__ uint32_t bits[TAIL ? kWords : 1];
+  __shared__ typename std::conditional<ONE, WaveList, int>::type list;
   BlockJoin across(slots);
   const int nc = (in.V + W - 1) / W;
   const int64_t items = in.n * sl.S;
@@ -229,7 +380,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     const int begin = slice * sl.cps, end = min(begin + sl.cps, nc);
     Share<T, W, U> sh;
     sh.place(begin + threadIdx.x, kBlock, end, in.V);
-    sh.load(in.x + r * in.ld);
+    sh.template load<PAST>(in.x + r * in.ld);
     if constexpr (TAIL) {
       // (the barrier of the former item's join came after its last read)
       for (int i = threadIdx.x; i < kWords; i += kBlock) bits[i] = 0;
@@ -244,11 +395,11 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     for (int u = 0; u < U; ++u)
       mask_out<T, W>(sh.raw[u], TAIL ? kill_bits<W>(bits, threadIdx.x + u * kBlock, sh.own[u]) : (1u << sh.own[u]) - 1u);
     float m = sh.largest(), s = 0.0f, t = 0.0f;
-    sh.template sums<false>(shift_of(m), in.c, s, t);
+    sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
     join<kWave>(m, s, t, in.c);
     across.run(m, s, t, in.c);
-    if (sl.S == 1) {
-      if (threadIdx.x < kWave) finish<T, kWave, TAIL>(in, o, r, threadIdx.x, m, s);
+    if constexpr (ONE) {
+      if (threadIdx.x < kWave) finish_wave<T, TAIL>(in, o, r, threadIdx.x, m, s, list);
     } else if (threadIdx.x == 0) {
       part[item] = make_float2(s == 0.0f ? -kInf : m, s);
     }
@@ -258,20 +409,21 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
 // Rows from their slices, a wavefront a row; lane i holds slice i.
 template <typename T, bool TAIL>
 __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, const float2* part) {
+  __shared__ WaveList lists[kWavesPerBlock];
   const int lane = lane_id();
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_id(); r < in.n; r += step) {
     const float2 p = lane < S ? part[r * S + lane] : make_float2(-kInf, 0.0f);
     float m = p.x, s = p.y, t = 0.0f;
     join<kWave>(m, s, t, in.c);
-    finish<T, kWave, TAIL>(in, o, r, lane, m, s);
+    finish_wave<T, TAIL>(in, o, r, lane, m, s, lists[wave_id()]);
   }
 }
 
 // grad_x of rows held by LPR threads (lanes, or LPR = 256: the slices of a
 // long row). A row without a listed class, or whose g is zero, is zeros,
 // whatever its logits hold.
-template <typename T, int W, int LPR, int U>
+template <typename T, int W, int LPR, int U, int PASS>
 __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, const Stats* stats, const float* p,
                                                       const float* g_loss, float temperature, T* gx) {
   using X = RowChunk<T, W>;
@@ -287,13 +439,14 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
     const int slice = active && S > 1 ? static_cast<int>(item - r * S) : 0;
     const int begin = slice * cps, end = min(begin + cps, nc);
     const Stats st = stats[r];
+    const Shift sf(st.mb, in.c);
     const float gt = g_loss[r] * temperature;
     const bool zero = gt == 0.0f || st.a == 0.0f;
     T* row = gx + r * in.V;
     if (active) {
       Share<T, W, U> sh;
       sh.place(begin + q, LPR, end, in.V);
-      if (!zero) sh.load(in.x + r * in.ld);
+      if (!zero) sh.template load<PASS == kPast>(in.x + r * in.ld);
       const float cb = gt * st.cb;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -303,10 +456,16 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
           for (int w = 0; w < W; ++w) v[w] = 0.0f;
         } else {
           X::unpack(sh.raw[u], v);
+          const auto turn = [&](auto of) {
 #pragma unroll
-          for (int w = 0; w < W; ++w) v[w] = cb * __builtin_amdgcn_exp2f(fmaf(v[w] - st.mb, in.c, -st.l2b));
+            for (int w = 0; w < W; ++w) v[w] = cb * __builtin_amdgcn_exp2f(of(v[w]) - st.l2b);
+          };
+          if (sf.far)
+            turn([&](float x) { return sf.far_d(x); });
+          else
+            turn([&](float x) { return sf.near_d(x); });
         }
-        Share<T, W, U>::store(row, sh.at[u], sh.own[u], v);
+        Share<T, W, U>::template store<PASS != kThrough>(row, sh.at[u], sh.own[u], v);
       }
     }
     __syncthreads();  // the listed classes are written over what another thread of this workgroup stored
@@ -315,7 +474,7 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
         const int64_t j = in.index[r * in.K + i];
         if (j < static_cast<int64_t>(begin) * W || j >= static_cast<int64_t>(end) * W || j >= in.V) continue;
         const float x = to_f32(in.x[r * in.ld + j]);
-        row[j] = from_f32<T>(gt * (st.a * __builtin_amdgcn_exp2f(fmaf(x - st.m, in.c, -st.l2s)) - p[r * in.K + i]));
+        row[j] = from_f32<T>(gt * (st.a * __builtin_amdgcn_exp2f(Shift(st.m, in.c).d(x) - st.l2s) - p[r * in.K + i]));
       }
   }
 }
@@ -363,7 +522,18 @@ int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void
   float2* part = static_cast<float2*>(workspace);
   const int rc = with_chunks<T>(sl.U, [&](auto UC) {
     constexpr int U = decltype(UC)::value;
-    hipLaunchKernelGGL((slice_kernel<T, U, TAIL>), dim3(grid_of(in.n * sl.S)), dim3(kBlock), 0, st, in, o, sl, part);
+    const int grid = grid_of(in.n * sl.S);
+    const auto launch = [&](auto OC, auto PC) {
+      hipLaunchKernelGGL((slice_kernel<T, U, TAIL, decltype(OC)::value, decltype(PC)::value>), dim3(grid), dim3(kBlock), 0,
+                         st, in, o, sl, part);
+    };
+    const bool past = pass_of<T>(in.n, in.V) == kPast;
+    if (sl.S == 1) {
+      if constexpr (U <= 8)  // 16 chunks a thread are for rows of more than 64 slices
+        past ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
+    } else {
+      past ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
+    }
     return check_launch(who);
   });
   if (rc || sl.S == 1) return rc;
@@ -421,9 +591,13 @@ int cign_distill_topk_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, con
     const auto launch = [&](auto WC, auto LC, auto UC, int S, int cps) {
       constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;
       constexpr int kRows = kBlock / LPR;
-      hipLaunchKernelGGL((grad_kernel<T, W, LPR, U>), dim3(grid_of((n * S + kRows - 1) / kRows)), dim3(kBlock), 0, st,
-                         in, S, cps, reinterpret_cast<const Stats*>(stats), teacher_mass, grad_loss, temperature,
-                         static_cast<T*>(grad_x));
+      // lane groups narrower than a wavefront: rows of a few classes, never that many bytes in earnest
+      with_pass(LPR < kWave ? kThrough : pass_of<T>(n, V), [&](auto PC) {
+        constexpr int PASS = LPR < kWave ? kThrough : decltype(PC)::value;
+        hipLaunchKernelGGL((grad_kernel<T, W, LPR, U, PASS>), dim3(grid_of((n * S + kRows - 1) / kRows)), dim3(kBlock), 0,
+                           st, in, S, cps, reinterpret_cast<const Stats*>(stats), teacher_mass, grad_loss, temperature,
+                           static_cast<T*>(grad_x));
+      });
       return check_launch(who);
     };
     constexpr int kW = kChunk<T>;

@@ -33,7 +33,22 @@ struct Shape {
   static constexpr int kSlots = NT > kWave ? 2 * (NT / kWave) : 1;     // LDS slots of its reductions
 };
 
-template <typename T, typename TW, int W, int NT, int V>
+// A chunk's own values of a result: whole chunks, value by value at a ragged end.
+template <typename T, int W, bool PAST>
+__device__ __forceinline__ void store_own(T* row, int at, int own, const float (&v)[W]) {
+  if (own == 0) {
+    if constexpr (PAST)
+      RowChunk<T, W>::store_past(row + at, v);
+    else
+      RowChunk<T, W>::store(row + at, v);
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      if (w >= own) row[at + w] = from_f32<T>(v[w]);
+  }
+}
+
+template <typename T, typename TW, int W, int NT, int V, bool PAST>
 __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int D, const T* x, int64_t ldx,
                                                                   const TW* weight, const TW* bias, float eps, T* y,
                                                                   float* mean, float* rstd) {
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int
 #pragma unroll
         for (int w = 0; w < W; ++w) o[w] += p[w];
       }
-      X::store(y + r * D + at[v], o);
+      store_own<T, W, PAST>(y + r * D, at[v], own[v], o);
     }
     if (q == 0 && mean) {
       mean[r] = mu;
@@ -109,7 +124,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int
 }
 
 // Rows [r0, r1) of workgroup b; part [2][nb][D] (weight, bias).
-template <typename T, typename TW, int W, int NT, int V>
+template <typename T, typename TW, int W, int NT, int V, bool PAST>
 __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int D, const T* gy, int64_t ldg,
                                                                   const T* x, int64_t ldx, const TW* weight,
                                                                   const float* mean, const float* rstd, T* gx,
@@ -136,19 +151,24 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
   const float inv = 1.0f / static_cast<float>(D);
   int64_t r0, r1;
   rowops::block_rows(n, nb, blockIdx.x, r0, r1);
+  // The next row's loads go out before this row's sums, except by 1024 threads,
+  // whose 128 registers do not hold both (spilled: see the measurements).
+  constexpr bool kAhead = NT < 1024;
   int64_t r = r0 + slot;
   typename X::Raw xn[V], gn[V];
   float mun = 0.0f, rsn = 0.0f;
-  if (r < r1) {
+  const auto load = [&](int64_t row) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      xn[v] = X::load(x + r * ldx + at[v]);
-      gn[v] = X::load(gy + r * ldg + at[v]);
+      xn[v] = X::load(x + row * ldx + at[v]);
+      gn[v] = X::load(gy + row * ldg + at[v]);
     }
-    mun = mean[r];
-    rsn = rstd[r];
-  }
+    mun = mean[row];
+    rsn = rstd[row];
+  };
+  if (kAhead && r < r1) load(r);
   for (; r < r1; r += kRows) {
+    if (!kAhead) load(r);
     float xh[V][W], g[V][W];
     const float mu = mun, rs = rsn;
 #pragma unroll
@@ -156,14 +176,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
       X::unpack(xn[v], xh[v]);
       X::unpack(gn[v], g[v]);
     }
-    const int64_t rn = r + kRows < r1 ? r + kRows : r;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      xn[v] = X::load(x + rn * ldx + at[v]);
-      gn[v] = X::load(gy + rn * ldg + at[v]);
-    }
-    mun = mean[rn];
-    rsn = rstd[rn];
+    if (kAhead) load(r + kRows < r1 ? r + kRows : r);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -193,7 +206,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
       float o[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) o[w] = rs * (g[v][w] - c1 - xh[v][w] * c2);
-      X::store(gx + r * D + at[v], o);
+      store_own<T, W, PAST>(gx + r * D, at[v], own[v], o);
     }
   }
   if (!part) return;
@@ -201,8 +214,8 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       if (own[v] >= W) continue;
-      RowChunk<float, W>::store(part + static_cast<int64_t>(blockIdx.x) * D + at[v], aw[v]);
-      RowChunk<float, W>::store(part + (static_cast<int64_t>(nb) + blockIdx.x) * D + at[v], ab[v]);
+      store_own<float, W, false>(part + static_cast<int64_t>(blockIdx.x) * D, at[v], own[v], aw[v]);
+      store_own<float, W, false>(part + (static_cast<int64_t>(nb) + blockIdx.x) * D, at[v], own[v], ab[v]);
     }
   } else {
     // the workgroup's row slots, added in order
@@ -316,11 +329,20 @@ int check_args(const char* who, int64_t n, int D, int x_dtype, int w_dtype) {
   return kOk;
 }
 
-// Workgroups of the backward: its partial rows.
-int bwd_blocks(int64_t n, int rows) {
-  const int64_t groups = (n + rows - 1) / rows;
-  return static_cast<int>(groups < 512 ? groups : 512);
+// Workgroups of the backward, its partial rows: what the card holds at a time
+// for rows of 512 threads and more (256 against 512 at 8192 bf16 columns: 171 +
+// 5 us against 176 + 9), two a CU for the others (256 was 10% slower at 1001
+// columns, 1024 12%).
+int bwd_blocks(int64_t n, int rows, int threads) {
+  const int64_t groups = (n + rows - 1) / rows, most = threads >= 512 ? 256 : 512;
+  return static_cast<int>(groups < most ? groups : most);
 }
+
+// Results of this many bytes and more are written past the cache (rowvec.h):
+// forward and backward of 125 MB take 99 us instead of 118, of 268 MB 256
+// instead of 273. With a kernel that reads each result at once: 96 MB 2%
+// slower, 125 MB 198 us instead of 218, 268 MB 454 instead of 438.
+constexpr int64_t kPastBytes = 112ll << 20;
 
 template <typename T>
 constexpr int kFwdV = sizeof(T) == 4 ? 5 : 4;
@@ -351,10 +373,13 @@ int cign_layernorm_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
     return with_shape<T, kFwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
       constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
       const int64_t groups = (n + Shape<NT>::kRows - 1) / Shape<NT>::kRows;
-      const int grid = static_cast<int>(groups < 4096 ? groups : 4096);
-      hipLaunchKernelGGL((fwd_kernel<T, TW, W, NT, V>), dim3(grid), dim3(Shape<NT>::kThreads), 0, st, n, D,
-                         static_cast<const T*>(x), x_stride, static_cast<const TW*>(weight),
-                         static_cast<const TW*>(bias), eps, static_cast<T*>(y), mean, rstd);
+      const int grid = static_cast<int>(groups < 2048 ? groups : 2048);
+      const auto launch = [&](auto PC) {
+        hipLaunchKernelGGL((fwd_kernel<T, TW, W, NT, V, decltype(PC)::value>), dim3(grid), dim3(Shape<NT>::kThreads), 0,
+                           st, n, D, static_cast<const T*>(x), x_stride, static_cast<const TW*>(weight),
+                           static_cast<const TW*>(bias), eps, static_cast<T*>(y), mean, rstd);
+      };
+      n * D * static_cast<int64_t>(sizeof(T)) >= kPastBytes ? launch(std::true_type()) : launch(std::false_type());
       return check_launch(who);
     });
   });
@@ -362,7 +387,7 @@ int cign_layernorm_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
 
 int64_t cign_layernorm_bwd_workspace_bytes(int64_t n, int32_t D) {
   if (n < 0 || D < 1 || D > kMaxWidth) return 0;
-  return 2 * static_cast<int64_t>(sizeof(float)) * bwd_blocks(n, 1) * D;
+  return 2 * static_cast<int64_t>(sizeof(float)) * bwd_blocks(n, 1, 1) * D;
 }
 
 int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, const void* grad_y,
@@ -387,10 +412,13 @@ int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
     if (n > 0) {
       const int err = with_shape<T, kBwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
         constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
-        nb = bwd_blocks(n, Shape<NT>::kRows);
-        hipLaunchKernelGGL((bwd_kernel<T, TW, W, NT, V>), dim3(nb), dim3(Shape<NT>::kThreads), 0, st, n, D,
-                           static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(x), x_stride,
-                           static_cast<const TW*>(weight), mean, rstd, static_cast<T*>(grad_x), part, nb);
+        nb = bwd_blocks(n, Shape<NT>::kRows, NT);
+        const auto launch = [&](auto PC) {
+          hipLaunchKernelGGL((bwd_kernel<T, TW, W, NT, V, decltype(PC)::value>), dim3(nb), dim3(Shape<NT>::kThreads), 0,
+                             st, n, D, static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(x), x_stride,
+                             static_cast<const TW*>(weight), mean, rstd, static_cast<T*>(grad_x), part, nb);
+        };
+        n * D * static_cast<int64_t>(sizeof(T)) >= kPastBytes ? launch(std::true_type()) : launch(std::false_type());
         return check_launch(who);
       });
       if (err) return err;

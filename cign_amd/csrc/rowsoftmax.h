@@ -2,10 +2,12 @@
 // distill.hip): how a row is laid over threads, and its softmax statistics.
 //
 // l = x / T is the row's logits at temperature T and c = log2(e) / T, so that
-// exp(l - l_max) = 2^((x - m) c) with m the largest x: the shift is taken from
-// x itself, before any rounding of a product, and one hardware exponential
-// (v_exp_f32) makes each term. A row's statistics are (m, s, t):
-//   s = sum 2^((x - m) c), t = sum 2^((x - m) c) (x - m) c,
+// exp(l - l_max) = 2^d with d = x c - m c and m the largest x: one fused
+// multiply-add and one hardware exponential (v_exp_f32) a term. The product
+// m c is rounded, the same way wherever it is formed, so its error shifts every
+// term and the result's own x alike and cancels (Shift); the fused form rounds d
+// alone. A row's statistics are (m, s, t):
+//   s = sum 2^d, t = sum 2^d d,
 // in float32; a masked class (-inf) adds nothing to either. A row of masked
 // classes alone has s = 0.
 //
@@ -67,17 +69,47 @@ bool wavefront_row(int V) {
 }
 
 // The slices of long rows: S a row, of cps chunks each, U chunks a thread
-// (256 U >= cps; U W <= 64 values). The longest that leave at least 1024
-// workgroups, so that few rows still spread over the card.
+// (256 U >= cps). Eight chunks a thread (128 bytes in flight: 16 took 84 us
+// where 8 took 73 over 777 x 50,001 floats with top classes, 4 took 187 where 8
+// took 130 over 2,048 x 131,072 bf16), 16 where 64 slices would not cover the
+// row, fewer while that leaves fewer than 1024 workgroups, so that few rows still
+// spread over the card.
+//
 struct Slicing {
   int U, S, cps;
 };
+
+// How the logits and their gradient pass the 256 MB cache behind the L2s: read
+// and written through it; from 144 MiB of logits on the gradient is written past
+// it, whose lines would push the logits and each other out; from 384 MiB on,
+// where nothing is left for the next pass anyway, the logits are read past it too,
+// both ways. Measured, forward and gradient together: 256 MB of bf16 logits
+// 176 us through, 146 with the gradient past, 149 with both past; 537 MB 300,
+// 285, 275; 1.6 GB 950, 905, 810. Followed at once by a kernel that reads the
+// gradient, 160 to 200 MB take 8% less past the cache, 268 MB and more 2 to 4%
+// more.
+enum Pass : int { kThrough = 0, kWritePast = 1, kPast = 2 };
+inline Pass pass_of(int64_t bytes) {
+  return bytes >= 384ll << 20 ? kPast : bytes >= 144ll << 20 ? kWritePast : kThrough;
+}
+template <typename T>
+Pass pass_of(int64_t n, int V) {
+  return pass_of(n * V * static_cast<int64_t>(sizeof(T)));
+}
+// f(IC<Pass>)
+template <class F>
+void with_pass(Pass p, F&& f) {
+  if (p == kThrough) f(IC<kThrough>());
+  else if (p == kWritePast) f(IC<kWritePast>());
+  else f(IC<kPast>());
+}
+
 template <typename T>
 Slicing slicing(int V, int64_t n) {
   constexpr int W = kChunk<T>;
   const int nc = (V + W - 1) / W;
-  int U = 64 / W;
   auto slices = [&](int u) { return (nc + kBlock * u - 1) / (kBlock * u); };
+  int U = slices(8) <= kMaxSlices ? 8 : 16;
   while (U > 1 && n * slices(U) < 1024 && slices(U / 2) <= kMaxSlices) U /= 2;
   const int S = slices(U), cps = (nc + S - 1) / S;
   while (U > 1 && kBlock * (U / 2) >= cps) U /= 2;
@@ -112,6 +144,23 @@ __device__ __forceinline__ void mask_out(typename RowChunk<T, W>::Raw& q, uint32
   }
 }
 
+// d = (x - m) log2(e) / T for the classes of a row. Where the scaled shift
+// nears float32's largest value (rows whose every logit is the type's lowest,
+// tiny temperatures) x c and m c overflow, and the difference is taken first.
+struct Shift {
+  float m, c, mc;
+  bool far;
+  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), c(c_), mc(m_ * c_), far(!(fabsf(m_ * c_) < 1e37f)) {}
+  __device__ __forceinline__ float near_d(float x) const { return fmaf(x, c, -mc); }
+  __device__ __forceinline__ float far_d(float x) const { return (x - m) * c; }
+  __device__ __forceinline__ float d(float x) const { return far ? far_d(x) : near_d(x); }
+  // of another shift: the difference of the two products as each was rounded
+  __device__ __forceinline__ float d_of(float other) const {
+#pragma clang fp contract(off)
+    return far ? far_d(other) : other * c - mc;
+  }
+};
+
 // A thread's share of a row: U chunks at positions first, first + stride, ...
 // below `end` (chunk numbers); places past the end repeat the last chunk and
 // own nothing.
@@ -130,35 +179,71 @@ struct Share {
       own[u] = c < end ? c * W - at[u] : W;
     }
   }
+  template <bool PAST = false>
   __device__ __forceinline__ void load(const T* row) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = X::load(row + at[u]);
+    for (int u = 0; u < U; ++u) {
+      if constexpr (PAST)
+        raw[u] = X::load_past(row + at[u]);
+      else
+        raw[u] = X::load(row + at[u]);
+    }
   }
   __device__ __forceinline__ void mask_foreign() {
 #pragma unroll
     for (int u = 0; u < U; ++u) mask_out<T, W>(raw[u], (1u << own[u]) - 1u);
   }
+  // The largest value; NaN may come out as itself or be passed over (the sums
+  // are NaN either way).
   __device__ __forceinline__ float largest() const {
-    float m = -kInf;
+    if constexpr (sizeof(T) == 2 && W > 1) {
+      // On the packed bits: the signed maximum is the largest value if any is
+      // positive, the unsigned minimum if none is: one instruction a value,
+      // where unpacking and a float maximum take two and a half.
+      typedef short i16x2 __attribute__((ext_vector_type(2)));
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      i16x2 top = __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[0][0]));
+      u16x2 low = __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[0][0]));
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float v[W];
-      X::unpack(raw[u], v);
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int w = 0; w < W; ++w) m = fmaxf(m, v[w]);
+        for (int w = 0; w < W / 2; ++w) {
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[u][w])));
+          low = __builtin_elementwise_min(low, __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[u][w])));
+        }
+      const short t = top.x > top.y ? top.x : top.y;
+      const unsigned short l = low.x < low.y ? low.x : low.y;
+      const uint32_t bits = t >= 0 ? static_cast<uint32_t>(static_cast<uint16_t>(t)) : static_cast<uint32_t>(l);
+      return __uint_as_float(bits << 16);
+    } else {
+      float m = -kInf;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[W];
+        X::unpack(raw[u], v);
+#pragma unroll
+        for (int w = 0; w < W; ++w) m = fmaxf(m, v[w]);
+      }
+      return m;
     }
-    return m;
   }
-  // Adds the share's s (and t) relative to m.
+  // Adds the share's s (and t) relative to the shift.
   template <bool WITH_T>
-  __device__ __forceinline__ void sums(float m, float c, float& s, float& t) const {
+  __device__ __forceinline__ void sums(const Shift& sf, float& s, float& t) const {
+    if (sf.far)
+      add<WITH_T>([&](float x) { return sf.far_d(x); }, s, t);
+    else
+      add<WITH_T>([&](float x) { return sf.near_d(x); }, s, t);
+  }
+  template <bool WITH_T, class D>
+  __device__ __forceinline__ void add(D&& of, float& s, float& t) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float v[W];
       X::unpack(raw[u], v);
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float d = (v[w] - m) * c;
+        const float d = of(v[w]);
         const float e = __builtin_amdgcn_exp2f(d);
         s += e;
         if constexpr (WITH_T) t = fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf counts nothing
@@ -166,9 +251,13 @@ struct Share {
     }
   }
   // Stores chunk u's own values of a result.
+  template <bool PAST = false>
   static __device__ __forceinline__ void store(T* row, int at, int own, const float (&v)[W]) {
     if (own == 0) {
-      X::store(row + at, v);
+      if constexpr (PAST)
+        X::store_past(row + at, v);
+      else
+        X::store(row + at, v);
     } else if (own < W) {
 #pragma unroll
       for (int w = 0; w < W; ++w)
@@ -190,7 +279,7 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
   float top = m;
   for_offsets<1, LPR>([&](auto OC) { top = fmaxf(top, xor_shfl<decltype(OC)::value>(top)); });
   top = shift_of(top);
-  const float d = (shift_of(m) - top) * c;
+  const float d = Shift(top, c).d_of(shift_of(m));
   const float e = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(d);
   t = s == 0.0f ? 0.0f : e * fmaf(s, fmaxf(d, -1e30f), t);
   s *= e;

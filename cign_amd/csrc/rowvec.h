@@ -31,11 +31,17 @@ template <>
 struct RowChunk<float, 4> {
   typedef float Raw __attribute__((ext_vector_type(4), aligned(4)));
   static __device__ __forceinline__ Raw load(const float* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ Raw load_past(const float* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+  }
   static __device__ __forceinline__ void unpack(const Raw& q, float (&v)[4]) {
     v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
   }
   static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
     *reinterpret_cast<Raw*>(p) = Raw{v[0], v[1], v[2], v[3]};
+  }
+  static __device__ __forceinline__ void store_past(float* p, const float (&v)[4]) {
+    __builtin_nontemporal_store(Raw{v[0], v[1], v[2], v[3]}, reinterpret_cast<Raw*>(p));
   }
 };
 
@@ -61,6 +67,9 @@ template <>
 struct RowChunk<bf16, 8> {
   typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
   static __device__ __forceinline__ Raw load(const bf16* p) { return *reinterpret_cast<const Raw*>(p); }
+  static __device__ __forceinline__ Raw load_past(const bf16* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const Raw*>(p));
+  }
   static __device__ __forceinline__ void unpack(const Raw& q, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -68,9 +77,12 @@ struct RowChunk<bf16, 8> {
       v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
     }
   }
-  static __device__ __forceinline__ void store(bf16* p, const float (&v)[8]) {
-    *reinterpret_cast<Raw*>(p) =
-        Raw{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+  static __device__ __forceinline__ Raw pack(const float (&v)[8]) {
+    return Raw{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+  }
+  static __device__ __forceinline__ void store(bf16* p, const float (&v)[8]) { *reinterpret_cast<Raw*>(p) = pack(v); }
+  static __device__ __forceinline__ void store_past(bf16* p, const float (&v)[8]) {
+    __builtin_nontemporal_store(pack(v), reinterpret_cast<Raw*>(p));
   }
 };
 
@@ -78,8 +90,10 @@ template <typename T>
 struct RowChunk<T, 1> {
   using Raw = T;
   static __device__ __forceinline__ Raw load(const T* p) { return *p; }
+  static __device__ __forceinline__ Raw load_past(const T* p) { return *p; }
   static __device__ __forceinline__ void unpack(const Raw& q, float (&v)[1]) { v[0] = to_f32(q); }
   static __device__ __forceinline__ void store(T* p, const float (&v)[1]) { *p = from_f32<T>(v[0]); }
+  static __device__ __forceinline__ void store_past(T* p, const float (&v)[1]) { store(p, v); }
 };
 
 // Values per 16-byte chunk of T.
