@@ -161,6 +161,22 @@ __device__ __forceinline__ uint64_t group_max(uint64_t k) {
   return k;
 }
 
+// How many of n keys in LDS (padded with zeros to a multiple of 16) are above
+// `key`: every thread of the workgroup reads the same ones, eight 16-byte reads
+// in flight.
+__device__ __forceinline__ int count_above(const uint64_t* keys, int n, uint64_t key) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  int above = 0;
+  for (int i = 0; i < n; i += 16) {
+    u64x2 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const u64x2*>(keys + i + 2 * k);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) above += (v[k].x > key) + (v[k].y > key);
+  }
+  return above;
+}
+
 // Rows that LPR lanes hold.
 template <typename T, int W, int LPR, int U, bool TOP>
 __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
@@ -198,8 +214,8 @@ template <typename T, int U, bool TOP, bool PAST>
 __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float4* part, uint64_t* keys) {
   constexpr int W = kChunk<T>;
   __shared__ float slots[2 * kWavesPerBlock][3];
-  __shared__ uint64_t sample[TOP ? kBlock : 1];
-  __shared__ uint64_t cand[TOP ? kCandidates : 1];
+  __shared__ __align__(16) uint64_t sample[TOP ? kBlock : 1];
+  __shared__ __align__(16) uint64_t cand[TOP ? kCandidates : 1];
   __shared__ uint64_t threshold;
   __shared__ int found;
   const int nc = (in.V + W - 1) / W;
@@ -223,7 +239,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
       found = 0;
     }
     uint64_t mine = 0;
-    const bool quads = TOP && o.K <= kBlock / 4;
+    const bool quads = TOP && o.K <= kBlock / 8;
     if constexpr (TOP) {
       mine = best_key(sh, top);
       uint64_t best = mine;
@@ -243,21 +259,18 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
     }
     if constexpr (TOP) {
-      // The K-th largest of the best keys of quads (K <= 64) or threads bounds
+      // The K-th largest of the best keys of quads (K <= 32) or threads bounds
       // the slice's K-th key from below; every key at or above it is a
       // candidate. Each quad counts the keys above its own, a quarter a lane.
       const int K = o.K;
       if (quads) {
         const uint64_t own = sample[threadIdx.x >> 2];
-        int above = 0;
-#pragma unroll
-        for (int i = 0; i < kBlock / 16; ++i) above += sample[(threadIdx.x & 3) * (kBlock / 16) + i] > own;
+        int above = count_above(sample + (threadIdx.x & 3) * (kBlock / 16), kBlock / 16, own);
         above += __float_as_int(xor_shfl<1>(__int_as_float(above)));
         above += __float_as_int(xor_shfl<2>(__int_as_float(above)));
         if (own != 0 && above == K - 1) threshold = own;  // one quad: keys differ
       } else {
-        int above = 0;
-        for (int i = 0; i < kBlock; ++i) above += sample[i] > mine;
+        const int above = count_above(sample, kBlock, mine);
         if (mine != 0 && above == K - 1) threshold = mine;
       }
       __syncthreads();
@@ -283,10 +296,11 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
       const int count = found;
       uint64_t* list = keys + item * K;
       if (count <= kCandidates) {
+        for (int i = count + threadIdx.x; i < ((count + 15) & ~15); i += kBlock) cand[i] = 0;
+        __syncthreads();
         for (int i = threadIdx.x; i < count; i += kBlock) {
           const uint64_t k = cand[i];
-          int rank = 0;
-          for (int j = 0; j < count; ++j) rank += cand[j] > k;
+          const int rank = count_above(cand, count, k);
           if (rank < K) {
             if (sl.S == 1)
               put_top(in, o, r, rank, k, m, l2s);
@@ -321,46 +335,89 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
   }
 }
 
-// Rows from their slices: a wavefront a row; lane i holds slice i. The top
-// classes are merged from the slices' falling lists, kept in LDS.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(kWave) void join_kernel(In<T> in, Out o, int S, const float4* part, const uint64_t* keys) {
-  extern __shared__ uint64_t lists[];
-  const int lane = threadIdx.x;
+// Rows from their slices, without top classes: a wavefront a row, lane i holds
+// slice i.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, const float4* part) {
+  const int lane = lane_id();
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_id(); r < in.n; r += step) {
+    const float4 p = lane < S ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
+    float m = p.x, s = p.y, t = p.z, l2s;
+    join<kWave>(m, s, t, in.c);
+    if (lane == 0) finish(in, o, r, m, s, t, l2s);
+  }
+}
+
+// With top classes, a workgroup a row: of the slices' falling lists, the K-th
+// largest among the first ceil(K / S) of each bounds the row's K-th key from
+// below, and the keys at or above it are ranked against each other (one row of
+// 131,072 with K = 20: 10.6 us by rounds of the lists' heads against each
+// other). Lists whose candidates overflow, such as the slices of a sorted row,
+// are merged by those rounds.
+constexpr int kHeldKeys = 8;  // list keys a thread reads ahead
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S, const float4* part,
+                                                          const uint64_t* keys) {
+  __shared__ __align__(16) uint64_t sample[kBlock];
+  __shared__ __align__(16) uint64_t cand[kCandidates];
+  __shared__ uint64_t threshold;
+  __shared__ int found;
+  const int lane = lane_id(), K = o.K, total = S * K;
+  const int heads = (K + S - 1) / S, list = threadIdx.x / heads;  // S heads <= K + S - 1 < kBlock
   for (int64_t r = blockIdx.x; r < in.n; r += gridDim.x) {
-    const bool has = lane < S;
-    const float4 p = has ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
+    const float4 p = lane < S ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
+    const uint64_t* lists = keys + r * total;  // [S][K]
+    const uint64_t mine = list < S ? lists[list * K + threadIdx.x - list * heads] : 0;
+    uint64_t held[kHeldKeys];
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; ++i) held[i] = lists[min(static_cast<int>(threadIdx.x) + i * kBlock, total - 1)];
     float m = p.x, s = p.y, t = p.z;
-    if constexpr (TOP) {
-      __syncthreads();
-      for (int i = lane; i < S * o.K; i += kWave) lists[i] = keys[r * S * o.K + i];
-      __syncthreads();
+    __syncthreads();  // the former row's candidates have been read
+    sample[threadIdx.x] = mine;
+    if (threadIdx.x == 0) {
+      threshold = 1;
+      found = 0;
     }
     join<kWave>(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
-    if (lane == 0) finish(in, o, r, m, s, t, l2s);
-    if constexpr (TOP) {
-      // the heads of the lists against each other; the winner's next comes in
-      // while the following round runs
-      int next = 1;
-      uint64_t mine = has ? lists[lane * o.K] : 0;
-      uint64_t then = has && o.K > 1 ? lists[lane * o.K + 1] : 0;
-      uint64_t won[kMaxList / kWave] = {};  // places lane, lane + 64
-      for (int k = 0; k < o.K; ++k) {
-        const uint64_t best = group_max<kWave>(mine);
-        if (mine == best) {  // one lane: keys differ
-          mine = then;
-          ++next;
-          then = next < o.K ? lists[lane * o.K + next] : 0;
-        }
+    __syncthreads();
+    if (mine != 0 && count_above(sample, S * heads, mine) == K - 1) threshold = mine;
+    __syncthreads();
+    const uint64_t bar = threshold;
+    const auto offer = [&](uint64_t k) {
+      if (k < bar) return;
+      const int at = atomicAdd(&found, 1);
+      if (at < kCandidates) cand[at] = k;
+    };
 #pragma unroll
-        for (int i = 0; i < kMaxList / kWave; ++i)
-          if (k == lane + i * kWave) won[i] = best;
+    for (int i = 0; i < kHeldKeys; ++i)
+      if (static_cast<int>(threadIdx.x) + i * kBlock < total) offer(held[i]);
+    for (int i = threadIdx.x + kHeldKeys * kBlock; i < total; i += kBlock) offer(lists[i]);
+    __syncthreads();
+    const int count = found;
+    if (count <= kCandidates) {
+      for (int i = count + threadIdx.x; i < ((count + 15) & ~15); i += kBlock) cand[i] = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < count; i += kBlock) {
+        const uint64_t k = cand[i];
+        const int rank = count_above(cand, count, k);
+        if (rank < K) put_top(in, o, r, rank, k, m, l2s);
       }
-#pragma unroll
-      for (int i = 0; i < kMaxList / kWave; ++i)
-        if (lane + i * kWave < o.K) put_top(in, o, r, lane + i * kWave, won[i], m, l2s);
+    } else if (threadIdx.x < kWave) {
+      int next = 1;
+      uint64_t head = lane < S ? lists[lane * K] : 0;
+      for (int k = 0; k < K; ++k) {
+        const uint64_t best = group_max<kWave>(head);
+        if (head == best) {  // one lane: keys differ
+          put_top(in, o, r, k, best, m, l2s);
+          head = next < K ? lists[lane * K + next] : 0;
+          ++next;
+        }
+      }
     }
+    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, l2s);
   }
 }
 
@@ -488,12 +545,11 @@ int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void
     return check_launch(who);
   });
   if (rc || sl.S == 1) return rc;
-  const int grid = grid_of(in.n);
   if (o.K > 0)
-    hipLaunchKernelGGL((join_kernel<T, true>), dim3(grid), dim3(kWave), sizeof(uint64_t) * sl.S * o.K, st, in, o, sl.S,
-                       part, keys);
+    hipLaunchKernelGGL((join_top_kernel<T>), dim3(grid_of(in.n)), dim3(kBlock), 0, st, in, o, sl.S, part, keys);
   else
-    hipLaunchKernelGGL((join_kernel<T, false>), dim3(grid), dim3(kWave), 0, st, in, o, sl.S, part, keys);
+    hipLaunchKernelGGL((join_kernel<T>), dim3(grid_of((in.n + kWavesPerBlock - 1) / kWavesPerBlock)), dim3(kBlock), 0, st,
+                       in, o, sl.S, part);
   return check_launch(who);
 }
 
