@@ -112,20 +112,37 @@ __device__ __forceinline__ uint64_t best_below(const Share<T, W, U>& sh, uint64_
   return best;
 }
 
-// The key of the share's largest value m (Share::largest), best_below(~0)
-// without making every value's key: the first own value equal to m. A share
-// whose m is -inf or NaN takes the long way.
+// f(IC<0>) ... f(IC<N - 1>)
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void for_each(F&& f) {
+  if constexpr (I < N) {
+    f(IC<I>());
+    for_each<N, I + 1>(f);
+  }
+}
+
+// The key of the share's largest value m, of those of its chunks: best_below(~0)
+// without making every value's key, the first own value equal to m of the first
+// chunk that has one. A share whose m is -inf or NaN takes the long way.
 template <typename T, int W, int U>
-__device__ __forceinline__ uint64_t best_key(const Share<T, W, U>& sh, float m) {
+__device__ __forceinline__ uint64_t best_key(const Share<T, W, U>& sh, const float (&of_chunk)[U], float m) {
   if (!(m > -kInf)) return best_below(sh, ~0ull);
+  auto raw = sh.raw[0];
+  int at = sh.at[0];
+#pragma unroll
+  for (int u = U - 1; u > 0; --u) {
+    const bool here = of_chunk[u] == m;
+    raw = here ? sh.raw[u] : raw;
+    at = here ? sh.at[u] : at;
+  }
+  const bool first = of_chunk[0] == m;
+  raw = first ? sh.raw[0] : raw;
+  at = first ? sh.at[0] : at;
+  float v[W];
+  RowChunk<T, W>::unpack(raw, v);
   int index = 0;
 #pragma unroll
-  for (int u = U - 1; u >= 0; --u) {
-    float v[W];
-    RowChunk<T, W>::unpack(sh.raw[u], v);
-#pragma unroll
-    for (int w = W - 1; w >= 0; --w) index = v[w] == m ? sh.at[u] + w : index;
-  }
+  for (int w = W - 1; w >= 0; --w) index = v[w] == m ? at + w : index;
   return key_of(m, index);
 }
 
@@ -230,8 +247,17 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     sh.place(slice * sl.cps + threadIdx.x, kBlock, end, in.V);
     sh.template load<PAST>(in.x + r * in.ld);
     sh.mask_foreign();
-    const float top = sh.largest();
-    float m = top, s = 0.0f, t = 0.0f;
+    float of_chunk[TOP ? U : 1], m = -kInf, s = 0.0f, t = 0.0f;
+    if constexpr (TOP) {
+      for_each<U>([&](auto UC) {
+        constexpr int u = decltype(UC)::value;
+        of_chunk[u] = sh.template largest<u, u + 1>();
+        m = fmaxf(m, of_chunk[u]);
+      });
+    } else {
+      m = sh.largest();
+    }
+    const float top = m;
     sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<kWave>(m, s, t, in.c);
     if (TOP && threadIdx.x == 0) {
@@ -241,7 +267,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     uint64_t mine = 0;
     const bool quads = TOP && o.K <= kBlock / 8;
     if constexpr (TOP) {
-      mine = best_key(sh, top);
+      mine = best_key(sh, of_chunk, top);
       uint64_t best = mine;
       if (quads) {
         best = group_max<4>(mine);
@@ -279,6 +305,8 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         const float low = key_value(bar);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          // (a chunk of NaN is looked at; on 4 values the test costs what it saves)
+          if (W == 8 && of_chunk[u] < low) continue;
           float v[W];
           RowChunk<T, W>::unpack(sh.raw[u], v);
 #pragma unroll

@@ -193,8 +193,9 @@ struct Share {
 #pragma unroll
     for (int u = 0; u < U; ++u) mask_out<T, W>(raw[u], (1u << own[u]) - 1u);
   }
-  // The largest value; NaN may come out as itself or be passed over (the sums
-  // are NaN either way).
+  // The largest value of chunks [U0, U1); NaN may come out as itself or be
+  // passed over (the sums are NaN either way).
+  template <int U0 = 0, int U1 = U>
   __device__ __forceinline__ float largest() const {
     if constexpr (sizeof(T) == 2 && W > 1) {
       // On the packed bits: the signed maximum is the largest value if any is
@@ -202,10 +203,10 @@ struct Share {
       // where unpacking and a float maximum take two and a half.
       typedef short i16x2 __attribute__((ext_vector_type(2)));
       typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-      i16x2 top = __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[0][0]));
-      u16x2 low = __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[0][0]));
+      i16x2 top = __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[U0][0]));
+      u16x2 low = __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[U0][0]));
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = U0; u < U1; ++u)
 #pragma unroll
         for (int w = 0; w < W / 2; ++w) {
           top = __builtin_elementwise_max(top, __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[u][w])));
@@ -218,7 +219,7 @@ struct Share {
     } else {
       float m = -kInf;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = U0; u < U1; ++u) {
         float v[W];
         X::unpack(raw[u], v);
 #pragma unroll
