@@ -14,10 +14,9 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._rows import as_rows, check_rows, on_device_of
+from ._rows import as_rows, check_rows, new_like, on_device_of, once
 
 MAX_CLASSES = 1 << 20
 MAX_TOP_K = 128
@@ -35,7 +34,7 @@ def _forward(logits, labels, top_k, temperature, ignore_index, with_stats):
     rows, stride = as_rows(logits)
     n, V = rows.shape
     lead = logits.shape[:-1]
-    new = lambda shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=logits.device)
+    new = lambda shape, dtype=torch.float32: logits.new_empty(shape, dtype=dtype)
     entropy = new(lead)
     logprob = None if labels is None else new(lead)
     top = (new((*lead, top_k)), new((*lead, top_k), torch.int64)) if top_k else (None, None)
@@ -62,7 +61,7 @@ class _ClassLogprobsFn(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad_logprob, grad_entropy, *unused):
         logits, labels, stats = ctx.saved_tensors
         if grad_logprob is None and grad_entropy is None:
@@ -72,7 +71,7 @@ class _ClassLogprobsFn(torch.autograd.Function):
         rows, stride = as_rows(logits)
         n, V = rows.shape
         gl, ge = (None if g is None else g.contiguous() for g in (grad_logprob, grad_entropy))
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = new_like(logits)
         with on_device_of(logits):
             lib.call("cign_class_logprobs_bwd", _lib.stream_ptr(logits.device), _lib.DTYPE_CODE[logits.dtype], n, V,
                      rows.data_ptr(), stride, temperature, _lib.ptr(labels), ignore_index, stats.data_ptr(),
@@ -96,7 +95,7 @@ def check_index(t, name: str, shape, device) -> torch.Tensor:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
-    return t.to(torch.int64).contiguous()
+    return (t if t.dtype == torch.int64 else t.to(torch.int64)).contiguous()
 
 
 def class_logprobs(logits, labels=None, top_k=0, temperature=1.0, ignore_index=-100) -> ClassLogprobs:

@@ -22,11 +22,10 @@ import itertools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check, check_input
-from ._rows import as_rows, check_rows, on_device_of
+from ._rows import as_rows, check_rows, new_like, on_device_of, once
 
 _EXT = None
 _EXT_ERROR = None
@@ -359,23 +358,24 @@ MAX_LAYERNORM_WIDTH = 16384
 
 
 def _layernorm_forward(x, weight, bias, eps, with_stats):
-    """(y, mean, rstd) of cign_layernorm_fwd; mean and rstd ([rows]) are None
+    """(y, stats) of cign_layernorm_fwd; stats [2, rows] (mean, rstd), None
     unless with_stats."""
     lib = _lib.load_library()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = new_like(x)
     rows, stride = as_rows(x)
     n, D = rows.shape
-    mean = rstd = None
+    stats, mean, rstd = None, None, None
     if with_stats:
-        mean = torch.empty((n,), dtype=torch.float32, device=x.device)
-        rstd = torch.empty((n,), dtype=torch.float32, device=x.device)
+        stats = rows.new_empty((2, n), dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
     param = weight if weight is not None else bias
-    code = _lib.DTYPE_CODE[x.dtype if param is None else param.dtype]
+    code = _lib.DTYPE_CODE[x.dtype]
     with on_device_of(x):
-        lib.call("cign_layernorm_fwd", _lib.stream_ptr(x.device), n, D, _lib.DTYPE_CODE[x.dtype], code,
-                 rows.data_ptr(), stride, _lib.ptr(weight), _lib.ptr(bias), eps, y.data_ptr(), _lib.ptr(mean),
-                 _lib.ptr(rstd))
-    return y, mean, rstd
+        lib.call("cign_layernorm_fwd", _lib.stream_ptr(x.device), n, D, code,
+                 code if param is None else _lib.DTYPE_CODE[param.dtype], rows.data_ptr(), stride, _lib.ptr(weight),
+                 _lib.ptr(bias), eps, y.data_ptr(), mean, rstd)
+    return y, stats
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -383,31 +383,34 @@ class _LayerNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _layernorm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = _layernorm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, grad_y):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         lib = _lib.load_library()
         rows, stride = as_rows(x)
         grads, grad_stride = as_rows(grad_y)
         n, D = rows.shape
-        new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=x.device)
-        gx = new(x.shape, x.dtype) if ctx.needs_input_grad[0] else None
-        gw = new((D,), weight.dtype) if ctx.needs_input_grad[1] else None
-        gb = new((D,), ctx.bias_dtype) if ctx.needs_input_grad[2] else None
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        gx = new_like(x) if need_x else None
+        gw = x.new_empty((D,), dtype=weight.dtype) if need_w else None
+        gb = x.new_empty((D,), dtype=ctx.bias_dtype) if need_b else None
         dtype = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
-        ws_bytes = 0 if gw is None and gb is None else int(lib.cign_layernorm_bwd_workspace_bytes(n, D))
-        ws = _lib.workspace(ws_bytes, x.device) if ws_bytes else None
+        ws, ws_bytes = None, 0
+        if need_w or need_b:
+            ws_bytes = int(lib.cign_layernorm_bwd_workspace_bytes(n, D))
+            ws = _lib.workspace(ws_bytes, x.device)
+        mean = stats.data_ptr()
         with on_device_of(x):
             lib.call("cign_layernorm_bwd", _lib.stream_ptr(x.device), n, D, _lib.DTYPE_CODE[x.dtype],
                      _lib.DTYPE_CODE[dtype], grads.data_ptr(), grad_stride, rows.data_ptr(), stride,
-                     _lib.ptr(weight), mean.data_ptr(), rstd.data_ptr(), _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb),
-                     _lib.ptr(ws), ws_bytes)
+                     _lib.ptr(weight), mean, mean + 4 * n, _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
+                     ws_bytes)
         return gx, gw, gb, None
 
 
@@ -429,7 +432,7 @@ def fused_layernorm(x, weight=None, bias=None, eps=1e-5):
             raise TypeError("LayerNorm weight/bias must both be float32 or both of x's type")
         if t.shape != (D,):
             raise ValueError(f"LayerNorm {name} must have shape [{D}], got {tuple(t.shape)}")
-        if t.device != x.device:
+        if t.get_device() != x.get_device():
             raise ValueError(f"LayerNorm {name} must be on {x.device}, got {t.device}")
         dtype = t.dtype
     eps = float(eps)
