@@ -1,5 +1,6 @@
-"""Builds libcign_amd.so (gfx950 HIP kernels + C-ABI) in-tree with hipcc, and
-_cign.so, the CPython binding of its entry points.
+"""Builds libcign_amd.so (gfx950 HIP kernels + C-ABI) in-tree with hipcc,
+_cign.so, the CPython binding of its entry points, and _cign_ops.so, the torch
+autograd nodes of the output operators.
 
 Run as ``python -m cign_amd._build`` or through ``__graft_entry__.build()``.
 Object files go to ``cign_amd/_build/`` and the library to
@@ -21,6 +22,8 @@ OBJ = PKG / "_build"
 LIB = PKG / "libcign_amd.so"
 BINDING_SRC = SRC / "python" / "binding.cpp"
 BINDING = PKG / "_cign.so"
+OPS_SRC = SRC / "python" / "output_ops.cpp"
+OPS = PKG / "_cign_ops.so"
 
 ARCH = "gfx950"
 
@@ -75,18 +78,37 @@ def _compile(hipcc: str, src: Path, force: bool) -> Path:
     return obj
 
 
-def build_binding() -> Path:
-    """Compiles the CPython binding against the library (host code only)."""
-    tmp = BINDING.with_suffix(".so.tmp")
+def _host_module(src: Path, out: Path, flags: list[str], libs: list[str]) -> Path:
+    """Compiles a CPython extension against the library (host code only)."""
+    tmp = out.with_suffix(".so.tmp")
     cxx = os.environ.get("CXX") or shutil.which("g++") or str(Path(_hipcc()).parent / "amdclang++")
     cmd = [cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-shared", f"-I{sysconfig.get_paths()['include']}",
-           f"-I{PKG.parent / 'include'}", str(BINDING_SRC), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}",
+           f"-I{PKG.parent / 'include'}", *flags, str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", *libs,
            "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"binding build failed:\n{res.stderr[-6000:]}")
-    os.replace(tmp, BINDING)
-    return BINDING
+        raise RuntimeError(f"{src.name} build failed:\n{res.stderr[-6000:]}")
+    os.replace(tmp, out)
+    return out
+
+
+def build_binding() -> Path:
+    """Compiles the CPython binding of the C-ABI."""
+    return _host_module(BINDING_SRC, BINDING, [], [])
+
+
+def build_output_ops() -> Path:
+    """Compiles the output operators' autograd nodes, against torch as it is
+    installed; its libraries are found by the process that imported torch."""
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    rocm = Path(_hipcc()).resolve().parents[1]
+    flags = [f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+             f"-isystem{rocm / 'include'}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    return _host_module(OPS_SRC, OPS, flags, [f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
+                                              "-ltorch_python"])
 
 
 def build(verbose: bool = False, jobs: int | None = None, force: bool = True) -> Path:
@@ -109,7 +131,9 @@ def build(verbose: bool = False, jobs: int | None = None, force: bool = True) ->
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr[-6000:]}")
     os.replace(tmp, LIB)
-    build_binding()
+    with cf.ThreadPoolExecutor(max_workers=2) as pool:
+        for done in [pool.submit(build_binding), pool.submit(build_output_ops)]:
+            done.result()
     if verbose:
         print(f"built {LIB} from {len(srcs)} sources", flush=True)
     return LIB

@@ -15,8 +15,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import _lib
-from ._rows import as_rows, check_rows, new_like, on_device_of, once
+from ._rows import check_rows, output_ops
 
 MAX_CLASSES = 1 << 20
 MAX_TOP_K = 128
@@ -27,56 +26,6 @@ class ClassLogprobs(NamedTuple):
     entropy: torch.Tensor                 # [...] float32, in nats
     top_logprobs: Optional[torch.Tensor]  # [..., top_k] float32, falling; None without top_k
     top_index: Optional[torch.Tensor]     # [..., top_k] int64
-
-
-def _forward(logits, labels, top_k, temperature, ignore_index, with_stats):
-    lib = _lib.load_library()
-    rows, stride = as_rows(logits)
-    n, V = rows.shape
-    lead = logits.shape[:-1]
-    new = lambda shape, dtype=torch.float32: logits.new_empty(shape, dtype=dtype)
-    entropy = new(lead)
-    logprob = None if labels is None else new(lead)
-    top = (new((*lead, top_k)), new((*lead, top_k), torch.int64)) if top_k else (None, None)
-    stats = new((n, 4)) if with_stats else None
-    code = _lib.DTYPE_CODE[logits.dtype]
-    ws_bytes = int(lib.cign_class_logprobs_workspace_bytes(code, n, V, top_k))
-    ws = _lib.workspace(ws_bytes, logits.device) if ws_bytes else None
-    with on_device_of(logits):
-        lib.call("cign_class_logprobs_fwd", _lib.stream_ptr(logits.device), code, n, V, rows.data_ptr(), stride,
-                 temperature, _lib.ptr(labels), ignore_index, top_k, _lib.ptr(logprob), entropy.data_ptr(),
-                 _lib.ptr(top[0]), _lib.ptr(top[1]), _lib.ptr(stats), _lib.ptr(ws), ws_bytes)
-    return ClassLogprobs(logprob, entropy, *top), stats
-
-
-class _ClassLogprobsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top_k, temperature, ignore_index):
-        out, stats = _forward(logits, labels, top_k, temperature, ignore_index, True)
-        ctx.save_for_backward(logits, labels, stats)
-        ctx.options = temperature, ignore_index
-        ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(out.top_logprobs, out.top_index)
-        return tuple(out)
-
-    @staticmethod
-    @once
-    def backward(ctx, grad_logprob, grad_entropy, *unused):
-        logits, labels, stats = ctx.saved_tensors
-        if grad_logprob is None and grad_entropy is None:
-            return (None,) * 5
-        temperature, ignore_index = ctx.options
-        lib = _lib.load_library()
-        rows, stride = as_rows(logits)
-        n, V = rows.shape
-        gl, ge = (None if g is None else g.contiguous() for g in (grad_logprob, grad_entropy))
-        grad = new_like(logits)
-        with on_device_of(logits):
-            lib.call("cign_class_logprobs_bwd", _lib.stream_ptr(logits.device), _lib.DTYPE_CODE[logits.dtype], n, V,
-                     rows.data_ptr(), stride, temperature, _lib.ptr(labels), ignore_index, stats.data_ptr(),
-                     _lib.ptr(gl), _lib.ptr(ge), grad.data_ptr())
-        return grad, None, None, None, None
 
 
 def check_temperature(temperature) -> float:
@@ -122,7 +71,4 @@ def class_logprobs(logits, labels=None, top_k=0, temperature=1.0, ignore_index=-
     temperature = check_temperature(temperature)
     if labels is not None:
         labels = check_index(labels, "labels", logits.shape[:-1], logits.device)
-    args = (logits, labels, top_k, temperature, int(ignore_index))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return ClassLogprobs(*_ClassLogprobsFn.apply(*args))
-    return _forward(*args, False)[0]
+    return ClassLogprobs(*output_ops().class_logprobs(logits, labels, top_k, temperature, int(ignore_index)))

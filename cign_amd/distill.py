@@ -11,61 +11,10 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
-from ._rows import as_rows, check_rows, new_like, on_device_of, once
+from ._rows import check_rows, output_ops
 from .class_logprobs import MAX_CLASSES, check_index, check_temperature
 
 MAX_LIST = 128
-
-
-STATS = 8  # floats a row that the backward reads, beside the list's masses
-
-
-def _forward(logits, teacher_logprobs, teacher_index, temperature, tail, with_stats):
-    """(loss, kept): kept holds the rows' statistics, then their lists' masses."""
-    lib = _lib.load_library()
-    rows, stride = as_rows(logits)
-    n, V = rows.shape
-    K = teacher_index.size(-1)
-    loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
-    kept = stats = mass = None
-    if with_stats:
-        kept = logits.new_empty((n * (STATS + K),), dtype=torch.float32)
-        stats = kept.data_ptr()
-        mass = stats + 4 * STATS * n
-    code = _lib.DTYPE_CODE[logits.dtype]
-    ws_bytes = int(lib.cign_distill_topk_workspace_bytes(code, n, V))
-    ws = _lib.workspace(ws_bytes, logits.device) if ws_bytes else None
-    with on_device_of(logits):
-        lib.call("cign_distill_topk_fwd", _lib.stream_ptr(logits.device), code, n, V, rows.data_ptr(), stride,
-                 temperature, int(tail), K, teacher_logprobs.data_ptr(), teacher_index.data_ptr(), loss.data_ptr(),
-                 stats, mass, _lib.ptr(ws), ws_bytes)
-    return loss, kept
-
-
-class _DistillTopkFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_logprobs, teacher_index, temperature, tail):
-        loss, kept = _forward(logits, teacher_logprobs, teacher_index, temperature, tail, True)
-        ctx.save_for_backward(logits, teacher_index, kept)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @once
-    def backward(ctx, grad_loss):
-        logits, teacher_index, kept = ctx.saved_tensors
-        lib = _lib.load_library()
-        rows, stride = as_rows(logits)
-        n, V = rows.shape
-        grad_loss = grad_loss.contiguous()
-        grad = new_like(logits)
-        stats = kept.data_ptr()
-        with on_device_of(logits):
-            lib.call("cign_distill_topk_bwd", _lib.stream_ptr(logits.device), _lib.DTYPE_CODE[logits.dtype], n, V,
-                     rows.data_ptr(), stride, ctx.temperature, teacher_index.size(-1), teacher_index.data_ptr(),
-                     stats, stats + 4 * STATS * n, grad_loss.data_ptr(), grad.data_ptr())
-        return grad, None, None, None, None
 
 
 def distill_topk_loss(logits, teacher_logprobs, teacher_index, temperature=1.0, tail=False) -> torch.Tensor:
@@ -102,7 +51,4 @@ def distill_topk_loss(logits, teacher_logprobs, teacher_index, temperature=1.0, 
     temperature = check_temperature(temperature)
     if teacher_logprobs.dtype != torch.float32:
         teacher_logprobs = teacher_logprobs.to(torch.float32)
-    args = (logits, teacher_logprobs.contiguous(), teacher_index, temperature, bool(tail))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _DistillTopkFn.apply(*args)
-    return _forward(*args, False)[0]
+    return output_ops().distill_topk(logits, teacher_logprobs.contiguous(), teacher_index, temperature, bool(tail))

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from ._lib import check, check_input
-from ._rows import as_rows, check_rows, new_like, on_device_of, once
+from ._rows import check_rows, output_ops
 
 _EXT = None
 _EXT_ERROR = None
@@ -357,63 +357,6 @@ def fused_dropout_gamma_residual(h, g, gamma, dropout_p):
 MAX_LAYERNORM_WIDTH = 16384
 
 
-def _layernorm_forward(x, weight, bias, eps, with_stats):
-    """(y, stats) of cign_layernorm_fwd; stats [2, rows] (mean, rstd), None
-    unless with_stats."""
-    lib = _lib.load_library()
-    y = new_like(x)
-    rows, stride = as_rows(x)
-    n, D = rows.shape
-    stats, mean, rstd = None, None, None
-    if with_stats:
-        stats = rows.new_empty((2, n), dtype=torch.float32)
-        mean = stats.data_ptr()
-        rstd = mean + 4 * n
-    param = weight if weight is not None else bias
-    code = _lib.DTYPE_CODE[x.dtype]
-    with on_device_of(x):
-        lib.call("cign_layernorm_fwd", _lib.stream_ptr(x.device), n, D, code,
-                 code if param is None else _lib.DTYPE_CODE[param.dtype], rows.data_ptr(), stride, _lib.ptr(weight),
-                 _lib.ptr(bias), eps, y.data_ptr(), mean, rstd)
-    return y, stats
-
-
-class _LayerNormFn(torch.autograd.Function):
-    """cign_layernorm_fwd / cign_layernorm_bwd."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _layernorm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once
-    def backward(ctx, grad_y):
-        x, weight, stats = ctx.saved_tensors
-        lib = _lib.load_library()
-        rows, stride = as_rows(x)
-        grads, grad_stride = as_rows(grad_y)
-        n, D = rows.shape
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        gx = new_like(x) if need_x else None
-        gw = x.new_empty((D,), dtype=weight.dtype) if need_w else None
-        gb = x.new_empty((D,), dtype=ctx.bias_dtype) if need_b else None
-        dtype = weight.dtype if weight is not None else ctx.bias_dtype or x.dtype
-        ws, ws_bytes = None, 0
-        if need_w or need_b:
-            ws_bytes = int(lib.cign_layernorm_bwd_workspace_bytes(n, D))
-            ws = _lib.workspace(ws_bytes, x.device)
-        mean = stats.data_ptr()
-        with on_device_of(x):
-            lib.call("cign_layernorm_bwd", _lib.stream_ptr(x.device), n, D, _lib.DTYPE_CODE[x.dtype],
-                     _lib.DTYPE_CODE[dtype], grads.data_ptr(), grad_stride, rows.data_ptr(), stride,
-                     _lib.ptr(weight), mean, mean + 4 * n, _lib.ptr(gx), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
-                     ws_bytes)
-        return gx, gw, gb, None
-
-
 def fused_layernorm(x, weight=None, bias=None, eps=1e-5):
     """LayerNorm over the last axis: (x - mean) / sqrt(var + eps) * weight +
     bias, var the biased variance, all sums in float32, the result in x's type.
@@ -438,8 +381,4 @@ def fused_layernorm(x, weight=None, bias=None, eps=1e-5):
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias))):
-        return _LayerNormFn.apply(x, weight, bias, eps)
-    return _layernorm_forward(x, weight, bias, eps, False)[0]
+    return output_ops().layernorm(x, weight, bias, eps)
