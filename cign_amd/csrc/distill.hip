@@ -509,7 +509,8 @@ int64_t workspace_bytes(int64_t n, int V) {
 
 template <typename T, bool TAIL>
 int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void* workspace, int64_t bytes) {
-  if (bytes < workspace_bytes<T>(in.n, in.V)) return set_error(kInvalid, "%s: workspace too small", who);
+  const int64_t needed = workspace_bytes<T>(in.n, in.V);
+  if (bytes < needed || (needed && !workspace)) return set_error(kInvalid, "%s: workspace too small", who);
   if (wavefront_row<T>(in.V))
     return with_lanes<T>(in.V, [&](auto WC, auto LC, auto UC) {
       constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;

@@ -36,7 +36,8 @@ import torch.nn.functional as F
 
 from . import _pack, lin_gat, pack_proj
 from .collapsed_gat import collapsed_gat_mean_bias_silu
-from .fused_block_ops import fused_add_layernorm_cat, fused_dropout_layernorm
+from .fused_block_ops import (MAX_LAYERNORM_WIDTH, fused_add_layernorm_cat, fused_dropout_layernorm,
+                              fused_layernorm)
 from .graph import selected_sparse_powers
 from .hop_gate import gated_clifford_pack, global_hop_gate, node_hop_gate
 from .linear import linear_attention_logits, linear_gamma_residual, mfma_linear
@@ -256,6 +257,23 @@ class GraphCliffordBlock(nn.Module):
                                      self.selective_amp_dtype)
 
 
+class FusedLayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over one axis, on fused_block_ops.fused_layernorm: the same
+    parameters and state dict, hooks called alike, rows of up to 16384 values in
+    float32 or bfloat16."""
+
+    def __init__(self, normalized_shape: int, *args, **kwargs):
+        super().__init__(normalized_shape, *args, **kwargs)
+        if len(self.normalized_shape) != 1 or not (1 <= self.normalized_shape[0] <= MAX_LAYERNORM_WIDTH):
+            raise ValueError(f"FusedLayerNorm needs one axis of 1 to {MAX_LAYERNORM_WIDTH} values, got "
+                             f"{tuple(self.normalized_shape)}")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() < 1 or x.size(-1) != self.normalized_shape[0]:
+            raise ValueError(f"expected rows of {self.normalized_shape[0]} values, got {tuple(x.shape)}")
+        return fused_layernorm(x, self.weight, self.bias, self.eps)
+
+
 class GraphCliffordNet(nn.Module):
     """The full CIGN model (generic_engine/model_cign.py:943-1210) on the HIP
     route: dual input projection (MFMA, selective bf16 autocast), the Clifford
@@ -263,7 +281,8 @@ class GraphCliffordNet(nn.Module):
     classifier (MFMA). Constructor arguments, parameter names and forward
     signature are the reference's. The input / output dropouts and the output
     LayerNorm (width hidden*(layers+1), beyond the fused row kernels' 256) are
-    torch ops, as in the reference."""
+    torch ops, as in the reference; with use_fused_output_norm the output
+    LayerNorm is fused_layernorm."""
 
     def __init__(self, in_dim: int, hidden_dim: int, out_dim: int, num_layers: int = 4, order_set=(1, 2, 3),
                  dropout: float = 0.28, gat_heads: int = 6, gat_dropout: float = 0.32, use_fused_gat: bool = False,
@@ -274,7 +293,7 @@ class GraphCliffordNet(nn.Module):
                  init_gamma: float = 0.49, gamma_mode: str = "vector", hop_gate_mode: str = "node",
                  alpha_score_mode: str = None, interaction_mode: str = None, alpha_weighting_mode: str = None,
                  layer_combine: str = "concat", use_dual_input_projection: bool = True, init_input_eta: float = 0.1,
-                 use_bias: bool = True):
+                 use_bias: bool = True, use_fused_output_norm: bool = False):
         super().__init__()
         # Validation of model_cign.py:978-1020 (the backend flags are accepted;
         # every combination runs the one HIP route).
@@ -340,7 +359,8 @@ class GraphCliffordNet(nn.Module):
             for _ in range(num_layers)
         ])
         final_dim = hidden_dim * (num_layers + 1) if layer_combine == "concat" else hidden_dim
-        self.output_norm = nn.LayerNorm(final_dim)
+        self.use_fused_output_norm = bool(use_fused_output_norm)
+        self.output_norm = (FusedLayerNorm if self.use_fused_output_norm else nn.LayerNorm)(final_dim)
         self.classifier = nn.Linear(final_dim, out_dim, bias=use_bias)
 
     @torch.no_grad()

@@ -18,7 +18,10 @@ to go from a dataset on disk to timed training steps.
     edge index with one self-loop per node, the fixed CSR operator and the
     multihop operator for the model's hops, and the fused-GAT graph format;
   * forward_model / train_one_epoch / evaluate_logits
-    (train_cign.py:1820-1821, 2103-2155).
+    (train_cign.py:1820-1821, 2103-2155);
+  * predict_nodes, teacher_targets, distill_one_epoch: what a node's logits say
+    (prediction, confidence, entropy), and training a model on another one's top
+    classes (no counterpart in the reference).
 
 The model itself runs on libcign_amd's HIP kernels; nothing here computes
 on the host beyond the one-time graph preparation and the metrics.
@@ -35,6 +38,8 @@ import torch
 import torch.nn.functional as F
 
 from . import graph
+from .class_logprobs import ClassLogprobs, class_logprobs
+from .distill import distill_topk_loss
 
 try:
     from sklearn.metrics import roc_auc_score
@@ -289,3 +294,60 @@ def evaluate_logits(model, data, graph_operator) -> torch.Tensor:
     """The single full-graph evaluation forward (train_cign.py:2151-2155)."""
     model.eval()
     return forward_model(model, data, graph_operator)
+
+
+def predict_nodes(model, data, graph_operator, top_k: int = 1, temperature: float = 1.0) -> ClassLogprobs:
+    """The evaluation forward read in one pass over its logits
+    (class_logprobs): each node's log probability of its label data.y, its
+    entropy, and its top_k classes (at most the model's) with their log
+    probabilities; top_index[:, 0] is the prediction ``accuracy`` takes."""
+    return class_logprobs(evaluate_logits(model, data, graph_operator), data.y.reshape(-1), top_k=top_k,
+                          temperature=temperature)
+
+
+@dataclass
+class TeacherTargets:
+    """A teacher's top classes a node, for distill_one_epoch."""
+    index: torch.Tensor     # [N, K] int64
+    logprobs: torch.Tensor  # [N, K] float32, at `temperature`
+    temperature: float
+
+
+def teacher_targets(model, data, graph_operator, top_k: int, temperature: float = 1.0) -> TeacherTargets:
+    """The top_k classes of each node by the teacher `model` in evaluation
+    mode, and their log probabilities at the temperature."""
+    top = class_logprobs(evaluate_logits(model, data, graph_operator), top_k=top_k, temperature=temperature)
+    return TeacherTargets(index=top.top_index, logprobs=top.top_logprobs, temperature=float(temperature))
+
+
+def distill_one_epoch(model, data, graph_operator, optimizer, device: torch.device, targets: TeacherTargets,
+                      weight: float = 0.5, tail: bool = True, grad_scaler=None) -> Tuple[float, float]:
+    """train_one_epoch against labels and a teacher: the loss is (1 - weight)
+    times the cross-entropy over the train mask plus weight times the mean over
+    all nodes of distill_topk_loss (with the tail: the classes outside a node's
+    list as one more). Returns the loss and the step's seconds."""
+    if not 0.0 <= float(weight) <= 1.0:
+        raise ValueError(f"weight must be in [0, 1], got {weight}")
+    model.train()
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise RuntimeError("distill_one_epoch: the model's kernels run on the GPU only")
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    optimizer.zero_grad()
+    logits = forward_model(model, data, graph_operator)
+    # nodes outside the mask are ignored, without gathering logits
+    labels = torch.where(data.train_mask, data.y, -100)
+    ce = -class_logprobs(logits, labels).logprob.sum() / data.train_mask.sum()
+    kl = distill_topk_loss(logits, targets.logprobs, targets.index, targets.temperature, tail).mean()
+    loss = (1.0 - weight) * ce + weight * kl
+    if grad_scaler is not None and grad_scaler.is_enabled():
+        grad_scaler.scale(loss).backward()
+        grad_scaler.step(optimizer)
+        grad_scaler.update()
+    else:
+        loss.backward()
+        optimizer.step()
+    end.record()
+    end.synchronize()
+    return float(loss.detach().item()), start.elapsed_time(end) / 1000.0
