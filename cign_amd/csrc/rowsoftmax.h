@@ -144,20 +144,27 @@ __device__ __forceinline__ void mask_out(typename RowChunk<T, W>::Raw& q, uint32
   }
 }
 
-// d = (x - m) log2(e) / T for the classes of a row. Where the scaled shift
-// nears float32's largest value (rows whose every logit is the type's lowest,
-// tiny temperatures) x c and m c overflow, and the difference is taken first.
+// d = (x - m) log2(e) / T for the classes of a row. The rounding of m c shifts
+// every d by up to 2^-24 |m c|, which must stay far from what an exponential
+// overflows at: from |m c| = 10^6 on (and where m c is no finite number: rows whose
+// every logit is the type's lowest, tiny temperatures) the difference is taken
+// first instead.
 struct Shift {
   float m, c, mc;
   bool far;
-  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), c(c_), mc(m_ * c_), far(!(fabsf(m_ * c_) < 1e37f)) {}
+  __device__ __forceinline__ Shift(float m_, float c_) : m(m_), c(c_), mc(m_ * c_), far(is_far(m_ * c_)) {}
+  static __device__ __forceinline__ bool is_far(float v) { return !(fabsf(v) < 1e6f); }
   __device__ __forceinline__ float near_d(float x) const { return fmaf(x, c, -mc); }
   __device__ __forceinline__ float far_d(float x) const { return (x - m) * c; }
   __device__ __forceinline__ float d(float x) const { return far ? far_d(x) : near_d(x); }
-  // of another shift: the difference of the two products as each was rounded
+  // of another shift's m, relative to which sums were taken: a near shift
+  // stands at its rounded product, a far one at the exact one
   __device__ __forceinline__ float d_of(float other) const {
 #pragma clang fp contract(off)
-    return far ? far_d(other) : other * c - mc;
+    const float oc = other * c;
+    const bool other_far = is_far(oc);
+    if (far) return other_far ? far_d(other) : fmaf(-m, c, oc);
+    return other_far ? fmaf(other, c, -mc) : oc - mc;
   }
 };
 

@@ -317,6 +317,23 @@ def test_large_offsets_and_temperatures():
         _check(x, labels, 4, T, g, h, name=f"T={T}")
 
 
+@pytest.mark.parametrize("V", [40, 3000, 40000])
+def test_rows_far_from_zero(V):
+    """Logits whose steps are 2^-4, 1, 64 and 2^13 (spreads of a few steps), and
+    rows half of which lies on either side of where the shift's rounded product
+    is given up for the difference (|x| log2(e) / T = 10^6)."""
+    for off, step in ((6.5e5, 0.0625), (-6.9314e5, 0.0625), (1e7, 1.0), (-1e9, 64.0), (1e11, 8192.0)):
+        x, labels, g, h = _logits(12, V, F32, V)
+        x = off + (x * 2).round() * step
+        T = max(1.0, step)
+        _check(x, labels, min(V, 4), T, g, h, name=f"offset {off}")
+    x, labels, g, h = _logits(12, V, F32, V + 1)
+    edge = 1e6 / 1.4426950408889634
+    x = edge + x.round()  # half of the values beyond
+    x[6:] *= -1
+    _check(x, labels, min(V, 4), 1.0, g, h, name="at the edge")
+
+
 def test_row_results_do_not_depend_on_the_call():
     """A row's values and gradient are the same in a call of its own, where
     its kernel shape is the same, and runs agree bit for bit."""

@@ -200,6 +200,21 @@ def test_masked_and_confident_students(V, tail):
         _check(x, t, index, g, 1.0, tail, f"V={V}")
 
 
+@pytest.mark.parametrize("V", [40, 3000, 40000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_rows_far_from_zero(V, tail):
+    """As in the log probabilities' tests: large steps, and rows on both sides
+    of |x| log2(e) / T = 10^6, the listed classes beyond it or not."""
+    for off, step in ((6.5e5, 0.0625), (1e7, 1.0), (-1e9, 64.0)):
+        x, t, index, g = _inputs(8, V, 5, F32, V)
+        _check(off + (x * 2).round() * step, t, index, g, max(1.0, step), tail, f"offset {off}")
+    x, t, index, g = _inputs(8, V, 5, F32, V + 1)
+    x = 1e6 / 1.4426950408889634 + x.round()
+    x[1] = x[1].scatter(0, index[1].clamp_min(0), x[1].max().item() + 5)
+    x[4:] *= -1
+    _check(x, t, index, g, 1.0, tail, "at the edge")
+
+
 @pytest.mark.parametrize("V", [6, 3000, 40000])
 def test_bad_rows_stay_in_their_rows(V):
     from cign_amd.distill import distill_topk_loss
