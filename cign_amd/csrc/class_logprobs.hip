@@ -123,10 +123,14 @@ __device__ __forceinline__ void for_each(F&& f) {
 
 // The key of the share's largest value m, of those of its chunks: best_below(~0)
 // without making every value's key, the first own value equal to m of the first
-// chunk that has one. A share whose m is -inf or NaN takes the long way.
+// chunk that has one. A share whose m is -inf, or with a chunk whose NaN hides
+// its other values, takes the long way.
 template <typename T, int W, int U>
 __device__ __forceinline__ uint64_t best_key(const Share<T, W, U>& sh, const float (&of_chunk)[U], float m) {
-  if (!(m > -kInf)) return best_below(sh, ~0ull);
+  bool hidden = !(m > -kInf);
+#pragma unroll
+  for (int u = 0; u < U; ++u) hidden = hidden || of_chunk[u] != of_chunk[u];
+  if (hidden) return best_below(sh, ~0ull);
   auto raw = sh.raw[0];
   int at = sh.at[0];
 #pragma unroll

@@ -242,6 +242,28 @@ def test_nonfinite_logits_stay_in_their_rows(V):
     assert not ga[6].any()  # an ignored row: zeros, whatever its logits hold
 
 
+@pytest.mark.parametrize("V", [6, 300, 3000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_top_lists_beside_nan(V, dtype):
+    """A NaN, of either sign, ranks as -inf and hides none of the classes read
+    with it."""
+    x = _logits(12, V, dtype, V)[0]
+    k = min(V, 20)
+    best = x.float().topk(min(3, V), dim=1).indices
+    for r in range(12):
+        # next to the row's best classes, and elsewhere
+        for i in {int(best[r, r % best.shape[1]]) ^ (1 + r % 3), (r * 37) % V}:
+            if i < V and i not in best[r].tolist()[:1]:
+                x[r, i] = math.nan if r % 2 else -math.nan
+    if dtype == BF16:  # the sign bit as well
+        x.view(torch.int16)[::2][x[::2].isnan()] = -64
+    from cign_amd.class_logprobs import class_logprobs
+
+    assert x.isnan().any(dim=1).sum() >= 8
+    got = class_logprobs(x, top_k=k).top_index.cpu().numpy()
+    assert np.array_equal(got, _top(_n(x), k))
+
+
 def test_labels_out_of_range_are_seen():
     from cign_amd.class_logprobs import class_logprobs
 
