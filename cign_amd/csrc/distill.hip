@@ -69,6 +69,12 @@ __device__ __forceinline__ double lanes_sum(double v) {
 }
 
 template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+  for_offsets<1, LPR>([&](auto OC) { v += xor_shfl<decltype(OC)::value>(v); });
+  return v;
+}
+
+template <int LPR>
 __device__ __forceinline__ float lanes_max(float v) {
   for_offsets<1, LPR>([&](auto OC) { v = fmaxf(v, xor_shfl<decltype(OC)::value>(v)); });
   return v;
@@ -122,11 +128,28 @@ __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t 
                        q.none ? kInf : static_cast<float>(q.lz * (1.0 / kLn2d)), static_cast<float>(a), {0.0f, 0.0f}};
 }
 
+// e^(t - top) of a list that is renormalised, to 2 ulp of float32: the
+// difference is taken in float64, what its rounding loses multiplied back. What a
+// list leaves of one (1 - sum e^t, near 0 for a confident teacher) takes the
+// exponential itself in float64.
+__device__ __forceinline__ double list_exp(float t, float top) {
+  const double d = static_cast<double>(t) - shift_of(top);
+  const float hi = static_cast<float>(d), e = expf(hi);
+  return hi == -kInf ? 0.0 : fmaf(e, static_cast<float>(d - hi), e);
+}
+
+template <bool TAIL>
+__device__ __forceinline__ double list_p(float t, float top, double inv_total) {
+  if constexpr (TAIL) return exp(static_cast<double>(t));
+  return list_exp(t, top) * inv_total;
+}
+
 // Row r by LPR < 64 lanes (lane q), from the joined statistics (m, s) of the
-// classes outside the list (TAIL) or of all classes. Rows this short have short
-// lists: each lane goes through its places once for every step.
+// classes outside the list (TAIL) or of all classes; `again`: a class is named
+// twice. Rows this short have short lists: each lane goes through its places
+// once for every step.
 template <typename T, int LPR, bool TAIL>
-__device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m, float s) {
+__device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m, float s, bool again) {
   const int64_t* index = in.index + r * in.K;
   const float* t = in.t + r * in.K;
   const T* row = in.x + r * in.ld;
@@ -140,45 +163,47 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
       continue;
     }
     top = fmaxf(top, t[i]);
-    top_x = fmaxf(top_x, to_f32(row[j]));
+    if (TAIL) top_x = fmaxf(top_x, to_f32(row[j]));
   }
   const ListSummary list{lanes_max<LPR>(top), lanes_max<LPR>(top_x), lanes_max<LPR>(any) != 0.0f,
                          lanes_max<LPR>(bad) != 0.0f};
   Student st(m, s, TAIL ? shift_of(fmaxf(s == 0.0f ? -kInf : m, list.top_x)) : m, in.c);
-  double members = 0.0, listed = 0.0, total = 0.0;
+  float members = 0.0f, listed = 0.0f;
+  double total = 0.0;
   for (int i = q; i < in.K; i += LPR) {
     const int64_t j = index[i];
     if (j < 0 || j >= in.V) continue;
     if constexpr (TAIL) {
       bool first = true;
-      for (int k = 0; k < i; ++k) first = first && index[k] != j;
+      if (again)
+        for (int k = 0; k < i; ++k) first = first && index[k] != j;
       if (!first) continue;
-      members += 1.0;
-      listed += exp2f(st.all.d(to_f32(row[j])));
+      members += 1.0f;
+      listed += __builtin_amdgcn_exp2f(st.all.d(to_f32(row[j])));
     } else {
-      total += exp(static_cast<double>(t[i]) - shift_of(list.top));
+      total += list_exp(t[i], list.top);
     }
   }
-  st.total(lanes_sum<LPR>(listed));
-  members = lanes_sum<LPR>(members);
+  st.total(group_sum<LPR>(listed));
+  members = group_sum<LPR>(members);
   total = lanes_sum<LPR>(total);
-  const double shift = total == 0.0 ? 0.0 : shift_of(list.top) + log(total);  // log p = t - shift
+  // log p = t - shift
+  const double shift = total == 0.0 ? 0.0 : static_cast<double>(shift_of(list.top)) + logf(static_cast<float>(total));
+  const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   for (int i = q; i < in.K; i += LPR) {
     const int64_t j = index[i];
     double at_class = 0.0;
     if (j >= 0 && j < in.V) {
-      const double lp = static_cast<double>(t[i]) - shift;
-      const double p = exp(lp);
+      const double p = list_p<TAIL>(t[i], list.top, inv);
       if (p != 0.0) {
-        loss += p * (lp - st.logq(to_f32(row[j])));
+        loss += p * (static_cast<double>(t[i]) - shift - st.logq(to_f32(row[j])));
         mass += p;
       }
-      if (o.p) {
-        at_class = p;
+      at_class = p;
+      if (o.p && again)
         for (int k = 0; k < in.K; ++k)
-          if (k != i && index[k] == j) at_class += exp(static_cast<double>(t[k]) - shift);
-      }
+          if (k != i && index[k] == j) at_class += list_p<TAIL>(t[k], list.top, inv);
     }
     if (o.p) o.p[r * in.K + i] = static_cast<float>(at_class);
   }
@@ -189,8 +214,8 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
 
 // The same by a whole wavefront: up to two places a lane in registers, the
 // list's classes and masses in the wavefront's part of LDS, where a place finds
-// the others that name its class.
-struct WaveList {
+// the others that name its class (repeats: 0 none do, 1 some, -1 not known).
+struct alignas(16) WaveList {
   int index[kMaxList];  // -1: names no class
   float p[kMaxList];
 };
@@ -199,7 +224,7 @@ __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOM
 
 template <typename T, bool TAIL, int E>
 __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int64_t r, int lane, float m, float s,
-                                              WaveList& lds) {
+                                              int repeats, WaveList& lds) {
   int at[E];
   float t[E], x[E];
   float top = -kInf, top_x = -kInf;
@@ -227,54 +252,57 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
       top_x = fmaxf(top_x, x[e]);
     }
   const ListSummary list{lanes_max<kWave>(top), lanes_max<kWave>(top_x), __any(any) != 0, __any(bad) != 0};
-  // the places that name the same class
+  // the places that name the same class, unless the caller knows of none
   bool first[E], again = false;
 #pragma unroll
   for (int e = 0; e < E; ++e) first[e] = at[e] >= 0;
-  for (int k = 0; k < in.K; k += 4) {
-    const int4 j = *reinterpret_cast<const int4*>(&lds.index[k]);
+  if (repeats != 0) {
+    for (int k = 0; k < in.K; k += 4) {
+      const int4 j = *reinterpret_cast<const int4*>(&lds.index[k]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int i = lane + e * kWave;
-      const bool b0 = j.x == at[e] && k != i, b1 = j.y == at[e] && k + 1 != i;
-      const bool b2 = j.z == at[e] && k + 2 != i, b3 = j.w == at[e] && k + 3 != i;
-      const bool same = at[e] >= 0 && (b0 || b1 || b2 || b3);
-      again = again || same;
-      if (same && ((b0 && k < i) || (b1 && k + 1 < i) || (b2 && k + 2 < i) || (b3 && k + 3 < i))) first[e] = false;
+      for (int e = 0; e < E; ++e) {
+        const int i = lane + e * kWave;
+        const bool b0 = j.x == at[e] && k != i, b1 = j.y == at[e] && k + 1 != i;
+        const bool b2 = j.z == at[e] && k + 2 != i, b3 = j.w == at[e] && k + 3 != i;
+        const bool same = at[e] >= 0 && (b0 || b1 || b2 || b3);
+        again = again || same;
+        if (same && ((b0 && k < i) || (b1 && k + 1 < i) || (b2 && k + 2 < i) || (b3 && k + 3 < i))) first[e] = false;
+      }
     }
   }
   Student st(m, s, TAIL ? shift_of(fmaxf(s == 0.0f ? -kInf : m, list.top_x)) : m, in.c);
-  double members = 0.0, listed = 0.0, total = 0.0;
-  const double top64 = shift_of(list.top);
+  float members = 0.0f, listed = 0.0f;
+  double total = 0.0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (at[e] < 0) continue;
     if constexpr (TAIL) {
-      members += first[e] ? 1.0 : 0.0;
-      listed += first[e] ? exp2f(st.all.d(x[e])) : 0.0f;
+      members += first[e] ? 1.0f : 0.0f;
+      listed += first[e] ? __builtin_amdgcn_exp2f(st.all.d(x[e])) : 0.0f;
     } else {
-      total += exp(static_cast<double>(t[e]) - top64);
+      total += list_exp(t[e], list.top);
     }
   }
   if constexpr (TAIL) {
-    listed = lanes_sum<kWave>(listed);
-    members = lanes_sum<kWave>(members);
+    listed = group_sum<kWave>(listed);
+    members = group_sum<kWave>(members);
   } else {
     total = lanes_sum<kWave>(total);
   }
   st.total(listed);
-  const double shift = total == 0.0 ? 0.0 : top64 + log(total);  // log p = t - shift
+  // log p = t - shift
+  const double shift = total == 0.0 ? 0.0 : static_cast<double>(shift_of(list.top)) + logf(static_cast<float>(total));
+  const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   float at_class[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     at_class[e] = 0.0f;
     if (at[e] < 0) continue;
-    const double lp = static_cast<double>(t[e]) - shift;
-    const double p = exp(lp);
+    const double p = list_p<TAIL>(t[e], list.top, inv);
     at_class[e] = static_cast<float>(p);
     if (p != 0.0) {
-      loss += p * (lp - st.logq(x[e]));
+      loss += p * (static_cast<double>(t[e]) - shift - st.logq(x[e]));
       mass += p;
     }
   }
@@ -302,12 +330,12 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
 
 template <typename T, bool TAIL>
 __device__ __forceinline__ void finish_wave(const In<T>& in, const Out& o, int64_t r, int lane, float m, float s,
-                                            WaveList& lds) {
+                                            int repeats, WaveList& lds) {
   static_assert(kMaxList == 2 * kWave, "one or two places a lane");
   if (in.K <= kWave)
-    finish_places<T, TAIL, 1>(in, o, r, lane, m, s, lds);
+    finish_places<T, TAIL, 1>(in, o, r, lane, m, s, repeats, lds);
   else
-    finish_places<T, TAIL, 2>(in, o, r, lane, m, s, lds);
+    finish_places<T, TAIL, 2>(in, o, r, lane, m, s, repeats, lds);
 }
 
 // The bits of a share's chunk c (W places from column c W of the bitmap's
@@ -318,16 +346,19 @@ __device__ __forceinline__ uint32_t kill_bits(const uint32_t* bits, int place, i
   return ((1u << own) - 1u) | ((listed << own) & ((1u << W) - 1u));
 }
 
-// Rows that LPR lanes hold.
+// Rows that LPR lanes hold. The bitmap also tells whether a list names a class
+// twice: a bit that was set (rows of 128 classes with whole lists: 933 us with
+// every place looking for others).
 template <typename T, int W, int LPR, int U, bool TAIL>
 __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
   constexpr int kRows = kBlock / LPR;
   constexpr int kWords = (LPR * U * W + 31) / 32;
-  __shared__ uint32_t bitmap[TAIL ? kRows * kWords : 1];
+  __shared__ uint32_t bitmap[kRows * kWords];
+  __shared__ int repeats[kRows];
   __shared__ WaveList lists[LPR == kWave ? kWavesPerBlock : 1];
   const int q = threadIdx.x & (LPR - 1);
   const int slot = threadIdx.x / LPR;
-  uint32_t* bits = bitmap + (TAIL ? slot * kWords : 0);
+  uint32_t* bits = bitmap + slot * kWords;
   const int nc = (in.V + W - 1) / W;
   Share<T, W, U> sh;
   sh.place(q, LPR, nc, in.V);
@@ -336,18 +367,20 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     const int64_t r = base + slot;
     const bool active = r < in.n;
     if (active) sh.load(in.x + r * in.ld);
-    if constexpr (TAIL) {
-      __syncthreads();  // the former rows' bits have been read
-      for (int i = q; i < kWords; i += LPR) bits[i] = 0;
-      __syncthreads();
-      if (active)
-        for (int i = q; i < in.K; i += LPR) {
-          const int64_t j = in.index[r * in.K + i];
-          if (j >= 0 && j < in.V) atomicOr(&bits[j >> 5], 1u << (j & 31));
-        }
-      __syncthreads();
-    }
+    __syncthreads();  // the former rows' bits have been read
+    for (int i = q; i < kWords; i += LPR) bits[i] = 0;
+    if (q == 0) repeats[slot] = 0;
+    __syncthreads();
+    if (active)
+      for (int i = q; i < in.K; i += LPR) {
+        const int64_t j = in.index[r * in.K + i];
+        if (j < 0 || j >= in.V) continue;
+        const uint32_t bit = 1u << (j & 31);
+        if (atomicOr(&bits[j >> 5], bit) & bit) repeats[slot] = 1;
+      }
+    __syncthreads();
     if (!active) continue;
+    const int again = repeats[slot];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       mask_out<T, W>(sh.raw[u], TAIL ? kill_bits<W>(bits, q + u * LPR, sh.own[u]) : (1u << sh.own[u]) - 1u);
@@ -355,9 +388,9 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
     join<LPR>(m, s, t, in.c);
     if constexpr (LPR == kWave)
-      finish_wave<T, TAIL>(in, o, r, q, m, s, lists[wave_id()]);
+      finish_wave<T, TAIL>(in, o, r, q, m, s, again, lists[wave_id()]);
     else
-      finish<T, LPR, TAIL>(in, o, r, q, m, s);
+      finish<T, LPR, TAIL>(in, o, r, q, m, s, again != 0);
   }
 }
 
@@ -399,7 +432,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     join<kWave>(m, s, t, in.c);
     across.run(m, s, t, in.c);
     if constexpr (ONE) {
-      if (threadIdx.x < kWave) finish_wave<T, TAIL>(in, o, r, threadIdx.x, m, s, list);
+      if (threadIdx.x < kWave) finish_wave<T, TAIL>(in, o, r, threadIdx.x, m, s, -1, list);
     } else if (threadIdx.x == 0) {
       part[item] = make_float2(s == 0.0f ? -kInf : m, s);
     }
@@ -416,7 +449,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
     const float2 p = lane < S ? part[r * S + lane] : make_float2(-kInf, 0.0f);
     float m = p.x, s = p.y, t = 0.0f;
     join<kWave>(m, s, t, in.c);
-    finish_wave<T, TAIL>(in, o, r, lane, m, s, lists[wave_id()]);
+    finish_wave<T, TAIL>(in, o, r, lane, m, s, -1, lists[wave_id()]);
   }
 }
 
