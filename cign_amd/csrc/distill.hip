@@ -97,35 +97,37 @@ struct ListSummary {
 struct Student {
   Shift rest, all;
   float s;    // relative to `rest`
-  double lz;  // log of the sum over all classes, relative to `all`
+  float lz;   // log of the sum over all classes, relative to `all`
   bool none;  // no class left
   __device__ __forceinline__ Student(float m, float s_, float mt, float c) : rest(m, c), all(mt, c), s(s_) {}
-  __device__ __forceinline__ void total(double listed) {
-    const double st = listed + (s == 0.0f ? 0.0 : static_cast<double>(s) * exp2f(all.d_of(rest.m)));
-    none = st == 0.0;
-    lz = none ? 0.0 : log(st);
+  __device__ __forceinline__ void total(float listed) {
+    const float st = listed + (s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(all.d_of(rest.m)));
+    none = st == 0.0f;
+    lz = none ? 0.0f : logf(st);
   }
   __device__ __forceinline__ double logq(float x) const { return none ? -kInfd : wide_d(all, x) * kLn2d - lz; }
 };
 
-// The row's loss and statistics from the sums over its list, by one lane.
+// The row's loss and statistics from the sums over its list, by one lane. The
+// logarithms are float32: of sums that are known to float32, and of a remainder
+// whose relative error is.
 template <typename T, bool TAIL>
 __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t r, const Student& q,
-                                         const ListSummary& list, double members, double loss, double mass) {
+                                         const ListSummary& list, float members, double loss, double mass) {
   double a = mass, cb = mass;
   if constexpr (TAIL) {
     const double left = list.any && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
     const double lrest =
-        q.s == 0.0f ? -kInfd : static_cast<double>(q.all.d_of(q.rest.m)) * kLn2d + log(static_cast<double>(q.s)) - q.lz;
-    if (left > 0.0) loss += left * (log(left) - lrest);
+        q.s == 0.0f ? -kInfd : static_cast<double>(q.all.d_of(q.rest.m)) * kLn2d + (logf(q.s) - q.lz);
+    if (left > 0.0) loss += left * (logf(static_cast<float>(left)) - lrest);
     a = mass + left;
-    cb = a * exp(lrest) - left;
+    cb = a * expf(static_cast<float>(lrest)) - left;
   }
   if (list.bad) loss = a = cb = __builtin_nan("");
   o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
   if (o.stats)
     o.stats[r] = Stats{q.rest.m, q.s == 0.0f ? kInf : log2f(q.s), static_cast<float>(cb), q.all.m,
-                       q.none ? kInf : static_cast<float>(q.lz * (1.0 / kLn2d)), static_cast<float>(a), {0.0f, 0.0f}};
+                       q.none ? kInf : q.lz * kLog2e, static_cast<float>(a), {0.0f, 0.0f}};
 }
 
 // e^(t - top) of a list that is renormalised, to 2 ulp of float32: the
