@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     sh.mask_foreign();
     float m = sh.largest(), s = 0.0f, t = 0.0f;
     sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
-    join<LPR>(m, s, t, in.c);
+    join<LPR, true>(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
     if (q == 0) finish(in, o, r, m, s, t, l2s);
     if constexpr (TOP) {
@@ -240,129 +240,126 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
   __shared__ uint64_t threshold;
   __shared__ int found;
   const int nc = (in.V + W - 1) / W;
-  const int64_t items = in.n * sl.S;
-  const int lane = lane_id();
+  const int lane = lane_id(), slice = blockIdx.x;
+  const int64_t r = slice_row();
+  if (r >= in.n) return;
   BlockJoin across(slots);
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t r = item / sl.S;
-    const int slice = static_cast<int>(item - r * sl.S);
-    const int end = min((slice + 1) * sl.cps, nc);
-    Share<T, W, U> sh;
-    sh.place(slice * sl.cps + threadIdx.x, kBlock, end, in.V);
-    sh.template load<PAST>(in.x + r * in.ld);
-    sh.mask_foreign();
-    float of_chunk[TOP ? U : 1], m = -kInf, s = 0.0f, t = 0.0f;
-    if constexpr (TOP) {
-      for_each<U>([&](auto UC) {
-        constexpr int u = decltype(UC)::value;
-        of_chunk[u] = sh.template largest<u, u + 1>();
-        m = fmaxf(m, of_chunk[u]);
-      });
+  const int64_t item = r * sl.S + slice;
+  const int end = min((slice + 1) * sl.cps, nc);
+  Share<T, W, U> sh;
+  sh.place(slice * sl.cps + threadIdx.x, kBlock, end, in.V);
+  sh.template load<PAST>(in.x + r * in.ld);
+  sh.mask_foreign();
+  float of_chunk[TOP ? U : 1], m = -kInf, s = 0.0f, t = 0.0f;
+  if constexpr (TOP) {
+    for_each<U>([&](auto UC) {
+      constexpr int u = decltype(UC)::value;
+      of_chunk[u] = sh.template largest<u, u + 1>();
+      m = fmaxf(m, of_chunk[u]);
+    });
+  } else {
+    m = sh.largest();
+  }
+  const float top = m;
+  sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
+  join<kWave, true>(m, s, t, in.c);
+  if (TOP && threadIdx.x == 0) {
+    threshold = 1;
+    found = 0;
+  }
+  uint64_t mine = 0;
+  const bool quads = TOP && o.K <= kBlock / 8;
+  if constexpr (TOP) {
+    mine = best_key(sh, of_chunk, top);
+    uint64_t best = mine;
+    if (quads) {
+      best = group_max<4>(mine);
+      if ((threadIdx.x & 3) == 0) sample[threadIdx.x >> 2] = best;
     } else {
-      m = sh.largest();
+      sample[threadIdx.x] = best;
     }
-    const float top = m;
-    sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
-    join<kWave>(m, s, t, in.c);
-    if (TOP && threadIdx.x == 0) {
-      threshold = 1;
-      found = 0;
+  }
+  across.run<true>(m, s, t, in.c);
+  float l2s = s == 0.0f ? 0.0f : log2f(s);
+  if (threadIdx.x == 0) {
+    if (sl.S == 1)
+      finish(in, o, r, m, s, t, l2s);
+    else
+      part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
+  }
+  if constexpr (TOP) {
+    // The K-th largest of the best keys of quads (K <= 32) or threads bounds
+    // the slice's K-th key from below; every key at or above it is a
+    // candidate. Each quad counts the keys above its own, a quarter a lane.
+    const int K = o.K;
+    if (quads) {
+      const uint64_t own = sample[threadIdx.x >> 2];
+      int above = count_above(sample + (threadIdx.x & 3) * (kBlock / 16), kBlock / 16, own);
+      above += __float_as_int(xor_shfl<1>(__int_as_float(above)));
+      above += __float_as_int(xor_shfl<2>(__int_as_float(above)));
+      if (own != 0 && above == K - 1) threshold = own;  // one quad: keys differ
+    } else {
+      const int above = count_above(sample, kBlock, mine);
+      if (mine != 0 && above == K - 1) threshold = mine;
     }
-    uint64_t mine = 0;
-    const bool quads = TOP && o.K <= kBlock / 8;
-    if constexpr (TOP) {
-      mine = best_key(sh, of_chunk, top);
-      uint64_t best = mine;
-      if (quads) {
-        best = group_max<4>(mine);
-        if ((threadIdx.x & 3) == 0) sample[threadIdx.x >> 2] = best;
-      } else {
-        sample[threadIdx.x] = best;
-      }
-    }
-    across.run(m, s, t, in.c);
-    float l2s = s == 0.0f ? 0.0f : log2f(s);
-    if (threadIdx.x == 0) {
-      if (sl.S == 1)
-        finish(in, o, r, m, s, t, l2s);
-      else
-        part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
-    }
-    if constexpr (TOP) {
-      // The K-th largest of the best keys of quads (K <= 32) or threads bounds
-      // the slice's K-th key from below; every key at or above it is a
-      // candidate. Each quad counts the keys above its own, a quarter a lane.
-      const int K = o.K;
-      if (quads) {
-        const uint64_t own = sample[threadIdx.x >> 2];
-        int above = count_above(sample + (threadIdx.x & 3) * (kBlock / 16), kBlock / 16, own);
-        above += __float_as_int(xor_shfl<1>(__int_as_float(above)));
-        above += __float_as_int(xor_shfl<2>(__int_as_float(above)));
-        if (own != 0 && above == K - 1) threshold = own;  // one quad: keys differ
-      } else {
-        const int above = count_above(sample, kBlock, mine);
-        if (mine != 0 && above == K - 1) threshold = mine;
-      }
-      __syncthreads();
-      const uint64_t bar = threshold;
-      if (mine >= bar) {
-        const float low = key_value(bar);
+    __syncthreads();
+    const uint64_t bar = threshold;
+    if (mine >= bar) {
+      const float low = key_value(bar);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          // (a chunk of NaN is looked at; on 4 values the test costs what it saves)
-          if (W == 8 && of_chunk[u] < low) continue;
-          float v[W];
-          RowChunk<T, W>::unpack(sh.raw[u], v);
+      for (int u = 0; u < U; ++u) {
+        // (a chunk of NaN is looked at; on 4 values the test costs what it saves)
+        if (W == 8 && of_chunk[u] < low) continue;
+        float v[W];
+        RowChunk<T, W>::unpack(sh.raw[u], v);
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            if (!(ranked(v[w]) >= low)) continue;
-            const uint64_t k = key_of(v[w], sh.at[u] + w);
-            if (w >= sh.own[u] && k >= bar) {
-              const int at = atomicAdd(&found, 1);
-              if (at < kCandidates) cand[at] = k;
-            }
+        for (int w = 0; w < W; ++w) {
+          if (!(ranked(v[w]) >= low)) continue;
+          const uint64_t k = key_of(v[w], sh.at[u] + w);
+          if (w >= sh.own[u] && k >= bar) {
+            const int at = atomicAdd(&found, 1);
+            if (at < kCandidates) cand[at] = k;
           }
         }
       }
+    }
+    __syncthreads();
+    const int count = found;
+    uint64_t* list = keys + item * K;
+    if (count <= kCandidates) {
+      for (int i = count + threadIdx.x; i < ((count + 15) & ~15); i += kBlock) cand[i] = 0;
       __syncthreads();
-      const int count = found;
-      uint64_t* list = keys + item * K;
-      if (count <= kCandidates) {
-        for (int i = count + threadIdx.x; i < ((count + 15) & ~15); i += kBlock) cand[i] = 0;
+      for (int i = threadIdx.x; i < count; i += kBlock) {
+        const uint64_t k = cand[i];
+        const int rank = count_above(cand, count, k);
+        if (rank < K) {
+          if (sl.S == 1)
+            put_top(in, o, r, rank, k, m, l2s);
+          else
+            list[rank] = k;
+        }
+      }
+      if (sl.S > 1)
+        for (int i = count + threadIdx.x; i < K; i += kBlock) list[i] = 0;
+    } else {
+      // More candidates than the buffer holds (many large values in few
+      // threads' chunks): K rounds over the registers.
+      uint64_t below = ~0ull;
+      for (int k = 0; k < K; ++k) {
+        const uint64_t w = group_max<kWave>(best_below(sh, below));
         __syncthreads();
-        for (int i = threadIdx.x; i < count; i += kBlock) {
-          const uint64_t k = cand[i];
-          const int rank = count_above(cand, count, k);
-          if (rank < K) {
-            if (sl.S == 1)
-              put_top(in, o, r, rank, k, m, l2s);
-            else
-              list[rank] = k;
-          }
+        if (lane == 0) sample[wave_id()] = w;
+        __syncthreads();
+        uint64_t best = sample[0];
+        for (int i = 1; i < kWavesPerBlock; ++i) best = sample[i] > best ? sample[i] : best;
+        if (threadIdx.x == 0) {
+          if (sl.S == 1)
+            put_top(in, o, r, k, best, m, l2s);
+          else
+            list[k] = best;
         }
-        if (sl.S > 1)
-          for (int i = count + threadIdx.x; i < K; i += kBlock) list[i] = 0;
-      } else {
-        // More candidates than the buffer holds (many large values in few
-        // threads' chunks): K rounds over the registers.
-        uint64_t below = ~0ull;
-        for (int k = 0; k < K; ++k) {
-          const uint64_t w = group_max<kWave>(best_below(sh, below));
-          __syncthreads();
-          if (lane == 0) sample[wave_id()] = w;
-          __syncthreads();
-          uint64_t best = sample[0];
-          for (int i = 1; i < kWavesPerBlock; ++i) best = sample[i] > best ? sample[i] : best;
-          if (threadIdx.x == 0) {
-            if (sl.S == 1)
-              put_top(in, o, r, k, best, m, l2s);
-            else
-              list[k] = best;
-          }
-          below = best;
-        }
+        below = best;
       }
-      __syncthreads();  // the next item's samples and candidates
     }
   }
 }
@@ -376,7 +373,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_id(); r < in.n; r += step) {
     const float4 p = lane < S ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
     float m = p.x, s = p.y, t = p.z, l2s;
-    join<kWave>(m, s, t, in.c);
+    join<kWave, true>(m, s, t, in.c);
     if (lane == 0) finish(in, o, r, m, s, t, l2s);
   }
 }
@@ -412,7 +409,7 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       threshold = 1;
       found = 0;
     }
-    join<kWave>(m, s, t, in.c);
+    join<kWave, true>(m, s, t, in.c);
     float l2s = s == 0.0f ? 0.0f : log2f(s);
     __syncthreads();
     if (mine != 0 && count_above(sample, S * heads, mine) == K - 1) threshold = mine;
@@ -497,7 +494,7 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
           for (int w = 0; w < W; ++w) {
             const float d = of(v[w]) - l2s;  // log2 p
             const float p = __builtin_amdgcn_exp2f(d);
-            v[w] = p * (ENT ? fmaf(b, fmaxf(d, -1e30f), a) : a);
+            v[w] = p * (ENT ? fmaf(b, fmaxf(d, kFloor), a) : a);
           }
         };
         if (sf.far)
@@ -565,10 +562,9 @@ int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void
   uint64_t* keys = reinterpret_cast<uint64_t*>(part + (sl.S == 1 ? 0 : in.n * sl.S));
   const int rc = with_chunks<T>(sl.U, [&](auto UC) {
     constexpr int U = decltype(UC)::value;
-    const int grid = grid_of(in.n * sl.S);
     const auto launch = [&](auto TC, auto SC) {
-      hipLaunchKernelGGL((slice_kernel<T, U, decltype(TC)::value, decltype(SC)::value>), dim3(grid), dim3(kBlock), 0, st,
-                         in, o, sl, part, keys);
+      hipLaunchKernelGGL((slice_kernel<T, U, decltype(TC)::value, decltype(SC)::value>), slice_grid(sl.S, in.n),
+                         dim3(kBlock), 0, st, in, o, sl, part, keys);
     };
     const bool past = pass_of<T>(in.n, in.V) == kPast;
     if (o.K > 0)

@@ -340,12 +340,19 @@ __device__ __forceinline__ void finish_wave(const In<T>& in, const Out& o, int64
     finish_places<T, TAIL, 2>(in, o, r, lane, m, s, repeats, lds);
 }
 
-// The bits of a share's chunk c (W places from column c W of the bitmap's
-// first column) moved to where its values are.
-template <int W>
-__device__ __forceinline__ uint32_t kill_bits(const uint32_t* bits, int place, int own) {
-  const uint32_t listed = bits[place * W >> 5] >> (place * W & 31);
-  return ((1u << own) - 1u) | ((listed << own) & ((1u << W) - 1u));
+// Masks a share's chunk: the values that another chunk owns and, TAIL, the
+// listed classes: the W bits of the bitmap from its place on, moved to where its
+// own values are.
+template <typename T, int W, bool TAIL>
+__device__ __forceinline__ void mask_chunk(typename RowChunk<T, W>::Raw& raw, const uint32_t* bits, int place, int own) {
+  uint32_t listed = 0;
+  if constexpr (TAIL) {
+    if constexpr (W == 8)
+      listed = reinterpret_cast<const uint8_t*>(bits)[place];
+    else
+      listed = bits[place * W >> 5] >> (place * W & 31) & ((1u << W) - 1u);
+  }
+  if ((listed | own) != 0) mask_out<T, W>(raw, ((1u << own) - 1u) | ((listed << own) & ((1u << W) - 1u)));
 }
 
 // Rows that LPR lanes hold. The bitmap also tells whether a list names a class
@@ -385,10 +392,10 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     const int again = repeats[slot];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      mask_out<T, W>(sh.raw[u], TAIL ? kill_bits<W>(bits, q + u * LPR, sh.own[u]) : (1u << sh.own[u]) - 1u);
+      mask_chunk<T, W, TAIL>(sh.raw[u], bits, q + u * LPR, sh.own[u]);
     float m = sh.largest(), s = 0.0f, t = 0.0f;
     sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
-    join<LPR>(m, s, t, in.c);
+    join<LPR, false>(m, s, t, in.c);
     if constexpr (LPR == kWave)
       finish_wave<T, TAIL>(in, o, r, q, m, s, again, lists[wave_id()]);
     else
@@ -396,48 +403,44 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
   }
 }
 
-// Slices of long rows: (m, s) to part[r * S + slice]; ONE: a row's only slice,
-// which finishes it (apart, since its registers would cost the others a
-// wavefront a SIMD).
-template <typename T, int U, bool TAIL, bool ONE, bool PAST>
+// Slices of long rows: (m, s) to part[r * S + slice]; a row's only slice finishes
+// it.
+template <typename T, int U, bool TAIL, bool PAST>
 __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float2* part) {
   constexpr int W = kChunk<T>;
   constexpr int kWords = kBlock * U * W / 32;
   __shared__ float slots[2 * kWavesPerBlock][3];
   __shared__ uint32_t bits[TAIL ? kWords : 1];
-  __shared__ typename std::conditional<ONE, WaveList, int>::type list;
+  __shared__ WaveList list;
   BlockJoin across(slots);
   const int nc = (in.V + W - 1) / W;
-  const int64_t items = in.n * sl.S;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t r = item / sl.S;
-    const int slice = static_cast<int>(item - r * sl.S);
-    const int begin = slice * sl.cps, end = min(begin + sl.cps, nc);
-    Share<T, W, U> sh;
-    sh.place(begin + threadIdx.x, kBlock, end, in.V);
-    sh.template load<PAST>(in.x + r * in.ld);
-    if constexpr (TAIL) {
-      // (the barrier of the former item's join came after its last read)
-      for (int i = threadIdx.x; i < kWords; i += kBlock) bits[i] = 0;
-      __syncthreads();
-      if (static_cast<int>(threadIdx.x) < in.K) {
-        const int64_t j = in.index[r * in.K + threadIdx.x] - static_cast<int64_t>(begin) * W;
-        if (j >= 0 && j < static_cast<int64_t>(end - begin) * W) atomicOr(&bits[j >> 5], 1u << (j & 31));
-      }
-      __syncthreads();
+  const int slice = blockIdx.x;
+  const int64_t r = slice_row();
+  if (r >= in.n) return;
+  const int begin = slice * sl.cps, end = min(begin + sl.cps, nc);
+  Share<T, W, U> sh;
+  sh.place(begin + threadIdx.x, kBlock, end, in.V);
+  sh.template load<PAST>(in.x + r * in.ld);
+  if constexpr (TAIL) {
+    for (int i = threadIdx.x; i < kWords; i += kBlock) bits[i] = 0;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < in.K) {
+      const int64_t j = in.index[r * in.K + threadIdx.x] - static_cast<int64_t>(begin) * W;
+      if (j >= 0 && j < static_cast<int64_t>(end - begin) * W) atomicOr(&bits[j >> 5], 1u << (j & 31));
     }
+    __syncthreads();
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      mask_out<T, W>(sh.raw[u], TAIL ? kill_bits<W>(bits, threadIdx.x + u * kBlock, sh.own[u]) : (1u << sh.own[u]) - 1u);
-    float m = sh.largest(), s = 0.0f, t = 0.0f;
-    sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
-    join<kWave>(m, s, t, in.c);
-    across.run(m, s, t, in.c);
-    if constexpr (ONE) {
-      if (threadIdx.x < kWave) finish_wave<T, TAIL>(in, o, r, threadIdx.x, m, s, -1, list);
-    } else if (threadIdx.x == 0) {
-      part[item] = make_float2(s == 0.0f ? -kInf : m, s);
-    }
+  for (int u = 0; u < U; ++u)
+    mask_chunk<T, W, TAIL>(sh.raw[u], bits, threadIdx.x + u * kBlock, sh.own[u]);
+  float m = sh.largest(), s = 0.0f, t = 0.0f;
+  sh.template sums<false>(Shift(shift_of(m), in.c), s, t);
+  join<kWave, false>(m, s, t, in.c);
+  across.run<false>(m, s, t, in.c);
+  if (sl.S == 1) {
+    if (threadIdx.x < kWave) finish_wave<T, TAIL>(in, o, r, threadIdx.x, m, s, -1, list);
+  } else if (threadIdx.x == 0) {
+    part[r * sl.S + slice] = make_float2(s == 0.0f ? -kInf : m, s);
   }
 }
 
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_id(); r < in.n; r += step) {
     const float2 p = lane < S ? part[r * S + lane] : make_float2(-kInf, 0.0f);
     float m = p.x, s = p.y, t = 0.0f;
-    join<kWave>(m, s, t, in.c);
+    join<kWave, false>(m, s, t, in.c);
     finish_wave<T, TAIL>(in, o, r, lane, m, s, -1, lists[wave_id()]);
   }
 }
@@ -558,18 +561,11 @@ int forward(const char* who, hipStream_t st, const In<T>& in, const Out& o, void
   float2* part = static_cast<float2*>(workspace);
   const int rc = with_chunks<T>(sl.U, [&](auto UC) {
     constexpr int U = decltype(UC)::value;
-    const int grid = grid_of(in.n * sl.S);
-    const auto launch = [&](auto OC, auto PC) {
-      hipLaunchKernelGGL((slice_kernel<T, U, TAIL, decltype(OC)::value, decltype(PC)::value>), dim3(grid), dim3(kBlock), 0,
-                         st, in, o, sl, part);
+    const auto launch = [&](auto PC) {
+      hipLaunchKernelGGL((slice_kernel<T, U, TAIL, decltype(PC)::value>), slice_grid(sl.S, in.n), dim3(kBlock), 0, st, in,
+                         o, sl, part);
     };
-    const bool past = pass_of<T>(in.n, in.V) == kPast;
-    if (sl.S == 1) {
-      if constexpr (U <= 8)  // 16 chunks a thread are for rows of more than 64 slices
-        past ? launch(std::true_type(), std::true_type()) : launch(std::true_type(), std::false_type());
-    } else {
-      past ? launch(std::false_type(), std::true_type()) : launch(std::false_type(), std::false_type());
-    }
+    pass_of<T>(in.n, in.V) == kPast ? launch(std::true_type()) : launch(std::false_type());
     return check_launch(who);
   });
   if (rc || sl.S == 1) return rc;

@@ -30,13 +30,37 @@ constexpr int kMaxSlices = 64;  // one lane of the joining wavefront each
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kInf = __builtin_huge_valf();
+// Below this power of two a float32 exponential is zero: what a logarithm that
+// multiplies it may be raised to, so that 0 * -inf counts nothing.
+constexpr float kFloor = -256.0f;
 
 template <int N>
 using IC = std::integral_constant<int, N>;
 
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// Value `at` of a row: a 32-bit offset, so that a row of the whole wavefront's
+// keeps its address in scalar registers.
+template <typename T>
+__device__ __forceinline__ T* within(T* row, int at) {
+  using Byte = typename std::conditional<std::is_const<T>::value, const char, char>::type;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + static_cast<uint32_t>(at) * static_cast<uint32_t>(sizeof(T)));
+}
+
 // Workgroups of a launch that strides over its items.
 constexpr int64_t kMaxGrid = 1 << 20;
 inline int grid_of(int64_t items) { return static_cast<int>(items < kMaxGrid ? items : kMaxGrid); }
+// Of one with a workgroup for each of a row's S slices, which follow each other,
+// and the row of a workgroup (at or past the last one: none). No loop over
+// rows, out of which the compiler would take the masks of every chunk, at twice
+// the registers.
+constexpr int64_t kGridRows = 65535;
+inline dim3 slice_grid(int S, int64_t rows) {
+  return dim3(S, static_cast<uint32_t>(rows < kGridRows ? rows : kGridRows),
+              static_cast<uint32_t>((rows + kGridRows - 1) / kGridRows));
+}
+__device__ __forceinline__ int64_t slice_row() { return blockIdx.z * kGridRows + blockIdx.y; }
 
 // f(IC<W>, IC<LPR>, IC<U>) for rows of V values of T that a wavefront holds,
 // -1 for longer ones.
@@ -139,8 +163,11 @@ __device__ __forceinline__ void mask_out(typename RowChunk<T, W>::Raw& q, uint32
       if (kill >> w & 1) q[w] = -kInf;
   } else {
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      if (kill >> w & 1) q[w / 2] = w & 1 ? (q[w / 2] & 0xffffu) | 0xff800000u : (q[w / 2] & 0xffff0000u) | 0xff80u;
+    for (int i = 0; i < W / 2; ++i) {
+      const uint32_t lo = static_cast<int32_t>(kill << (31 - 2 * i)) >> 31, hi = static_cast<int32_t>(kill << (30 - 2 * i)) >> 31;
+      const uint32_t mask = (lo & 0xffffu) | (hi & 0xffff0000u);
+      q[i] = (q[i] & ~mask) | (0xff80ff80u & mask);
+    }
   }
 }
 
@@ -179,11 +206,12 @@ struct Share {
   int own[U];  // its own values start here (W: none)
 
   __device__ __forceinline__ void place(int first, int stride, int end, int V) {
+    const int last = min(end * W, V) - W;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = first + u * stride;
-      at[u] = chunk_start<W>(c < end ? c : end - 1, V);
-      own[u] = c < end ? c * W - at[u] : W;
+      const int i = (first + u * stride) * W;
+      at[u] = min(i, last);
+      own[u] = min(i - at[u], W);
     }
   }
   template <bool PAST = false>
@@ -191,14 +219,25 @@ struct Share {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (PAST)
-        raw[u] = X::load_past(row + at[u]);
+        raw[u] = X::load_past(within(row, at[u]));
       else
-        raw[u] = X::load(row + at[u]);
+        raw[u] = X::load(within(row, at[u]));
     }
   }
   __device__ __forceinline__ void mask_foreign() {
 #pragma unroll
-    for (int u = 0; u < U; ++u) mask_out<T, W>(raw[u], (1u << own[u]) - 1u);
+    for (int u = 0; u < U; ++u)
+      if (own[u] != 0) mask_out<T, W>(raw[u], (1u << own[u]) - 1u);
+  }
+  // f over the packed values of chunks [U0, U1) of a bf16 row.
+  template <class P, int U0, int U1, class F>
+  __device__ __forceinline__ P fold(F&& f) const {
+    P v = __builtin_bit_cast(P, static_cast<uint32_t>(raw[U0][0]));
+#pragma unroll
+    for (int u = U0; u < U1; ++u)
+#pragma unroll
+      for (int w = u == U0; w < W / 2; ++w) v = f(v, __builtin_bit_cast(P, static_cast<uint32_t>(raw[u][w])));
+    return v;
   }
   // The largest value of chunks [U0, U1); NaN may come out as itself or be
   // passed over (the sums are NaN either way).
@@ -206,22 +245,15 @@ struct Share {
   __device__ __forceinline__ float largest() const {
     if constexpr (sizeof(T) == 2 && W > 1) {
       // On the packed bits: the signed maximum is the largest value if any is
-      // positive, the unsigned minimum if none is: one instruction a value,
-      // where unpacking and a float maximum take two and a half.
-      typedef short i16x2 __attribute__((ext_vector_type(2)));
-      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-      i16x2 top = __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[U0][0]));
-      u16x2 low = __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[U0][0]));
-#pragma unroll
-      for (int u = U0; u < U1; ++u)
-#pragma unroll
-        for (int w = 0; w < W / 2; ++w) {
-          top = __builtin_elementwise_max(top, __builtin_bit_cast(i16x2, static_cast<uint32_t>(raw[u][w])));
-          low = __builtin_elementwise_min(low, __builtin_bit_cast(u16x2, static_cast<uint32_t>(raw[u][w])));
-        }
+      // positive, the unsigned minimum if none is: half an instruction a value or
+      // one, where unpacking and a float maximum take two and a half.
+      const i16x2 top = fold<i16x2, U0, U1>([](i16x2 a, i16x2 b) { return __builtin_elementwise_max(a, b); });
       const short t = top.x > top.y ? top.x : top.y;
-      const unsigned short l = low.x < low.y ? low.x : low.y;
-      const uint32_t bits = t >= 0 ? static_cast<uint32_t>(static_cast<uint16_t>(t)) : static_cast<uint32_t>(l);
+      uint32_t bits = static_cast<uint16_t>(t);
+      if (t < 0) {
+        const u16x2 low = fold<u16x2, U0, U1>([](u16x2 a, u16x2 b) { return __builtin_elementwise_min(a, b); });
+        bits = low.x < low.y ? low.x : low.y;
+      }
       return __uint_as_float(bits << 16);
     } else {
       float m = -kInf;
@@ -235,15 +267,23 @@ struct Share {
       return m;
     }
   }
-  // Adds the share's s (and t) relative to the shift.
+  // Adds the share's s (and t) relative to the shift. t needs its d raised where
+  // a class is masked; wavefronts of bf16 rows without one, which half an
+  // instruction a value tells, do without.
   template <bool WITH_T>
   __device__ __forceinline__ void sums(const Shift& sf, float& s, float& t) const {
-    if (sf.far)
-      add<WITH_T>([&](float x) { return sf.far_d(x); }, s, t);
-    else
-      add<WITH_T>([&](float x) { return sf.near_d(x); }, s, t);
+    const auto near_d = [&](float x) { return sf.near_d(x); };
+    if (sf.far) return add<WITH_T>([&](float x) { return sf.far_d(x); }, s, t);
+    if constexpr (WITH_T && sizeof(T) == 2 && W > 1) {
+      // the unsigned maximum: the lowest value, or a NaN, if any is negative
+      const u16x2 low = fold<u16x2, 0, U>([](u16x2 a, u16x2 b) { return __builtin_elementwise_max(a, b); });
+      const uint32_t bits = low.x > low.y ? low.x : low.y;
+      if (__all(near_d(__uint_as_float(bits >= 0x8000u ? bits << 16 : 0u)) > -1e30f))
+        return add<WITH_T, false>(near_d, s, t);
+    }
+    add<WITH_T>(near_d, s, t);
   }
-  template <bool WITH_T, class D>
+  template <bool WITH_T, bool MASKED = true, class D>
   __device__ __forceinline__ void add(D&& of, float& s, float& t) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -254,7 +294,7 @@ struct Share {
         const float d = of(v[w]);
         const float e = __builtin_amdgcn_exp2f(d);
         s += e;
-        if constexpr (WITH_T) t = fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf counts nothing
+        if constexpr (WITH_T) t = fmaf(e, MASKED ? fmaxf(d, kFloor) : d, t);
       }
     }
   }
@@ -263,9 +303,9 @@ struct Share {
   static __device__ __forceinline__ void store(T* row, int at, int own, const float (&v)[W]) {
     if (own == 0) {
       if constexpr (PAST)
-        X::store_past(row + at, v);
+        X::store_past(within(row, at), v);
       else
-        X::store(row + at, v);
+        X::store(within(row, at), v);
     } else if (own < W) {
 #pragma unroll
       for (int w = 0; w < W; ++w)
@@ -281,7 +321,7 @@ __device__ __forceinline__ float shift_of(float m) { return m == -kInf ? 0.0f : 
 // largest() gave it, s and t relative to shift_of(m)). m becomes the shift.
 // Every lane gets the same bits: a lane that contracted its own product into
 // the first addition would round differently from its partner.
-template <int LPR>
+template <int LPR, bool WITH_T>
 __device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
 #pragma clang fp contract(off)
   float top = m;
@@ -289,12 +329,12 @@ __device__ __forceinline__ void join(float& m, float& s, float& t, float c) {
   top = shift_of(top);
   const float d = Shift(top, c).d_of(shift_of(m));
   const float e = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(d);
-  t = s == 0.0f ? 0.0f : e * fmaf(s, fmaxf(d, -1e30f), t);
+  if constexpr (WITH_T) t = s == 0.0f ? 0.0f : e * fmaf(s, fmaxf(d, kFloor), t);
   s *= e;
   for_offsets<1, LPR>([&](auto OC) {
     constexpr int o = decltype(OC)::value;
     s += xor_shfl<o>(s);
-    t += xor_shfl<o>(t);
+    if constexpr (WITH_T) t += xor_shfl<o>(t);
   });
   m = top;
 }
@@ -307,6 +347,7 @@ struct BlockJoin {
   int turn = 0;
   __device__ explicit BlockJoin(float (*p)[3]) : slots(p) {}
 
+  template <bool WITH_T>
   __device__ __forceinline__ void run(float& m, float& s, float& t, float c) {
     static_assert(kWavesPerBlock == 4, "one quad joins the wavefronts");
     float(*p)[3] = slots + turn * kWavesPerBlock;
@@ -314,14 +355,14 @@ struct BlockJoin {
     if (lane_id() == 0) {
       p[wave_id()][0] = s == 0.0f ? -kInf : m;
       p[wave_id()][1] = s;
-      p[wave_id()][2] = t;
+      if constexpr (WITH_T) p[wave_id()][2] = t;
     }
     __syncthreads();
     const int k = lane_id() & 3;
     m = p[k][0];
     s = p[k][1];
-    t = p[k][2];
-    join<4>(m, s, t, c);  // the same in every quad
+    if constexpr (WITH_T) t = p[k][2];
+    join<4, WITH_T>(m, s, t, c);  // the same in every quad
   }
 };
 

@@ -356,6 +356,36 @@ def test_rows_far_from_zero(V):
     _check(x, labels, min(V, 4), 1.0, g, h, name="at the edge")
 
 
+def test_large_gradients_beside_masks():
+    """Gradients of the entropy of 10^9 and more, as a scaled loss or a small
+    temperature makes them: a masked class's stays 0."""
+    for V in (6, 300, 3000, 40000):
+        for dtype in (F32, BF16):
+            print(f"large gradients V={V} {dtype}", flush=True)
+            x, labels, g, h = _logits(6, V, dtype, V + 3)
+            x[:, 1::3] = -math.inf
+            x[1, 2::3] = torch.finfo(dtype).min
+            labels = torch.zeros_like(labels)
+            _check(x, labels, 0, 1.0, g * 1e9, h * 1e12, name=f"V={V}")
+            _check(x, labels, 0, 2.0 ** -6, g, h * 1e9, name=f"V={V}, small T")
+
+
+def test_more_rows_than_a_grid_dimension():
+    """131,100 rows of a slice each: the grid's second dimension ends at 65,535."""
+    from cign_amd.class_logprobs import class_logprobs
+
+    n, V = 131100, 601
+    x, labels, _, _ = _logits(n, V, BF16, 1)
+    r = class_logprobs(x, labels, top_k=3)
+    for a in (0, 65530, 131066):
+        xn, at = _n(x[a:a + 34]), labels[a:a + 34].cpu().numpy()
+        o = _oracle(xn, 1.0, at)
+        want = _top(xn, 3)
+        assert_within(_n(r.entropy[a:a + 34]), o["H"], o["e_h"], f"entropy from row {a}")
+        assert_within(_n(r.logprob[a:a + 34]), o["logprob"], o["e_logprob"], f"logprob from row {a}")
+        assert np.array_equal(r.top_index[a:a + 34].cpu().numpy(), want)
+
+
 def test_row_results_do_not_depend_on_the_call():
     """A row's values and gradient are the same in a call of its own, where
     its kernel shape is the same, and runs agree bit for bit."""

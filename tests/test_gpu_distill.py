@@ -294,6 +294,22 @@ def test_gradient_against_differences():
         assert_within(_n(got), num, 2e-6 + 1e-5 * np.abs(num), "gradient")
 
 
+def test_more_rows_than_a_grid_dimension():
+    """65,600 rows of a slice each: the grid's second dimension ends at 65,535."""
+    from cign_amd.distill import distill_topk_loss
+
+    n, V, K = 65600, 4105, 3
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(n, V, generator=gen, device="cuda", dtype=BF16)
+    index = torch.randint(0, V // K, (n, K), generator=gen, device="cuda") * K + torch.arange(K, device="cuda")
+    t = torch.log_softmax(torch.randn(n, K, generator=gen, device="cuda"), dim=1) - 0.1
+    loss = distill_topk_loss(x, t, index, tail=True)
+    for a in (0, 65520, 65580):
+        at = slice(a, a + 20)
+        el, bl, _, _ = _oracle(_n(x[at]), _n(t[at]), index[at].cpu().numpy(), 1.0, True, np.ones(20))
+        _within(_n(loss[at]), el, bl, f"loss from row {a}")
+
+
 def test_offsets_beyond_32_bits():
     from cign_amd.distill import distill_topk_loss
 
