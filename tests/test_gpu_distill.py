@@ -180,6 +180,31 @@ def test_lists(V, tail):
         assert loss[0] == 0 and not grad[0].any()
 
 
+@pytest.mark.parametrize("V", [300, 5000, 40000])
+@pytest.mark.parametrize("tail", [False, True])
+def test_repeats_in_long_lists(V, tail):
+    """Lists that name one class 128 times, some classes a few times, two places
+    one class, and none twice, among classes far apart and next to each other."""
+    for dtype in (F32, BF16):
+        for K in (64, 65, 128):
+            print(f"repeats V={V} K={K} {dtype} tail={tail}", flush=True)
+            x, t, index, g = _inputs(12, V, K, dtype, V + K, padded=0.05, mass=0.7)
+            empty = index < 0
+            index[0] = V - 1
+            index[1] = index[1] % 60
+            index[2] = index[2] % 2 * (V - 1)
+            index[3, -1], index[4, 1], index[5, 63] = index[3, 0], index[4, 0], index[5, K - 1]
+            index[6] = torch.arange(K, device="cuda") + 7
+            index[7] = torch.arange(K, device="cuda") * (V // K)
+            index[8] = torch.arange(K, device="cuda").flip(0) // 2
+            # places of one class agree on its probability
+            p = torch.zeros(12, V, device="cuda").scatter_(1, index.clamp_min(0), t.nan_to_num(nan=-9.0))
+            count = torch.zeros(12, V, device="cuda").scatter_add_(1, index.clamp_min(0), torch.ones_like(t))
+            t = (p - count.clamp_min(1).log()).gather(1, index.clamp_min(0)) - 1
+            index, t = torch.where(empty, -1, index), torch.where(empty, math.nan, t)
+            _check(x, t, index, g, 1.0, tail, f"V={V} K={K}")
+
+
 @pytest.mark.parametrize("V", [6, 300, 3000, 40000])
 @pytest.mark.parametrize("tail", [False, True])
 def test_masked_and_confident_students(V, tail):
