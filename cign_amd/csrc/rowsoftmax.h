@@ -93,28 +93,28 @@ bool wavefront_row(int V) {
 }
 
 // The slices of long rows: S a row, of cps chunks each, U chunks a thread
-// (256 U >= cps). Eight chunks a thread (128 bytes in flight: 16 took 84 us
-// where 8 took 73 over 777 x 50,001 floats with top classes, 4 took 187 where 8
-// took 130 over 2,048 x 131,072 bf16), 16 where 64 slices would not cover the
-// row, fewer while that leaves fewer than 1024 workgroups, so that few rows still
-// spread over the card.
-//
+// (256 U >= cps). Eight chunks a thread (128 bytes in flight: 777 x 50,001 floats
+// with top classes 34 us, 53 with 16 chunks and 35 with 4; 2,048 x 131,072 bf16
+// with a list 82, 86 with 4), 16 where 64 slices would not cover the row, fewer
+// while that leaves fewer than 1024 workgroups, so that few rows still spread over
+// the card.
 struct Slicing {
   int U, S, cps;
 };
 
 // How the logits and their gradient pass the 256 MB cache behind the L2s: read
 // and written through it; from 144 MiB of logits on the gradient is written past
-// it, whose lines would push the logits and each other out; from 384 MiB on,
+// it, whose lines would push the logits and each other out; from 320 MiB on,
 // where nothing is left for the next pass anyway, the logits are read past it too,
-// both ways. Measured, forward and gradient together: 256 MB of bf16 logits
-// 176 us through, 146 with the gradient past, 149 with both past; 537 MB 300,
-// 285, 275; 1.6 GB 950, 905, 810. Followed at once by a kernel that reads the
+// both ways. Measured, forward and gradient of a list's loss: 128 MiB of bf16
+// logits 75 us through, 76 with the gradient past, 80 with both past; 160 MiB 92,
+// 88, 91; 256 MiB 167, 137, 137 (of float32 161, 127, 142); 384 MiB 255, 221,
+// 201; 512 MiB 334, 300, 264; 1.5 GiB 941, 896, 835. Followed at once by a kernel that reads the
 // gradient, 160 to 200 MB take 8% less past the cache, 268 MB and more 2 to 4%
 // more.
 enum Pass : int { kThrough = 0, kWritePast = 1, kPast = 2 };
 inline Pass pass_of(int64_t bytes) {
-  return bytes >= 384ll << 20 ? kPast : bytes >= 144ll << 20 ? kWritePast : kThrough;
+  return bytes >= 320ll << 20 ? kPast : bytes >= 144ll << 20 ? kWritePast : kThrough;
 }
 template <typename T>
 Pass pass_of(int64_t n, int V) {
