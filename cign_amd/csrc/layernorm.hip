@@ -96,7 +96,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int w = 0; w < W; ++w) s[0] += w >= own[v] ? xv[v][w] : 0.0f;
-    reduce.template run<AddOp>(s);
+    reduce.sum(s);
     const float mu = s[0] * inv;
     s[0] = 0.0f;
 #pragma unroll
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void fwd_kernel(int64_t n, int
         xv[v][w] -= mu;
         s[0] += w >= own[v] ? xv[v][w] * xv[v][w] : 0.0f;
       }
-    reduce.template run<AddOp>(s);
+    reduce.sum(s);
     const float rs = 1.0f / sqrtf(s[0] * inv + eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(Shape<NT>::kThreads) void bwd_kernel(int64_t n, int
       }
     }
     if (!gx) continue;  // only the parameters' gradients are asked for
-    reduce.template run<AddOp>(s);
+    reduce.sum(s);
     const float c1 = s[0] * inv, c2 = s[1] * inv;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -352,9 +352,9 @@ int check_args(const char* who, int64_t n, int D, int x_dtype, int w_dtype) {
 }
 
 // Workgroups of the backward, its partial rows: what the card holds at a time
-// for rows of 512 threads and more (256 against 512 at 8192 bf16 columns: 171 +
-// 5 us against 176 + 9), two a CU for the others (256 was 10% slower at 1001
-// columns, 1024 12%).
+// for rows of 512 threads and more (16,384 rows of 8192 bf16 142 + 5 us, 146 + 8
+// by 512), two a CU for the others (10,007 rows of 1001 bf16 14.5 us, 17 by 256 or
+// 1024; 22,369 of 3000 69, 90 and 80).
 int bwd_blocks(int64_t n, int rows, int threads) {
   const int64_t groups = (n + rows - 1) / rows, most = threads >= 512 ? 256 : 512;
   return static_cast<int>(groups < most ? groups : most);

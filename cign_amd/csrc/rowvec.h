@@ -108,19 +108,12 @@ __device__ __forceinline__ int chunk_start(int c, int n) {
 }
 
 // ---------------------------------------------------------------------------
-// Reductions over the NT threads of a row: lanes of one wavefront (NT <= 64, a
+// Sums over the NT threads of a row: lanes of one wavefront (NT <= 64, a
 // power of two, by butterflies) or the whole workgroup (NT = 256, 512, 1024:
 // butterflies, then one LDS round). The LDS slots alternate between two sets,
 // so one barrier a reduction is enough: a thread writes a set again only after
 // the next reduction's barrier, which every reader of the former one passed.
 // ---------------------------------------------------------------------------
-struct AddOp {
-  static __device__ __forceinline__ float f(float a, float b) { return a + b; }
-};
-struct MaxOp {
-  static __device__ __forceinline__ float f(float a, float b) { return fmaxf(a, b); }
-};
-
 template <int NT, int N>
 struct GroupReduce {
   static constexpr int kWaves = NT / kWave;
@@ -128,12 +121,11 @@ struct GroupReduce {
   int turn = 0;
   __device__ explicit GroupReduce(float (*s)[N]) : slots(s) {}
 
-  template <class Op>
-  __device__ __forceinline__ void run(float (&v)[N]) {
+  __device__ __forceinline__ void sum(float (&v)[N]) {
     for_offsets<1, (NT < kWave ? NT : kWave)>([&](auto OC) {
       constexpr int o = decltype(OC)::value;
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = Op::f(v[i], xor_shfl<o>(v[i]));
+      for (int i = 0; i < N; ++i) v[i] += xor_shfl<o>(v[i]);
     });
     if constexpr (NT > kWave) {
       float (*s)[N] = slots + turn * kWaves;
@@ -146,7 +138,7 @@ struct GroupReduce {
 #pragma unroll
       for (int k = 1; k < kWaves; ++k)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = Op::f(v[i], s[k][i]);
+        for (int i = 0; i < N; ++i) v[i] += s[k][i];
       turn ^= 1;
     }
   }
