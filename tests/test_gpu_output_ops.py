@@ -158,3 +158,52 @@ def test_distillation_step_in_a_graph(tmp_path):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want)), i
+
+
+def test_calls_at_once_on_two_streams_and_in_two_graphs():
+    """Long rows (slices, joins and their workspaces) on two streams at a time,
+    then in two captured graphs replayed in turn: each has the values of a call of
+    its own."""
+    from cign_amd.class_logprobs import class_logprobs
+    from cign_amd.distill import distill_topk_loss
+    from cign_amd.fused_block_ops import fused_layernorm
+
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    sets = []
+    for V in (20011, 40000):
+        x = torch.randn(60, V, generator=gen, device="cuda")
+        index = torch.randint(0, V, (60, 128), generator=gen, device="cuda")
+        t = torch.log_softmax(torch.randn(60, 128, generator=gen, device="cuda"), dim=1)
+        sets.append((x, index[:, 0].contiguous(), t, index))
+
+    def calls(x, labels, t, index):
+        x = x.detach().requires_grad_()
+        r = class_logprobs(x, labels, top_k=20)
+        loss = distill_topk_loss(x, t, index, tail=True)
+        gx, = torch.autograd.grad([r.logprob, r.entropy, loss], x, [torch.ones_like(loss)] * 3)
+        return [*r, loss, gx, fused_layernorm(x.detach()[:, :9001])]
+
+    want = [calls(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for s, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(calls(*s))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+    del got
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(calls(*s))
+    for _ in range(3):
+        for o in outs:
+            for v in o:
+                v.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(outs, want) for a, b in zip(g, w))
