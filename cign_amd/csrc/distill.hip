@@ -118,7 +118,7 @@ __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t 
   if constexpr (TAIL) {
     const double left = list.any && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
     const double lrest =
-        q.s == 0.0f ? -kInfd : static_cast<double>(q.all.d_of(q.rest.m)) * kLn2d + (logf(q.s) - q.lz);
+        q.s == 0.0f ? -kInfd : (q.rest.origin() - q.all.origin()) * kLn2d + (logf(q.s) - q.lz);
     if (left > 0.0) loss += left * (logf(static_cast<float>(left)) - lrest);
     a = mass + left;
     cb = a * expf(static_cast<float>(lrest)) - left;

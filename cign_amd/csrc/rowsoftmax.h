@@ -193,6 +193,9 @@ struct Shift {
     if (far) return other_far ? far_d(other) : fmaf(-m, c, oc);
     return other_far ? fmaf(other, c, -mc) : oc - mc;
   }
+  // where d is taken from, for differences of two shifts that float32 may not
+  // hold: at T < log2(e) two ends of the type's range lie further apart
+  __device__ __forceinline__ double origin() const { return far ? static_cast<double>(m) * c : mc; }
 };
 
 // A thread's share of a row: U chunks at positions first, first + stride, ...

@@ -460,3 +460,37 @@ def test_operators_together():
     assert abs(loss.item() - loss64.item()) <= 1e-5 * abs(loss64.item())
     for a, e in zip(got, want):
         assert (a.double() - e).norm() <= 2e-5 * e.norm()
+
+
+@pytest.mark.parametrize("V", [6, 300, 3000, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_unlisted_classes_at_the_lowest_value(V, dtype):
+    """A mask of the type's lowest value and a list of the classes that are not
+    masked: the others lie further off, in units of log 2, than float32 holds
+    for T < log2(e), and the loss is finite."""
+    from cign_amd.distill import distill_topk_loss
+
+    for T in (1.0, 0.75, 2.0):
+        print(f"lowest outside the list V={V} {dtype} T={T}", flush=True)
+        x, t, index, g = _inputs(6, V, 4, dtype, V, padded=0.0, mass=0.8)
+        member = torch.zeros(6, V, dtype=torch.bool, device="cuda").scatter_(1, index, True)
+        x = torch.where(member, x, torch.finfo(dtype).min)
+        x[1, int((~member[1]).nonzero()[-1])] = 0.5  # one class outside the list is not masked
+        x[2, index[2, 0]] = torch.finfo(dtype).min  # a masked class in the list
+        xr = x.requires_grad_()
+        loss = distill_topk_loss(xr, t, index, T, tail=True)
+        grad, = torch.autograd.grad(loss, xr, g)
+        el, bl, _, bg = _oracle(_n(x), _n(t), index.cpu().numpy(), T, True, _n(g))
+        # T^2 times 3e38 may pass float32's largest value: infinity is its rounding
+        el = np.where(el > np.finfo(np.float32).max, np.inf, el)
+        _within(_n(loss), el, bl, f"loss V={V} T={T}")
+        # the oracle's share of a class outside the list is exp(log q - log q_rest), where 3e38 hides log 2:
+        # here the softmax of the classes outside the list
+        z, p = x.detach().double() / T, t.double().exp()
+        mass = torch.zeros_like(z).scatter_(1, index, p)
+        left = 1 - p.sum(1, keepdim=True)
+        eg = g.double()[:, None] * T * (torch.softmax(z, 1) - mass - left * torch.softmax(
+            z.masked_fill(member, -math.inf), 1))
+        eg = _n(eg)
+        _within(_n(grad), eg, bg + HALF[dtype] * (np.abs(eg) + bg) + 2.0 ** -126, f"grad V={V} T={T}")
+        assert loss[[0, 1, 3, 4, 5]].isfinite().all()
