@@ -189,8 +189,10 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
   st.total(group_sum<LPR>(listed));
   members = group_sum<LPR>(members);
   total = lanes_sum<LPR>(total);
-  // log p = t - shift
-  const double shift = total == 0.0 ? 0.0 : static_cast<double>(shift_of(list.top)) + logf(static_cast<float>(total));
+  // log p = (t - from) - norm, the difference first: a sum of both subtrahends
+  // would round norm away where all places are at -3e38
+  const double from = TAIL ? 0.0 : shift_of(list.top);
+  const double norm = total == 0.0 ? 0.0 : logf(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   for (int i = q; i < in.K; i += LPR) {
@@ -199,7 +201,7 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
     if (j >= 0 && j < in.V) {
       const double p = list_p<TAIL>(t[i], list.top, inv);
       if (p != 0.0) {
-        loss += p * (static_cast<double>(t[i]) - shift - st.logq(to_f32(row[j])));
+        loss += p * (static_cast<double>(t[i]) - from - norm - st.logq(to_f32(row[j])));
         mass += p;
       }
       at_class = p;
@@ -326,8 +328,10 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
     total = lanes_sum<kWave>(total);
   }
   st.total(listed);
-  // log p = t - shift
-  const double shift = total == 0.0 ? 0.0 : static_cast<double>(shift_of(list.top)) + logf(static_cast<float>(total));
+  // log p = (t - from) - norm, the difference first: a sum of both subtrahends
+  // would round norm away where all places are at -3e38
+  const double from = TAIL ? 0.0 : shift_of(list.top);
+  const double norm = total == 0.0 ? 0.0 : logf(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   float at_class[E];
@@ -338,7 +342,7 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
     const double p = list_p<TAIL>(t[e], list.top, inv);
     at_class[e] = static_cast<float>(p);
     if (p != 0.0) {
-      loss += p * (static_cast<double>(t[e]) - shift - st.logq(x[e]));
+      loss += p * (static_cast<double>(t[e]) - from - norm - st.logq(x[e]));
       mass += p;
     }
   }

@@ -494,3 +494,21 @@ def test_unlisted_classes_at_the_lowest_value(V, dtype):
         eg = _n(eg)
         _within(_n(grad), eg, bg + HALF[dtype] * (np.abs(eg) + bg) + 2.0 ** -126, f"grad V={V} T={T}")
         assert loss[[0, 1, 3, 4, 5]].isfinite().all()
+
+
+@pytest.mark.parametrize("V", [6, 100, 300, 40000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_renormalised_lists_far_from_zero(V, dtype):
+    """Any constant may be added to a row of the teacher's values: rows at the
+    type's lowest value and others so large that log K is below their step."""
+    for K in {4, min(V, 100)}:
+        print(f"far lists V={V} K={K} {dtype}", flush=True)
+        x, t, index, g = _inputs(8, V, K, dtype, V + K)
+        present = index >= 0
+        place = torch.arange(K, device="cuda")
+        rows = (torch.full((K,), torch.finfo(F32).min, device="cuda"), torch.full((K,), -1e30, device="cuda"),
+                torch.full((K,), 1e18, device="cuda"), torch.full((K,), 3e38, device="cuda"),
+                torch.where(place % 2 == 0, -3.4e38, -3.0e38), torch.where(place % 2 == 0, 2.0 ** 60, -math.inf))
+        for r, v in enumerate(rows):
+            t[r] = torch.where(present[r], v.to(F32), math.nan)
+        _check(x, t, index, g, 1.0, False, f"V={V} K={K}")
