@@ -14,9 +14,16 @@ _OPS = None
 def output_ops():
     """The module of the autograd nodes. Raises RuntimeError if it or the
     library is not built, or if no HIP device is visible."""
-    global _OPS
     _lib.load_library()
+    return _OPS or load_output_ops()
+
+
+def load_output_ops():
+    """The same without a device: the operators torch.ops.cign_amd.*, on meta
+    tensors."""
+    global _OPS
     if _OPS is None:
+        _lib.load_library(require_gpu=False)
         try:
             from . import _cign_ops
         except ImportError as exc:

@@ -207,3 +207,111 @@ def test_calls_at_once_on_two_streams_and_in_two_graphs():
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(outs, want) for a, b in zip(g, w))
+
+
+def _operators():
+    """name -> (function of rows, the rows' width)."""
+    from cign_amd.class_logprobs import class_logprobs
+    from cign_amd.distill import distill_topk_loss
+    from cign_amd.fused_block_ops import fused_layernorm
+
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    rn = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    w, b, t = rn(40), rn(40), torch.log_softmax(rn(6, 3), 1)
+    labels = torch.randint(0, 40, (6,), generator=gen, device="cuda")
+    index = torch.randint(0, 40, (6, 3), generator=gen, device="cuda")
+    return {
+        "norm": lambda x: fused_layernorm(x, w, b),
+        "norm, no parameters": lambda x: fused_layernorm(x),
+        "log probabilities": lambda x: class_logprobs(x, labels).logprob,
+        "entropy": lambda x: class_logprobs(x).entropy,
+        "list": lambda x: distill_topk_loss(x, t, index),
+        "list and tail": lambda x: distill_topk_loss(x, t, index, 2.0, tail=True),
+    }
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Not zero: with and without gradients, of every input that has one."""
+    import torch.autograd.forward_ad as fwd
+
+    from cign_amd.distill import distill_topk_loss
+    from cign_amd.fused_block_ops import fused_layernorm
+
+    x = torch.randn(6, 40, device="cuda")
+    tangent = torch.ones_like(x)
+    with fwd.dual_level():
+        for name, f in _operators().items():
+            for leaf in (x, x.clone().requires_grad_()):
+                dual = fwd.make_dual(leaf, tangent)
+                with pytest.raises(RuntimeError, match="jvp"):
+                    f(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                    f(dual)
+            assert f(x).isfinite().all(), name
+        w = fwd.make_dual(torch.ones(40, device="cuda"), torch.ones(40, device="cuda"))
+        for args in ((w, None), (None, w)):
+            with pytest.raises(RuntimeError, match="jvp"):
+                fused_layernorm(x, *args)
+        t = fwd.make_dual(torch.zeros(6, 3, device="cuda"), torch.ones(6, 3, device="cuda"))
+        with pytest.raises(RuntimeError, match="jvp"):
+            distill_topk_loss(x, t, torch.zeros(6, 3, dtype=torch.int64, device="cuda"))
+    for name, f in _operators().items():
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (tangent,))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: f(v).sum())(x)
+
+
+def test_traced_calls_compute():
+    """A traced call computes what the call does, on other values, with and
+    without a gradient, after a save as well; so does a graph of tensor
+    operations."""
+    import io
+
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, other = torch.randn(6, 40, device="cuda"), torch.randn(6, 40, device="cuda")
+    for name, f in _operators().items():
+        want = f(other)
+        leaf = other.clone().requires_grad_()
+        up = torch.randn_like(want)
+        grad, = torch.autograd.grad(f(leaf), leaf, up)
+        for example in (x, x.clone().requires_grad_()):
+            traced = torch.jit.trace(f, (example,))
+            buffer = io.BytesIO()
+            torch.jit.save(traced, buffer)
+            buffer.seek(0)
+            for g in (traced, torch.jit.load(buffer)):
+                assert torch.equal(g(other), want), name
+                leaf = other.clone().requires_grad_()
+                assert torch.equal(torch.autograd.grad(g(leaf), leaf, up)[0], grad), name
+        assert torch.equal(make_fx(f)(x)(other), want), name
+        if not name.startswith("norm") and name != "entropy":  # labels and lists of six rows
+            with pytest.raises(RuntimeError, match="must have shape"):
+                traced(other[:4])
+    from cign_amd.model_cign import FusedLayerNorm
+
+    norm = FusedLayerNorm(40).cuda()
+    with torch.no_grad():
+        norm.weight.normal_()
+    assert torch.equal(torch.jit.trace(norm, (x,))(other), norm(other))
+
+
+def test_memory_errors_are_torch_s():
+    """A result that no memory holds: the error other calls of torch raise."""
+    for name, f in {"norm": lambda x: _operators()["norm, no parameters"](x),
+                    "entropy": lambda x: _operators()["entropy"](x)}.items():
+        with pytest.raises(torch.OutOfMemoryError):
+            f(torch.zeros(1, 40, device="cuda").expand(1 << 44, 40))
+
+
+def test_predictions_outside_inference_mode(tmp_path):
+    """Logits of the evaluation forward are inference tensors; what is read from
+    them is not."""
+    T, model, data, op = _setup(tmp_path)
+    r = T.predict_nodes(model, data, op, top_k=2)
+    assert not any(v.is_inference() or v.requires_grad for v in r)
+    from cign_amd.distill import distill_topk_loss
+
+    x = torch.randn(300, 5, device="cuda").requires_grad_()
+    assert torch.autograd.grad(distill_topk_loss(x, r.top_logprobs, r.top_index).sum(), x)[0].isfinite().all()

@@ -141,3 +141,88 @@ def test_slices_cover_every_class_once_in_bounds(W, n):
         assert lib.cign_class_logprobs_workspace_bytes(int(W == 8), n, V, 5) == want
         long = V > 512 * W
         assert lib.cign_distill_topk_workspace_bytes(int(W == 8), n, V) == (n * S * 8 if long and S > 1 else 0)
+
+
+def _meta_operators():
+    """The operators as a trace repeats them, on meta tensors: name -> (call,
+    its tensors by name)."""
+    from cign_amd._rows import load_output_ops
+
+    load_output_ops()
+    ops = torch.ops.cign_amd
+    m = lambda *s, t=torch.float32: torch.zeros(*s, dtype=t, device="meta")
+    long = torch.int64
+    return {
+        "layernorm": (lambda x, w, b: ops.layernorm(x, w, b, 1e-5), dict(x=m(4, 6, 32), w=m(32), b=m(32))),
+        "layernorm_backward": (lambda g, x, w, s: ops.layernorm_backward(g, x, w, s, torch.float32, True, True, True),
+                               dict(g=m(4, 32), x=m(4, 32), w=m(32), s=m(2, 4))),
+        "class_logprobs": (lambda x, y: ops.class_logprobs(x, y, 3, 1.0, -100), dict(x=m(4, 6, 32), y=m(4, 6, t=long))),
+        "class_logprobs_backward": (lambda h, g, x, y, s: ops.class_logprobs_backward(h, g, x, y, s, 1.0, -100),
+                                    dict(h=m(4), g=m(4), x=m(4, 32), y=m(4, t=long), s=m(4, 4))),
+        "distill_topk": (lambda x, t, j: ops.distill_topk(x, t, j, 1.0, True),
+                         dict(x=m(4, 6, 32), t=m(4, 6, 3), j=m(4, 6, 3, t=long))),
+        "distill_topk_backward": (lambda g, x, j, s: ops.distill_topk_backward(g, x, j, s, 1.0),
+                                  dict(g=m(4), x=m(4, 32), j=m(4, 3, t=long), s=m(4 * 11))),
+    }
+
+
+def test_operators_check_what_their_accesses_rest_on():
+    """A trace repeats the operators without the Python functions' checks: a
+    tensor of another shape, type or device is refused by the operator itself."""
+    for name, (call, args) in _meta_operators().items():
+        first = next(iter(args))
+        out = call(**args)
+        out = list(out) if isinstance(out, (list, tuple)) else [out]
+        assert out[0].shape[: args[first].dim() - 1] == args[first].shape[:-1] or name.endswith("backward"), name
+        for key, t in args.items():
+            shorter = t[:-1] if key != "s" or name != "layernorm_backward" else t[:, :-1]
+            if (name, key) == ("layernorm", "x"):  # nothing else has its rows
+                shorter = t[..., :-1]
+            for bad in (shorter, t[..., None], t.double(), t.half(), torch.zeros(t.shape, dtype=t.dtype)):
+                with pytest.raises((RuntimeError, TypeError, ValueError)):
+                    call(**{**args, key: bad})
+        if "w" in args:
+            with pytest.raises((RuntimeError, TypeError, ValueError)):
+                call(**{**args, "w": args["w"].bfloat16()})
+    ops, x = torch.ops.cign_amd, torch.zeros(4, 32, device="meta")
+    for k in (-1, 33, 1 << 32):
+        with pytest.raises(ValueError, match="top_k"):
+            ops.class_logprobs(x, None, k, 1.0, -100)
+    for t in (torch.zeros(4, 0, device="meta"), torch.zeros((), device="meta")):
+        with pytest.raises(ValueError):
+            ops.layernorm(t, None, None, 1e-5)
+    with pytest.raises(ValueError, match="detach"):
+        ops.distill_topk(x, torch.zeros(4, 3, device="meta").requires_grad_(),
+                         torch.zeros(4, 3, dtype=torch.int64, device="meta"), 1.0, True)
+    for call, args in _meta_operators().values():  # on the host: no kernel
+        with pytest.raises((RuntimeError, TypeError)):
+            call(**{k: torch.zeros(t.shape, dtype=t.dtype) for k, t in args.items()})
+
+
+def test_traces_and_forward_mode_on_the_host():
+    """A trace holds the call, with and without a gradient, and a forward-mode
+    derivative raises."""
+    import torch.autograd.forward_ad as fwd
+
+    for name, (call, args) in _meta_operators().items():
+        if name.endswith("backward"):
+            continue
+        rest = {k: t for k, t in args.items() if k != "x"}
+        f = lambda x: call(x=x, **rest)
+        for x in (args["x"], args["x"].clone().requires_grad_()):
+            graph = torch.jit.trace(f, (x,), check_trace=False).graph
+            assert f"cign_amd::{name}(" in str(graph) and "aten::empty" not in str(graph)
+            with fwd.dual_level():
+                dual = fwd.make_dual(x, torch.zeros_like(args["x"]))
+                with pytest.raises(RuntimeError, match="jvp"):
+                    f(dual)
+                with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+                    f(dual)
+        for key, t in rest.items():
+            if t.is_floating_point():
+                with fwd.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+                    call(**{**args, key: fwd.make_dual(t, torch.zeros_like(t))})
+        leaf = args["x"].clone().requires_grad_()
+        out = call(**{**args, "x": leaf})
+        grad, = torch.autograd.grad(out[0].sum() if name == "class_logprobs" else out.sum(), leaf)
+        assert grad.shape == leaf.shape
