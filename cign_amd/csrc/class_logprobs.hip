@@ -58,41 +58,42 @@ struct In {
   float c, inv_t;  // log2(e) / T, 1 / T
 };
 
-__device__ __forceinline__ float logprob_of(float x, const Shift& sf, float l2s, float inv_t) {
-  const float d = sf.d(x);
-  // a class at the type's lowest value: log2 p overflows, log p may not
-  return d == -kInf ? (x - sf.m) * inv_t - l2s * kLn2 : (d - l2s) * kLn2;
+// log p of the class of logit x, ls = log s (0 for a row without a class: -inf
+// comes out). In float64, rounded once: a difference of values that may be much
+// larger, and one that float32 does not hold between the ends of its range.
+__device__ __forceinline__ float logprob_of(float x, const Shift& sf, double ls) {
+  return static_cast<float>(sf.wide_d(x) * kLn2d - ls);
 }
+__device__ __forceinline__ double log_sum(float s) { return s == 0.0f ? 0.0 : log_of(s); }
 
-// Label, entropy and statistics of row r from its joined (m, s, t); l2s is
-// what logprob_of takes, 0 for a row without a class (-inf then comes out).
+// Label, entropy and statistics of row r from its joined (m, s, t) and ls =
+// log_sum(s). The entropy's difference is float64, as log p is.
 template <typename T>
-__device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t, float& l2s) {
+__device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t, double ls) {
   const bool none = s == 0.0f;
-  l2s = none ? 0.0f : log2f(s);
-  const float H = none ? 0.0f : kLn2 * (l2s - t / s);
+  const float H = none ? 0.0f : static_cast<float>(ls - kLn2d * (static_cast<double>(t) / s));
   o.entropy[r] = H;
   if (o.label) {
     const int64_t y = o.label[r];
     float lp = 0.0f;
     if (y != o.ignore)
-      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), Shift(m, in.c), l2s, in.inv_t) : __builtin_nanf("");
+      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), Shift(m, in.c), ls) : __builtin_nanf("");
     o.logprob[r] = lp;
   }
   if (o.stats) {
     float* p = o.stats + 4 * r;
     p[0] = m;
-    p[1] = none ? kInf : l2s;
+    p[1] = none ? kInf : static_cast<float>(ls * (1.0 / kLn2d));
     p[2] = H;
   }
 }
 
 template <typename T>
 __device__ __forceinline__ void put_top(const In<T>& in, const Out& o, int64_t r, int rank, uint64_t key, float m,
-                                        float l2s) {
+                                        double ls) {
   const int i = key_index(key);
   o.top_index[r * o.K + rank] = i;
-  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), Shift(m, in.c), l2s, in.inv_t);
+  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), Shift(m, in.c), ls);
 }
 
 // The largest key below `below` of a share's own values.
@@ -214,14 +215,14 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     float m = sh.largest(), s = 0.0f, t = 0.0f;
     sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<LPR, true>(m, s, t, in.c);
-    float l2s = s == 0.0f ? 0.0f : log2f(s);
-    if (q == 0) finish(in, o, r, m, s, t, l2s);
+    const double ls = log_sum(s);
+    if (q == 0) finish(in, o, r, m, s, t, ls);
     if constexpr (TOP) {
       uint64_t mine = best_below(sh, ~0ull);
       for (int k = 0; k < o.K; ++k) {
         const uint64_t best = group_max<LPR>(mine);
         if (mine == best) {  // one lane: keys differ
-          put_top(in, o, r, k, best, m, l2s);
+          put_top(in, o, r, k, best, m, ls);
           mine = best_below(sh, best);
         }
       }
@@ -287,10 +288,10 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     }
   }
   across.run<true>(m, s, t, in.c);
-  float l2s = s == 0.0f ? 0.0f : log2f(s);
+  const double ls = log_sum(s);
   if (threadIdx.x == 0) {
     if (sl.S == 1)
-      finish(in, o, r, m, s, t, l2s);
+      finish(in, o, r, m, s, t, ls);
     else
       part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
   }
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         const int rank = count_above(cand, count, k);
         if (rank < K) {
           if (sl.S == 1)
-            put_top(in, o, r, rank, k, m, l2s);
+            put_top(in, o, r, rank, k, m, ls);
           else
             list[rank] = k;
         }
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         for (int i = 1; i < kWavesPerBlock; ++i) best = sample[i] > best ? sample[i] : best;
         if (threadIdx.x == 0) {
           if (sl.S == 1)
-            put_top(in, o, r, k, best, m, l2s);
+            put_top(in, o, r, k, best, m, ls);
           else
             list[k] = best;
         }
@@ -380,9 +381,9 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_id(); r < in.n; r += step) {
     const float4 p = lane < S ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
-    float m = p.x, s = p.y, t = p.z, l2s;
+    float m = p.x, s = p.y, t = p.z;
     join<kWave, true>(m, s, t, in.c);
-    if (lane == 0) finish(in, o, r, m, s, t, l2s);
+    if (lane == 0) finish(in, o, r, m, s, t, log_sum(s));
   }
 }
 
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       found = 0;
     }
     join<kWave, true>(m, s, t, in.c);
-    float l2s = s == 0.0f ? 0.0f : log2f(s);
+    const double ls = log_sum(s);
     __syncthreads();
     if (mine != 0 && count_above(sample, S * heads, mine) == K - 1) threshold = mine;
     __syncthreads();
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       for (int i = threadIdx.x; i < count; i += kBlock) {
         const uint64_t k = cand[i];
         const int rank = count_above(cand, count, k);
-        if (rank < K) put_top(in, o, r, rank, k, m, l2s);
+        if (rank < K) put_top(in, o, r, rank, k, m, ls);
       }
     } else if (threadIdx.x < kWave) {
       int next = 1;
@@ -448,13 +449,13 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       for (int k = 0; k < K; ++k) {
         const uint64_t best = group_max<kWave>(head);
         if (head == best) {  // one lane: keys differ
-          put_top(in, o, r, k, best, m, l2s);
+          put_top(in, o, r, k, best, m, ls);
           head = next < K ? lists[lane * K + next] : 0;
           ++next;
         }
       }
     }
-    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, l2s);
+    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, ls);
   }
 }
 

@@ -18,9 +18,13 @@
 // The forward reads the logits once (rowsoftmax.h); with the tail, listed
 // classes are marked in a bitmap in LDS and left out of the sums, which a
 // subtraction from the whole sum could not recover where the list holds nearly
-// all of the mass. What remains is K values a row, which its lanes finish in
-// float64: log p - log q is a difference of near values. The backward reads the
-// logits, writes the gradient of a class outside the list for every class, and
+// all of the mass. What remains is K values a row, which its lanes finish. log p
+// - log q is a difference of near values: the logarithms, differences, products
+// and sums over the list are float64, the logarithm of a float32 sum to 2^-24
+// (log_of), and so are the exponentials of the tail's masses, whose sum is taken
+// from one. Those of a renormalised list are float32 to 2 ulp (exp_of): an error of
+// the masses, which the backward keeps in float32 as well. The backward reads
+// the logits, writes the gradient of a class outside the list for every class, and
 // after a barrier the listed ones over it.
 #include "rowsoftmax.h"
 
@@ -54,8 +58,6 @@ struct Out {
   float* p;      // [n, K]: the teacher's mass at the place's class, over all places that name it
 };
 
-constexpr double kLn2d = 0.6931471805599453, kInfd = __builtin_huge_val();
-
 template <int LPR>
 __device__ __forceinline__ double lanes_sum(double v) {
   for_offsets<1, LPR>([&](auto OC) {
@@ -80,12 +82,6 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-// Shift::d in float64 (relative to the same rounded product).
-__device__ __forceinline__ double wide_d(const Shift& sf, float x) {
-  const double xd = x;
-  return sf.far ? (xd - sf.m) * sf.c : xd * sf.c - sf.mc;
-}
-
 // What is known of a row's list once its lanes have been through it once.
 struct ListSummary {
   float top, top_x;    // the teacher's largest value, the student's largest logit (of a listed class)
@@ -97,47 +93,50 @@ struct ListSummary {
 struct Student {
   Shift rest, all;
   float s;    // relative to `rest`
-  float lz;   // log of the sum over all classes, relative to `all`
+  double lz;  // log of the sum over all classes, relative to `all`
   bool none;  // no class left
   __device__ __forceinline__ Student(float m, float s_, float mt, float c) : rest(m, c), all(mt, c), s(s_) {}
   __device__ __forceinline__ void total(float listed) {
     const float st = listed + (s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(all.d_of(rest.m)));
     none = st == 0.0f;
-    lz = none ? 0.0f : logf(st);
+    lz = none ? 0.0 : log_of(st);
   }
-  __device__ __forceinline__ double logq(float x) const { return none ? -kInfd : wide_d(all, x) * kLn2d - lz; }
+  __device__ __forceinline__ double logq(float x) const { return none ? -kInfd : all.wide_d(x) * kLn2d - lz; }
 };
 
-// The row's loss and statistics from the sums over its list, by one lane. The
-// logarithms are float32: of sums that are known to float32, and of a remainder
-// whose relative error is.
+// e^v of a float64 difference v to 2 ulp of float32: what rounding v loses is
+// multiplied back.
+__device__ __forceinline__ double exp_of(double v) {
+  const float hi = static_cast<float>(v), e = expf(hi);
+  return hi == -kInf ? 0.0 : fmaf(e, static_cast<float>(v - hi), e);
+}
+
+// The row's loss and statistics from the sums over its list, by one lane.
 template <typename T, bool TAIL>
 __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t r, const Student& q,
                                          const ListSummary& list, float members, double loss, double mass) {
   double a = mass, cb = mass;
   if constexpr (TAIL) {
     const double left = list.any && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
-    const double lrest =
-        q.s == 0.0f ? -kInfd : (q.rest.origin() - q.all.origin()) * kLn2d + (logf(q.s) - q.lz);
-    if (left > 0.0) loss += left * (logf(static_cast<float>(left)) - lrest);
+    const double lrest = q.s == 0.0f ? -kInfd : (q.rest.origin() - q.all.origin()) * kLn2d + (log_of(q.s) - q.lz);
+    if (left > 0.0) {  // its logarithm: that of the nearest float32, and what the rounding left
+      const float l = static_cast<float>(left);
+      loss += left * (log_of(l) + static_cast<float>(left - l) / l - lrest);
+    }
     a = mass + left;
-    cb = a * expf(static_cast<float>(lrest)) - left;
+    cb = a * exp_of(lrest) - left;
   }
   if (list.bad) loss = a = cb = __builtin_nan("");
   o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
   if (o.stats)
     o.stats[r] = Stats{q.rest.m, q.s == 0.0f ? kInf : log2f(q.s), static_cast<float>(cb), q.all.m,
-                       q.none ? kInf : q.lz * kLog2e, static_cast<float>(a), {0.0f, 0.0f}};
+                       q.none ? kInf : static_cast<float>(q.lz * (1.0 / kLn2d)), static_cast<float>(a), {0.0f, 0.0f}};
 }
 
-// e^(t - top) of a list that is renormalised, to 2 ulp of float32: the
-// difference is taken in float64, what its rounding loses multiplied back. What a
-// list leaves of one (1 - sum e^t, near 0 for a confident teacher) takes the
-// exponential itself in float64.
+// e^(t - top) of a list that is renormalised. What a list leaves of one (1 - sum
+// e^t, near 0 for a confident teacher) takes the exponential itself in float64.
 __device__ __forceinline__ double list_exp(float t, float top) {
-  const double d = static_cast<double>(t) - shift_of(top);
-  const float hi = static_cast<float>(d), e = expf(hi);
-  return hi == -kInf ? 0.0 : fmaf(e, static_cast<float>(d - hi), e);
+  return exp_of(static_cast<double>(t) - shift_of(top));
 }
 
 template <bool TAIL>
@@ -192,7 +191,7 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
   // log p = (t - from) - norm, the difference first: a sum of both subtrahends
   // would round norm away where all places are at -3e38
   const double from = TAIL ? 0.0 : shift_of(list.top);
-  const double norm = total == 0.0 ? 0.0 : logf(static_cast<float>(total));
+  const double norm = total == 0.0 ? 0.0 : log_of(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   for (int i = q; i < in.K; i += LPR) {
@@ -331,7 +330,7 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
   // log p = (t - from) - norm, the difference first: a sum of both subtrahends
   // would round norm away where all places are at -3e38
   const double from = TAIL ? 0.0 : shift_of(list.top);
-  const double norm = total == 0.0 ? 0.0 : logf(static_cast<float>(total));
+  const double norm = total == 0.0 ? 0.0 : log_of(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
   double loss = 0.0, mass = 0.0;
   float at_class[E];

@@ -30,6 +30,7 @@ constexpr int kMaxSlices = 64;  // one lane of the joining wavefront each
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kInf = __builtin_huge_valf();
+constexpr double kLn2d = 0.6931471805599453, kInfd = __builtin_huge_val();
 // Below this power of two a float32 exponential is zero: what a logarithm that
 // multiplies it may be raised to, so that 0 * -inf counts nothing.
 constexpr float kFloor = -256.0f;
@@ -193,6 +194,11 @@ struct Shift {
     if (far) return other_far ? far_d(other) : fmaf(-m, c, oc);
     return other_far ? fmaf(other, c, -mc) : oc - mc;
   }
+  // d in float64 (relative to the same rounded product)
+  __device__ __forceinline__ double wide_d(float x) const {
+    const double xd = x;
+    return far ? (xd - m) * c : xd * c - mc;
+  }
   // where d is taken from, for differences of two shifts that float32 may not
   // hold: at T < log2(e) two ends of the type's range lie further apart
   __device__ __forceinline__ double origin() const { return far ? static_cast<double>(m) * c : mc; }
@@ -319,6 +325,21 @@ struct Share {
 
 // The shift of a row whose largest value is m: 0 for a row without any.
 __device__ __forceinline__ float shift_of(float m) { return m == -kInf ? 0.0f : m; }
+
+// log s of a float32 sum: the exponent's part in float64, the rest the logarithm
+// of a value in [0.7, 1.42), at most 0.35, whose float32 error is below 2^-24.
+// A float32 logarithm of the whole is off by half a step of itself, 2^-22 for s =
+// 50,001, more than the sum that it is taken of; float64 functions of the lists'
+// sums cost 24,492 x 18 with 5 places 1.8 us more, 24,492 x 1000 with 64 17.
+__device__ __forceinline__ double log_of(float s) {
+  float f = __builtin_amdgcn_frexp_mantf(s);
+  int e = __builtin_amdgcn_frexp_expf(s);
+  if (f < 0.70710678f) {
+    f += f;
+    --e;
+  }
+  return e * kLn2d + logf(f);
+}
 
 // Joins statistics over the LPR lanes of a group (one (m, s, t) a lane; m as
 // largest() gave it, s and t relative to shift_of(m)). m becomes the shift.

@@ -497,3 +497,34 @@ def test_refusals():
     grad, = torch.autograd.grad(r.logprob.pow(2).sum(), xr, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("V", [2, 3, 5, 37, 100, 129, 300, 1000, 1025, 3001, 5001, 20011, 50001, 131071])
+def test_logarithms_of_the_sums(V):
+    """Classes that are all equal: every sum is a whole number, exact in
+    float32, so log p = -log V and the entropy log V up to a logarithm's error of
+    at most 2^-24, however large it is, and half a step of the result."""
+    from cign_amd.class_logprobs import class_logprobs
+
+    want = math.log(V)
+    bound = U + float(np.spacing(np.float32(want))) / 2
+    for n in (3, 700):
+        for dtype in (F32, BF16):
+            x = torch.full((n, V), 0.75, dtype=dtype, device="cuda")
+            r = class_logprobs(x, torch.full((n,), V - 1, device="cuda"), top_k=2)
+            for v in (-r.logprob, r.entropy, -r.top_logprobs):
+                assert (v.double() - want).abs().max() <= bound, (V, n, dtype)
+
+
+def test_log_probabilities_further_off_than_float32_differences():
+    """log p = -1.5e38 at T = 4 of a class at one end of the type's range beside
+    one at the other: their difference alone overflows."""
+    from cign_amd.class_logprobs import class_logprobs
+
+    for V in (5, 300, 3000, 40000):
+        x = torch.full((2, V), -3.0e38, device="cuda")
+        x[:, 1] = 3.0e38
+        r = class_logprobs(x, torch.tensor([0, 1], device="cuda"), top_k=3, temperature=4.0)
+        assert abs(r.logprob[0].item() + 1.5e38) <= 4 * U * 1.5e38 and r.logprob[1] == 0
+        assert r.top_index[0].tolist() == [1, 0, 2] and (r.top_logprobs[:, 1:] + 1.5e38).abs().max() <= 4 * U * 1.5e38
+        assert not r.entropy.any()

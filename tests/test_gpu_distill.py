@@ -512,3 +512,30 @@ def test_renormalised_lists_far_from_zero(V, dtype):
         for r, v in enumerate(rows):
             t[r] = torch.where(present[r], v.to(F32), math.nan)
         _check(x, t, index, g, 1.0, False, f"V={V} K={K}")
+
+
+def _whole(V, n=3):
+    return torch.full((n, V), 0.75, device="cuda")
+
+
+@pytest.mark.parametrize("V", [3, 37, 100, 129, 300, 1000, 1025, 5001, 20011, 50001])
+def test_logarithms_of_the_sums(V):
+    """Classes that are all equal: every sum is a whole number, exact in
+    float32, so what is left is the logarithms' error, each at most 2^-24 (of
+    log s, however large), and the result's half step. The teacher's own
+    float32 values are what the definition takes; its masses agree with it to
+    1e-12, or to 2^-22 of themselves where they are renormalised."""
+    for K in sorted({1, min(V, 5), min(V, 100), min(V, 128)}):
+        index = torch.arange(K, device="cuda").mul(max(1, V // K)).expand(3, K).contiguous()
+        t = torch.full((3, K), -math.log(V), device="cuda")
+        from cign_amd.distill import distill_topk_loss
+
+        p, t0 = math.exp(t[0, 0].item()), t[0, 0].item()
+        left = 0.0 if K == V else 1.0 - K * p
+        want = K * p * (t0 + math.log(V)) + (left * (math.log(left) - math.log((V - K) / V)) if left else 0.0)
+        got = distill_topk_loss(_whole(V), t, index, tail=True)
+        assert (got.double() - want).abs().max() <= 2 * U * K * p + 4 * U * left + U * abs(want), (V, K)
+        want = math.log(V) - math.log(K)
+        got = distill_topk_loss(_whole(V), t, index)
+        half = float(np.spacing(np.float32(max(want, 1.0)))) / 2
+        assert (got.double() - want).abs().max() <= 2 * U + half + 2.0 ** -22 * want, (V, K)
