@@ -12,8 +12,8 @@
 // passes with the statistics a gradient takes and the gradients: a trace, or
 // another mode that records operators, records the calls and not the allocations
 // in them, and transforms that have no rule for them refuse. The autograd key's
-// kernel applies the node whether or not a gradient is needed, so that a
-// forward-mode derivative of any input raises. A trace repeats a call without the
+// kernel applies the node where a gradient is needed or an input has a
+// forward-mode derivative, which the node refuses. A trace repeats a call without the
 // checks of the Python functions, with other shapes if it likes, so what a
 // kernel's accesses rest on is checked here.
 //
@@ -97,6 +97,10 @@ void check_beside(const Tensor& t, const Tensor& x, const char* name, at::Scalar
   TORCH_CHECK_VALUE(t.sizes() == shape, name, " must have shape ", shape, ", got ", t.sizes());
   TORCH_CHECK_VALUE(t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
 }
+
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+
+bool has_tangent(const Optional& t) { return t && has_tangent(*t); }
 
 // A gradient that a graph was asked for: differentiating it raises.
 variable_list sealed(variable_list grads, const char* name) {
@@ -228,8 +232,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layernorm_autograd(const Tensor& x, const Optional& weight, const Optional& bias, double eps) {
-  const bool needed = x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad());
-  return LayerNorm::apply(x, optional(whole(weight)), optional(whole(bias)), eps, needed && at::GradMode::is_enabled());
+  const bool graph = at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) ||
+                                                    (bias && bias->requires_grad()));
+  if (!graph && !has_tangent(x) && !has_tangent(weight) && !has_tangent(bias)) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call_layernorm(x, weight, bias, eps);
+  }
+  return LayerNorm::apply(x, optional(whole(weight)), optional(whole(bias)), eps, graph);
 }
 
 // ---- log probabilities -------------------------------------------------------
@@ -337,7 +346,12 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
 variable_list class_logprobs_autograd(const Tensor& x, const Optional& labels, int64_t top_k, double temperature,
                                       int64_t ignore_index) {
-  return Logprobs::apply(x, labels, top_k, temperature, ignore_index, x.requires_grad() && at::GradMode::is_enabled());
+  const bool graph = at::GradMode::is_enabled() && x.requires_grad();
+  if (!graph && !has_tangent(x)) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call_class_logprobs(x, labels, top_k, temperature, ignore_index);
+  }
+  return Logprobs::apply(x, labels, top_k, temperature, ignore_index, graph);
 }
 
 // ---- distillation ------------------------------------------------------------
@@ -436,7 +450,12 @@ Tensor distill_topk_autograd(const Tensor& x, const Tensor& teacher, const Tenso
                              bool tail) {
   const bool grad = at::GradMode::is_enabled();
   TORCH_CHECK_VALUE(!(grad && teacher.requires_grad()), "teacher_logprobs is a constant of the loss: detach it");
-  return Distill::apply(x, teacher, index, temperature, tail, grad && x.requires_grad());
+  const bool graph = grad && x.requires_grad();
+  if (!graph && !has_tangent(x) && !has_tangent(teacher)) {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return call_distill_topk(x, teacher, index, temperature, tail);
+  }
+  return Distill::apply(x, teacher, index, temperature, tail, graph);
 }
 
 // ---- the operators -------------------------------------------------------------

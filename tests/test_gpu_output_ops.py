@@ -315,3 +315,15 @@ def test_predictions_outside_inference_mode(tmp_path):
 
     x = torch.randn(300, 5, device="cuda").requires_grad_()
     assert torch.autograd.grad(distill_topk_loss(x, r.top_logprobs, r.top_index).sum(), x)[0].isfinite().all()
+
+
+def test_transforms_agree_or_refuse():
+    """vmap over rows of rows: the values of the calls one by one, or an error."""
+    xs = torch.randn(3, 6, 40, device="cuda")
+    for name, f in _operators().items():
+        want = torch.stack([f(x) for x in xs])
+        try:
+            got = torch.func.vmap(f)(xs)
+        except RuntimeError:
+            continue
+        assert torch.equal(got, want), name
