@@ -9,6 +9,9 @@
 //   with the tail:  p_i = e^(listed value), r = max(0, 1 - sum p) and q_rest =
 //     the mass q leaves outside the list,
 //     loss = T^2 [sum_i p_i (log p_i - log q_i) + r (log r - log q_rest)].
+// The sums over i are over places: places that name one class count with their
+// masses each, sum p_i log(P / p_i) below the term of their joined mass P, a constant
+// of the logits. q_rest and the gradient's p_j are of classes.
 // With A = sum p + r, the gradient of x_j is g T (A q_j - p_j) for a listed
 // class and g T (A q_rest - r) q_j / q_rest for the others (r = 0, q_rest = 1
 // for a renormalised list): one exponential a class, relative to the statistics
@@ -204,9 +207,11 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
         mass += p;
       }
       at_class = p;
-      if (o.p && again)
+      if (o.p && again) {  // in the list's order: places of one class get the same bits
+        at_class = 0.0;
         for (int k = 0; k < in.K; ++k)
-          if (k != i && index[k] == j) at_class += list_p<TAIL>(t[k], list.top, inv);
+          if (index[k] == j) at_class += list_p<TAIL>(t[k], list.top, inv);
+      }
     }
     if (o.p) o.p[r * in.K + i] = static_cast<float>(at_class);
   }

@@ -33,9 +33,13 @@ def distill_topk_loss(logits, teacher_logprobs, teacher_index, temperature=1.0, 
 
     A negative index marks an empty place, whose teacher_logprobs is not
     looked at. A row without a listed class has loss 0 and no gradient; an
-    index of V or more makes its row's loss and gradient NaN. A class named
-    twice counts with both masses. The loss's gradient is that of the logits
-    (their type, once differentiable); the teacher's tensors are constants."""
+    index of V or more makes its row's loss and gradient NaN. The divergence is
+    summed over places, p_i (log p_i - log q of the place's class): a class named
+    twice counts with both masses, place by place, which is less than the KL of
+    its joined mass P by the sum of p_i log(P / p_i) over its places (the loss may
+    be negative then) and has the same gradient. The loss's gradient is that of
+    the logits (their type, once differentiable); the teacher's tensors are
+    constants."""
     check_rows(logits, "logits", MAX_CLASSES)
     if not isinstance(teacher_logprobs, torch.Tensor) or teacher_logprobs.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("teacher_logprobs must be a float32 or bfloat16 tensor")

@@ -406,6 +406,8 @@ int64_t cign_distill_topk_workspace_bytes(int32_t dtype, int64_t n, int32_t V);
  * the same temperature. tail 0: p is the list renormalised; 1: the mass the
  * list leaves, max(0, 1 - sum e^teacher_logprob), is one more class, all
  * classes outside the list together (none where the list names every class).
+ * The sum is over places: a class named twice counts with both masses, place by
+ * place, by sum p_i log(P / p_i) less than its joined mass P would.
  * A row without a listed class has loss 0. stats [n, 8] and teacher_mass
  * [n, K], float32, both or neither, are what the backward reads. No
  * counterpart in the reference, which trains on labels alone

@@ -539,3 +539,28 @@ def test_logarithms_of_the_sums(V):
         got = distill_topk_loss(_whole(V), t, index)
         half = float(np.spacing(np.float32(max(want, 1.0)))) / 2
         assert (got.double() - want).abs().max() <= 2 * U + half + 2.0 ** -22 * want, (V, K)
+
+
+@pytest.mark.parametrize("V", [5, 100, 300, 40000])
+def test_a_class_named_twice_counts_place_by_place(V):
+    """Sum over places of p_i (log p_i - log q of its class): below the KL of
+    the joined masses by sum p_i log(mass of the class / p_i), a constant of the
+    logits, so the gradient is that of the joined masses."""
+    from cign_amd.distill import distill_topk_loss
+
+    x = torch.zeros(3, V, device="cuda")
+    x[:, 2] = 60.0  # sure of the class, up to e^-60
+    index = torch.full((3, 2), 2, device="cuda")
+    t = torch.log(torch.tensor([[0.5, 0.5], [0.25, 0.75], [0.125, 0.25]], device="cuda"))
+    loss = distill_topk_loss(x, t, index, temperature=2.0)
+    p = torch.tensor([[0.5, 0.5], [0.25, 0.75], [1 / 3, 2 / 3]], dtype=torch.float64, device="cuda")
+    lq = torch.log_softmax(x.double() / 2, 1)[:, 2]
+    want = 4 * ((p * p.log()).sum(1) - lq)
+    assert (loss.double() - want).abs().max() <= 4 * 2.0 ** -22
+    one, joined = (v.clone().requires_grad_() for v in (x, x))
+    g = torch.ones(3, device="cuda")
+    a, = torch.autograd.grad(distill_topk_loss(one, t, index, 2.0, tail=True), one, g)
+    b, = torch.autograd.grad(distill_topk_loss(joined, t.exp().sum(1, keepdim=True).log(), index[:, :1], 2.0, tail=True),
+                             joined, g)
+    # the masses agree to 2^-22 of themselves; 2 is the temperature
+    assert (a.double() - b.double()).abs().max() <= 2 * 2 * 2.0 ** -22
