@@ -325,7 +325,8 @@ def distill_one_epoch(model, data, graph_operator, optimizer, device: torch.devi
     """train_one_epoch against labels and a teacher: the loss is (1 - weight)
     times the cross-entropy over the train mask plus weight times the mean over
     all nodes of distill_topk_loss (with the tail: the classes outside a node's
-    list as one more). Returns the loss and the step's seconds."""
+    list as one more); a part of weight 0 is left out, so that weight = 1 needs no
+    labelled node. Returns the loss and the step's seconds."""
     if not 0.0 <= float(weight) <= 1.0:
         raise ValueError(f"weight must be in [0, 1], got {weight}")
     model.train()
@@ -336,11 +337,15 @@ def distill_one_epoch(model, data, graph_operator, optimizer, device: torch.devi
     start.record()
     optimizer.zero_grad()
     logits = forward_model(model, data, graph_operator)
-    # nodes outside the mask are ignored, without gathering logits
-    labels = torch.where(data.train_mask, data.y, -100)
-    ce = -class_logprobs(logits, labels).logprob.sum() / data.train_mask.sum()
-    kl = distill_topk_loss(logits, targets.logprobs, targets.index, targets.temperature, tail).mean()
-    loss = (1.0 - weight) * ce + weight * kl
+    parts = []
+    if weight < 1.0:
+        # nodes outside the mask are ignored, without gathering logits
+        labels = torch.where(data.train_mask, data.y, -100)
+        ce = -class_logprobs(logits, labels).logprob.sum() / data.train_mask.sum()
+        parts.append((1.0 - weight) * ce)
+    if weight > 0.0:
+        parts.append(weight * distill_topk_loss(logits, targets.logprobs, targets.index, targets.temperature, tail).mean())
+    loss = sum(parts[1:], parts[0])
     if grad_scaler is not None and grad_scaler.is_enabled():
         grad_scaler.scale(loss).backward()
         grad_scaler.step(optimizer)

@@ -327,3 +327,22 @@ def test_transforms_agree_or_refuse():
         except RuntimeError:
             continue
         assert torch.equal(got, want), name
+
+
+def test_distillation_without_labelled_nodes(tmp_path):
+    """weight = 1 leaves the labels out, also where no node has one; weight = 0
+    leaves the lists out."""
+    T, model, data, op = _setup(tmp_path, seed=1)
+    targets = T.teacher_targets(model, data, op, top_k=3)
+    opt = torch.optim.SGD(model.parameters(), lr=0.0)
+    step = lambda weight: T.distill_one_epoch(model, data, op, opt, torch.device("cuda"), targets, weight=weight)[0]
+    both = step(0.25), step(0.0), step(1.0)
+    # 300 float32 terms below 20, as in test_distillation_steps
+    assert abs(both[0] - 0.75 * both[1] - 0.25 * both[2]) <= 1e-5 * max(1.0, abs(both[0]))
+    mask = data.train_mask
+    data.train_mask = torch.zeros_like(mask)
+    assert step(1.0) == both[2]
+    assert all(p.grad is None or p.grad.isfinite().all() for p in model.parameters())
+    data.train_mask = mask
+    targets.index[:] = data.y[:, None].new_full(targets.index.shape, 5)  # out of range: a loss of NaN
+    assert step(0.0) == both[1] and step(0.5) != step(0.5)
