@@ -3,6 +3,7 @@ distill_topk_loss): what the C-ABI and the Python functions refuse before any
 launch, workspace sizes, and the places the row kernels read."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -226,3 +227,52 @@ def test_traces_and_forward_mode_on_the_host():
         out = call(**{**args, "x": leaf})
         grad, = torch.autograd.grad(out[0].sum() if name == "class_logprobs" else out.sum(), leaf)
         assert grad.shape == leaf.shape
+
+
+def _owners(V, W, first, stride, end, threads, U):
+    """How often each value of a row of V is some thread's own: Share::place of
+    `threads` threads whose chunks lie `stride` apart from `first` on, below
+    chunk `end`; every access inside the row."""
+    i = (first + np.arange(threads)[:, None] + stride * np.arange(U)[None, :]) * W
+    at = np.minimum(i, min(end * W, V) - W)
+    own = np.minimum(i - at, W)
+    assert at.min() >= 0 and at.max() + W <= V
+    value = at[..., None] + np.arange(W)
+    return np.bincount(value[np.arange(W) >= own[..., None]], minlength=V)
+
+
+def _ragged():
+    """Widths at, just below and just past what chunks, slices and their numbers
+    of chunks a thread end at."""
+    edges = {512, 1024, 2048, 4096, 8192, 16384, 32768, 50001, 65536, 131072, 300007, 524288, 1 << 20}
+    return sorted(v for e in edges for v in (e - 9, e - 1, e, e + 1, e + 3, e + 4, e + 9) if v <= 1 << 20)
+
+
+@pytest.mark.parametrize("W", [4, 8])
+@pytest.mark.parametrize("n", [1, 3, 100, 5000])
+def test_each_value_of_a_sliced_row_has_one_owner(W, n):
+    """slice_kernel of both operators, as rowsoftmax.h places it."""
+    for V in _ragged():
+        U, S, cps = _slicing(V, n, W)
+        nc = -(-V // W)
+        count = sum(_owners(V, W, s * cps, 256, min((s + 1) * cps, nc), 256, U) for s in range(S))
+        assert (count == 1).all(), (V, np.flatnonzero(count != 1)[:5])
+
+
+@pytest.mark.parametrize("W", [4, 8])
+def test_each_value_of_a_gradient_has_one_owner(W):
+    """grad_kernel: slices of 32 values a thread, and the rows of lane groups."""
+    for V in _ragged() + list(range(1, 600)):
+        nc = -(-V // W)
+        if nc > 512:
+            U = 32 // W
+            S = -(-nc // (256 * U))
+            cps = -(-nc // S)
+            count = sum(_owners(V, W, s * cps, 256, min((s + 1) * cps, nc), 256, U) for s in range(S))
+        else:  # with_lanes
+            w = W if V >= W else 1
+            chunks = -(-V // w)
+            lanes = min(64, 1 << (chunks - 1).bit_length())
+            U = 1 << (-(-chunks // lanes) - 1).bit_length()
+            count = _owners(V, w, 0, lanes, chunks, lanes, U)
+        assert (count == 1).all(), (V, np.flatnonzero(count != 1)[:5])
