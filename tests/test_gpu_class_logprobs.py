@@ -528,3 +528,17 @@ def test_log_probabilities_further_off_than_float32_differences():
         assert abs(r.logprob[0].item() + 1.5e38) <= 4 * U * 1.5e38 and r.logprob[1] == 0
         assert r.top_index[0].tolist() == [1, 0, 2] and (r.top_logprobs[:, 1:] + 1.5e38).abs().max() <= 4 * U * 1.5e38
         assert not r.entropy.any()
+
+
+def test_zero_rows():
+    from cign_amd.class_logprobs import class_logprobs
+
+    for V in (7, 300, 40000):
+        x = torch.empty(0, V, device="cuda").requires_grad_()
+        labels = torch.empty(0, dtype=torch.int64, device="cuda")
+        r = class_logprobs(x, labels, top_k=2)
+        assert r.logprob.shape == (0,) and r.top_logprobs.shape == (0, 2)
+        e = torch.empty(0, device="cuda")
+        for outs in ([r.logprob, r.entropy], [r.logprob], [r.entropy]):
+            grad, = torch.autograd.grad(outs, x, [e] * len(outs), retain_graph=True)
+            assert grad.shape == x.shape

@@ -564,3 +564,15 @@ def test_a_class_named_twice_counts_place_by_place(V):
                              joined, g)
     # the masses agree to 2^-22 of themselves; 2 is the temperature
     assert (a.double() - b.double()).abs().max() <= 2 * 2 * 2.0 ** -22
+
+
+def test_zero_rows():
+    from cign_amd.distill import distill_topk_loss
+
+    for V in (7, 300, 40000):
+        x = torch.empty(0, V, device="cuda").requires_grad_()
+        loss = distill_topk_loss(x, torch.empty(0, 2, device="cuda"), torch.empty(0, 2, dtype=torch.int64, device="cuda"))
+        grad, = torch.autograd.grad(loss, x, torch.empty(0, device="cuda"))
+        assert loss.shape == (0,) and grad.shape == x.shape
+        assert torch.autograd.grad(distill_topk_loss(x, torch.empty(0, 2, device="cuda"), torch.empty(
+            0, 2, dtype=torch.int32, device="cuda"), tail=True).sum(), x)[0].shape == x.shape
