@@ -56,44 +56,49 @@ struct In {
   const T* x;
   int64_t ld;
   float c, inv_t;  // log2(e) / T, 1 / T
+  double c_ln2;    // c ln 2
 };
 
-// log p of the class of logit x, ls = log s (0 for a row without a class: -inf
-// comes out). In float64, rounded once: a difference of values that may be much
-// larger, and one that float32 does not hold between the ends of its range.
-__device__ __forceinline__ float logprob_of(float x, const Shift& sf, double ls) {
-  return static_cast<float>(sf.wide_d(x) * kLn2d - ls);
-}
+// log p and the entropy are float64 differences of values that may be much larger,
+// rounded once. A row without a class has log s = 0, so that -inf comes out.
 __device__ __forceinline__ double log_sum(float s) { return s == 0.0f ? 0.0 : log_of(s); }
-
-// Label, entropy and statistics of row r from its joined (m, s, t) and ls =
-// log_sum(s). The entropy's difference is float64, as log p is.
 template <typename T>
-__device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t, double ls) {
+__device__ __forceinline__ LogProb log_prob(const In<T>& in, float m, double log_s) {
+  return LogProb(Shift(m, in.c), in.c_ln2, log_s);
+}
+
+// Label, entropy and statistics of row r from its joined (m, s, t) and log s.
+template <typename T>
+__device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t,
+                                       double log_s) {
   const bool none = s == 0.0f;
-  const float H = none ? 0.0f : static_cast<float>(ls - kLn2d * (static_cast<double>(t) / s));
+  // t / s: a float32 reciprocal and one step in float64
+  const double inv = __builtin_amdgcn_rcpf(s), first = t * inv;
+  const double mean = fma(fma(-first, static_cast<double>(s), static_cast<double>(t)), inv, first);
+  const float H = none ? 0.0f : static_cast<float>(log_s - kLn2d * mean);
   o.entropy[r] = H;
   if (o.label) {
     const int64_t y = o.label[r];
     float lp = 0.0f;
     if (y != o.ignore)
-      lp = y >= 0 && y < in.V ? logprob_of(to_f32(in.x[r * in.ld + y]), Shift(m, in.c), ls) : __builtin_nanf("");
+      lp = y >= 0 && y < in.V ? static_cast<float>(log_prob(in, m, log_s)(to_f32(in.x[r * in.ld + y])))
+                              : __builtin_nanf("");
     o.logprob[r] = lp;
   }
   if (o.stats) {
     float* p = o.stats + 4 * r;
     p[0] = m;
-    p[1] = none ? kInf : static_cast<float>(ls * (1.0 / kLn2d));
+    p[1] = none ? kInf : static_cast<float>(log_s * (1.0 / kLn2d));
     p[2] = H;
   }
 }
 
 template <typename T>
-__device__ __forceinline__ void put_top(const In<T>& in, const Out& o, int64_t r, int rank, uint64_t key, float m,
-                                        double ls) {
+__device__ __forceinline__ void put_top(const In<T>& in, const Out& o, int64_t r, int rank, uint64_t key,
+                                        const LogProb& log_p) {
   const int i = key_index(key);
   o.top_index[r * o.K + rank] = i;
-  o.top_logprob[r * o.K + rank] = logprob_of(to_f32(in.x[r * in.ld + i]), Shift(m, in.c), ls);
+  o.top_logprob[r * o.K + rank] = static_cast<float>(log_p(to_f32(in.x[r * in.ld + i])));
 }
 
 // The largest key below `below` of a share's own values.
@@ -215,14 +220,15 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     float m = sh.largest(), s = 0.0f, t = 0.0f;
     sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<LPR, true>(m, s, t, in.c);
-    const double ls = log_sum(s);
-    if (q == 0) finish(in, o, r, m, s, t, ls);
+    const double log_s = log_sum(s);
+    if (q == 0) finish(in, o, r, m, s, t, log_s);
     if constexpr (TOP) {
+      const LogProb log_p = log_prob(in, m, log_s);
       uint64_t mine = best_below(sh, ~0ull);
       for (int k = 0; k < o.K; ++k) {
         const uint64_t best = group_max<LPR>(mine);
         if (mine == best) {  // one lane: keys differ
-          put_top(in, o, r, k, best, m, ls);
+          put_top(in, o, r, k, best, log_p);
           mine = best_below(sh, best);
         }
       }
@@ -288,10 +294,9 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
     }
   }
   across.run<true>(m, s, t, in.c);
-  const double ls = log_sum(s);
   if (threadIdx.x == 0) {
     if (sl.S == 1)
-      finish(in, o, r, m, s, t, ls);
+      finish(in, o, r, m, s, t, log_sum(s));
     else
       part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
   }
@@ -342,7 +347,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         const int rank = count_above(cand, count, k);
         if (rank < K) {
           if (sl.S == 1)
-            put_top(in, o, r, rank, k, m, ls);
+            put_top(in, o, r, rank, k, log_prob(in, m, log_sum(s)));
           else
             list[rank] = k;
         }
@@ -362,7 +367,7 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
         for (int i = 1; i < kWavesPerBlock; ++i) best = sample[i] > best ? sample[i] : best;
         if (threadIdx.x == 0) {
           if (sl.S == 1)
-            put_top(in, o, r, k, best, m, ls);
+            put_top(in, o, r, k, best, log_prob(in, m, log_sum(s)));
           else
             list[k] = best;
         }
@@ -419,7 +424,8 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       found = 0;
     }
     join<kWave, true>(m, s, t, in.c);
-    const double ls = log_sum(s);
+    const double log_s = log_sum(s);
+    const LogProb log_p = log_prob(in, m, log_s);
     __syncthreads();
     if (mine != 0 && count_above(sample, S * heads, mine) == K - 1) threshold = mine;
     __syncthreads();
@@ -441,7 +447,7 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       for (int i = threadIdx.x; i < count; i += kBlock) {
         const uint64_t k = cand[i];
         const int rank = count_above(cand, count, k);
-        if (rank < K) put_top(in, o, r, rank, k, m, ls);
+        if (rank < K) put_top(in, o, r, rank, k, log_p);
       }
     } else if (threadIdx.x < kWave) {
       int next = 1;
@@ -449,13 +455,13 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
       for (int k = 0; k < K; ++k) {
         const uint64_t best = group_max<kWave>(head);
         if (head == best) {  // one lane: keys differ
-          put_top(in, o, r, k, best, m, ls);
+          put_top(in, o, r, k, best, log_p);
           head = next < K ? lists[lane * K + next] : 0;
           ++next;
         }
       }
     }
-    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, ls);
+    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, log_s);
   }
 }
 
@@ -529,6 +535,12 @@ int check_args(const char* who, int dtype, int64_t n, int V, int64_t ld, float t
   if (ld < 0) return set_error(kInvalid, "%s: negative row stride", who);
   if (!(temperature > 0.0f && temperature < kInf)) return set_error(kInvalid, "%s: temperature must be positive", who);
   return kOk;
+}
+
+template <typename T>
+In<T> input(int64_t n, int V, const void* x, int64_t ld, float temperature) {
+  const float c = kLog2e / temperature;
+  return In<T>{n, V, static_cast<const T*>(x), ld, c, 1.0f / temperature, c * kLn2d};
 }
 
 // Whether slices take the row: longer than a wavefront holds, or than its
@@ -620,7 +632,7 @@ int cign_class_logprobs_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, c
   const Out o{label, ignore_index, logprob, entropy, stats, top_k, top_logprob, top_index};
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const In<T> in{n, V, static_cast<const T*>(x), x_stride, kLog2e / temperature, 1.0f / temperature};
+    const In<T> in = input<T>(n, V, x, x_stride, temperature);
     return forward(who, static_cast<hipStream_t>(stream), in, o, workspace, workspace_bytes);
   });
 }
@@ -636,7 +648,7 @@ int cign_class_logprobs_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, c
   hipStream_t st = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    const In<T> in{n, V, static_cast<const T*>(x), x_stride, kLog2e / temperature, 1.0f / temperature};
+    const In<T> in = input<T>(n, V, x, x_stride, temperature);
     const auto launch = [&](auto WC, auto LC, auto UC, int S, int cps) {
       constexpr int W = decltype(WC)::value, LPR = decltype(LC)::value, U = decltype(UC)::value;
       constexpr int kRows = kBlock / LPR;

@@ -41,7 +41,8 @@ struct In {
   int V;
   const T* x;
   int64_t ld;
-  float c;  // log2(e) / T
+  float c;       // log2(e) / T
+  double c_ln2;  // c ln 2
   double temperature;
   int K;
   const float* t;        // [n, K]
@@ -95,16 +96,17 @@ struct ListSummary {
 // (TAIL; over all classes otherwise) and the listed logits' sum.
 struct Student {
   Shift rest, all;
-  float s;    // relative to `rest`
-  double lz;  // log of the sum over all classes, relative to `all`
-  bool none;  // no class left
+  float s;       // relative to `rest`
+  double log_s;  // of the sum over all classes, relative to the exact product m c of `all` (LogProb::base)
+  bool none;     // no class left
   __device__ __forceinline__ Student(float m, float s_, float mt, float c) : rest(m, c), all(mt, c), s(s_) {}
   __device__ __forceinline__ void total(float listed) {
     const float st = listed + (s == 0.0f ? 0.0f : s * __builtin_amdgcn_exp2f(all.d_of(rest.m)));
     none = st == 0.0f;
-    lz = none ? 0.0 : log_of(st);
+    log_s = (none ? 0.0 : log_of(st)) + all.rounding() * kLn2d;
   }
-  __device__ __forceinline__ double logq(float x) const { return none ? -kInfd : all.wide_d(x) * kLn2d - lz; }
+  // (no class left: every logit is -inf, and so is log q)
+  __device__ __forceinline__ LogProb log_q(double c_ln2) const { return LogProb(all.m, c_ln2, log_s); }
 };
 
 // e^v of a float64 difference v to 2 ulp of float32: what rounding v loses is
@@ -121,7 +123,7 @@ __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t 
   double a = mass, cb = mass;
   if constexpr (TAIL) {
     const double left = list.any && members < in.V ? fmax(0.0, 1.0 - mass) : 0.0;
-    const double lrest = q.s == 0.0f ? -kInfd : (q.rest.origin() - q.all.origin()) * kLn2d + (log_of(q.s) - q.lz);
+    const double lrest = q.s == 0.0f ? -kInfd : (q.rest.origin() - q.all.exact()) * kLn2d + (log_of(q.s) - q.log_s);
     if (left > 0.0) {  // its logarithm: that of the nearest float32, and what the rounding left
       const float l = static_cast<float>(left);
       loss += left * (log_of(l) + static_cast<float>(left - l) / l - lrest);
@@ -133,7 +135,7 @@ __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t 
   o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
   if (o.stats)
     o.stats[r] = Stats{q.rest.m, q.s == 0.0f ? kInf : log2f(q.s), static_cast<float>(cb), q.all.m,
-                       q.none ? kInf : static_cast<float>(q.lz * (1.0 / kLn2d)), static_cast<float>(a), {0.0f, 0.0f}};
+                       q.none ? kInf : static_cast<float>(q.log_s * (1.0 / kLn2d) - q.all.rounding()), static_cast<float>(a), {0.0f, 0.0f}};
 }
 
 // e^(t - top) of a list that is renormalised. What a list leaves of one (1 - sum
@@ -196,6 +198,7 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
   const double from = TAIL ? 0.0 : shift_of(list.top);
   const double norm = total == 0.0 ? 0.0 : log_of(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
+  const LogProb log_q = st.log_q(in.c_ln2);
   double loss = 0.0, mass = 0.0;
   for (int i = q; i < in.K; i += LPR) {
     const int64_t j = index[i];
@@ -203,7 +206,7 @@ __device__ void finish(const In<T>& in, const Out& o, int64_t r, int q, float m,
     if (j >= 0 && j < in.V) {
       const double p = list_p<TAIL>(t[i], list.top, inv);
       if (p != 0.0) {
-        loss += p * (static_cast<double>(t[i]) - from - norm - st.logq(to_f32(row[j])));
+        loss += p * (static_cast<double>(t[i]) - from - norm - log_q(to_f32(row[j])));
         mass += p;
       }
       at_class = p;
@@ -337,6 +340,7 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
   const double from = TAIL ? 0.0 : shift_of(list.top);
   const double norm = total == 0.0 ? 0.0 : log_of(static_cast<float>(total));
   const double inv = total == 0.0 ? 1.0 : 1.0 / total;
+  const LogProb log_q = st.log_q(in.c_ln2);
   double loss = 0.0, mass = 0.0;
   float at_class[E];
 #pragma unroll
@@ -346,7 +350,7 @@ __device__ __forceinline__ void finish_places(const In<T>& in, const Out& o, int
     const double p = list_p<TAIL>(t[e], list.top, inv);
     at_class[e] = static_cast<float>(p);
     if (p != 0.0) {
-      loss += p * (static_cast<double>(t[e]) - from - norm - st.logq(x[e]));
+      loss += p * (static_cast<double>(t[e]) - from - norm - log_q(x[e]));
       mass += p;
     }
   }
@@ -402,8 +406,10 @@ __device__ __forceinline__ void mask_chunk(typename RowChunk<T, W>::Raw& raw, co
 // 933 with every place looking for others). 24,492 x 18 float32 with 5 places
 // 6.2 us, 24,492 x 1000 bf16 with 64 31 us: what they read takes 0.7 and 14 us,
 // the rest is the dependent loads of the list and its logits, and its sums.
+// Eight float32 chunks a lane are held to three wavefronts a SIMD, the tail's one
+// register more than they have (24,492 x 2000 with 64 places: two 65 us, three 50).
 template <typename T, int W, int LPR, int U, bool TAIL>
-__global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
+__global__ __launch_bounds__(kBlock, W == 4 && U == 8 ? 3 : 1) void lanes_kernel(In<T> in, Out o) {
   constexpr int kRows = kBlock / LPR;
   constexpr int kWords = (LPR * U * W + 31) / 32;
   __shared__ uint32_t bitmap[kRows * kWords];
@@ -583,7 +589,8 @@ int with_type(int dtype, F&& f) {
 template <typename T>
 In<T> input(int64_t n, int V, const void* x, int64_t ld, float temperature, int K, const float* t,
             const int64_t* index) {
-  return In<T>{n, V, static_cast<const T*>(x), ld, kLog2e / temperature, temperature, K, t, index};
+  const float c = kLog2e / temperature;
+  return In<T>{n, V, static_cast<const T*>(x), ld, c, c * kLn2d, temperature, K, t, index};
 }
 
 template <typename T>

@@ -194,14 +194,12 @@ struct Shift {
     if (far) return other_far ? far_d(other) : fmaf(-m, c, oc);
     return other_far ? fmaf(other, c, -mc) : oc - mc;
   }
-  // d in float64 (relative to the same rounded product)
-  __device__ __forceinline__ double wide_d(float x) const {
-    const double xd = x;
-    return far ? (xd - m) * c : xd * c - mc;
-  }
-  // where d is taken from, for differences of two shifts that float32 may not
-  // hold: at T < log2(e) two ends of the type's range lie further apart
-  __device__ __forceinline__ double origin() const { return far ? static_cast<double>(m) * c : mc; }
+  // Where d is taken from, for differences of two shifts that float32 may not
+  // hold (at T < log2(e) two ends of the type's range lie further apart): the
+  // product as rounded where near, the exact one where far.
+  __device__ __forceinline__ double exact() const { return static_cast<double>(m) * c; }
+  __device__ __forceinline__ double origin() const { return far ? exact() : mc; }
+  __device__ __forceinline__ double rounding() const { return far ? 0.0 : mc - exact(); }
 };
 
 // A thread's share of a row: U chunks at positions first, first + stride, ...
@@ -326,11 +324,12 @@ struct Share {
 // The shift of a row whose largest value is m: 0 for a row without any.
 __device__ __forceinline__ float shift_of(float m) { return m == -kInf ? 0.0f : m; }
 
-// log s of a float32 sum: the exponent's part in float64, the rest the logarithm
-// of a value in [0.7, 1.42), at most 0.35, whose float32 error is below 2^-24.
-// A float32 logarithm of the whole is off by half a step of itself, 2^-21 for s =
-// 50,001, more than the sum that it is taken of; float64 functions of the lists'
-// sums cost 24,492 x 18 with 5 places 1.8 us more, 24,492 x 1000 with 64 17.
+// log s of a float32 sum: the exponent apart, the hardware's base-2 logarithm
+// (v_log_f32, 1 ulp) of a value in [0.7, 1.42), at most 0.5, and float64 for the
+// rest: below 2^-24 off. A float32 logarithm of the whole is off by half a step of
+// itself, 2^-21 for s = 50,001, more than the sum that it is taken of. Lists of
+// 24,492 x 100 with 64 places: 19.7 us, 20.7 with logf of the same value; float64
+// functions cost 24,492 x 18 with 5 places 1.8 us more, x 1000 with 64 17.
 __device__ __forceinline__ double log_of(float s) {
   float f = __builtin_amdgcn_frexp_mantf(s);
   int e = __builtin_amdgcn_frexp_expf(s);
@@ -338,8 +337,20 @@ __device__ __forceinline__ double log_of(float s) {
     f += f;
     --e;
   }
-  return e * kLn2d + logf(f);
+  return (e + static_cast<double>(__builtin_amdgcn_logf(f))) * kLn2d;
 }
+
+// log p of a row's logits in float64: (x - m) c ln 2 - base, the difference of
+// logits first, since their products with c may be far larger; base is log s and
+// what the shift's product was rounded by, times ln 2.
+struct LogProb {
+  float m;
+  double c, base;  // c ln 2 (of the whole launch: scalar registers)
+  __device__ __forceinline__ LogProb(float m_, double c_ln2, double base_) : m(m_), c(c_ln2), base(base_) {}
+  __device__ __forceinline__ LogProb(const Shift& sf, double c_ln2, double log_s)
+      : LogProb(sf.m, c_ln2, log_s + sf.rounding() * kLn2d) {}
+  __device__ __forceinline__ double operator()(float x) const { return fma(static_cast<double>(x) - m, c, -base); }
+};
 
 // Joins statistics over the LPR lanes of a group (one (m, s, t) a lane; m as
 // largest() gave it, s and t relative to shift_of(m)). m becomes the shift.
