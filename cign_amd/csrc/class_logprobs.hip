@@ -43,7 +43,7 @@ struct Out {
   int64_t ignore;
   float* logprob;
   float* entropy;
-  float* stats;  // [n, 4]: m, log2 s (inf: no class left), entropy, unused; NULL: not kept
+  float* stats;  // [n, 4]: m, log2 s (inf: no class left), entropy, 1 / s; NULL: not kept
   int K;
   float* top_logprob;
   int64_t* top_index;
@@ -90,6 +90,7 @@ __device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r,
     p[0] = m;
     p[1] = none ? kInf : static_cast<float>(log_s * (1.0 / kLn2d));
     p[2] = H;
+    p[3] = static_cast<float>(inv * fma(-inv, static_cast<double>(s), 2.0));
   }
 }
 
@@ -488,8 +489,10 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
     if (g_lp && y != ignore) g = y >= 0 && y < in.V ? g_lp[r] : __builtin_nanf("");
     if (ENT) h = g_ent[r];
     if (l2s == kInf) g = h = 0.0f;  // no class left
-    // p_j (a + b log2 p_j), and g at the label
-    const float a = -(g + h * stats[4 * r + 2]) * in.inv_t, b = -h * kLn2 * in.inv_t;
+    // 2^d (a + b log2 p_j), p_j = 2^d / s (2^(d - log2 s) would round the exponent
+    // once more), and g at the label
+    const float inv_s = stats[4 * r + 3] * in.inv_t;
+    const float a = -(g + h * stats[4 * r + 2]) * inv_s, b = -h * kLn2 * inv_s;
     const float gl = g * in.inv_t;
     const bool zero = g == 0.0f && h == 0.0f;
     const Shift sf(m, in.c);
@@ -508,9 +511,9 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
         const auto turn = [&](auto of) {
 #pragma unroll
           for (int w = 0; w < W; ++w) {
-            const float d = of(v[w]) - l2s;  // log2 p
-            const float p = __builtin_amdgcn_exp2f(d);
-            v[w] = p * (ENT ? fmaf(b, fmaxf(d, kFloor), a) : a);
+            const float d = of(v[w]);
+            const float e = __builtin_amdgcn_exp2f(d);
+            v[w] = e * (ENT ? fmaf(b, fmaxf(d - l2s, kFloor), a) : a);
           }
         };
         if (sf.far)

@@ -51,9 +51,9 @@ struct In {
 
 // What the backward takes of a row.
 struct Stats {
-  float mb, l2b, cb;  // gradient of a class outside the list: cb 2^(d - l2b), d by Shift(mb)
-  float m, l2s, a;    // of a listed class: a 2^(d - l2s) - p, d by Shift(m)
-  float pad[2];
+  float mb, cb;     // gradient of a class outside the list: cb 2^d, d by Shift(mb)
+  float m, l2s, a;  // of a listed class: a 2^(d - l2s) - p, d by Shift(m)
+  float pad[3];
 };
 
 struct Out {
@@ -134,8 +134,11 @@ __device__ __forceinline__ void conclude(const In<T>& in, const Out& o, int64_t 
   if (list.bad) loss = a = cb = __builtin_nan("");
   o.loss[r] = static_cast<float>(loss * in.temperature * in.temperature);
   if (o.stats)
-    o.stats[r] = Stats{q.rest.m, q.s == 0.0f ? kInf : log2f(q.s), static_cast<float>(cb), q.all.m,
-                       q.none ? kInf : static_cast<float>(q.log_s * (1.0 / kLn2d) - q.all.rounding()), static_cast<float>(a), {0.0f, 0.0f}};
+    o.stats[r] = Stats{q.rest.m,  // (no class outside the list: 0, or NaN as it is)
+                       q.s == 0.0f ? 0.0f * static_cast<float>(cb) : static_cast<float>(cb) / q.s, q.all.m,
+                       q.none ? kInf : static_cast<float>(q.log_s * (1.0 / kLn2d) - q.all.rounding()),
+                       static_cast<float>(a),
+                       {0.0f, 0.0f, 0.0f}};
 }
 
 // e^(t - top) of a list that is renormalised. What a list leaves of one (1 - sum
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(In<T> in, int S, int cps, 
           X::unpack(sh.raw[u], v);
           const auto turn = [&](auto of) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) v[w] = cb * __builtin_amdgcn_exp2f(of(v[w]) - st.l2b);
+            for (int w = 0; w < W; ++w) v[w] = cb * __builtin_amdgcn_exp2f(of(v[w]));
           };
           if (sf.far)
             turn([&](float x) { return sf.far_d(x); });
