@@ -32,7 +32,7 @@ def check_temperature(temperature) -> float:
     t = float(temperature)
     # the kernels take 1 / T in float32
     if not (1e-30 < t < 1e30):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+        raise ValueError(f"temperature must be between 1e-30 and 1e30, got {temperature}")
     return t
 
 
@@ -50,7 +50,7 @@ def check_index(t, name: str, shape, device) -> torch.Tensor:
 def class_logprobs(logits, labels=None, top_k=0, temperature=1.0, ignore_index=-100) -> ClassLogprobs:
     """For each row of logits ([..., V], float32 or bfloat16, 1 <= V <=
     1048576; row-strided views are read in place), with l = logits /
-    temperature and log p = l - logsumexp(l):
+    temperature (between 1e-30 and 1e30) and log p = l - logsumexp(l):
 
     - logprob: log p of labels ([...], int64 or int32); 0, without gradient,
       where the label is ignore_index, NaN where it is another value outside

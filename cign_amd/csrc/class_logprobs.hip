@@ -241,8 +241,8 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
 // largest keys, in falling order, to keys[(r * S + slice) * K ...] (0: the
 // slice has no more). With S = 1 the row's outputs are written at once.
 //
-// Measured: 8,192 x 32,000 bf16 87 to 100 us (524 MB at 5.2 to 6.0 TB/s; the
-// VALU is 80% busy with 8.5 instructions and a quarter-rate exponential a value,
+// Measured: 8,192 x 32,000 bf16 82 to 101 us (524 MB at 5.2 to 6.4 TB/s; the
+// VALU is 78% busy with 8.5 instructions and a quarter-rate exponential a value,
 // so the clock decides); 777 x 50,001 float32 with 5 top classes 34 us (155 MB at
 // 4.6 TB/s; the selection's LDS rounds); one row of 131,072 bf16 with 20 over 64
 // workgroups 6 us (latency).

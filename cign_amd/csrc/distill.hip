@@ -405,10 +405,11 @@ __device__ __forceinline__ void mask_chunk(typename RowChunk<T, W>::Raw& raw, co
 }
 
 // Rows that LPR lanes hold. The bitmap also tells whether a list names a class
-// twice: a bit that was set (60,000 rows of 128 classes with whole lists: 77 us,
+// twice: a bit that was set (60,000 rows of 128 classes with whole lists: 72 us,
 // 933 with every place looking for others). 24,492 x 18 float32 with 5 places
-// 6.2 us, 24,492 x 1000 bf16 with 64 31 us: what they read takes 0.7 and 14 us,
-// the rest is the dependent loads of the list and its logits, and its sums.
+// 6.0 us, 24,492 x 1000 bf16 with 64 25 us, 28 with the tail: what they read takes
+// 0.7 and 14 us, the rest is the dependent loads of the list and its logits, and
+// its sums.
 // Eight float32 chunks a lane are held to three wavefronts a SIMD, the tail's one
 // register more than they have (24,492 x 2000 with 64 places: two 65 us, three 50).
 template <typename T, int W, int LPR, int U, bool TAIL>

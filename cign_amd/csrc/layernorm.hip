@@ -297,8 +297,9 @@ __global__ __launch_bounds__(kParamThreads) void param_kernel(const float* part,
 // rows take a workgroup of 256, 512 or 1024 threads. 512 threads go as far as
 // their registers hold the next row's values too: up to 12,288 columns (backward of
 // 11,000 float32 columns, 268 MB: 146 us against 198 by 1024 threads, of bf16 67
-// against 98; with 8 and 4 chunks a thread at 16,384 columns they spill: 316 and
-// 101 us against 151 and 78).
+// against 98; with 8 and 4 chunks a thread at 16,384 columns 316 and 101 us
+// against 151 and 78 by 1024 threads, which spill too, 56 and 20 bytes of their 128
+// registers each, but hold one row at a time).
 template <typename T, class F>
 int with_shape(int D, F&& f) {
   constexpr int W = kChunk<T>;
