@@ -70,7 +70,7 @@ __device__ __forceinline__ LogProb log_prob(const In<T>& in, float m, double log
 // Label, entropy and statistics of row r from its joined (m, s, t) and log s.
 template <typename T>
 __device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r, float m, float s, float t,
-                                       double log_s) {
+                                       double log_s, const LogProb& log_p) {
   const bool none = s == 0.0f;
   // t / s: a float32 reciprocal and one step in float64
   const double inv = __builtin_amdgcn_rcpf(s), first = t * inv;
@@ -81,8 +81,7 @@ __device__ __forceinline__ void finish(const In<T>& in, const Out& o, int64_t r,
     const int64_t y = o.label[r];
     float lp = 0.0f;
     if (y != o.ignore)
-      lp = y >= 0 && y < in.V ? static_cast<float>(log_prob(in, m, log_s)(to_f32(in.x[r * in.ld + y])))
-                              : __builtin_nanf("");
+      lp = y >= 0 && y < in.V ? static_cast<float>(log_p(to_f32(in.x[r * in.ld + y]))) : __builtin_nanf("");
     o.logprob[r] = lp;
   }
   if (o.stats) {
@@ -222,9 +221,9 @@ __global__ __launch_bounds__(kBlock) void lanes_kernel(In<T> in, Out o) {
     sh.template sums<true>(Shift(shift_of(m), in.c), s, t);
     join<LPR, true>(m, s, t, in.c);
     const double log_s = log_sum(s);
-    if (q == 0) finish(in, o, r, m, s, t, log_s);
+    const LogProb log_p = log_prob(in, m, log_s);
+    if (q == 0) finish(in, o, r, m, s, t, log_s, log_p);
     if constexpr (TOP) {
-      const LogProb log_p = log_prob(in, m, log_s);
       uint64_t mine = best_below(sh, ~0ull);
       for (int k = 0; k < o.K; ++k) {
         const uint64_t best = group_max<LPR>(mine);
@@ -296,10 +295,12 @@ __global__ __launch_bounds__(kBlock) void slice_kernel(In<T> in, Out o, Slicing 
   }
   across.run<true>(m, s, t, in.c);
   if (threadIdx.x == 0) {
-    if (sl.S == 1)
-      finish(in, o, r, m, s, t, log_sum(s));
-    else
+    if (sl.S == 1) {
+      const double log_s = log_sum(s);
+      finish(in, o, r, m, s, t, log_s, log_prob(in, m, log_s));
+    } else {
       part[item] = make_float4(s == 0.0f ? -kInf : m, s, t, 0.0f);
+    }
   }
   if constexpr (TOP) {
     // The K-th largest of the best keys of quads (K <= 32) or threads bounds
@@ -389,7 +390,8 @@ __global__ __launch_bounds__(kBlock) void join_kernel(In<T> in, Out o, int S, co
     const float4 p = lane < S ? part[r * S + lane] : make_float4(-kInf, 0.0f, 0.0f, 0.0f);
     float m = p.x, s = p.y, t = p.z;
     join<kWave, true>(m, s, t, in.c);
-    if (lane == 0) finish(in, o, r, m, s, t, log_sum(s));
+    const double log_s = log_sum(s);
+    if (lane == 0) finish(in, o, r, m, s, t, log_s, log_prob(in, m, log_s));
   }
 }
 
@@ -462,7 +464,7 @@ __global__ __launch_bounds__(kBlock) void join_top_kernel(In<T> in, Out o, int S
         }
       }
     }
-    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, log_s);
+    if (threadIdx.x == kBlock - 1) finish(in, o, r, m, s, t, log_s, log_p);
   }
 }
 
