@@ -22,7 +22,7 @@ OBJ = PKG / "_build"
 LIB = PKG / "libcign_amd.so"
 BINDING_SRC = SRC / "python" / "binding.cpp"
 BINDING = PKG / "_cign.so"
-OPS_SRC = SRC / "python" / "output_ops.cpp"
+OPS_SRCS = [SRC / "python" / "output_ops.cpp", SRC / "python" / "step_ops.cpp"]
 OPS = PKG / "_cign_ops.so"
 
 ARCH = "gfx950"
@@ -78,27 +78,37 @@ def _compile(hipcc: str, src: Path, force: bool) -> Path:
     return obj
 
 
-def _host_module(src: Path, out: Path, flags: list[str], libs: list[str]) -> Path:
-    """Compiles a CPython extension against the library (host code only)."""
+def _host_module(srcs: list[Path], out: Path, flags: list[str], libs: list[str]) -> Path:
+    """Compiles a CPython extension against the library (host code only), a
+    source at a time on a core of its own."""
     tmp = out.with_suffix(".so.tmp")
     cxx = os.environ.get("CXX") or shutil.which("g++") or str(Path(_hipcc()).parent / "amdclang++")
-    cmd = [cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-shared", f"-I{sysconfig.get_paths()['include']}",
-           f"-I{PKG.parent / 'include'}", *flags, str(src), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", *libs,
-           "-Wl,-rpath,$ORIGIN"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"{src.name} build failed:\n{res.stderr[-6000:]}")
+    objs = [OBJ / f"{src.stem}.host.o" for src in srcs]
+
+    def run(cmd, what):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{what} build failed:\n{res.stderr[-6000:]}")
+
+    def compile_one(src, obj):
+        run([cxx, "-O2", "-fPIC", "-std=c++17", "-Wall", "-c", f"-I{sysconfig.get_paths()['include']}",
+             f"-I{PKG.parent / 'include'}", *flags, str(src), "-o", str(obj)], src.name)
+
+    with cf.ThreadPoolExecutor(max_workers=len(srcs)) as pool:
+        list(pool.map(compile_one, srcs, objs))
+    run([cxx, "-shared", *map(str, objs), "-o", str(tmp), f"-L{PKG}", f"-l:{LIB.name}", *libs, "-Wl,-rpath,$ORIGIN"],
+        out.name)
     os.replace(tmp, out)
     return out
 
 
 def build_binding() -> Path:
     """Compiles the CPython binding of the C-ABI."""
-    return _host_module(BINDING_SRC, BINDING, [], [])
+    return _host_module([BINDING_SRC], BINDING, [], [])
 
 
 def build_output_ops() -> Path:
-    """Compiles the output operators' autograd nodes, against torch as it is
+    """Compiles the torch operators and their autograd nodes, against torch as it is
     installed; its libraries are found by the process that imported torch."""
     import torch
 
@@ -107,7 +117,7 @@ def build_output_ops() -> Path:
     flags = [f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
              f"-isystem{rocm / 'include'}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    return _host_module(OPS_SRC, OPS, flags, [f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
+    return _host_module(OPS_SRCS, OPS, flags, [f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
                                               "-ltorch_python"])
 
 

@@ -86,6 +86,22 @@ _SIGNATURES = {
     "cign_distill_topk_workspace_bytes": (_I64, [_I32, _I64, _I32]),
     "cign_distill_topk_fwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _I32, _I32, _P, _P, _P, _P, _P, _P, _I64]),
     "cign_distill_topk_bwd": (C.c_int, [_P, _I32, _I64, _I32, _P, _I64, _F32, _I32, _P, _P, _P, _P, _P]),
+    # boundary of two blocks (block_boundary.hip)
+    "cign_block_boundary_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P, _I64, _P, _I64]
+                                + [_P] * 5 + [_F32, _P, _P, _P]),
+    "cign_block_boundary_bwd_workspace_bytes": (_I64, [_I64, _I32]),
+    "cign_block_boundary_bwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _I32, _I32] + [_P, _I64] * 5 + [_P] * 14
+                                + [_I64]),
+    # cross entropy of a linear classifier (linear_xent.hip)
+    "cign_linear_xent_workspace_bytes": (_I64, [_I32, _I64, _I32, _I32, _P, _I64, _P, _I64, _I32]),
+    "cign_linear_xent_fwd": (C.c_int, [_P, _I32, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I32, _P, _I64, _P, _P, _P,
+                                       _I64]),
+    "cign_linear_xent_bwd": (C.c_int, [_P, _I32, _I64, _I32, _I32, _P, _I64, _P, _I64, _P, _I32, _P, _I64] + [_P] * 7
+                             + [_I64]),
+    # global norm of gradients (grad_norm.hip)
+    "cign_grad_norm_workspace_bytes": (_I64, [_I32, _P]),
+    "cign_grad_norm": (C.c_int, [_P, _I32, _P, _P, _P, _P, _P, _I64]),
+    "cign_clip_grad_norm": (C.c_int, [_P, _I32, _P, _P, _P, _F32, _P, _P, _P, _I64]),
     # hop gate (gate.hip)
     "cign_hop_gate_bwd_workspace_bytes": (_I64, [_I64, _I32, _I32]),
     "cign_hop_gate_fwd": (C.c_int, [_P, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P]),

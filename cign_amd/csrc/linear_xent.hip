@@ -1,0 +1,931 @@
+// Cross entropy of a linear classifier over many classes, z = x W^T + b, by
+// pieces of the classes, without keeping the logits:
+//   lse = log sum_v e^(z_v), loss = lse - z_label,
+//   dz_v = (g_loss + g_lse) e^(z_v - lse) - g_loss [v = label],
+//   grad_x = dz W, grad_W = dz^T x, grad_b = sum over rows of dz.
+//
+// Forward: tiles of 256 rows by 256 classes (nt_gemm.h), whose largest logit and
+// sum of exponentials a row leave the tile; join_kernel brings them together. Few
+// rows (up to 64) stream W through the matrix units instead (few_kernel).
+// Backward: a piece's logits are formed again, and their gradient is stored in
+// bf16 as it stands and transposed, so that every product is one of rows that run
+// along the summed axis. float32 operands are held as three bf16 parts of 8 bits
+// each and multiplied in six products, the smallest first: the dropped ones lie
+// below 2^-26 of a product, so the sums are float32's own.
+#include <algorithm>
+
+#include "nt_gemm.h"
+#include "rowvec.h"
+
+namespace cign {
+namespace xent {
+using ntgemm::bf16x8;
+using ntgemm::f32x4;
+using ntgemm::kFragA;
+using ntgemm::kFragB;
+using ntgemm::kStep;
+using ntgemm::kTile;
+using ntgemm::Operand;
+using ntgemm::Place;
+
+constexpr int kMaxClasses = 1 << 20;
+constexpr int kMaxWidth = 1 << 16;
+constexpr int kMaxRows = 1 << 23;  // 32-bit offsets in a tile of the transposed gradient
+constexpr int kFewRows = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int N>
+using IC = std::integral_constant<int, N>;
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// e^d for d = z - m <= 0: relative error |d| 2^-24 and less.
+__device__ __forceinline__ float exp_of(float d) { return exp2_of(d * kLog2e); }
+
+__device__ __forceinline__ uint16_t round_bf16(float v) { return from_f32<bf16>(v).bits; }
+
+// v as PARTS bf16 values whose sum it is to 8 bits each. Parts below a value that
+// is not finite are zero.
+template <int PARTS>
+__device__ __forceinline__ void split(float v, uint16_t (&part)[PARTS]) {
+  part[0] = round_bf16(v);
+  float rest = v;
+#pragma unroll
+  for (int k = 1; k < PARTS; ++k) {
+    rest -= __uint_as_float(static_cast<uint32_t>(part[k - 1]) << 16);
+    part[k] = isfinite(rest) ? round_bf16(rest) : 0;
+  }
+}
+
+// A class's bias, of storage code `f32`.
+__device__ __forceinline__ float bias_at(const void* bias, int f32, int64_t v) {
+  return f32 ? static_cast<const float*>(bias)[v] : to_f32(static_cast<const bf16*>(bias)[v]);
+}
+
+// What the logits of a piece of classes are formed from.
+struct Logits {
+  Operand w, x;             // classes of the piece; rows
+  int ksteps;
+  const void* bias;         // of the whole vocabulary, or null
+  int bias_f32;
+  int64_t first;            // first class of the piece
+  const int32_t* count;     // rows at work, on the device, or null for x.rows
+  const int64_t* labels;
+  __device__ __forceinline__ float bias_of(int64_t v) const {
+    return bias ? bias_at(bias, bias_f32, first + v) : 0.0f;
+  }
+};
+
+__device__ __forceinline__ int tiles(int64_t rows) { return static_cast<int>((rows + kTile - 1) / kTile); }
+
+// (largest, sum of e^(value - largest)) of two sets
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  const float by = top == -INFINITY ? 0.0f : top;
+  s = s * exp_of(m - by) + s2 * exp_of(m2 - by);
+  m = top;
+}
+
+// Statistics of a tile: part[tile of classes][row], and the logit of each row's label.
+template <int SEGS>
+__global__ __launch_bounds__(ntgemm::kThreads, 1) void stats_kernel(Logits f, int64_t n, float2* part, int first_tile,
+                                                                    float* chosen) {
+  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  int ia, ib;
+  ntgemm::tile_of(blockIdx.x, tiles(f.w.rows), tiles(n), ia, ib);
+  f32x4 acc[kFragA][kFragB];
+  ntgemm::product<SEGS>(f.w, f.x, ia, ib, f.ksteps, lds, acc);
+  const Place at(ia, ib);
+  float2* red = reinterpret_cast<float2*>(lds);  // [2][kTile]
+  const int wave = threadIdx.x / kWave, l = lane_id();
+  float bias[kFragA][4];
+#pragma unroll
+  for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
+#pragma unroll
+  for (int fb = 0; fb < kFragB; ++fb) {
+    const int64_t row = at.b(fb);
+    const int64_t want = f.labels && row < n ? f.labels[row] - f.first : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float z = bias[fa][r] == -INFINITY ? -INFINITY : acc[fa][fb][r] + bias[fa][r];
+        acc[fa][fb][r] = z;
+        m = fmaxf(m, z);
+        if (at.a(fa) + r == want && want < f.w.rows) chosen[row] = z;
+      }
+    const float by = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += exp_of(acc[fa][fb][r] - by);
+    join(m, s, xor_shfl<16>(m), xor_shfl<16>(s));
+    join(m, s, xor_shfl<32>(m), xor_shfl<32>(s));
+    if (l < 16) red[(wave & 1) * kTile + (wave >> 1) * 64 + fb * 16 + l] = make_float2(m, s);
+  }
+  __syncthreads();
+  const int64_t row = static_cast<int64_t>(ib) * kTile + threadIdx.x;
+  if (threadIdx.x < kTile && row < n) {
+    float2 a = red[threadIdx.x];
+    const float2 b = red[kTile + threadIdx.x];
+    join(a.x, a.y, b.x, b.y);
+    part[static_cast<int64_t>(first_tile + ia) * n + row] = a;
+  }
+}
+
+// Up to 16 T rows: a wavefront takes 64 classes, four tiles of 16, and reads W
+// where it lies; values are fed to the matrix units in the order in which a lane's
+// 16-byte chunks come, rows of x alike. part[workgroup][row] as above.
+template <typename T>
+struct Few;
+template <>
+struct Few<bf16> {
+  static constexpr int kLane = 8;  // values of a lane's chunk
+  using Raw = bf16x8;
+  static __device__ __forceinline__ f32x4 mul(const Raw& a, const Raw& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Few<float> {
+  static constexpr int kLane = 4;
+  using Raw = f32x4;
+  static __device__ __forceinline__ f32x4 mul(const Raw& a, const Raw& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ typename Few<T>::Raw few_load(const T* p) {
+  return __builtin_bit_cast(typename Few<T>::Raw, rowvec::RowChunk<T, Few<T>::kLane>::load(p));
+}
+
+// the values before `left` of a chunk, zeros behind
+template <typename T>
+__device__ __forceinline__ typename Few<T>::Raw few_tail(const T* p, int left) {
+  T v[Few<T>::kLane];
+#pragma unroll
+  for (int i = 0; i < Few<T>::kLane; ++i) v[i] = i < left ? p[i] : from_f32<T>(0.0f);
+  return __builtin_bit_cast(typename Few<T>::Raw, v);
+}
+
+constexpr int kFewClasses = 256;  // of a workgroup
+
+template <typename T, int TOKENS>
+__global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, const T* x, int64_t ldx, const T* w,
+                                                     int64_t ldw, const void* bias, int bias_f32,
+                                                     const int64_t* labels, float2* part, float* chosen) {
+  using F = Few<T>;
+  constexpr int L = F::kLane, TA = 4, TB = TOKENS / 16;
+  __shared__ float2 red[kWavesPerBlock][TOKENS];
+  const int l = lane_id(), wave = wave_id();
+  const int c0 = blockIdx.x * kFewClasses + wave * 64;
+  const int q = l >> 4;
+  const T *wp[TA], *xp[TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i) wp[i] = w + static_cast<int64_t>(min(c0 + i * 16 + (l & 15), V - 1)) * ldw + q * L;
+#pragma unroll
+  for (int i = 0; i < TB; ++i) xp[i] = x + min(static_cast<int64_t>(i * 16 + (l & 15)), n - 1) * ldx + q * L;
+  f32x4 acc[TA][TB];
+#pragma unroll
+  for (int a = 0; a < TA; ++a)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  int k = 0;
+#pragma unroll 4
+  for (; k + 4 * L <= D; k += 4 * L) {
+    typename F::Raw a[TA], b[TB];
+#pragma unroll
+    for (int i = 0; i < TA; ++i) a[i] = few_load(wp[i] + k);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) b[i] = few_load(xp[i] + k);
+#pragma unroll
+    for (int i = 0; i < TA; ++i)
+#pragma unroll
+      for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
+  }
+  if (k < D) {
+    typename F::Raw a[TA], b[TB];
+    const int left = D - k - q * L;
+#pragma unroll
+    for (int i = 0; i < TA; ++i) a[i] = few_tail(wp[i] + k, left);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) b[i] = few_tail(xp[i] + k, left);
+#pragma unroll
+    for (int i = 0; i < TA; ++i)
+#pragma unroll
+      for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
+  }
+#pragma unroll
+  for (int b = 0; b < TB; ++b) {
+    const int64_t row = b * 16 + (l & 15);
+    const int64_t want = labels && row < n ? labels[row] : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < TA; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = c0 + a * 16 + q * 4 + r;
+        float z = -INFINITY;
+        if (v < V) {
+          const float add = bias ? bias_at(bias, bias_f32, v) : 0.0f;
+          if (add != -INFINITY) z = acc[a][b][r] + add;
+          if (v == want) chosen[row] = z;
+        }
+        acc[a][b][r] = z;
+        m = fmaxf(m, z);
+      }
+    const float by = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int a = 0; a < TA; ++a)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += exp_of(acc[a][b][r] - by);
+    join(m, s, xor_shfl<16>(m), xor_shfl<16>(s));
+    join(m, s, xor_shfl<32>(m), xor_shfl<32>(s));
+    if (l < 16) red[wave][b * 16 + l] = make_float2(m, s);
+  }
+  __syncthreads();
+  if (threadIdx.x < TOKENS && threadIdx.x < n) {
+    float2 t = red[0][threadIdx.x];
+#pragma unroll
+    for (int k2 = 1; k2 < kWavesPerBlock; ++k2) join(t.x, t.y, red[k2][threadIdx.x].x, red[k2][threadIdx.x].y);
+    part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = t;
+  }
+}
+
+// loss and lse of 32 rows a workgroup, eight threads a row over its nt tiles; the
+// logarithm and the differences in float64, rounded once.
+constexpr int kJoinRows = 32;
+__global__ __launch_bounds__(kBlock) void join_kernel(int64_t n, int V, int nt, const float2* part,
+                                                      const int64_t* labels, int64_t ignore, const float* chosen,
+                                                      float* loss, float* lse) {
+  constexpr int kParts = kBlock / kJoinRows;
+  __shared__ float2 red[kParts][kJoinRows];
+  const int j = threadIdx.x % kJoinRows, k = threadIdx.x / kJoinRows;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + j;
+  float m = -INFINITY, s = 0.0f;
+  if (row < n)
+    for (int t = k; t < nt; t += kParts) {
+      const float2 p = part[static_cast<int64_t>(t) * n + row];
+      join(m, s, p.x, p.y);
+    }
+  red[k][j] = make_float2(m, s);
+  __syncthreads();
+  if (k || row >= n) return;
+#pragma unroll
+  for (int t = 1; t < kParts; ++t) join(m, s, red[t][j].x, red[t][j].y);
+  const double logs = log(static_cast<double>(s));
+  lse[row] = static_cast<float>(static_cast<double>(m) + logs);
+  if (!loss) return;
+  const int64_t y = labels[row];
+  float out = 0.0f;
+  if (y != ignore) {
+    if (y < 0 || y >= V)
+      out = NAN;
+    else if (s == 0.0f || chosen[row] == -INFINITY)
+      out = isnan(s) ? NAN : INFINITY;
+    else
+      out = static_cast<float>(static_cast<double>(m) - static_cast<double>(chosen[row]) + logs);
+  }
+  loss[row] = out;
+}
+
+// Rows with a gradient, in order: list[0..count), and each row's place in it or -1.
+__global__ __launch_bounds__(1024) void rows_kernel(int64_t n, const int64_t* labels, int64_t ignore,
+                                                    const float* g_loss, const float* g_lse, int32_t* list,
+                                                    int32_t* place, int32_t* count) {
+  __shared__ int32_t sums[16], base;
+  constexpr int kEach = 8;
+  if (threadIdx.x == 0) base = 0;
+  __syncthreads();
+  for (int64_t b = 0; b < n; b += 1024 * kEach) {
+    const int64_t r0 = b + threadIdx.x * kEach;
+    bool on[kEach];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t r = r0 + i;
+      on[i] = r < n && ((g_loss && labels[r] != ignore && g_loss[r] != 0.0f) || (g_lse && g_lse[r] != 0.0f));
+      mine += on[i];
+    }
+    int before = mine;
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int t = __shfl_up(before, o, kWave);
+      if (lane_id() >= o) before += t;
+    }
+    if (lane_id() == kWave - 1) sums[wave_id()] = before;
+    __syncthreads();
+    int at = base + before - mine, total = 0;
+    for (int wv = 0; wv < 16; ++wv) {
+      if (wv < wave_id()) at += sums[wv];
+      total += sums[wv];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (r0 + i >= n) continue;
+      place[r0 + i] = on[i] ? at : -1;
+      if (on[i]) list[at++] = static_cast<int32_t>(r0 + i);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = base;
+}
+
+// Rows of D values of T as bf16 parts, Kp values apart with zeros behind the
+// row's own; rows of a list where there is one.
+template <typename T, int PARTS>
+__global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* count, const int32_t* list, int D,
+                                                      const T* src, int64_t ld, uint16_t* dst, int Kp, int64_t part) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  const int per = Kp / 8;
+  const int64_t r = i / per;
+  const int c = static_cast<int>(i - r * per) * 8;
+  if (r >= (count ? *count : n)) return;
+  const T* row = src + (list ? list[r] : r) * ld;
+  float v[8];
+  if (c + 8 <= D) {
+    rowvec::RowChunk<T, 8>::unpack(rowvec::RowChunk<T, 8>::load(row + c), v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c + k < D ? to_f32(row[c + k]) : 0.0f;
+  }
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  u16x8 o[PARTS];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint16_t p[PARTS];
+    split<PARTS>(v[k], p);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) o[q][k] = p[q];
+  }
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) *reinterpret_cast<u16x8*>(dst + q * part + r * Kp + c) = o[q];
+}
+
+// The same transposed: dst[c][r], rows of dst Rp values apart, zeros for rows
+// from the last one to the next multiple of kStep, and for classes that a bias of
+// -inf masks (whose gradients are zero, which a NaN would not stay). 64 x 64 values a workgroup.
+template <typename T, int PARTS>
+__global__ __launch_bounds__(kBlock) void pack_t_kernel(int64_t n, const int32_t* count, const int32_t* list, int D,
+                                                        const T* src, int64_t ld, const void* bias, int bias_f32,
+                                                        uint16_t* dst, int64_t Rp, int64_t part) {
+  __shared__ float tile[64][65];
+  const int64_t rows = count ? *count : n;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
+  const int c0 = blockIdx.y * 64;
+  if (r0 >= rows) return;
+  const int a = threadIdx.x >> 2, b = (threadIdx.x & 3) * 16;
+  {
+    const int64_t r = r0 + a;
+    const bool on = r < rows && !(bias && bias_at(bias, bias_f32, r) == -INFINITY);
+    const T* row = src + (on ? (list ? list[r] : r) : 0) * ld;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + b + 8 * h;
+      float v[8];
+      if (on && c + 8 <= D) {
+        rowvec::RowChunk<T, 8>::unpack(rowvec::RowChunk<T, 8>::load(row + c), v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = on && c + k < D ? to_f32(row[c + k]) : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) tile[a][b + 8 * h + k] = v[k];
+    }
+  }
+  __syncthreads();
+  if (c0 + a >= D) return;
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u16x8 o[PARTS];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint16_t p[PARTS];
+      split<PARTS>(tile[b + 8 * h + k][a], p);
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) o[q][k] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q)
+      *reinterpret_cast<u16x8*>(dst + q * part + static_cast<int64_t>(c0 + a) * Rp + r0 + b + 8 * h) = o[q];
+  }
+}
+
+// The gradient of a piece's logits, in bf16 parts: dz[row][class] and
+// dzt[class][row], zeros up to the next multiple of kStep of each axis; and the
+// tile's sums over its rows, for the bias.
+struct Grads {
+  const int32_t* list;
+  const float* lse;
+  const float* g_loss;     // null: none
+  const float* g_lse;      // null: none
+  int64_t ignore;
+  int64_t V;
+  uint16_t* dz;
+  int64_t ld, part;
+  uint16_t* dzt;
+  int64_t ldt, partt;
+  float* bias_part;        // [tile of rows][class of the piece] or null
+};
+
+template <int SEGS>
+__global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Grads g) {
+  constexpr int PARTS = SEGS > 1 ? 3 : 1;
+  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  const int64_t n = *f.count;
+  const int ta = tiles(f.w.rows), tb = tiles(n);
+  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(ta) * tb) return;
+  int ia, ib;
+  ntgemm::tile_of(blockIdx.x, ta, tb, ia, ib);
+  f32x4 acc[kFragA][kFragB];
+  Operand x = f.x;
+  x.rows = n;
+  ntgemm::product<SEGS>(f.w, x, ia, ib, f.ksteps, lds, acc);
+  const Place at(ia, ib);
+  const int wave = threadIdx.x / kWave, l = lane_id();
+  const int64_t Vp = (f.w.rows + kStep - 1) / kStep * kStep, np = (n + kStep - 1) / kStep * kStep;
+  float sums[kFragA][4];
+  float bias[kFragA][4];
+#pragma unroll
+  for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sums[fa][r] = 0.0f;
+      bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
+    }
+#pragma unroll
+  for (int fb = 0; fb < kFragB; ++fb) {
+    const int64_t row = at.b(fb);
+    float own = 0.0f, all = 0.0f, shift = 0.0f;
+    int64_t want = -1;
+    bool some = false;
+    if (row < n) {
+      const int64_t src = g.list[row];
+      const int64_t y = f.labels ? f.labels[src] : g.ignore;
+      if (y != g.ignore && g.g_loss) {
+        own = g.g_loss[src];
+        if (y < 0 || y >= g.V) own = NAN;
+      }
+      want = y - f.first;
+      all = own + (g.g_lse ? g.g_lse[src] : 0.0f);
+      shift = g.lse[src];
+      some = shift != -INFINITY;  // a class is left
+    }
+#pragma unroll
+    for (int fa = 0; fa < kFragA; ++fa) {
+      float d[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float z = acc[fa][fb][r] + bias[fa][r];
+        const float p = bias[fa][r] == -INFINITY || !some ? 0.0f : exp_of(z - shift);
+        d[r] = all * p;
+        if (some && at.a(fa) + r == want && want < f.w.rows) d[r] -= own;
+        if (row >= n || at.a(fa) + r >= f.w.rows) d[r] = 0.0f;
+        sums[fa][r] += d[r];
+      }
+      uint16_t o[4][PARTS];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) split<PARTS>(d[r], o[r]);
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+        if (g.dz && row < n && at.a(fa) < Vp)
+          *reinterpret_cast<uint2*>(g.dz + q * g.part + row * g.ld + at.a(fa)) =
+              make_uint2(o[0][q] | (static_cast<uint32_t>(o[1][q]) << 16), o[2][q] | (static_cast<uint32_t>(o[3][q]) << 16));
+        if (g.dzt && row < np)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (at.a(fa) + r < f.w.rows) g.dzt[q * g.partt + (at.a(fa) + r) * g.ldt + row] = o[r][q];
+      }
+    }
+  }
+  if (!g.bias_part) return;
+  float* red = reinterpret_cast<float*>(lds);  // [4][kTile]
+#pragma unroll
+  for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float s = sums[fa][r];
+      s += xor_shfl<1>(s);
+      s += xor_shfl<2>(s);
+      s += xor_shfl<4>(s);
+      s += xor_shfl<8>(s);
+      if ((l & 15) == 0) red[(wave >> 1) * kTile + (wave & 1) * 128 + fa * 16 + (l >> 4) * 4 + r] = s;
+    }
+  __syncthreads();
+  const int64_t v = static_cast<int64_t>(ia) * kTile + threadIdx.x;
+  if (threadIdx.x < kTile && v < f.w.rows)
+    g.bias_part[static_cast<int64_t>(ib) * f.w.rows + v] = (red[threadIdx.x] + red[kTile + threadIdx.x]) +
+                                                           (red[2 * kTile + threadIdx.x] + red[3 * kTile + threadIdx.x]);
+}
+
+// out[b][a] = sum_k A[a][k] B[b][k]: the weight's gradient (SLOT false: rounded to
+// T, ldo = a row's values), or a part of the rows' gradient (float32, added to
+// what earlier pieces left; blockIdx.y takes a run of the K steps).
+template <typename T, int SEGS, bool SLOT>
+__global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Operand b, int ksteps,
+                                                                  const int32_t* count, T* out, int64_t ldo,
+                                                                  int64_t slot, int accumulate) {
+  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  if (SLOT) {
+    b.rows = *count;
+    const int each = (ksteps + gridDim.y - 1) / gridDim.y, from = blockIdx.y * each;
+    ksteps = max(0, min(each, ksteps - from));
+    a.p += static_cast<int64_t>(from) * kStep;
+    b.p += static_cast<int64_t>(from) * kStep;
+    out += blockIdx.y * slot;
+  } else {
+    ksteps = (*count + kStep - 1) / kStep;
+  }
+  const int ta = tiles(a.rows), tb = tiles(b.rows);
+  if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(ta) * tb) return;
+  int ia, ib;
+  ntgemm::tile_of(blockIdx.x, ta, tb, ia, ib);
+  f32x4 acc[kFragA][kFragB];
+  ntgemm::product<SEGS>(a, b, ia, ib, ksteps, lds, acc);
+  const Place at(ia, ib);
+#pragma unroll
+  for (int fb = 0; fb < kFragB; ++fb) {
+    if (at.b(fb) >= b.rows) continue;
+    T* row = out + at.b(fb) * ldo;
+#pragma unroll
+    for (int fa = 0; fa < kFragA; ++fa) {
+      const int64_t i = at.a(fa);
+      if (i >= a.rows) continue;
+      if constexpr (SLOT) {  // rows of a multiple of four floats
+        f32x4* to = reinterpret_cast<f32x4*>(row + i);
+        *to = accumulate ? *to + acc[fa][fb] : acc[fa][fb];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i + r < a.rows) row[i + r] = from_f32<T>(acc[fa][fb][r]);
+      }
+    }
+  }
+}
+
+// grad_x of all rows from the slots of those with a gradient, zeros elsewhere.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, const int32_t* place, const float* slots,
+                                                          int ns, int64_t slot, int Dp, T* gx) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  const int per = Dp / 4;
+  const int64_t r = i / per;
+  const int c = static_cast<int>(i - r * per) * 4;
+  if (r >= n) return;
+  const int p = place[r];
+  f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+  if (p >= 0)
+    for (int s = 0; s < ns; ++s) v += *reinterpret_cast<const f32x4*>(slots + s * slot + static_cast<int64_t>(p) * Dp + c);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (c + k < D) gx[r * D + c + k] = from_f32<T>(v[k]);
+}
+
+// grad_b of a piece from the tiles' sums.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void bias_kernel(const int32_t* count, int64_t V, const float* part, T* gb) {
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  if (v >= V) return;
+  const int nt = tiles(*count);
+  float s = 0.0f;
+  for (int t = 0; t < nt; ++t) s += part[t * V + v];
+  gb[v] = from_f32<T>(s);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// Rows that the tiles read where they lie (their offsets in a tile are 32 bits).
+bool in_place(int dtype, int D, const void* p, int64_t ld) {
+  return dtype == kBF16 && D % kStep == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 &&
+         ld <= (1 << 24);
+}
+
+struct Cut {
+  int parts, Kp;
+  int64_t fwd_piece;         // classes packed at a time by the forward
+  int64_t piece;             // classes of a piece of the backward
+  int64_t rows_p;            // rows to the next multiple of kStep
+  int splits;                // slots of the rows' gradient
+  int Dp;
+};
+
+constexpr int64_t kPieceValues = 64ll << 20;   // of dz in a piece
+constexpr int64_t kPackValues = 256ll << 20;   // of packed classes in a piece of the forward
+
+Cut cut(int dtype, int64_t n, int64_t V, int D) {
+  Cut c;
+  c.parts = dtype == kF32 ? 3 : 1;
+  c.Kp = static_cast<int>(up(D, kStep));
+  const auto even = [&](int64_t most) {
+    most = std::max<int64_t>(kTile, most / kTile * kTile);
+    const int64_t pieces = (V + most - 1) / most;
+    return up((V + pieces - 1) / pieces, kTile);
+  };
+  c.fwd_piece = even(kPackValues / (c.parts * static_cast<int64_t>(c.Kp)));
+  c.rows_p = up(n, kStep);
+  c.piece = even(std::min<int64_t>(kPieceValues / std::max<int64_t>(kStep, c.rows_p),
+                                   kPackValues / (c.parts * static_cast<int64_t>(c.Kp))));
+  c.Dp = static_cast<int>(up(D, 4));
+  // workgroups for every CU, two rounds of them
+  const int64_t t = ((n + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
+  const int64_t most = std::max<int64_t>(1, up(std::min(c.piece, V), kStep) / kStep / 8);
+  c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, t), most, 32})));
+  return c;
+}
+
+// Bytes of a workspace's regions, 256-byte aligned.
+struct Regions {
+  int64_t total = 0;
+  char* base;
+  explicit Regions(void* p) : base(static_cast<char*>(p)) {}
+  template <typename T>
+  T* take(int64_t values) {
+    T* p = base ? reinterpret_cast<T*>(base + total) : nullptr;
+    total += up(values * static_cast<int64_t>(sizeof(T)), 256);
+    return p;
+  }
+};
+
+struct FwdSpace {
+  float2* part;
+  float* chosen;
+  uint16_t *x, *w;
+};
+
+// x_in, w_in: read in place
+int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void* p, FwdSpace* s) {
+  Regions r(p);
+  FwdSpace f;
+  f.part = r.take<float2>(n * ((V + kTile - 1) / kTile));
+  f.chosen = r.take<float>(n);
+  f.x = f.w = nullptr;
+  if (n > kFewRows) {
+    if (!x_in) f.x = r.take<uint16_t>(c.parts * n * c.Kp);
+    if (!w_in) f.w = r.take<uint16_t>(c.parts * std::min(c.fwd_piece, V) * c.Kp);
+  }
+  if (s) *s = f;
+  return r.total;
+}
+
+struct BwdSpace {
+  int32_t *list, *place, *count;
+  uint16_t *x, *xt, *w, *wt, *dz, *dzt;
+  float *slots, *bias;
+};
+
+int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, void* p, BwdSpace* s) {
+  Regions r(p);
+  BwdSpace b{};
+  const int64_t vc = std::min(c.piece, up(V, kStep));
+  b.list = r.take<int32_t>(n);
+  b.place = r.take<int32_t>(n);
+  b.count = r.take<int32_t>(1);
+  b.x = r.take<uint16_t>(c.parts * n * c.Kp);
+  if (!w_in) b.w = r.take<uint16_t>(c.parts * vc * c.Kp);
+  if (of & 1) {
+    b.wt = r.take<uint16_t>(c.parts * vc * D);
+    b.dz = r.take<uint16_t>(c.parts * n * vc);
+    b.slots = r.take<float>(c.splits * n * c.Dp);
+  }
+  if (of & 2) {
+    b.xt = r.take<uint16_t>(c.parts * c.rows_p * D);
+    b.dzt = r.take<uint16_t>(c.parts * c.rows_p * vc);
+  }
+  if (of & 4) b.bias = r.take<float>(((n + kTile - 1) / kTile) * vc);
+  if (s) *s = b;
+  return r.total;
+}
+
+int check_args(const char* who, int dtype, int64_t n, int64_t V, int64_t D) {
+  if (dtype != kF32 && dtype != kBF16) return set_error(kInvalid, "%s: dtype is 0 or 1", who);
+  if (n < 0) return set_error(kInvalid, "%s: negative row count", who);
+  if (n > kMaxRows) return set_error(kInvalid, "%s: more than %d rows", who, kMaxRows);
+  if (V < 1 || V > kMaxClasses) return set_error(kInvalid, "%s: requires 1<=V<=%d", who, kMaxClasses);
+  if (D < 1 || D > kMaxWidth) return set_error(kInvalid, "%s: requires 1<=D<=%d", who, kMaxWidth);
+  return kOk;
+}
+
+dim3 grid_of(int64_t threads) { return dim3(static_cast<uint32_t>((threads + kBlock - 1) / kBlock)); }
+
+template <typename T, int PARTS>
+int pack(hipStream_t st, int64_t n, const int32_t* count, const int32_t* list, int D, const T* src, int64_t ld,
+         uint16_t* dst, int Kp, int64_t part) {
+  hipLaunchKernelGGL((pack_kernel<T, PARTS>), grid_of(n * (Kp / 8)), dim3(kBlock), 0, st, n, count, list, D, src, ld,
+                     dst, Kp, part);
+  return check_launch("cign_linear_xent (pack)");
+}
+
+template <typename T, int PARTS>
+int pack_t(hipStream_t st, int64_t n, const int32_t* count, const int32_t* list, int D, const T* src, int64_t ld,
+           const void* bias, int bias_f32, uint16_t* dst, int64_t Rp, int64_t part) {
+  hipLaunchKernelGGL((pack_t_kernel<T, PARTS>), dim3(static_cast<uint32_t>((n + 63) / 64), (D + 63) / 64), dim3(kBlock),
+                     0, st, n, count, list, D, src, ld, bias, bias_f32, dst, Rp, part);
+  return check_launch("cign_linear_xent (transpose)");
+}
+
+const void* bias_of(const void* bias, int f32, int64_t v) {
+  return bias ? static_cast<const char*>(bias) + v * (f32 ? 4 : 2) : nullptr;
+}
+
+uint32_t tile_count(int64_t a, int64_t b) {
+  return static_cast<uint32_t>(((a + kTile - 1) / kTile) * ((b + kTile - 1) / kTile));
+}
+
+template <typename T>
+int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, const T* w, int64_t ldw, const void* bias,
+            int bias_f32, const int64_t* labels, int64_t ignore, float* loss, float* lse, void* ws) {
+  constexpr int dtype = std::is_same_v<T, float> ? kF32 : kBF16;
+  constexpr int PARTS = dtype == kF32 ? 3 : 1, SEGS = PARTS == 3 ? 6 : 1;
+  const Cut c = cut(dtype, n, V, D);
+  const bool xin = in_place(dtype, D, x, ldx), win = in_place(dtype, D, w, ldw);
+  FwdSpace s;
+  fwd_space(c, n, V, xin, win, ws, &s);
+  const int nt = (V + kTile - 1) / kTile;
+  if (n <= kFewRows) {
+    const auto launch = [&](auto TC) {
+      hipLaunchKernelGGL((few_kernel<T, decltype(TC)::value>), dim3(nt), dim3(kBlock), 0, st, n, V, D, x, ldx, w, ldw,
+                         bias, bias_f32, labels, s.part, s.chosen);
+    };
+    if (n <= 16) launch(IC<16>());
+    else if (n <= 32) launch(IC<32>());
+    else launch(IC<64>());
+    if (const int rc = check_launch("cign_linear_xent_fwd")) return rc;
+  } else {
+    Operand xo{reinterpret_cast<const uint16_t*>(x), n, ldx, 0};
+    if (!xin) {
+      xo = Operand{s.x, n, c.Kp, n * c.Kp};
+      if (const int rc = pack<T, PARTS>(st, n, nullptr, nullptr, D, x, ldx, s.x, c.Kp, xo.part)) return rc;
+    }
+    const int64_t piece = win ? V : c.fwd_piece;
+    for (int64_t v = 0; v < V; v += piece) {
+      const int64_t vn = std::min<int64_t>(piece, V - v);
+      Operand wo{reinterpret_cast<const uint16_t*>(w + v * ldw), vn, ldw, 0};
+      if (!win) {
+        wo = Operand{s.w, vn, c.Kp, vn * c.Kp};
+        if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, w + v * ldw, ldw, s.w, c.Kp, wo.part)) return rc;
+      }
+      const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, nullptr, labels};
+      hipLaunchKernelGGL((stats_kernel<SEGS>), dim3(tile_count(vn, n)), dim3(ntgemm::kThreads), 0, st, f, n, s.part,
+                         static_cast<int>(v / kTile), s.chosen);
+      if (const int rc = check_launch("cign_linear_xent_fwd")) return rc;
+    }
+  }
+  hipLaunchKernelGGL(join_kernel, dim3(static_cast<uint32_t>((n + kJoinRows - 1) / kJoinRows)), dim3(kBlock), 0, st, n, V,
+                     nt, s.part, labels, ignore, s.chosen, loss, lse);
+  return check_launch("cign_linear_xent_fwd");
+}
+
+template <typename T>
+int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, const T* w, int64_t ldw,
+             const void* bias, int bias_f32, const int64_t* labels, int64_t ignore, const float* lse, const float* g_loss,
+             const float* g_lse, T* gx, T* gw, void* gb, void* ws) {
+  constexpr int dtype = std::is_same_v<T, float> ? kF32 : kBF16;
+  constexpr int PARTS = dtype == kF32 ? 3 : 1, SEGS = PARTS == 3 ? 6 : 1;
+  const char* who = "cign_linear_xent_bwd";
+  const Cut c = cut(dtype, n, V, D);
+  const bool win = in_place(dtype, D, w, ldw);
+  const int of = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
+  BwdSpace s;
+  bwd_space(c, n, V, D, win, of, ws, &s);
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, n, labels, ignore, g_loss, g_lse, s.list, s.place,
+                     s.count);
+  if (const int rc = check_launch(who)) return rc;
+  const Operand xo{s.x, n, c.Kp, n * c.Kp};
+  if (const int rc = pack<T, PARTS>(st, n, s.count, s.list, D, x, ldx, s.x, c.Kp, xo.part)) return rc;
+  const Operand xt{s.xt, D, c.rows_p, c.rows_p * D};
+  if (gw)
+    if (const int rc = pack_t<T, PARTS>(st, n, s.count, s.list, D, x, ldx, nullptr, 0, s.xt, xt.ld, xt.part)) return rc;
+  for (int64_t v = 0; v < V; v += c.piece) {
+    const int64_t vn = std::min<int64_t>(c.piece, V - v), vp = up(vn, kStep);
+    const T* wv = w + v * ldw;
+    Operand wo{reinterpret_cast<const uint16_t*>(wv), vn, ldw, 0};
+    if (!win) {
+      wo = Operand{s.w, vn, c.Kp, vn * c.Kp};
+      if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, wv, ldw, s.w, c.Kp, wo.part)) return rc;
+    }
+    const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, s.count, labels};
+    const Grads g{s.list, lse,   g_loss, g_lse,    ignore,     V,    s.dz, vp,
+                  n * vp, s.dzt, c.rows_p, c.rows_p * vn, s.bias};
+    hipLaunchKernelGGL((grad_kernel<SEGS>), dim3(tile_count(vn, n)), dim3(ntgemm::kThreads), 0, st, f, g);
+    if (const int rc = check_launch(who)) return rc;
+    if (gx) {
+      const Operand wt{s.wt, D, vp, vp * D};
+      if (const int rc = pack_t<T, PARTS>(st, vn, nullptr, nullptr, D, wv, ldw, bias_of(bias, bias_f32, v), bias_f32, s.wt,
+                                            vp, wt.part))
+        return rc;
+      const Operand dz{s.dz, n, vp, n * vp};
+      hipLaunchKernelGGL((out_kernel<float, SEGS, true>), dim3(tile_count(D, n), c.splits), dim3(ntgemm::kThreads), 0, st,
+                         wt, dz, static_cast<int>(vp / kStep), s.count, s.slots, static_cast<int64_t>(c.Dp),
+                         n * c.Dp, v > 0);
+      if (const int rc = check_launch(who)) return rc;
+    }
+    if (gw) {
+      const Operand dzt{s.dzt, vn, c.rows_p, c.rows_p * vn};
+      hipLaunchKernelGGL((out_kernel<T, SEGS, false>), dim3(tile_count(D, vn)), dim3(ntgemm::kThreads), 0, st, xt, dzt, 0,
+                         s.count, gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0);
+      if (const int rc = check_launch(who)) return rc;
+    }
+    if (gb) {
+      if (bias_f32)
+        hipLaunchKernelGGL((bias_kernel<float>), grid_of(vn), dim3(kBlock), 0, st, s.count, vn, s.bias,
+                           static_cast<float*>(gb) + v);
+      else
+        hipLaunchKernelGGL((bias_kernel<bf16>), grid_of(vn), dim3(kBlock), 0, st, s.count, vn, s.bias,
+                           static_cast<bf16*>(gb) + v);
+      if (const int rc = check_launch(who)) return rc;
+    }
+  }
+  if (gx) {
+    hipLaunchKernelGGL((rows_out_kernel<T>), grid_of(n * (c.Dp / 4)), dim3(kBlock), 0, st, n, D, s.place, s.slots,
+                       c.splits, n * c.Dp, c.Dp, gx);
+    return check_launch(who);
+  }
+  return kOk;
+}
+
+}  // namespace xent
+}  // namespace cign
+
+using namespace cign;
+using namespace cign::xent;
+
+extern "C" {
+
+int64_t cign_linear_xent_workspace_bytes(int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x,
+                                         int64_t x_stride, const void* weight, int64_t weight_stride, int32_t of) {
+  if (check_args("cign_linear_xent_workspace_bytes", dtype, n, V, D) || of < 0 || of > 7 || n == 0) return 0;
+  const Cut c = cut(dtype, n, V, D);
+  const bool xin = in_place(dtype, D, x, x_stride), win = in_place(dtype, D, weight, weight_stride);
+  return of ? bwd_space(c, n, V, D, win, of, nullptr, nullptr) : fwd_space(c, n, V, xin, win, nullptr, nullptr);
+}
+
+int cign_linear_xent_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,
+                         const void* weight, int64_t weight_stride, const void* bias, int32_t bias_dtype,
+                         const int64_t* labels, int64_t ignore_index, float* loss, float* logsumexp, void* workspace,
+                         int64_t workspace_bytes) {
+  const char* who = "cign_linear_xent_fwd";
+  if (const int rc = check_args(who, dtype, n, V, D)) return rc;
+  if (bias && bias_dtype != kF32 && bias_dtype != dtype) return set_error(kInvalid, "%s: bias dtype", who);
+  if (n == 0) return kOk;
+  if (!x || !weight || !logsumexp || (loss == nullptr) != (labels == nullptr))
+    return set_error(kInvalid, "%s: null argument", who);
+  if (x_stride < 0 || weight_stride < 0) return set_error(kInvalid, "%s: negative row stride", who);
+  if (!workspace ||
+      workspace_bytes <
+          cign_linear_xent_workspace_bytes(dtype, n, V, D, x, x_stride, weight, weight_stride, 0))
+    return set_error(kInvalid, "%s: workspace too small", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == kF32)
+    return forward<float>(st, n, V, D, static_cast<const float*>(x), x_stride, static_cast<const float*>(weight),
+                          weight_stride, bias, bias_dtype == kF32, labels, ignore_index, loss, logsumexp, workspace);
+  return forward<bf16>(st, n, V, D, static_cast<const bf16*>(x), x_stride, static_cast<const bf16*>(weight),
+                       weight_stride, bias, bias_dtype == kF32, labels, ignore_index, loss, logsumexp, workspace);
+}
+
+int cign_linear_xent_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,
+                         const void* weight, int64_t weight_stride, const void* bias, int32_t bias_dtype,
+                         const int64_t* labels, int64_t ignore_index, const float* logsumexp, const float* grad_loss,
+                         const float* grad_logsumexp, void* grad_x, void* grad_weight, void* grad_bias,
+                         void* workspace, int64_t workspace_bytes) {
+  const char* who = "cign_linear_xent_bwd";
+  if (const int rc = check_args(who, dtype, n, V, D)) return rc;
+  if ((bias || grad_bias) && bias_dtype != kF32 && bias_dtype != dtype)
+    return set_error(kInvalid, "%s: bias dtype", who);
+  const int of = (grad_x ? 1 : 0) | (grad_weight ? 2 : 0) | (grad_bias ? 4 : 0);
+  if (!of) return kOk;
+  if (n == 0) return set_error(kInvalid, "%s: no rows", who);
+  if (!x || !weight || !logsumexp || (!grad_loss && !grad_logsumexp) || (grad_loss && !labels))
+    return set_error(kInvalid, "%s: null argument", who);
+  if (x_stride < 0 || weight_stride < 0) return set_error(kInvalid, "%s: negative row stride", who);
+  if (!workspace ||
+      workspace_bytes <
+          cign_linear_xent_workspace_bytes(dtype, n, V, D, x, x_stride, weight, weight_stride, of))
+    return set_error(kInvalid, "%s: workspace too small", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == kF32)
+    return backward<float>(st, n, V, D, static_cast<const float*>(x), x_stride, static_cast<const float*>(weight),
+                           weight_stride, bias, bias_dtype == kF32, labels, ignore_index, logsumexp, grad_loss,
+                           grad_logsumexp, static_cast<float*>(grad_x), static_cast<float*>(grad_weight), grad_bias,
+                           workspace);
+  return backward<bf16>(st, n, V, D, static_cast<const bf16*>(x), x_stride, static_cast<const bf16*>(weight),
+                        weight_stride, bias, bias_dtype == kF32, labels, ignore_index, logsumexp, grad_loss,
+                        grad_logsumexp, static_cast<bf16*>(grad_x), static_cast<bf16*>(grad_weight), grad_bias,
+                        workspace);
+}
+
+}  // extern "C"

@@ -103,6 +103,15 @@ PyMethodDef methods[] = {
     CIGN_ENTRY(cign_distill_topk_workspace_bytes),
     CIGN_ENTRY(cign_distill_topk_fwd),
     CIGN_ENTRY(cign_distill_topk_bwd),
+    CIGN_ENTRY(cign_block_boundary_fwd),
+    CIGN_ENTRY(cign_block_boundary_bwd_workspace_bytes),
+    CIGN_ENTRY(cign_block_boundary_bwd),
+    CIGN_ENTRY(cign_linear_xent_workspace_bytes),
+    CIGN_ENTRY(cign_linear_xent_fwd),
+    CIGN_ENTRY(cign_linear_xent_bwd),
+    CIGN_ENTRY(cign_grad_norm_workspace_bytes),
+    CIGN_ENTRY(cign_grad_norm),
+    CIGN_ENTRY(cign_clip_grad_norm),
     CIGN_ENTRY(cign_hop_gate_bwd_workspace_bytes),
     CIGN_ENTRY(cign_hop_gate_fwd),
     CIGN_ENTRY(cign_hop_gate_bwd),

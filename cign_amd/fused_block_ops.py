@@ -382,3 +382,57 @@ def fused_layernorm(x, weight=None, bias=None, eps=1e-5):
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     return output_ops().layernorm(x, weight, bias, eps)
+
+
+MAX_BOUNDARY_WIDTH = 8192
+
+
+def fused_gated_residual_norm(branch, residual, post_weight=None, post_bias=None, scale=None, gate=None,
+                              next_weight=None, next_bias=None, eps=1e-5, norm="layer"):
+    """The boundary of two blocks over the last axis, one pass each way:
+
+        v = N(branch) * post_weight + post_bias
+        hidden = residual + scale * sigmoid(gate) * v
+        normed = N(hidden) * next_weight + next_bias
+
+    N(t) = (t - mean) / sqrt(var + eps) for norm "layer" (var the biased
+    variance), t / sqrt(mean(t^2) + eps) for "rms". Returns (hidden, normed):
+    what the next block adds to and what it reads.
+
+    branch, residual: [..., D], both float32 or both bfloat16, 1 <= D <= 8192;
+    row-strided views are read in place. gate: their type, [..., D], or [..., 1]
+    for one gate a row (for D = 1 these are the same), or None for no gate. The
+    five vectors: [D], all float32 or all of branch's type, or None for ones and
+    zeros. Sums are float32; normed is the norm of hidden before it is rounded.
+    Gradients of every input, once differentiable; those of the vectors are summed
+    over the rows in float32, in an order that depends on the shape alone."""
+    D = check_rows(branch, "branch", MAX_BOUNDARY_WIDTH)
+    for t, name in ((residual, "residual"), (gate, "gate")):
+        if t is None and name == "gate":
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != branch.dtype:
+            raise TypeError(f"{name} must be a tensor of branch's type ({branch.dtype})")
+        if t.shape != branch.shape and not (name == "gate" and t.shape == (*branch.shape[:-1], 1)):
+            raise ValueError(f"{name} must have shape {tuple(branch.shape)}"
+                             f"{f' or {(*branch.shape[:-1], 1)}' if name == 'gate' else ''}, got {tuple(t.shape)}")
+        if t.device != branch.device:
+            raise ValueError(f"{name} must be on {branch.device}, got {t.device}")
+    dtype = None
+    for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (scale, "scale"),
+                    (next_weight, "next_weight"), (next_bias, "next_bias")):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, branch.dtype) or dtype not in (None, t.dtype):
+            raise TypeError("the vectors must all be float32 or all of branch's type")
+        if t.shape != (D,):
+            raise ValueError(f"{name} must have shape [{D}], got {tuple(t.shape)}")
+        if t.device != branch.device:
+            raise ValueError(f"{name} must be on {branch.device}, got {t.device}")
+        dtype = t.dtype
+    if norm not in ("layer", "rms"):
+        raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    return output_ops().block_boundary(branch, residual, post_weight, post_bias, scale, gate, next_weight, next_bias,
+                                       eps, norm == "layer")

@@ -41,6 +41,7 @@ from .fused_block_ops import (MAX_LAYERNORM_WIDTH, fused_add_layernorm_cat, fuse
 from .graph import selected_sparse_powers
 from .hop_gate import gated_clifford_pack, global_hop_gate, node_hop_gate
 from .linear import linear_attention_logits, linear_gamma_residual, mfma_linear
+from .linear_cross_entropy import LinearCrossEntropy, linear_cross_entropy
 from .partition import ShardedGAT, prepare_sharded_gat_graph, sharded_collapsed_gat_mean_bias_silu
 
 
@@ -395,8 +396,8 @@ class GraphCliffordNet(nn.Module):
         }
         return dict(self._fused_gat_graph_info)
 
-    def _forward_impl(self, x: torch.Tensor, edge_index: torch.Tensor, graph_operator):
-        """model_cign.py:1160-1204."""
+    def _features(self, x: torch.Tensor, edge_index: torch.Tensor, graph_operator) -> torch.Tensor:
+        """model_cign.py:1160-1200: what the classifier reads."""
         H_in = F.dropout(x, p=self.dropout, training=self.training)
         amp, amp_dtype = self.use_selective_amp, self.selective_amp_dtype
         if self.use_dual_input_projection:
@@ -413,8 +414,22 @@ class GraphCliffordNet(nn.Module):
         # Final LayerNorm and classifier stay in fp32 (the classifier on the
         # fp32 MFMA kernel).
         H_out = self.output_norm(H_out.float())
-        H_out = F.dropout(H_out, p=self.dropout, training=self.training)
-        return mfma_linear(self.classifier, H_out, False).float()
+        return F.dropout(H_out, p=self.dropout, training=self.training)
+
+    def _forward_impl(self, x: torch.Tensor, edge_index: torch.Tensor, graph_operator):
+        """model_cign.py:1160-1204."""
+        return mfma_linear(self.classifier, self._features(x, edge_index, graph_operator), False).float()
+
+    def node_losses(self, x: torch.Tensor, edge_index: torch.Tensor, graph_operator, labels: torch.Tensor,
+                    ignore_index: int = -100) -> LinearCrossEntropy:
+        """Each node's cross entropy against its label (0 where it is
+        ignore_index) and the logsumexp of its logits, differentiable, without
+        the logits [N, out_dim] ever being stored: for classifiers over many
+        classes."""
+        if graph_operator is None:
+            raise ValueError("GraphCliffordNet requires a sparse graph operator as the third input.")
+        return linear_cross_entropy(self._features(x, edge_index, graph_operator), self.classifier.weight, labels,
+                                    bias=self.classifier.bias, ignore_index=ignore_index)
 
     def forward(self, x: torch.Tensor, edge_index: torch.Tensor, graph_operator=None) -> torch.Tensor:
         if graph_operator is None:

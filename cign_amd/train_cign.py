@@ -40,6 +40,7 @@ import torch.nn.functional as F
 from . import graph
 from .class_logprobs import ClassLogprobs, class_logprobs
 from .distill import distill_topk_loss
+from .grad_norm import clip_grad_norm
 
 try:
     from sklearn.metrics import roc_auc_score
@@ -263,11 +264,31 @@ def forward_model(model, data, graph_operator):
     return model(data.x, data.edge_index, graph_operator)
 
 
-def train_one_epoch(model, data, graph_operator, optimizer, device: torch.device,
-                    grad_scaler=None) -> Tuple[float, float]:
+def _optimizer_step(loss, optimizer, grad_scaler, max_grad_norm) -> None:
+    """backward, the parameters' gradients clipped to max_grad_norm (None: not)
+    as they stand after a scaler's unscaling, optimizer step."""
+    scaled = grad_scaler is not None and grad_scaler.is_enabled()
+    (grad_scaler.scale(loss) if scaled else loss).backward()
+    if max_grad_norm is not None:
+        if scaled:
+            grad_scaler.unscale_(optimizer)
+        grads = [p.grad for group in optimizer.param_groups for p in group["params"] if p.grad is not None]
+        if grads:
+            clip_grad_norm(grads, max_grad_norm)
+    if scaled:
+        grad_scaler.step(optimizer)
+        grad_scaler.update()
+    else:
+        optimizer.step()
+
+
+def train_one_epoch(model, data, graph_operator, optimizer, device: torch.device, grad_scaler=None,
+                    max_grad_norm=None, fused_loss: bool = False) -> Tuple[float, float]:
     """One parameter update (zero_grad -> forward -> cross-entropy over the
     train mask -> backward -> optimizer step) and its seconds, timed with
-    events on the GPU as train_cign.py:2103-2148 times it."""
+    events on the GPU as train_cign.py:2103-2148 times it. max_grad_norm clips the
+    optimizer's gradients to that global norm before its step; fused_loss takes the
+    cross-entropy from model.node_losses, without the logits (many classes)."""
     model.train()
     dev = torch.device(device)
     if dev.type != "cuda":
@@ -275,15 +296,14 @@ def train_one_epoch(model, data, graph_operator, optimizer, device: torch.device
     start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
     start.record()
     optimizer.zero_grad()
-    logits = forward_model(model, data, graph_operator)
-    loss = F.cross_entropy(logits[data.train_mask], data.y[data.train_mask])
-    if grad_scaler is not None and grad_scaler.is_enabled():
-        grad_scaler.scale(loss).backward()
-        grad_scaler.step(optimizer)
-        grad_scaler.update()
+    if fused_loss:
+        labels = torch.where(data.train_mask, data.y, -100)
+        losses = model.node_losses(data.x, data.edge_index, graph_operator, labels).loss
+        loss = losses.sum() / data.train_mask.sum()
     else:
-        loss.backward()
-        optimizer.step()
+        logits = forward_model(model, data, graph_operator)
+        loss = F.cross_entropy(logits[data.train_mask], data.y[data.train_mask])
+    _optimizer_step(loss, optimizer, grad_scaler, max_grad_norm)
     end.record()
     end.synchronize()
     return float(loss.detach().item()), start.elapsed_time(end) / 1000.0
@@ -321,12 +341,14 @@ def teacher_targets(model, data, graph_operator, top_k: int, temperature: float 
 
 
 def distill_one_epoch(model, data, graph_operator, optimizer, device: torch.device, targets: TeacherTargets,
-                      weight: float = 0.5, tail: bool = True, grad_scaler=None) -> Tuple[float, float]:
+                      weight: float = 0.5, tail: bool = True, grad_scaler=None,
+                      max_grad_norm=None) -> Tuple[float, float]:
     """train_one_epoch against labels and a teacher: the loss is (1 - weight)
     times the cross-entropy over the train mask plus weight times the mean over
     all nodes of distill_topk_loss (with the tail: the classes outside a node's
     list as one more); a part of weight 0 is left out, so that weight = 1 needs no
-    labelled node. Returns the loss and the step's seconds."""
+    labelled node. max_grad_norm as in train_one_epoch. Returns the loss and the
+    step's seconds."""
     if not 0.0 <= float(weight) <= 1.0:
         raise ValueError(f"weight must be in [0, 1], got {weight}")
     model.train()
@@ -346,13 +368,7 @@ def distill_one_epoch(model, data, graph_operator, optimizer, device: torch.devi
     if weight > 0.0:
         parts.append(weight * distill_topk_loss(logits, targets.logprobs, targets.index, targets.temperature, tail).mean())
     loss = sum(parts[1:], parts[0])
-    if grad_scaler is not None and grad_scaler.is_enabled():
-        grad_scaler.scale(loss).backward()
-        grad_scaler.step(optimizer)
-        grad_scaler.update()
-    else:
-        loss.backward()
-        optimizer.step()
+    _optimizer_step(loss, optimizer, grad_scaler, max_grad_norm)
     end.record()
     end.synchronize()
     return float(loss.detach().item()), start.elapsed_time(end) / 1000.0

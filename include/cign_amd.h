@@ -423,6 +423,98 @@ int cign_distill_topk_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, con
                           float temperature, int32_t K, const int64_t* teacher_index, const float* stats,
                           const float* teacher_mass, const float* grad_loss, void* grad_x);
 
+/* ---- block boundary (float32 or bfloat16, 1 <= D <= 8192) ------------------- */
+
+/* For rows of D values: v = N(branch) * post_weight + post_bias, hidden =
+ * residual + scale * s * v, y = N(hidden) * next_weight + next_bias. N(t) =
+ * (t - mean) / sqrt(var + eps) with layer 1, t / sqrt(mean(t^2) + eps) with 0. s =
+ * sigmoid(gate): gate_kind 0 none (s = 1), 1 one value a row (row r at
+ * r * gate_stride), 2 a value each. x_dtype 0 or 1, of rows and gate; w_dtype, of
+ * the five vectors [D], 0 or x_dtype; each vector may be NULL (ones, zeros).
+ * branch, residual and gate rows lie their strides apart (0 or below D allowed:
+ * they are only read). hidden and y are [n, D]; y is the norm of hidden before
+ * its rounding to x_dtype. stats [4, n] float32 (means and 1 / sigma of branch and
+ * of hidden), or NULL: an evaluation that keeps none. No alignment beyond the
+ * type's own. No counterpart in the reference: its blocks norm before the branch
+ * and have a residual scale (generic_engine/model_cign.py:751-937). */
+int cign_block_boundary_fwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, int32_t layer,
+                            int32_t gate_kind, const void* branch, int64_t branch_stride, const void* residual,
+                            int64_t residual_stride, const void* gate, int64_t gate_stride, const void* post_weight,
+                            const void* post_bias, const void* scale, const void* next_weight, const void* next_bias,
+                            float eps, void* hidden, void* y, float* stats);
+
+/* Workspace bytes of cign_block_boundary_bwd with a vector's gradient. */
+int64_t cign_block_boundary_bwd_workspace_bytes(int64_t n, int32_t D);
+
+/* Gradients of the above given those of hidden and y (one of them may be NULL:
+ * zeros; rows their strides apart): grad_branch, grad_residual [n, D], grad_gate
+ * ([n] or [n, D], x_dtype) and the vectors' [D] (w_dtype), each may be NULL. The
+ * vectors' are float32 sums over the rows in an order that depends on (n, D) alone,
+ * rounded once; without them the workspace may be NULL. */
+int cign_block_boundary_bwd(void* stream, int64_t n, int32_t D, int32_t x_dtype, int32_t w_dtype, int32_t layer,
+                            int32_t gate_kind, const void* grad_hidden, int64_t grad_hidden_stride, const void* grad_y,
+                            int64_t grad_y_stride, const void* branch, int64_t branch_stride, const void* residual,
+                            int64_t residual_stride, const void* gate, int64_t gate_stride, const void* post_weight,
+                            const void* post_bias, const void* scale, const void* next_weight, const float* stats,
+                            void* grad_branch, void* grad_residual, void* grad_gate, void* grad_post_weight,
+                            void* grad_post_bias, void* grad_scale, void* grad_next_weight, void* grad_next_bias,
+                            void* workspace, int64_t workspace_bytes);
+
+/* ---- cross entropy of a linear classifier (1 <= V <= 1048576, D <= 65536) ---- */
+
+/* Workspace bytes of cign_linear_xent_fwd (of 0) and of cign_linear_xent_bwd (of:
+ * 1 grad_x, 2 grad_weight, 4 grad_bias, added up). x and weight are looked at for
+ * their alignment only: rows of bfloat16 that start 16-byte aligned and are a
+ * multiple of 64 values wide are read where they lie, others packed. */
+int64_t cign_linear_xent_workspace_bytes(int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x,
+                                         int64_t x_stride, const void* weight, int64_t weight_stride, int32_t of);
+
+/* For the logits z = x weight^T + bias of n rows (at most 2^23; x [n, D], weight
+ * [V, D], dtype 0 or 1, rows their strides apart; bias [V], bias_dtype 0 or dtype,
+ * or NULL), which are never stored: logsumexp[r] = log sum_v e^z, loss[r] =
+ * logsumexp[r] - z[label[r]], 0 where label[r] is ignore_index, NaN where it is
+ * another value outside [0, V). label and loss may both be NULL. A bias of -inf
+ * masks its class whatever its weight holds; a row without any class left has
+ * logsumexp -inf and loss inf. Products are float32's for dtype 0 (within 2^-22),
+ * exact for 1, sums float32. No counterpart in the reference: torch's Linear and
+ * cross-entropy (generic_engine/model_cign.py:1199, train_cign.py:2123). */
+int cign_linear_xent_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,
+                         const void* weight, int64_t weight_stride, const void* bias, int32_t bias_dtype,
+                         const int64_t* label, int64_t ignore_index, float* loss, float* logsumexp, void* workspace,
+                         int64_t workspace_bytes);
+
+/* Gradients for those of loss and logsumexp (each may be NULL): grad_x [n, D],
+ * grad_weight [V, D] (dtype), grad_bias [V] (bias_dtype), each may be NULL. Rows
+ * whose gradients are zero, an ignored label's among them, take no part whatever
+ * they hold; rows without any class left have none. The sums' order depends on the
+ * shapes and on which rows take part. n >= 1. */
+int cign_linear_xent_bwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,
+                         const void* weight, int64_t weight_stride, const void* bias, int32_t bias_dtype,
+                         const int64_t* label, int64_t ignore_index, const float* logsumexp, const float* grad_loss,
+                         const float* grad_logsumexp, void* grad_x, void* grad_weight, void* grad_bias,
+                         void* workspace, int64_t workspace_bytes);
+
+/* ---- global norm of gradients (float32 and bfloat16) -------------------------- */
+
+/* Workspace bytes of cign_grad_norm and cign_clip_grad_norm for tensors of these
+ * sizes (host array). */
+int64_t cign_grad_norm_workspace_bytes(int32_t count, const int64_t* sizes);
+
+/* norm[0] = sqrt(sum over count tensors of their values' squares), squares and sums
+ * in float64. grads: host array of device pointers; sizes, dtypes (0 or 1): host
+ * arrays. No alignment beyond the type's own. No counterpart in the reference,
+ * whose step does not clip (generic_engine/train_cign.py:2103-2148). */
+int cign_grad_norm(void* stream, int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes,
+                   float* norm, void* workspace, int64_t workspace_bytes);
+
+/* The same, and out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), the factor
+ * float32: NaN where the norm is, 0 where it is infinite. out[i] is grads[i], which
+ * a factor of one leaves alone, or memory that no gradient and no other output
+ * lies in. max_norm >= 0. */
+int cign_clip_grad_norm(void* stream, int32_t count, const void* const* grads, const int64_t* sizes,
+                        const int32_t* dtypes, float max_norm, void* const* out, float* norm, void* workspace,
+                        int64_t workspace_bytes);
+
 /* ---- hop gate (float32) ------------------------------------------------- */
 
 /* Node-mode hop gate: alpha [n,K] = softmax_k(score @ weight^T + bias), score
