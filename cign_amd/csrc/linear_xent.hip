@@ -36,24 +36,23 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int N>
 using IC = std::integral_constant<int, N>;
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // e^d for d = z - m <= 0: relative error |d| 2^-24 and less.
 __device__ __forceinline__ float exp_of(float d) { return exp2_of(d * kLog2e); }
 
-__device__ __forceinline__ uint16_t round_bf16(float v) { return from_f32<bf16>(v).bits; }
-
-// v as PARTS bf16 values whose sum it is to 8 bits each. Parts below a value that
-// is not finite are zero.
+// Two values as PARTS pairs of bf16 whose sums they are to 8 bits each. Parts below a
+// value that is not finite are zero.
 template <int PARTS>
-__device__ __forceinline__ void split(float v, uint16_t (&part)[PARTS]) {
-  part[0] = round_bf16(v);
-  float rest = v;
+__device__ __forceinline__ void split(float lo, float hi, uint32_t (&part)[PARTS]) {
+  part[0] = rowvec::pack_bf16(lo, hi);
 #pragma unroll
   for (int k = 1; k < PARTS; ++k) {
-    rest -= __uint_as_float(static_cast<uint32_t>(part[k - 1]) << 16);
-    part[k] = isfinite(rest) ? round_bf16(rest) : 0;
+    lo -= __uint_as_float(part[k - 1] << 16);
+    hi -= __uint_as_float(part[k - 1] & 0xffff0000u);
+    part[k] = rowvec::pack_bf16(isfinite(lo) ? lo : 0.0f, isfinite(hi) ? hi : 0.0f);
   }
 }
 
@@ -98,26 +97,35 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void stats_kernel(Logits f, in
   const Place at(ia, ib);
   float2* red = reinterpret_cast<float2*>(lds);  // [2][kTile]
   const int wave = threadIdx.x / kWave, l = lane_id();
+  const bool plain = !f.bias && (ia + 1) * kTile <= f.w.rows;  // no class masked or behind the last
   float bias[kFragA][4];
-#pragma unroll
-  for (int fa = 0; fa < kFragA; ++fa)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
-#pragma unroll
-  for (int fb = 0; fb < kFragB; ++fb) {
-    const int64_t row = at.b(fb);
-    const int64_t want = f.labels && row < n ? f.labels[row] - f.first : -1;
-    float m = -INFINITY;
+  if (!plain)
 #pragma unroll
     for (int fa = 0; fa < kFragA; ++fa)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float z = bias[fa][r] == -INFINITY ? -INFINITY : acc[fa][fb][r] + bias[fa][r];
-        acc[fa][fb][r] = z;
-        m = fmaxf(m, z);
-        if (at.a(fa) + r == want && want < f.w.rows) chosen[row] = z;
+      for (int r = 0; r < 4; ++r)
+        bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
+#pragma unroll
+  for (int fb = 0; fb < kFragB; ++fb) {
+    const int64_t row = at.b(fb);
+    // the label's place behind the lane's first class
+    const int64_t in = (f.labels && row < n ? f.labels[row] : -1) - f.first;
+    const int want = in >= at.a0 && in < f.w.rows && in - at.a0 < 128 ? static_cast<int>(in - at.a0) : -1;
+    float m = -INFINITY;
+#pragma unroll
+    for (int fa = 0; fa < kFragA; ++fa) {
+      if (!plain)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[fa][fb][r] = bias[fa][r] == -INFINITY ? -INFINITY : acc[fa][fb][r] + bias[fa][r];
+      const f32x4 z = acc[fa][fb];
+      m = fmaxf(fmaxf(m, fmaxf(z[0], z[1])), fmaxf(z[2], z[3]));
+      if ((want >> 4) == fa) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if ((want & 15) == r) chosen[row] = z[r];
       }
+    }
     const float by = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
@@ -138,9 +146,9 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void stats_kernel(Logits f, in
   }
 }
 
-// Up to 16 T rows: a wavefront takes 64 classes, four tiles of 16, and reads W
-// where it lies; values are fed to the matrix units in the order in which a lane's
-// 16-byte chunks come, rows of x alike. part[workgroup][row] as above.
+// Up to 64 rows: a wavefront takes 64 classes, four tiles of 16; values are fed to the
+// matrix units in the order in which a lane's 16-byte chunks come, those of x alike.
+// part[workgroup][row] as above.
 template <typename T>
 struct Few;
 template <>
@@ -176,53 +184,14 @@ __device__ __forceinline__ typename Few<T>::Raw few_tail(const T* p, int left) {
   return __builtin_bit_cast(typename Few<T>::Raw, v);
 }
 
-constexpr int kFewClasses = 256;  // of a workgroup
+constexpr int kFewClasses = 64;  // of a wavefront
 
-template <typename T, int TOKENS>
-__global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, const T* x, int64_t ldx, const T* w,
-                                                     int64_t ldw, const void* bias, int bias_f32,
-                                                     const int64_t* labels, float2* part, float* chosen) {
-  using F = Few<T>;
-  constexpr int L = F::kLane, TA = 4, TB = TOKENS / 16;
-  __shared__ float2 red[kWavesPerBlock][TOKENS];
-  const int l = lane_id(), wave = wave_id();
-  const int c0 = blockIdx.x * kFewClasses + wave * 64;
-  const int q = l >> 4;
-  const T *wp[TA], *xp[TB];
-#pragma unroll
-  for (int i = 0; i < TA; ++i) wp[i] = w + static_cast<int64_t>(min(c0 + i * 16 + (l & 15), V - 1)) * ldw + q * L;
-#pragma unroll
-  for (int i = 0; i < TB; ++i) xp[i] = x + min(static_cast<int64_t>(i * 16 + (l & 15)), n - 1) * ldx + q * L;
-  f32x4 acc[TA][TB];
-#pragma unroll
-  for (int a = 0; a < TA; ++a)
-#pragma unroll
-    for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  int k = 0;
-#pragma unroll 4
-  for (; k + 4 * L <= D; k += 4 * L) {
-    typename F::Raw a[TA], b[TB];
-#pragma unroll
-    for (int i = 0; i < TA; ++i) a[i] = few_load(wp[i] + k);
-#pragma unroll
-    for (int i = 0; i < TB; ++i) b[i] = few_load(xp[i] + k);
-#pragma unroll
-    for (int i = 0; i < TA; ++i)
-#pragma unroll
-      for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
-  }
-  if (k < D) {
-    typename F::Raw a[TA], b[TB];
-    const int left = D - k - q * L;
-#pragma unroll
-    for (int i = 0; i < TA; ++i) a[i] = few_tail(wp[i] + k, left);
-#pragma unroll
-    for (int i = 0; i < TB; ++i) b[i] = few_tail(xp[i] + k, left);
-#pragma unroll
-    for (int i = 0; i < TA; ++i)
-#pragma unroll
-      for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
-  }
+// Statistics of a wavefront's classes from their products.
+template <int TOKENS>
+__device__ __forceinline__ void few_stats(f32x4 (&acc)[4][TOKENS / 16], int c0, int64_t n, int V, const void* bias,
+                                          int bias_f32, const int64_t* labels, float2* part, float* chosen) {
+  constexpr int TA = 4, TB = TOKENS / 16;
+  const int l = lane_id();
 #pragma unroll
   for (int b = 0; b < TB; ++b) {
     const int64_t row = b * 16 + (l & 15);
@@ -232,7 +201,7 @@ __global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, co
     for (int a = 0; a < TA; ++a)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int v = c0 + a * 16 + q * 4 + r;
+        const int v = c0 + a * 16 + (l >> 4) * 4 + r;
         float z = -INFINITY;
         if (v < V) {
           const float add = bias ? bias_at(bias, bias_f32, v) : 0.0f;
@@ -250,27 +219,175 @@ __global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, co
       for (int r = 0; r < 4; ++r) s += exp_of(acc[a][b][r] - by);
     join(m, s, xor_shfl<16>(m), xor_shfl<16>(s));
     join(m, s, xor_shfl<32>(m), xor_shfl<32>(s));
-    if (l < 16) red[wave][b * 16 + l] = make_float2(m, s);
-  }
-  __syncthreads();
-  if (threadIdx.x < TOKENS && threadIdx.x < n) {
-    float2 t = red[0][threadIdx.x];
-#pragma unroll
-    for (int k2 = 1; k2 < kWavesPerBlock; ++k2) join(t.x, t.y, red[k2][threadIdx.x].x, red[k2][threadIdx.x].y);
-    part[static_cast<int64_t>(blockIdx.x) * n + threadIdx.x] = t;
+    if (l < 16 && row < n) part[static_cast<int64_t>(c0 / kFewClasses) * n + row] = make_float2(m, s);
   }
 }
 
-// loss and lse of 32 rows a workgroup, eight threads a row over its nt tiles; the
-// logarithm and the differences in float64, rounded once.
-constexpr int kJoinRows = 32;
+// Rows of any alignment and width, read from where they lie into registers.
+template <typename T, int TOKENS>
+__global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, const T* x, int64_t ldx, const T* w,
+                                                     int64_t ldw, const void* bias, int bias_f32,
+                                                     const int64_t* labels, float2* part, float* chosen) {
+  using F = Few<T>;
+  constexpr int L = F::kLane, TA = 4, TB = TOKENS / 16;
+  const int l = lane_id();
+  const int c0 = (blockIdx.x * kWavesPerBlock + wave_id()) * kFewClasses;
+  if (c0 >= V) return;
+  const int q = l >> 4;
+  const T *wp[TA], *xp[TB];
+#pragma unroll
+  for (int i = 0; i < TA; ++i) wp[i] = w + static_cast<int64_t>(min(c0 + i * 16 + (l & 15), V - 1)) * ldw + q * L;
+#pragma unroll
+  for (int i = 0; i < TB; ++i) xp[i] = x + min(static_cast<int64_t>(i * 16 + (l & 15)), n - 1) * ldx + q * L;
+  f32x4 acc[TA][TB];
+#pragma unroll
+  for (int a = 0; a < TA; ++a)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto steps = [&](auto UC, int k) {
+    constexpr int U = decltype(UC)::value;
+    typename F::Raw a[U][TA], b[U][TB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < TA; ++i) a[u][i] = few_load(wp[i] + k + u * 4 * L);
+#pragma unroll
+      for (int i = 0; i < TB; ++i) b[u][i] = few_load(xp[i] + k + u * 4 * L);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < TA; ++i)
+#pragma unroll
+        for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[u][i], b[u][j], acc[i][j]);
+  };
+  const int blocks = D / (16 * L), skew = blocks ? blockIdx.x * 13 % blocks : 0;
+  for (int i = 0; i < blocks; ++i) steps(IC<4>(), (i + skew < blocks ? i + skew : i + skew - blocks) * 16 * L);
+  int k = blocks * 16 * L;
+  for (; k + 4 * L <= D; k += 4 * L) steps(IC<1>(), k);
+  if (k < D) {
+    typename F::Raw a[TA], b[TB];
+    const int left = D - k - q * L;
+#pragma unroll
+    for (int i = 0; i < TA; ++i) a[i] = few_tail(wp[i] + k, left);
+#pragma unroll
+    for (int i = 0; i < TB; ++i) b[i] = few_tail(xp[i] + k, left);
+#pragma unroll
+    for (int i = 0; i < TA; ++i)
+#pragma unroll
+      for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
+  }
+  few_stats<TOKENS>(acc, c0, n, V, bias, bias_f32, labels, part, chosen);
+}
+
+// Four 16-byte reads of LDS, 2048 bytes apart, and one, waited for in the same statement.
+__device__ __forceinline__ void read_four(uint32_t at, U32x4 (&v)[4]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n"
+      "ds_read_b128 %1, %4 offset:2048\n"
+      "ds_read_b128 %2, %4 offset:4096\n"
+      "ds_read_b128 %3, %4 offset:6144\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+      : "v"(at)
+      : "memory");
+}
+__device__ __forceinline__ U32x4 read_one(uint32_t at) {
+  U32x4 v;
+  asm volatile("ds_read_b128 %0, %1\ns_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(at) : "memory");
+  return v;
+}
+
+// Rows that start 16-byte aligned and are a multiple of 128 bytes wide: a workgroup is
+// one wavefront; steps of 128 bytes of its 64 classes and of the rows of x go to LDS
+// without passing registers, in a ring of steps. Nothing waits for another wavefront,
+// and what finishes early makes room for the next. Each starts at another step, 13
+// further on than the one before: rows of 8 KB read from their beginnings at the same
+// time lie on few memory channels (one row against 131,072 x 4096 bf16: 186 us = 5.8
+// TB/s, 218 from the beginning; float32 360 and 404). Two steps in the ring are
+// enough for the memory (three 195 us, four 188). float32 rows beyond 16 are bounded
+// by the matrix units, whose SIMDs have to have as many wavefronts each: rings, or
+// room kept free, of 36 to 40 KB, four wavefronts a CU (40 rows: 640 us; five
+// wavefronts a CU 1,010).
+template <typename T, int TOKENS>
+__global__ __launch_bounds__(kWave) void stream_kernel(int64_t n, int V, int D, const T* x, int64_t ldx, const T* w,
+                                                       int64_t ldw, const void* bias, int bias_f32,
+                                                       const int64_t* labels, float2* part, float* chosen) {
+  using F = Few<T>;
+  constexpr int TB = TOKENS / 16;
+  constexpr int kWide = 128 / sizeof(T);                    // values of a step
+  constexpr int kStepBytes = (kFewClasses + TOKENS) * 128;
+  constexpr int kLoads = 8 + 2 * TB;                        // of a step
+  constexpr bool kBound = sizeof(T) == 4 && TOKENS > 16;    // by the matrix units
+  constexpr int RING = kBound && TOKENS == 32 ? 3 : 2;
+  constexpr int kRingBytes = RING * kStepBytes, kKept = kBound && kRingBytes < (33 << 10) ? 40 << 10 : kRingBytes;
+  static_assert(kLoads * (RING - 1) < 63, "vmcnt");
+  __shared__ __attribute__((aligned(1024))) char mine[kKept];
+  const int l = lane_id();
+  const int c0 = blockIdx.x * kFewClasses;
+  const int r8 = l >> 3, chunk = ((l & 7) ^ r8) * (16 / static_cast<int>(sizeof(T)));
+  const T *wp[8], *xp[2 * TB];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wp[j] = w + static_cast<int64_t>(min(c0 + j * 8 + r8, V - 1)) * ldw + chunk;
+#pragma unroll
+  for (int j = 0; j < 2 * TB; ++j) xp[j] = x + min(static_cast<int64_t>(j * 8 + r8), n - 1) * ldx + chunk;
+  const int total = D / kWide;
+  const int skew = blockIdx.x * 13 % total;
+  const auto load = [&](int step) {
+    char* to = mine + (step % RING) * kStepBytes;
+    const int t = step + skew < total ? step + skew : step + skew - total;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      __builtin_amdgcn_global_load_lds((ntgemm::GlobalPtr)(wp[j] + t * kWide), (ntgemm::LdsPtr)(to + j * 1024), 16, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2 * TB; ++j)
+      __builtin_amdgcn_global_load_lds((ntgemm::GlobalPtr)(xp[j] + t * kWide), (ntgemm::LdsPtr)(to + 8192 + j * 1024), 16,
+                                       0, 0);
+  };
+  f32x4 acc[4][TB];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < RING - 1 && t < total; ++t) load(t);
+  const int row = l & 15;
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((ntgemm::LdsPtr)mine)) + row * 128;
+  for (int t = 0; t < total; ++t) {
+    // what step t - 1 held was read and waited for
+    if (t + RING - 1 < total) {
+      load(t + RING - 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads * (RING - 1)) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const uint32_t from = base + (t % RING) * kStepBytes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t at = from + (((4 * h + (l >> 4)) ^ (row & 7)) << 4);
+      U32x4 a[4];
+      read_four(at, a);
+#pragma unroll
+      for (int j = 0; j < TB; ++j) {
+        const U32x4 b = read_one(at + 8192 + j * 2048);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[i][j] = F::mul(__builtin_bit_cast(typename F::Raw, a[i]), __builtin_bit_cast(typename F::Raw, b), acc[i][j]);
+      }
+    }
+  }
+  few_stats<TOKENS>(acc, c0, n, V, bias, bias_f32, labels, part, chosen);
+}
+
+// loss and lse of ROWS rows a workgroup, 256 / ROWS threads a row over its nt tiles;
+// the logarithm and the differences in float64, rounded once.
+template <int ROWS>
 __global__ __launch_bounds__(kBlock) void join_kernel(int64_t n, int V, int nt, const float2* part,
                                                       const int64_t* labels, int64_t ignore, const float* chosen,
                                                       float* loss, float* lse) {
-  constexpr int kParts = kBlock / kJoinRows;
-  __shared__ float2 red[kParts][kJoinRows];
-  const int j = threadIdx.x % kJoinRows, k = threadIdx.x / kJoinRows;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + j;
+  constexpr int kParts = kBlock / ROWS;
+  __shared__ float2 red[kParts][ROWS];
+  const int j = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + j;
   float m = -INFINITY, s = 0.0f;
   if (row < n)
     for (int t = k; t < nt; t += kParts) {
@@ -279,9 +396,14 @@ __global__ __launch_bounds__(kBlock) void join_kernel(int64_t n, int V, int nt, 
     }
   red[k][j] = make_float2(m, s);
   __syncthreads();
+  for (int h = kParts / 2; h > 0; h >>= 1) {
+    if (k < h) {
+      join(m, s, red[k + h][j].x, red[k + h][j].y);
+      red[k][j] = make_float2(m, s);
+    }
+    __syncthreads();
+  }
   if (k || row >= n) return;
-#pragma unroll
-  for (int t = 1; t < kParts; ++t) join(m, s, red[t][j].x, red[t][j].y);
   const double logs = log(static_cast<double>(s));
   lse[row] = static_cast<float>(static_cast<double>(m) + logs);
   if (!loss) return;
@@ -299,43 +421,54 @@ __global__ __launch_bounds__(kBlock) void join_kernel(int64_t n, int V, int nt, 
 }
 
 // Rows with a gradient, in order: list[0..count), and each row's place in it or -1.
+// One workgroup, 8192 rows at a time: a vote a wavefront for each 64 rows, the votes'
+// counts added up in the rows' order.
 __global__ __launch_bounds__(1024) void rows_kernel(int64_t n, const int64_t* labels, int64_t ignore,
                                                     const float* g_loss, const float* g_lse, int32_t* list,
                                                     int32_t* place, int32_t* count) {
-  __shared__ int32_t sums[16], base;
-  constexpr int kEach = 8;
-  if (threadIdx.x == 0) base = 0;
-  __syncthreads();
+  constexpr int kEach = 8, kWaves = 1024 / kWave;
+  __shared__ int32_t sums[kEach * kWaves];
+  int32_t base = 0;
+  const uint64_t below = (1ull << lane_id()) - 1;
   for (int64_t b = 0; b < n; b += 1024 * kEach) {
-    const int64_t r0 = b + threadIdx.x * kEach;
-    bool on[kEach];
-    int mine = 0;
+    uint64_t votes[kEach];
+    int64_t y[kEach];
+    float g[kEach], h[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {  // every load before the first test
+      const int64_t r = min(b + i * 1024 + threadIdx.x, n - 1);
+      y[i] = g_loss ? labels[r] : 0;
+      g[i] = g_loss ? g_loss[r] : 0.0f;
+      h[i] = g_lse ? g_lse[r] : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int64_t r = r0 + i;
-      on[i] = r < n && ((g_loss && labels[r] != ignore && g_loss[r] != 0.0f) || (g_lse && g_lse[r] != 0.0f));
-      mine += on[i];
+      const bool on = b + i * 1024 + threadIdx.x < n && ((y[i] != ignore && g[i] != 0.0f) || h[i] != 0.0f);
+      votes[i] = __ballot(on);
+      if (lane_id() == 0) sums[i * kWaves + wave_id()] = __popcll(votes[i]);
     }
-    int before = mine;
+    __syncthreads();
+    // sums[k]: rows before the 64 of vote k, in every wavefront's lanes two by two
+    const int a = sums[2 * lane_id()], c = sums[2 * lane_id() + 1];
+    int upto = a + c;
     for (int o = 1; o < kWave; o <<= 1) {
-      const int t = __shfl_up(before, o, kWave);
-      if (lane_id() >= o) before += t;
+      const int t = __shfl_up(upto, o, kWave);
+      if (lane_id() >= o) upto += t;
     }
-    if (lane_id() == kWave - 1) sums[wave_id()] = before;
-    __syncthreads();
-    int at = base + before - mine, total = 0;
-    for (int wv = 0; wv < 16; ++wv) {
-      if (wv < wave_id()) at += sums[wv];
-      total += sums[wv];
-    }
+    const int all = __shfl(upto, kWave - 1, kWave);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      if (r0 + i >= n) continue;
-      place[r0 + i] = on[i] ? at : -1;
-      if (on[i]) list[at++] = static_cast<int32_t>(r0 + i);
+      const int k = i * kWaves + wave_id();
+      const int before = __shfl(k & 1 ? upto - c : upto - a - c, k >> 1, kWave);
+      const int64_t r = b + i * 1024 + threadIdx.x;
+      const int at = base + before + __popcll(votes[i] & below);
+      if (r < n) {
+        const bool on = votes[i] >> lane_id() & 1;
+        place[r] = on ? at : -1;
+        if (on) list[at] = static_cast<int32_t>(r);
+      }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) base += total;
+    base += all;
     __syncthreads();
   }
   if (threadIdx.x == 0) *count = base;
@@ -359,17 +492,16 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* 
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = c + k < D ? to_f32(row[c + k]) : 0.0f;
   }
-  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-  u16x8 o[PARTS];
+  U32x4 o[PARTS];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    uint16_t p[PARTS];
-    split<PARTS>(v[k], p);
+  for (int k = 0; k < 4; ++k) {
+    uint32_t p[PARTS];
+    split<PARTS>(v[2 * k], v[2 * k + 1], p);
 #pragma unroll
     for (int q = 0; q < PARTS; ++q) o[q][k] = p[q];
   }
 #pragma unroll
-  for (int q = 0; q < PARTS; ++q) *reinterpret_cast<u16x8*>(dst + q * part + r * Kp + c) = o[q];
+  for (int q = 0; q < PARTS; ++q) *reinterpret_cast<U32x4*>(dst + q * part + r * Kp + c) = o[q];
 }
 
 // The same transposed: dst[c][r], rows of dst Rp values apart, zeros for rows
@@ -405,20 +537,19 @@ __global__ __launch_bounds__(kBlock) void pack_t_kernel(int64_t n, const int32_t
   }
   __syncthreads();
   if (c0 + a >= D) return;
-  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    u16x8 o[PARTS];
+    U32x4 o[PARTS];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      uint16_t p[PARTS];
-      split<PARTS>(tile[b + 8 * h + k][a], p);
+    for (int k = 0; k < 4; ++k) {
+      uint32_t p[PARTS];
+      split<PARTS>(tile[b + 8 * h + 2 * k][a], tile[b + 8 * h + 2 * k + 1][a], p);
 #pragma unroll
       for (int q = 0; q < PARTS; ++q) o[q][k] = p[q];
     }
 #pragma unroll
     for (int q = 0; q < PARTS; ++q)
-      *reinterpret_cast<u16x8*>(dst + q * part + static_cast<int64_t>(c0 + a) * Rp + r0 + b + 8 * h) = o[q];
+      *reinterpret_cast<U32x4*>(dst + q * part + static_cast<int64_t>(c0 + a) * Rp + r0 + b + 8 * h) = o[q];
   }
 }
 
@@ -439,6 +570,56 @@ struct Grads {
   float* bias_part;        // [tile of rows][class of the piece] or null
 };
 
+// A tile of 256 x 256 16-bit values in LDS, rows of 512 bytes and 16 more, so that
+// neither a column's nor a row's accesses meet on few banks.
+constexpr int kStageRow = kTile * 2 + 16;
+static_assert(kTile * kStageRow <= ntgemm::kLdsBytes, "a tile of results fits the operands' LDS");
+
+// Writes the staged tile to global rows `ld` values apart, 16 bytes a lane, 512 a
+// row: rows below `rows`, values below `cols` (of the tile), chunks whole where cols
+// is a multiple of 8, value by value at a ragged end.
+template <bool RAGGED>
+__device__ __forceinline__ void store_tile(const char* lds, uint16_t* out, int64_t ld, int rows, int cols) {
+  typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
+  const int c = (threadIdx.x & 31) * 8;
+#pragma unroll 4
+  for (int r = threadIdx.x >> 5; r < kTile; r += ntgemm::kThreads / 32) {
+    if (r >= rows || c >= cols) continue;
+    const U32x4 v = *reinterpret_cast<const U32x4*>(lds + r * kStageRow + c * 2);
+    uint16_t* to = out + r * ld + c;
+    if (!RAGGED) {
+      *reinterpret_cast<U32x4*>(to) = v;
+    } else if (c + 8 <= cols) {
+      *reinterpret_cast<Any*>(to) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < cols) to[i] = static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// Stages four consecutive rows of A by one of B a lane: [row of B][row of A].
+__device__ __forceinline__ void stage(char* lds, int fa, int fb, uint32_t first, uint32_t second) {
+  const int w = threadIdx.x / kWave, l = lane_id();
+  *reinterpret_cast<uint2*>(lds + ((w >> 1) * 64 + fb * 16 + (l & 15)) * kStageRow +
+                            ((w & 1) * 128 + fa * 16 + (l >> 4) * 4) * 2) = make_uint2(first, second);
+}
+
+// The same transposed, [row of A][row of B]: two neighbouring lanes exchange two of
+// their values, so that each has two rows of A for both of its rows of B.
+__device__ __forceinline__ void stage_t(char* lds, int fa, int fb, uint32_t first, uint32_t second) {
+  const int w = threadIdx.x / kWave, l = lane_id();
+  const bool odd = l & 1;
+  const uint32_t give = odd ? first : second, keep = odd ? second : first;
+  const uint32_t got = __float_as_uint(dpp<0xB1>(__uint_as_float(give)));  // of the lane beside
+  const uint32_t even_lane = odd ? got : keep, odd_lane = odd ? keep : got;
+  char* to = lds + ((w & 1) * 128 + fa * 16 + (l >> 4) * 4 + 2 * odd) * kStageRow +
+             ((w >> 1) * 64 + fb * 16 + (l & 14)) * 2;
+  *reinterpret_cast<uint32_t*>(to) = (even_lane & 0xffff) | (odd_lane << 16);
+  *reinterpret_cast<uint32_t*>(to + kStageRow) = (even_lane >> 16) | (odd_lane & 0xffff0000u);
+}
+
 template <int SEGS>
 __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Grads g) {
   constexpr int PARTS = SEGS > 1 ? 3 : 1;
@@ -454,98 +635,151 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
   ntgemm::product<SEGS>(f.w, x, ia, ib, f.ksteps, lds, acc);
   const Place at(ia, ib);
   const int wave = threadIdx.x / kWave, l = lane_id();
-  const int64_t Vp = (f.w.rows + kStep - 1) / kStep * kStep, np = (n + kStep - 1) / kStep * kStep;
-  float sums[kFragA][4];
-  float bias[kFragA][4];
-#pragma unroll
-  for (int fa = 0; fa < kFragA; ++fa)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sums[fa][r] = 0.0f;
-      bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
-    }
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kTile), n - static_cast<int64_t>(ib) * kTile));
+  const int classes = static_cast<int>(min(static_cast<int64_t>(kTile), f.w.rows - static_cast<int64_t>(ia) * kTile));
+  const int a0 = (wave & 1) * 128 + (l >> 4) * 4;  // the lane's first class in the tile
+  float own[kFragB], all[kFragB], shift[kFragB];
+  int want[kFragB];  // the label's place behind the lane's first class
 #pragma unroll
   for (int fb = 0; fb < kFragB; ++fb) {
     const int64_t row = at.b(fb);
-    float own = 0.0f, all = 0.0f, shift = 0.0f;
-    int64_t want = -1;
-    bool some = false;
+    own[fb] = all[fb] = 0.0f;
+    shift[fb] = INFINITY;  // e^(z - inf) = 0
+    want[fb] = -1;
     if (row < n) {
       const int64_t src = g.list[row];
       const int64_t y = f.labels ? f.labels[src] : g.ignore;
       if (y != g.ignore && g.g_loss) {
-        own = g.g_loss[src];
-        if (y < 0 || y >= g.V) own = NAN;
+        own[fb] = g.g_loss[src];
+        if (y < 0 || y >= g.V) own[fb] = NAN;
       }
-      want = y - f.first;
-      all = own + (g.g_lse ? g.g_lse[src] : 0.0f);
-      shift = g.lse[src];
-      some = shift != -INFINITY;  // a class is left
-    }
-#pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa) {
-      float d[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float z = acc[fa][fb][r] + bias[fa][r];
-        const float p = bias[fa][r] == -INFINITY || !some ? 0.0f : exp_of(z - shift);
-        d[r] = all * p;
-        if (some && at.a(fa) + r == want && want < f.w.rows) d[r] -= own;
-        if (row >= n || at.a(fa) + r >= f.w.rows) d[r] = 0.0f;
-        sums[fa][r] += d[r];
-      }
-      uint16_t o[4][PARTS];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) split<PARTS>(d[r], o[r]);
-#pragma unroll
-      for (int q = 0; q < PARTS; ++q) {
-        if (g.dz && row < n && at.a(fa) < Vp)
-          *reinterpret_cast<uint2*>(g.dz + q * g.part + row * g.ld + at.a(fa)) =
-              make_uint2(o[0][q] | (static_cast<uint32_t>(o[1][q]) << 16), o[2][q] | (static_cast<uint32_t>(o[3][q]) << 16));
-        if (g.dzt && row < np)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (at.a(fa) + r < f.w.rows) g.dzt[q * g.partt + (at.a(fa) + r) * g.ldt + row] = o[r][q];
+      all[fb] = own[fb] + (g.g_lse ? g.g_lse[src] : 0.0f);
+      const float lse = g.lse[src];
+      if (lse != -INFINITY) {  // a class is left
+        shift[fb] = lse;
+        const int64_t in = y - f.first - static_cast<int64_t>(ia) * kTile;
+        if (in >= 0 && in < classes) want[fb] = static_cast<int>(in) - a0;
       }
     }
   }
-  if (!g.bias_part) return;
   float* red = reinterpret_cast<float*>(lds);  // [4][kTile]
+  // PLAIN: a whole tile without bias, where nothing is masked
+  const auto gradients = [&](auto PLAIN) {
 #pragma unroll
-  for (int fa = 0; fa < kFragA; ++fa)
+    for (int fa = 0; fa < kFragA; ++fa) {
+      float bias[4], sum[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float s = sums[fa][r];
-      s += xor_shfl<1>(s);
-      s += xor_shfl<2>(s);
-      s += xor_shfl<4>(s);
-      s += xor_shfl<8>(s);
-      if ((l & 15) == 0) red[(wave >> 1) * kTile + (wave & 1) * 128 + fa * 16 + (l >> 4) * 4 + r] = s;
+      for (int r = 0; r < 4; ++r) {
+        sum[r] = 0.0f;
+        if (!PLAIN) bias[r] = a0 + fa * 16 + r < classes ? f.bias_of(at.a(fa) + r) : -INFINITY;
+      }
+#pragma unroll
+      for (int fb = 0; fb < kFragB; ++fb) {
+        float d[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (PLAIN) {
+            d[r] = all[fb] * exp_of(acc[fa][fb][r] - shift[fb]);
+          } else {
+            d[r] = all[fb] * exp_of(acc[fa][fb][r] + bias[r] - shift[fb]);
+            // rows behind the last, classes masked or behind the last: whatever they hold
+            if (bias[r] == -INFINITY || shift[fb] == INFINITY) d[r] = 0.0f;
+          }
+        }
+        if ((want[fb] >> 4) == fa) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if ((want[fb] & 15) == r) d[r] -= own[fb];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[fa][fb][r] = d[r];
+          sum[r] += d[r];
+        }
+      }
+      if (!PLAIN && g.bias_part) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          sum[r] += xor_shfl<1>(sum[r]);
+          sum[r] += xor_shfl<2>(sum[r]);
+          sum[r] += xor_shfl<4>(sum[r]);
+          sum[r] += xor_shfl<8>(sum[r]);
+          if ((l & 15) == 0) red[(wave >> 1) * kTile + a0 + fa * 16 + r] = sum[r];
+        }
+      }
     }
-  __syncthreads();
-  const int64_t v = static_cast<int64_t>(ia) * kTile + threadIdx.x;
-  if (threadIdx.x < kTile && v < f.w.rows)
-    g.bias_part[static_cast<int64_t>(ib) * f.w.rows + v] = (red[threadIdx.x] + red[kTile + threadIdx.x]) +
-                                                           (red[2 * kTile + threadIdx.x] + red[3 * kTile + threadIdx.x]);
+  };
+  if (!f.bias && rows == kTile && classes == kTile) {
+    gradients(std::true_type());
+  } else {
+    gradients(std::false_type());
+    if (g.bias_part) {
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < classes)
+        g.bias_part[static_cast<int64_t>(ib) * f.w.rows + static_cast<int64_t>(ia) * kTile + threadIdx.x] =
+            (red[threadIdx.x] + red[kTile + threadIdx.x]) + (red[2 * kTile + threadIdx.x] + red[3 * kTile + threadIdx.x]);
+      __syncthreads();
+    }
+  }
+  // each part as it stands, then transposed, through LDS; zeros up to the next
+  // multiple of kStep of either axis
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    const auto part = [&](const f32x4& d, uint32_t& first, uint32_t& second) {
+      uint32_t lo[PARTS], hi[PARTS];
+      split<PARTS>(d[0], d[1], lo);
+      split<PARTS>(d[2], d[3], hi);
+      first = lo[q];
+      second = hi[q];
+    };
+    if (g.dz) {
+#pragma unroll
+      for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+        for (int fb = 0; fb < kFragB; ++fb) {
+          uint32_t first, second;
+          part(acc[fa][fb], first, second);
+          stage(lds, fa, fb, first, second);
+        }
+      __syncthreads();
+      store_tile<false>(lds, g.dz + q * g.part + static_cast<int64_t>(ib) * kTile * g.ld + static_cast<int64_t>(ia) * kTile,
+                        g.ld, rows, (classes + kStep - 1) / kStep * kStep);
+      __syncthreads();
+    }
+    if (g.dzt) {
+#pragma unroll
+      for (int fa = 0; fa < kFragA; ++fa)
+#pragma unroll
+        for (int fb = 0; fb < kFragB; ++fb) {
+          uint32_t first, second;
+          part(acc[fa][fb], first, second);
+          stage_t(lds, fa, fb, first, second);
+        }
+      __syncthreads();
+      store_tile<false>(lds, g.dzt + q * g.partt + static_cast<int64_t>(ia) * kTile * g.ldt + static_cast<int64_t>(ib) * kTile,
+                        g.ldt, classes, (rows + kStep - 1) / kStep * kStep);
+      __syncthreads();
+    }
+  }
 }
 
-// out[b][a] = sum_k A[a][k] B[b][k]: the weight's gradient (SLOT false: rounded to
-// T, ldo = a row's values), or a part of the rows' gradient (float32, added to
-// what earlier pieces left; blockIdx.y takes a run of the K steps).
+// out[b][a] = sum_k A[a][k] B[b][k], rows of out `ldo` values apart. SLOT: float32
+// sums of a run of the K steps, blockIdx.y's, added to what earlier pieces left
+// (accumulate); else rounded to T. The rows at work are the gradient's rows of B
+// (rows_of_b) or the K axis.
 template <typename T, int SEGS, bool SLOT>
-__global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Operand b, int ksteps,
+__global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Operand b, int ksteps, bool rows_of_b,
                                                                   const int32_t* count, T* out, int64_t ldo,
                                                                   int64_t slot, int accumulate) {
   __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  if (rows_of_b) b.rows = *count;
+  else ksteps = (*count + kStep - 1) / kStep;
   if (SLOT) {
-    b.rows = *count;
     const int each = (ksteps + gridDim.y - 1) / gridDim.y, from = blockIdx.y * each;
     ksteps = max(0, min(each, ksteps - from));
     a.p += static_cast<int64_t>(from) * kStep;
     b.p += static_cast<int64_t>(from) * kStep;
     out += blockIdx.y * slot;
-  } else {
-    ksteps = (*count + kStep - 1) / kStep;
   }
   const int ta = tiles(a.rows), tb = tiles(b.rows);
   if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(ta) * tb) return;
@@ -554,27 +788,44 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Ope
   f32x4 acc[kFragA][kFragB];
   ntgemm::product<SEGS>(a, b, ia, ib, ksteps, lds, acc);
   const Place at(ia, ib);
+  if constexpr (std::is_same_v<T, bf16>) {
 #pragma unroll
-  for (int fb = 0; fb < kFragB; ++fb) {
-    if (at.b(fb) >= b.rows) continue;
-    T* row = out + at.b(fb) * ldo;
+    for (int fb = 0; fb < kFragB; ++fb)
 #pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa) {
-      const int64_t i = at.a(fa);
-      if (i >= a.rows) continue;
-      if constexpr (SLOT) {  // rows of a multiple of four floats
-        f32x4* to = reinterpret_cast<f32x4*>(row + i);
-        *to = accumulate ? *to + acc[fa][fb] : acc[fa][fb];
-      } else {
+      for (int fa = 0; fa < kFragA; ++fa) {
+        const f32x4 v = acc[fa][fb];
+        stage(lds, fa, fb, rowvec::pack_bf16(v[0], v[1]), rowvec::pack_bf16(v[2], v[3]));
+      }
+    __syncthreads();
+    uint16_t* to = reinterpret_cast<uint16_t*>(out) + static_cast<int64_t>(ib) * kTile * ldo + static_cast<int64_t>(ia) * kTile;
+    store_tile<true>(lds, to, ldo, static_cast<int>(min(static_cast<int64_t>(kTile), b.rows - static_cast<int64_t>(ib) * kTile)),
+                     static_cast<int>(min(static_cast<int64_t>(kTile), a.rows - static_cast<int64_t>(ia) * kTile)));
+  } else {
+    typedef float Any __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (i + r < a.rows) row[i + r] = from_f32<T>(acc[fa][fb][r]);
+    for (int fb = 0; fb < kFragB; ++fb) {
+      if (at.b(fb) >= b.rows) continue;
+      T* row = out + at.b(fb) * ldo;
+#pragma unroll
+      for (int fa = 0; fa < kFragA; ++fa) {
+        const int64_t i = at.a(fa);
+        if (SLOT) {  // rows of a multiple of four floats
+          f32x4* to = reinterpret_cast<f32x4*>(row + i);
+          if (i < a.rows) *to = accumulate ? *to + acc[fa][fb] : acc[fa][fb];
+        } else if (i + 4 <= a.rows) {
+          *reinterpret_cast<Any*>(row + i) = acc[fa][fb];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (i + r < a.rows) row[i + r] = acc[fa][fb][r];
+        }
       }
     }
   }
 }
 
-// grad_x of all rows from the slots of those with a gradient, zeros elsewhere.
+// Rows of a gradient from its slots' sums: grad_x of all rows from those of the rows
+// with a gradient, by their places (zeros elsewhere), or without places.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, const int32_t* place, const float* slots,
                                                           int ns, int64_t slot, int Dp, T* gx) {
@@ -583,23 +834,33 @@ __global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, cons
   const int64_t r = i / per;
   const int c = static_cast<int>(i - r * per) * 4;
   if (r >= n) return;
-  const int p = place[r];
+  const int64_t p = place ? place[r] : r;
   f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
   if (p >= 0)
-    for (int s = 0; s < ns; ++s) v += *reinterpret_cast<const f32x4*>(slots + s * slot + static_cast<int64_t>(p) * Dp + c);
+    for (int s = 0; s < ns; ++s) v += *reinterpret_cast<const f32x4*>(slots + s * slot + p * Dp + c);
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (c + k < D) gx[r * D + c + k] = from_f32<T>(v[k]);
 }
 
-// grad_b of a piece from the tiles' sums.
+// grad_b of a piece from the tiles' sums: 32 classes a workgroup, eight slices of the
+// tiles, then the slices in order.
+constexpr int kBiasCols = 32;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void bias_kernel(const int32_t* count, int64_t V, const float* part, T* gb) {
-  const int64_t v = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-  if (v >= V) return;
+  constexpr int kSlices = kBlock / kBiasCols;
+  __shared__ float red[kSlices][kBiasCols];
+  const int c = threadIdx.x % kBiasCols, k = threadIdx.x / kBiasCols;
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kBiasCols + c;
   const int nt = tiles(*count);
   float s = 0.0f;
-  for (int t = 0; t < nt; ++t) s += part[t * V + v];
+  if (v < V)
+    for (int t = k; t < nt; t += kSlices) s += part[t * V + v];
+  red[k][c] = s;
+  __syncthreads();
+  if (k || v >= V) return;
+#pragma unroll
+  for (int t = 1; t < kSlices; ++t) s += red[t][c];
   gb[v] = from_f32<T>(s);
 }
 
@@ -609,10 +870,14 @@ __global__ __launch_bounds__(kBlock) void bias_kernel(const int32_t* count, int6
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
+// Rows that start 16-byte aligned.
+bool rows_aligned(const void* p, int64_t ld, int64_t size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+}
+
 // Rows that the tiles read where they lie (their offsets in a tile are 32 bits).
 bool in_place(int dtype, int D, const void* p, int64_t ld) {
-  return dtype == kBF16 && D % kStep == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 &&
-         ld <= (1 << 24);
+  return dtype == kBF16 && D % kStep == 0 && rows_aligned(p, ld, 2) && ld <= (1 << 24);
 }
 
 struct Cut {
@@ -621,9 +886,11 @@ struct Cut {
   int64_t piece;             // classes of a piece of the backward
   int64_t rows_p;            // rows to the next multiple of kStep
   int splits;                // slots of the rows' gradient
+  int wsplits;               // slots of the weight's gradient, 1: none
   int Dp;
 };
 
+constexpr int kCus = 256;
 constexpr int64_t kPieceValues = 64ll << 20;   // of dz in a piece
 constexpr int64_t kPackValues = 256ll << 20;   // of packed classes in a piece of the forward
 
@@ -641,10 +908,14 @@ Cut cut(int dtype, int64_t n, int64_t V, int D) {
   c.piece = even(std::min<int64_t>(kPieceValues / std::max<int64_t>(kStep, c.rows_p),
                                    kPackValues / (c.parts * static_cast<int64_t>(c.Kp))));
   c.Dp = static_cast<int>(up(D, 4));
-  // workgroups for every CU, two rounds of them
-  const int64_t t = ((n + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
-  const int64_t most = std::max<int64_t>(1, up(std::min(c.piece, V), kStep) / kStep / 8);
-  c.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(1, t), most, 32})));
+  // Few tiles: their K steps cut into slots, so that all 256 CUs have a workgroup, as
+  // long as a slot keeps eight steps.
+  const auto slots = [](int64_t tiles, int64_t steps) {
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kCus / std::max<int64_t>(1, tiles), steps / 8, 32})));
+  };
+  const int64_t cols = (D + kTile - 1) / kTile, most = std::min(c.piece, V);
+  c.splits = slots((n + kTile - 1) / kTile * cols, up(most, kStep) / kStep);
+  c.wsplits = slots((most + kTile - 1) / kTile * cols, c.rows_p / kStep);
   return c;
 }
 
@@ -661,6 +932,12 @@ struct Regions {
   }
 };
 
+// Sets of classes whose statistics are joined.
+int64_t stat_tiles(int64_t n, int64_t V) {
+  const int64_t classes = n <= kFewRows ? kFewClasses : kTile;
+  return (V + classes - 1) / classes;
+}
+
 struct FwdSpace {
   float2* part;
   float* chosen;
@@ -671,7 +948,7 @@ struct FwdSpace {
 int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void* p, FwdSpace* s) {
   Regions r(p);
   FwdSpace f;
-  f.part = r.take<float2>(n * ((V + kTile - 1) / kTile));
+  f.part = r.take<float2>(n * stat_tiles(n, V));
   f.chosen = r.take<float>(n);
   f.x = f.w = nullptr;
   if (n > kFewRows) {
@@ -685,7 +962,7 @@ int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void
 struct BwdSpace {
   int32_t *list, *place, *count;
   uint16_t *x, *xt, *w, *wt, *dz, *dzt;
-  float *slots, *bias;
+  float *slots, *wslots, *bias;
 };
 
 int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, void* p, BwdSpace* s) {
@@ -705,6 +982,7 @@ int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, 
   if (of & 2) {
     b.xt = r.take<uint16_t>(c.parts * c.rows_p * D);
     b.dzt = r.take<uint16_t>(c.parts * c.rows_p * vc);
+    if (c.wsplits > 1) b.wslots = r.take<float>(c.wsplits * vc * c.Dp);
   }
   if (of & 4) b.bias = r.take<float>(((n + kTile - 1) / kTile) * vc);
   if (s) *s = b;
@@ -755,11 +1033,17 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
   const bool xin = in_place(dtype, D, x, ldx), win = in_place(dtype, D, w, ldw);
   FwdSpace s;
   fwd_space(c, n, V, xin, win, ws, &s);
-  const int nt = (V + kTile - 1) / kTile;
+  const int nt = static_cast<int>(stat_tiles(n, V));
   if (n <= kFewRows) {
+    const bool stream = rows_aligned(x, ldx, sizeof(T)) && rows_aligned(w, ldw, sizeof(T)) && D % (128 / sizeof(T)) == 0;
     const auto launch = [&](auto TC) {
-      hipLaunchKernelGGL((few_kernel<T, decltype(TC)::value>), dim3(nt), dim3(kBlock), 0, st, n, V, D, x, ldx, w, ldw,
-                         bias, bias_f32, labels, s.part, s.chosen);
+      constexpr int TOKENS = decltype(TC)::value;
+      if (stream)
+        hipLaunchKernelGGL((stream_kernel<T, TOKENS>), dim3(nt), dim3(kWave), 0, st, n, V, D, x, ldx, w, ldw, bias,
+                           bias_f32, labels, s.part, s.chosen);
+      else
+        hipLaunchKernelGGL((few_kernel<T, TOKENS>), dim3((nt + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlock), 0, st, n, V, D, x, ldx, w, ldw, bias, bias_f32,
+                           labels, s.part, s.chosen);
     };
     if (n <= 16) launch(IC<16>());
     else if (n <= 32) launch(IC<32>());
@@ -785,8 +1069,14 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
       if (const int rc = check_launch("cign_linear_xent_fwd")) return rc;
     }
   }
-  hipLaunchKernelGGL(join_kernel, dim3(static_cast<uint32_t>((n + kJoinRows - 1) / kJoinRows)), dim3(kBlock), 0, st, n, V,
-                     nt, s.part, labels, ignore, s.chosen, loss, lse);
+  // a workgroup a row where there are few rows, 8 rows (64 bytes of a tile's) otherwise
+  const auto joined = [&](auto RC) {
+    constexpr int ROWS = decltype(RC)::value;
+    hipLaunchKernelGGL((join_kernel<ROWS>), dim3(static_cast<uint32_t>((n + ROWS - 1) / ROWS)), dim3(kBlock), 0, st, n, V,
+                       nt, s.part, labels, ignore, s.chosen, loss, lse);
+  };
+  if (n <= kFewRows) joined(IC<1>());
+  else joined(IC<8>());
   return check_launch("cign_linear_xent_fwd");
 }
 
@@ -830,22 +1120,31 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
         return rc;
       const Operand dz{s.dz, n, vp, n * vp};
       hipLaunchKernelGGL((out_kernel<float, SEGS, true>), dim3(tile_count(D, n), c.splits), dim3(ntgemm::kThreads), 0, st,
-                         wt, dz, static_cast<int>(vp / kStep), s.count, s.slots, static_cast<int64_t>(c.Dp),
+                         wt, dz, static_cast<int>(vp / kStep), true, s.count, s.slots, static_cast<int64_t>(c.Dp),
                          n * c.Dp, v > 0);
       if (const int rc = check_launch(who)) return rc;
     }
     if (gw) {
       const Operand dzt{s.dzt, vn, c.rows_p, c.rows_p * vn};
-      hipLaunchKernelGGL((out_kernel<T, SEGS, false>), dim3(tile_count(D, vn)), dim3(ntgemm::kThreads), 0, st, xt, dzt, 0,
-                         s.count, gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0);
+      if (c.wsplits > 1) {
+        hipLaunchKernelGGL((out_kernel<float, SEGS, true>), dim3(tile_count(D, vn), c.wsplits), dim3(ntgemm::kThreads), 0,
+                           st, xt, dzt, 0, false, s.count, s.wslots, static_cast<int64_t>(c.Dp), vn * c.Dp, 0);
+        if (const int rc = check_launch(who)) return rc;
+        hipLaunchKernelGGL((rows_out_kernel<T>), grid_of(vn * (c.Dp / 4)), dim3(kBlock), 0, st, vn, D,
+                           static_cast<const int32_t*>(nullptr), s.wslots, c.wsplits, vn * c.Dp, c.Dp, gw + v * D);
+      } else {
+        hipLaunchKernelGGL((out_kernel<T, SEGS, false>), dim3(tile_count(D, vn)), dim3(ntgemm::kThreads), 0, st, xt, dzt, 0,
+                           false, s.count, gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0);
+      }
       if (const int rc = check_launch(who)) return rc;
     }
     if (gb) {
+      const dim3 bias_grid(static_cast<uint32_t>((vn + kBiasCols - 1) / kBiasCols));
       if (bias_f32)
-        hipLaunchKernelGGL((bias_kernel<float>), grid_of(vn), dim3(kBlock), 0, st, s.count, vn, s.bias,
+        hipLaunchKernelGGL((bias_kernel<float>), bias_grid, dim3(kBlock), 0, st, s.count, vn, s.bias,
                            static_cast<float*>(gb) + v);
       else
-        hipLaunchKernelGGL((bias_kernel<bf16>), grid_of(vn), dim3(kBlock), 0, st, s.count, vn, s.bias,
+        hipLaunchKernelGGL((bias_kernel<bf16>), bias_grid, dim3(kBlock), 0, st, s.count, vn, s.bias,
                            static_cast<bf16*>(gb) + v);
       if (const int rc = check_launch(who)) return rc;
     }

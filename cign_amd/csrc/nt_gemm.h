@@ -1,5 +1,25 @@
 // Products of two bf16 matrices whose rows run along the summed axis:
-// C[b][a] = sum_k A[a][k] B[b][k], float32 sums, a 256 x 256 tile of C a workgroup.
+// C[b][a] = sum_k A[a][k] B[b][k], float32 sums, a 256 x 256 tile of C a workgroup of
+// eight wavefronts, 128 rows of A by 64 of B each: 32 results of 16 x 16 in 128
+// registers, v_mfma_f32_16x16x32_bf16 (16 cycles).
+//
+// Steps of 64 values go to LDS without passing registers (16-byte direct loads, rows
+// of 128 bytes an eight lanes), into a ring of five units of 32 KB, 64 values of 256
+// rows of one operand each: the two in use, the other operand's next, and the two
+// after. A wavefront reads half a step's fragments (12 ds_read_b128), then multiplies
+// (32 MFMAs, 512 cycles), with a barrier after each; the wavefronts 4 to 7, one on
+// each SIMD beside one of 0 to 3, run one barrier behind, so that a SIMD's matrix
+// unit works for one of its two wavefronts while the other reads. A row's 16-byte
+// chunk c lies at place c ^ (row mod 8): 16 lanes read from all banks (no conflicts
+// counted). The loads for the steps to come are issued while reading and waited for
+// with vmcnt(4), the youngest unit left in flight, two to three phases before use.
+//
+// Measured, 8192 x 32000 x 4096 with the loss's statistics behind it: 1.65 ms, 1,300
+// TFLOP/s (the library's product of that shape with its bf16 result stored 1,360); a
+// double buffer of both operands with one barrier a step 957; a ring of four stages of
+// 32 values (rows of 64 bytes: twice the L2 requests) 1,260; four units released by
+// halves of A's rows 1,286; the loads between the MFMAs 1,114, at their head 1,135.
+// The clock falls to 1.65 GHz under this load; MFMAs are busy 64 to 70% of it.
 #pragma once
 
 #include "common.h"
@@ -11,12 +31,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 256;                    // rows of A and of B of a workgroup's tile
-constexpr int kStep = 64;                     // values of a row in LDS at a time
+constexpr int kStep = 64;                     // rows are a multiple of this many values
+constexpr int kUnits = 5;                     // LDS: a ring of kStep values of 256 rows of A or of B
 constexpr int kThreads = 512;
 constexpr int kFragA = 8, kFragB = 4;         // 16 x 16 results of a wavefront: 128 rows of A, 64 of B
-constexpr int kOperandBytes = kTile * kStep * 2;
-constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kLdsBytes = 2 * kStageBytes;
+constexpr int kUnitBytes = kTile * kStep * 2;
+constexpr int kLdsBytes = kUnits * kUnitBytes;
 
 // Rows of bf16 values, ld values apart, 16-byte aligned, of a multiple of kStep
 // values (zeros beyond their own); `part` values on lies the next part of values
@@ -41,7 +61,8 @@ struct Place {
 };
 
 // Tile of workgroup id: workgroups go round the 8 XCDs, each of which takes a
-// contiguous run of tiles, in bands of 8 tiles of B, tile of A by tile of A.
+// contiguous run of tiles, in bands of 8 tiles of B, tile of A by tile of A: the 32
+// tiles at work on an XCD share 4 tiles of A and 8 of B in its L2.
 __device__ __forceinline__ void tile_of(int id, int ta, int tb, int& ia, int& ib) {
   const int total = ta * tb, x = id & 7, k = id >> 3;
   const int each = total >> 3, more = total & 7;
@@ -59,6 +80,37 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 __device__ __forceinline__ int seg_a(int s) { return (0x001102 >> (4 * s)) & 0xF; }
 __device__ __forceinline__ int seg_b(int s) { return (0x010120 >> (4 * s)) & 0xF; }
 
+// The twelve fragments of half a step from LDS, waited for in the same statement.
+__device__ __forceinline__ void read_fragments(uint32_t at_a, uint32_t at_b, bf16x8 (&a)[kFragA], bf16x8 (&b)[kFragB]) {
+  asm volatile(
+      "ds_read_b128 %0, %13\n"
+      "ds_read_b128 %1, %13 offset:2048\n"
+      "ds_read_b128 %2, %13 offset:4096\n"
+      "ds_read_b128 %3, %13 offset:6144\n"
+      "ds_read_b128 %4, %12\n"
+      "ds_read_b128 %5, %12 offset:2048\n"
+      "ds_read_b128 %6, %12 offset:4096\n"
+      "ds_read_b128 %7, %12 offset:6144\n"
+      "ds_read_b128 %8, %12 offset:8192\n"
+      "ds_read_b128 %9, %12 offset:10240\n"
+      "ds_read_b128 %10, %12 offset:12288\n"
+      "ds_read_b128 %11, %12 offset:14336\n"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]), "=&v"(b[3]), "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]),
+        "=&v"(a[4]), "=&v"(a[5]), "=&v"(a[6]), "=&v"(a[7])
+      : "v"(at_a), "v"(at_b)
+      : "memory");
+}
+
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The tile (ia, ib) of the product over ksteps steps of each of SEGS segments; ends
+// with a barrier behind the last use of lds. Rows past an operand's last repeat it:
+// their results are not to be used.
 template <int SEGS>
 __device__ __forceinline__ void product(const Operand& A, const Operand& B, int ia, int ib, int ksteps, char* lds,
                                         f32x4 (&acc)[kFragA][kFragB]) {
@@ -75,58 +127,85 @@ __device__ __forceinline__ void product(const Operand& A, const Operand& B, int 
     oa[j] = static_cast<uint32_t>(min(r, ra)) * static_cast<uint32_t>(A.ld) + chunk * 8;
     ob[j] = static_cast<uint32_t>(min(r, rb)) * static_cast<uint32_t>(B.ld) + chunk * 8;
   }
-  int seg = 0, k = 0;
-  const auto load = [&](int stage) {
-    const uint16_t* sa = pa + k * kStep;
-    const uint16_t* sb = pb + k * kStep;
-    if (SEGS > 1) {
-      sa += seg_a(seg) * A.part;
-      sb += seg_b(seg) * B.part;
-    }
-    char* to = lds + stage * kStageBytes + w * 4096;
+  const int total = ksteps * SEGS;
+  // the next unit of each operand: its step, the step in its segment, its segment
+  int na = 0, ka = 0, ga = 0, nb = 0, kb = 0, gb = 0;
+  int slot = 0;  // of the next unit
+  const auto to_lds = [&](const uint16_t* src, const uint32_t (&o)[4]) {
+    char* to = lds + slot * kUnitBytes + w * 4096;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      __builtin_amdgcn_global_load_lds((GlobalPtr)(sa + oa[j]), (LdsPtr)(to + j * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((GlobalPtr)(sb + ob[j]), (LdsPtr)(to + kOperandBytes + j * 1024), 16, 0, 0);
-    }
+    for (int j = 0; j < 4; ++j)
+      __builtin_amdgcn_global_load_lds((GlobalPtr)(src + o[j]), (LdsPtr)(to + j * 1024), 16, 0, 0);
+  };
+  const auto next = [&](int& k, int& g) {
     if (++k == ksteps) {
       k = 0;
-      ++seg;
+      ++g;
     }
+    slot = slot == kUnits - 1 ? 0 : slot + 1;
+  };
+  const auto load_a = [&]() {
+    if (na >= total) return;
+    to_lds(pa + ka * kStep + (SEGS > 1 ? seg_a(ga) * A.part : 0), oa);
+    next(ka, ga);
+    ++na;
+  };
+  const auto load_b = [&]() {
+    if (nb >= total) return;
+    to_lds(pb + kb * kStep + (SEGS > 1 ? seg_b(gb) * B.part : 0), ob);
+    next(kb, gb);
+    ++nb;
   };
 #pragma unroll
   for (int fa = 0; fa < kFragA; ++fa)
 #pragma unroll
     for (int fb = 0; fb < kFragB; ++fb) acc[fa][fb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int total = ksteps * SEGS;
-  if (total > 0) load(0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  if (total == 0) return;
+  load_a();
+  load_b();
+  load_a();
   const int row = l & 15;
-  const char* fa0 = lds + ((w & 1) * 128 + row) * 128;
-  const char* fb0 = lds + kOperandBytes + ((w >> 1) * 64 + row) * 128;
+  const uint32_t base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((LdsPtr)lds)) + row * 128;
+  const uint32_t at_a = base + (w & 1) * 16384, at_b = base + (w >> 1) * 8192;
+  const uint32_t half[2] = {static_cast<uint32_t>(((l >> 4) ^ (row & 7)) << 4),
+                            static_cast<uint32_t>(((4 + (l >> 4)) ^ (row & 7)) << 4)};
+  const bool second = w >= 4;
+  if (total > 1) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  barrier();
+  if (second) barrier();
+  uint32_t ua = 0, ub = kUnitBytes;  // units of this step
   for (int t = 0; t < total; ++t) {
-    const int off = (t & 1) * kStageBytes;
-    bf16x8 a[2][kFragA], b[2][kFragB];
+    const bool more = t + 2 < total;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int slot = ((kk * 4 + (l >> 4)) ^ (row & 7)) * 16 + off;
-#pragma unroll
-      for (int f = 0; f < kFragB; ++f) b[kk][f] = *reinterpret_cast<const bf16x8*>(fb0 + f * 2048 + slot);
-#pragma unroll
-      for (int f = 0; f < kFragA; ++f) a[kk][f] = *reinterpret_cast<const bf16x8*>(fa0 + f * 2048 + slot);
-    }
-    if (t + 1 < total) load((t + 1) & 1);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int h = 0; h < 2; ++h) {
+      bf16x8 a[kFragA], b[kFragB];
+      if (h == 0) load_b();
+      else load_a();
+      read_fragments(at_a + ua + half[h], at_b + ub + half[h], a, b);
+      if (h == 1 && second) {
+        if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      barrier();
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int fa = 0; fa < kFragA; ++fa)
 #pragma unroll
         for (int fb = 0; fb < kFragB; ++fb)
-          acc[fa][fb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[kk][fa], b[kk][fb], acc[fa][fb], 0, 0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+          acc[fa][fb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[fa], b[fb], acc[fa][fb], 0, 0, 0);
+      __builtin_amdgcn_s_setprio(0);
+      if (h == 1 && !second) {
+        if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      }
+      barrier();
+    }
+    ua = ua >= 3 * kUnitBytes ? ua - 3 * kUnitBytes : ua + 2 * kUnitBytes;
+    ub = ub >= 3 * kUnitBytes ? ub - 3 * kUnitBytes : ub + 2 * kUnitBytes;
   }
+  if (!second) barrier();
+  __syncthreads();
 }
 
 }  // namespace ntgemm
