@@ -1,13 +1,17 @@
 // The global norm of many tensors, sqrt(sum of all squares), and the tensors
 // scaled by min(1, max_norm / (norm + 1e-6)): the clipping of a training step.
 //
-// Tensors are read as flat runs of values, float32 or bf16, in chunks of one
-// tensor each; the table of tensors travels in the kernel's arguments, 128 of them
-// a launch, so that nothing is copied to the device. A workgroup adds its chunk's
-// squares in float64, where no gradient over- or underflows (the VALU's float64
-// rate is half of float32's here), and stores one partial sum; the scaling kernel's workgroups each
-// add the partial sums up in one order and scale their chunk. No atomics: the same
-// bits in every run.
+// Tensors are read as flat runs of values, float32 or bf16, in chunks of one tensor
+// each; the table of tensors travels in the kernel's arguments, 128 of them a launch,
+// so that nothing is copied to the device. A workgroup adds its chunk's squares in
+// float64, where no gradient over- or underflows (the VALU multiplies float64 at half
+// of float32's rate here, and is about half busy), and stores one partial sum; the
+// scaling kernel's workgroups each add the partial sums up in one order and scale
+// their chunk. No atomics: the same bits in every run.
+//
+// HBM bounds the large ones: 500,000,000 bf16 in 200 tensors, the norm 182 us (5.5
+// TB/s), clipped into one packed buffer 562 us (3 GB, 5.3 TB/s; a copy moves 4.75).
+// Launches bound the small ones: 62 tensors of 2,600,000 float32 in all 8 us and 12.5.
 #include <algorithm>
 
 #include "rowvec.h"
@@ -17,8 +21,13 @@ namespace gradnorm {
 using rowvec::RowChunk;
 
 constexpr int kTable = 128;       // tensors of a launch
-constexpr int kGroups = 1536;     // chunks aimed at: six workgroups a CU
-constexpr int64_t kLeast = 8192;  // values of a chunk at least
+constexpr int kGroups = 1536, kManyGroups = 4096;  // chunks aimed at
+constexpr int64_t kLeast = 8192, kMost = 32768;  // values of a chunk: at least; beyond, more chunks
+
+// Tensors of this many bytes and more are scaled from the last to the first and
+// written past the cache (1 GB of bf16 562 us, 597 through the cache, 588 in order);
+// what is smaller stays in it for the optimizer.
+constexpr int64_t kLargeBytes = 192ll << 20;
 
 struct Table {
   const void* p[kTable];
@@ -34,16 +43,14 @@ struct Part {
   int64_t from, to;
 };
 
-__device__ __forceinline__ Part part_of(const Table& table, int64_t chunk) {
-  int lo = 0, hi = table.count;
-  const int b = blockIdx.x;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (table.first[mid] <= b) lo = mid;
-    else hi = mid;
-  }
-  const int64_t from = static_cast<int64_t>(b - table.first[lo]) * chunk;
-  return Part{lo, from, min(from + chunk, table.n[lo])};
+// The workgroup's tensor: the last one whose first chunk is not behind it, by a vote
+// over the table's two halves (a search would be seven loads behind each other).
+__device__ __forceinline__ Part part_of(const Table& table, int64_t chunk, int b) {
+  const int l = lane_id();
+  const int lo = l < table.count && table.first[l] <= b, hi = l + 64 < table.count && table.first[l + 64] <= b;
+  const int t = __popcll(__ballot(lo)) + __popcll(__ballot(hi)) - 1;
+  const int64_t from = static_cast<int64_t>(b - table.first[t]) * chunk;
+  return Part{t, from, min(from + chunk, table.n[t])};
 }
 
 // The sum of v over the workgroup, in every thread.
@@ -59,23 +66,23 @@ __device__ __forceinline__ double group_sum(double v, double* lds) {
 
 template <typename T>
 __device__ __forceinline__ double squares(const T* p, int64_t from, int64_t to) {
-  constexpr int U = 4;
+  constexpr int W = rowvec::kChunk<T>, U = 4;
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
-  int64_t i = from + threadIdx.x * 8;
-  for (; i + (U - 1) * 8 * kBlock + 8 <= to; i += U * 8 * kBlock) {
-    typename RowChunk<T, 8>::Raw q[U];
+  int64_t i = from + threadIdx.x * W;
+  for (; i + (U - 1) * W * kBlock + W <= to; i += U * W * kBlock) {
+    typename RowChunk<T, W>::Raw q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = RowChunk<T, 8>::load(p + i + u * 8 * kBlock);
+    for (int u = 0; u < U; ++u) q[u] = RowChunk<T, W>::load(p + i + u * W * kBlock);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float v[8];
-      RowChunk<T, 8>::unpack(q[u], v);
+      float v[W];
+      RowChunk<T, W>::unpack(q[u], v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[k & 3] = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), acc[k & 3]);
+      for (int k = 0; k < W; ++k) acc[k & 3] = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), acc[k & 3]);
     }
   }
-  for (; i < to; i += 8 * kBlock)
-    for (int k = 0; k < 8 && i + k < to; ++k) {
+  for (; i < to; i += W * kBlock)
+    for (int k = 0; k < W && i + k < to; ++k) {
       const double v = to_f32(p[i + k]);
       acc[0] = fma(v, v, acc[0]);
     }
@@ -84,7 +91,7 @@ __device__ __forceinline__ double squares(const T* p, int64_t from, int64_t to) 
 
 __global__ __launch_bounds__(kBlock) void squares_kernel(Table table, int64_t chunk, double* part) {
   __shared__ double lds[kWavesPerBlock];
-  const Part c = part_of(table, chunk);
+  const Part c = part_of(table, chunk, blockIdx.x);
   const double mine = table.bf16[c.t] ? squares(static_cast<const bf16*>(table.p[c.t]), c.from, c.to)
                                       : squares(static_cast<const float*>(table.p[c.t]), c.from, c.to);
   const double s = group_sum(mine, lds);
@@ -103,42 +110,53 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(const double* part, int pa
   if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
-template <typename T>
-__device__ __forceinline__ void scale(const T* p, T* out, int64_t from, int64_t to, float by) {
-  constexpr int U = 4;
-  int64_t i = from + threadIdx.x * 8;
-  for (; i + (U - 1) * 8 * kBlock + 8 <= to; i += U * 8 * kBlock) {
-    typename RowChunk<T, 8>::Raw q[U];
+// out = p by `by`, of the chunk's values; all chunks are moved on to where out's lines
+// of 128 bytes begin (a packed buffer's tensors lie anywhere), so that stores are
+// whole lines and only loads are not aligned.
+template <bool PAST, typename T>
+__device__ __forceinline__ void scale(const T* p, T* out, int64_t from, int64_t to, int64_t n, float by) {
+  constexpr int W = rowvec::kChunk<T>, U = 4;
+  const int head = static_cast<int>(-(reinterpret_cast<uintptr_t>(out) / sizeof(T)) & (128 / sizeof(T) - 1));
+  const int64_t begin = from == 0 ? min(static_cast<int64_t>(head), n) : min(from + head, n);
+  if (from == 0 && threadIdx.x < begin) out[threadIdx.x] = from_f32<T>(to_f32(p[threadIdx.x]) * by);
+  to = to == n ? n : min(to + head, n);
+  int64_t i = begin + threadIdx.x * W;
+  for (; i + (U - 1) * W * kBlock + W <= to; i += U * W * kBlock) {
+    typename RowChunk<T, W>::Raw q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = RowChunk<T, 8>::load(p + i + u * 8 * kBlock);
+    for (int u = 0; u < U; ++u) q[u] = RowChunk<T, W>::load(p + i + u * W * kBlock);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float v[8];
-      RowChunk<T, 8>::unpack(q[u], v);
+      float v[W];
+      RowChunk<T, W>::unpack(q[u], v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= by;
-      RowChunk<T, 8>::store(out + i + u * 8 * kBlock, v);
+      for (int k = 0; k < W; ++k) v[k] *= by;
+      if constexpr (PAST) RowChunk<T, W>::store_past(out + i + u * W * kBlock, v);
+      else RowChunk<T, W>::store(out + i + u * W * kBlock, v);
     }
   }
-  for (; i < to; i += 8 * kBlock)
-    for (int k = 0; k < 8 && i + k < to; ++k) out[i + k] = from_f32<T>(to_f32(p[i + k]) * by);
+  for (; i < to; i += W * kBlock)
+    for (int k = 0; k < W && i + k < to; ++k) out[i + k] = from_f32<T>(to_f32(p[i + k]) * by);
 }
 
+// LARGE: from the last chunk to the first, the squares' pass having left the last ones
+// in the 256 MB cache, and stores past it.
+template <bool LARGE>
 __global__ __launch_bounds__(kBlock) void scale_kernel(Table table, int64_t chunk, const double* part, int parts,
-                                                       double max_norm, float* norm) {
+                                                       float max_norm, float* norm) {
   __shared__ double lds[kWavesPerBlock];
   const double total = norm_of(part, parts, lds);
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(total);
-  double by = max_norm / (total + 1e-6);
+  double by = static_cast<double>(max_norm) / (total + 1e-6);
   if (by > 1.0) by = 1.0;  // a NaN stays
-  const Part c = part_of(table, chunk);
+  const Part c = part_of(table, chunk, LARGE ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
   if (by == 1.0 && table.out[c.t] == table.p[c.t]) return;
   if (table.bf16[c.t])
-    scale(static_cast<const bf16*>(table.p[c.t]), static_cast<bf16*>(table.out[c.t]), c.from, c.to,
-          static_cast<float>(by));
+    scale<LARGE>(static_cast<const bf16*>(table.p[c.t]), static_cast<bf16*>(table.out[c.t]), c.from, c.to, table.n[c.t],
+                 static_cast<float>(by));
   else
-    scale(static_cast<const float*>(table.p[c.t]), static_cast<float*>(table.out[c.t]), c.from, c.to,
-          static_cast<float>(by));
+    scale<LARGE>(static_cast<const float*>(table.p[c.t]), static_cast<float*>(table.out[c.t]), c.from, c.to, table.n[c.t],
+                 static_cast<float>(by));
 }
 
 // Values of a chunk, and the chunks of all tensors; a multiple of 8 so that every
@@ -146,7 +164,9 @@ __global__ __launch_bounds__(kBlock) void scale_kernel(Table table, int64_t chun
 int64_t chunk_of(int32_t count, const int64_t* sizes, int64_t* chunks) {
   int64_t total = 0;
   for (int32_t i = 0; i < count; ++i) total += sizes[i];
-  const int64_t chunk = std::max(kLeast, ((total + kGroups - 1) / kGroups + 2047) / 2048 * 2048);
+  const auto share = [&](int64_t groups) { return (total + groups - 1) / groups; };
+  const int64_t want = std::max(kLeast, std::min(share(kGroups), std::max(kMost, share(kManyGroups))));
+  const int64_t chunk = (want + 2047) / 2048 * 2048;
   *chunks = 0;
   for (int32_t i = 0; i < count; ++i) *chunks += (sizes[i] + chunk - 1) / chunk;
   return chunk;
@@ -164,34 +184,39 @@ int check_tensors(const char* who, int32_t count, const void* const* grads, cons
   return kOk;
 }
 
-// f(table, blocks, chunks before) for runs of up to kTable tensors that are not empty
+// f(table, blocks, chunks before) for runs of up to kTable tensors that are not empty,
+// or from the last run to the first.
 template <class F>
 int for_tables(int32_t count, const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes,
-               int64_t chunk, F&& f) {
-  Table t;
-  t.count = 0;
-  t.first[0] = 0;
-  int32_t before = 0;
-  for (int32_t i = 0; i <= count; ++i) {
-    if (t.count == kTable || (i == count && t.count > 0)) {
-      if (const int rc = f(t, t.first[t.count], before)) return rc;
-      before += t.first[t.count];
-      t.count = 0;
+               int64_t chunk, bool backwards, F&& f) {
+  int32_t full = 0;
+  for (int32_t i = 0; i < count; ++i) full += sizes[i] > 0;
+  const int32_t runs = (full + kTable - 1) / kTable;
+  for (int32_t r = 0; r < runs; ++r) {
+    const int32_t run = backwards ? runs - 1 - r : r;
+    Table t;
+    t.count = 0;
+    t.first[0] = 0;
+    int32_t before = 0, seen = 0;
+    for (int32_t i = 0; i < count; ++i) {
+      if (sizes[i] == 0) continue;
+      const int32_t chunks = static_cast<int32_t>((sizes[i] + chunk - 1) / chunk), at = seen++ / kTable;
+      if (at < run) before += chunks;
+      if (at != run) continue;
+      const int k = t.count++;
+      t.p[k] = grads[i];
+      t.out[k] = out ? out[i] : nullptr;
+      t.n[k] = sizes[i];
+      t.bf16[k] = dtypes[i] == kBF16;
+      t.first[k + 1] = t.first[k] + chunks;
     }
-    if (i == count) break;
-    if (sizes[i] == 0) continue;
-    const int k = t.count++;
-    t.p[k] = grads[i];
-    t.out[k] = out ? out[i] : nullptr;
-    t.n[k] = sizes[i];
-    t.bf16[k] = dtypes[i] == kBF16;
-    t.first[k + 1] = t.first[k] + static_cast<int32_t>((sizes[i] + chunk - 1) / chunk);
+    if (const int rc = f(t, t.first[t.count], before)) return rc;
   }
   return kOk;
 }
 
 int run(const char* who, void* stream, int32_t count, const void* const* grads, const int64_t* sizes,
-        const int32_t* dtypes, double max_norm, void* const* out, float* norm, void* workspace,
+        const int32_t* dtypes, float max_norm, void* const* out, float* norm, void* workspace,
         int64_t workspace_bytes) {
   int64_t chunks;
   const int64_t chunk = chunk_of(count, sizes, &chunks);
@@ -201,7 +226,8 @@ int run(const char* who, void* stream, int32_t count, const void* const* grads, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   const int parts = static_cast<int>(chunks);
-  int rc = for_tables(count, grads, out, sizes, dtypes, chunk, [&](const Table& t, int32_t blocks, int32_t before) {
+  int rc = for_tables(count, grads, out, sizes, dtypes, chunk, false,
+                      [&](const Table& t, int32_t blocks, int32_t before) {
     hipLaunchKernelGGL(squares_kernel, dim3(blocks), dim3(kBlock), 0, st, t, chunk, part + before);
     return check_launch(who);
   });
@@ -210,8 +236,14 @@ int run(const char* who, void* stream, int32_t count, const void* const* grads, 
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kBlock), 0, st, part, parts, norm);
     return check_launch(who);
   }
-  return for_tables(count, grads, out, sizes, dtypes, chunk, [&](const Table& t, int32_t blocks, int32_t) {
-    hipLaunchKernelGGL(scale_kernel, dim3(blocks), dim3(kBlock), 0, st, t, chunk, part, parts, max_norm, norm);
+  int64_t bytes = 0;
+  for (int32_t i = 0; i < count; ++i) bytes += sizes[i] * (dtypes[i] == kF32 ? 4 : 2);
+  const bool large = bytes >= kLargeBytes;
+  return for_tables(count, grads, out, sizes, dtypes, chunk, large, [&](const Table& t, int32_t blocks, int32_t) {
+    if (large)
+      hipLaunchKernelGGL((scale_kernel<true>), dim3(blocks), dim3(kBlock), 0, st, t, chunk, part, parts, max_norm, norm);
+    else
+      hipLaunchKernelGGL((scale_kernel<false>), dim3(blocks), dim3(kBlock), 0, st, t, chunk, part, parts, max_norm, norm);
     return check_launch(who);
   });
 }
@@ -238,7 +270,7 @@ int cign_grad_norm(void* stream, int32_t count, const void* const* grads, const 
   const char* who = "cign_grad_norm";
   if (const int rc = check_tensors(who, count, grads, sizes, dtypes)) return rc;
   if (!norm) return set_error(kInvalid, "%s: null argument", who);
-  return run(who, stream, count, grads, sizes, dtypes, 0.0, nullptr, norm, workspace, workspace_bytes);
+  return run(who, stream, count, grads, sizes, dtypes, 0.0f, nullptr, norm, workspace, workspace_bytes);
 }
 
 int cign_clip_grad_norm(void* stream, int32_t count, const void* const* grads, const int64_t* sizes,

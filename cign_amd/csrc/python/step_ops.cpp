@@ -5,7 +5,7 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <algorithm>
-#include <cmath>
+#include <array>
 
 #include "ops.h"
 
@@ -40,15 +40,12 @@ Boundary check_boundary(const Tensor& branch, const Tensor& residual, const Opti
     check_beside(*gate, branch, "gate", branch.scalar_type(), b.kind == kRowGate ? at::IntArrayRef(one) : branch.sizes());
   }
   b.params = branch.scalar_type();
-  for (const Optional& v : vec)
-    if (v) {
-      b.params = v->scalar_type();
-      break;
-    }
-  TORCH_CHECK_TYPE(b.params == at::kFloat || b.params == branch.scalar_type(),
-                   "the vectors must all be float32 or all of branch's type");
+  for (int i = 4; i >= 0; --i)
+    if (vec[i]) b.params = vec[i]->scalar_type();
   for (int i = 0; i < 5; ++i)
     if (vec[i]) {
+      TORCH_CHECK_TYPE(vec[i]->scalar_type() == b.params && (b.params == at::kFloat || b.params == branch.scalar_type()),
+                       "the vectors must all be float32 or all of branch's type");
       check_beside(*vec[i], branch, names[i], b.params, {b.D});
       b.vec[i] = vec[i]->contiguous();
     }
@@ -183,6 +180,7 @@ struct BlockBoundary : torch::autograd::Function<BlockBoundary> {
     for (int i = 0; i < 8; ++i) place[bit[i]] = i;
     {
       const at::NoGradGuard no_grad;
+      const at::AutoDispatchBelowADInplaceOrView below;
       const variable_list got = call_block_boundary_backward(
           optional(grads[0]), optional(grads[1]), saved[0], saved[1], optional(saved[2]), optional(saved[3]),
           optional(saved[4]), optional(saved[5]), optional(saved[6]), saved[7],
@@ -324,6 +322,7 @@ struct LinearXent : torch::autograd::Function<LinearXent> {
     if (!grads[0].defined() && !grads[1].defined()) return out;
     {
       const at::NoGradGuard no_grad;
+      const at::AutoDispatchBelowADInplaceOrView below;
       const bool of[3] = {ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                           saved[3].defined() && ctx->needs_input_grad(3)};
       const variable_list got =
@@ -535,8 +534,10 @@ TORCH_LIBRARY_IMPL(cign_amd, Autograd, m) {
 
 Tensor bound_global_grad_norm(const std::vector<Tensor>& grads) { return call_global_grad_norm(at::TensorList(grads)); }
 
-Tensor bound_clip_grad_norm(const std::vector<Tensor>& grads, double max_norm, const std::vector<Tensor>& out) {
-  return call_clip_grad_norm(at::TensorList(grads), max_norm, at::TensorList(out));
+// in place without `out`
+Tensor bound_clip_grad_norm(const std::vector<Tensor>& grads, double max_norm,
+                            const std::optional<std::vector<Tensor>>& out) {
+  return call_clip_grad_norm(at::TensorList(grads), max_norm, at::TensorList(out ? *out : grads));
 }
 
 }  // namespace

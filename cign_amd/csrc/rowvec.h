@@ -61,6 +61,12 @@ struct RowChunk<float, 8> {
     *reinterpret_cast<RowChunk<float, 4>::Raw*>(p) = RowChunk<float, 4>::Raw{v[0], v[1], v[2], v[3]};
     *reinterpret_cast<RowChunk<float, 4>::Raw*>(p + 4) = RowChunk<float, 4>::Raw{v[4], v[5], v[6], v[7]};
   }
+  static __device__ __forceinline__ void store_past(float* p, const float (&v)[8]) {
+    __builtin_nontemporal_store(RowChunk<float, 4>::Raw{v[0], v[1], v[2], v[3]},
+                                reinterpret_cast<RowChunk<float, 4>::Raw*>(p));
+    __builtin_nontemporal_store(RowChunk<float, 4>::Raw{v[4], v[5], v[6], v[7]},
+                                reinterpret_cast<RowChunk<float, 4>::Raw*>(p + 4));
+  }
 };
 
 template <>

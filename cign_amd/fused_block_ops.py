@@ -406,29 +406,7 @@ def fused_gated_residual_norm(branch, residual, post_weight=None, post_bias=None
     zeros. Sums are float32; normed is the norm of hidden before it is rounded.
     Gradients of every input, once differentiable; those of the vectors are summed
     over the rows in float32, in an order that depends on the shape alone."""
-    D = check_rows(branch, "branch", MAX_BOUNDARY_WIDTH)
-    for t, name in ((residual, "residual"), (gate, "gate")):
-        if t is None and name == "gate":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype != branch.dtype:
-            raise TypeError(f"{name} must be a tensor of branch's type ({branch.dtype})")
-        if t.shape != branch.shape and not (name == "gate" and t.shape == (*branch.shape[:-1], 1)):
-            raise ValueError(f"{name} must have shape {tuple(branch.shape)}"
-                             f"{f' or {(*branch.shape[:-1], 1)}' if name == 'gate' else ''}, got {tuple(t.shape)}")
-        if t.device != branch.device:
-            raise ValueError(f"{name} must be on {branch.device}, got {t.device}")
-    dtype = None
-    for t, name in ((post_weight, "post_weight"), (post_bias, "post_bias"), (scale, "scale"),
-                    (next_weight, "next_weight"), (next_bias, "next_bias")):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, branch.dtype) or dtype not in (None, t.dtype):
-            raise TypeError("the vectors must all be float32 or all of branch's type")
-        if t.shape != (D,):
-            raise ValueError(f"{name} must have shape [{D}], got {tuple(t.shape)}")
-        if t.device != branch.device:
-            raise ValueError(f"{name} must be on {branch.device}, got {t.device}")
-        dtype = t.dtype
+    check_rows(branch, "branch", MAX_BOUNDARY_WIDTH)  # the operator checks the others against it
     if norm not in ("layer", "rms"):
         raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
     eps = float(eps)

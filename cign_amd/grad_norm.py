@@ -10,13 +10,15 @@ import torch
 from ._rows import ROW_DTYPES, output_ops
 
 
-def _tensors(tensors, name: str) -> list:
+def _listed(tensors, name: str) -> list:
+    """The tensors as a list that is not empty; the first one checked here, where
+    no device need be present, the others by the operators."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         raise ValueError(f"{name} must not be empty")
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in ROW_DTYPES or t.layout != torch.strided:
-            raise TypeError(f"{name} must be CUDA float32 or bfloat16 tensors")
+    t = tensors[0]
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in ROW_DTYPES:
+        raise TypeError(f"{name} must be CUDA float32 or bfloat16 tensors")
     return tensors
 
 
@@ -25,7 +27,7 @@ def global_grad_norm(grads) -> torch.Tensor:
     any shapes and strides, on one device), a float32 scalar on their device:
     squares and sums in float64, in an order that depends on the sizes alone. Not
     differentiable."""
-    grads = _tensors(grads, "grads")
+    grads = _listed(grads, "grads")
     return output_ops().global_grad_norm(grads)
 
 
@@ -39,23 +41,10 @@ def clip_grad_norm(grads, max_norm, out=None) -> torch.Tensor:
     Tensors that are written must not share memory with each other or with
     another gradient (from the first to the last value of each); out[i] may be
     grads[i]. max_norm >= 0, taken as float32 (inf: no clipping)."""
-    grads = _tensors(grads, "grads")
+    grads = _listed(grads, "grads")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    if out is None:
-        out = grads
-    else:
-        out = _tensors(out, "out")
-        if len(out) != len(grads):
-            raise ValueError(f"out must have {len(grads)} tensors, got {len(out)}")
-        for g, o in zip(grads, out):
-            if o.dtype != g.dtype:
-                raise TypeError(f"out must have the gradients' types, got {o.dtype} for {g.dtype}")
-            if o.shape != g.shape or o.device != g.device:
-                raise ValueError(f"out must have the gradients' shapes and device, got {tuple(o.shape)} for "
-                                 f"{tuple(g.shape)}")
-    for g in grads:
-        if g.device != grads[0].device:
-            raise ValueError(f"gradients must be on one device, got {grads[0].device} and {g.device}")
+    if out is not None:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
     return output_ops().clip_grad_norm(grads, max_norm, out)

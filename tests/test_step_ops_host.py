@@ -110,7 +110,10 @@ def test_grad_norm_refusals():
                           ({"_7": ws - 1}, "workspace")):
         _refused("cign_grad_norm", _with(norm, **change), match)
     many = (C.c_int64 * 3)(0, 1, 10**9)
-    assert lib.cign_grad_norm_workspace_bytes(3, a(many)) == 8 * (1 + -(-10**9 // (-(-(-(-(10**9 + 1) // 1536)) // 2048) * 2048)))
+    # chunks of 10^9 / 4096 values, to the next multiple of 2048
+    assert lib.cign_grad_norm_workspace_bytes(3, a(many)) == 8 * (1 + -(-10**9 // (-(-(-(-(10**9 + 1) // 4096)) // 2048) * 2048)))
+    few = (C.c_int64 * 2)(8192, 8193)  # chunks of at least 8192
+    assert lib.cign_grad_norm_workspace_bytes(2, a(few)) == 8 * 3
     assert lib.cign_grad_norm_workspace_bytes(0, a(many)) == lib.cign_grad_norm_workspace_bytes(3, None) == 0
 
 
