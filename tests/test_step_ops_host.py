@@ -38,7 +38,7 @@ def test_block_boundary_refusals():
     lib = _lib.load_library(require_gpu=False)
     ws = lib.cign_block_boundary_bwd_workspace_bytes(4, 32)
     assert ws == 5 * 4 * 4 * 32
-    assert lib.cign_block_boundary_bwd_workspace_bytes(10**6, 8192) == 5 * 4 * 512 * 8192
+    assert lib.cign_block_boundary_bwd_workspace_bytes(10**6, 8192) == 5 * 4 * 1024 * 8192
     assert lib.cign_block_boundary_bwd_workspace_bytes(-1, 32) == lib.cign_block_boundary_bwd_workspace_bytes(1, 8193) == 0
     #      stream n D  xt wt ly gk g1  ld1 g2  ld2 u   ldu h   ldh a   lda
     bwd = (None, 4, 32, 0, 0, 1, 2, BIG, 32, BIG, 32, BIG, 32, BIG, 32, BIG, 32,
