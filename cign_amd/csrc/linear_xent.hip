@@ -21,12 +21,11 @@ namespace cign {
 namespace xent {
 using ntgemm::bf16x8;
 using ntgemm::f32x4;
-using ntgemm::kFragA;
-using ntgemm::kFragB;
 using ntgemm::kStep;
-using ntgemm::kTile;
+using ntgemm::Large;
 using ntgemm::Operand;
 using ntgemm::Place;
+using ntgemm::Small;
 
 constexpr int kMaxClasses = 1 << 20;
 constexpr int kMaxWidth = 1 << 16;
@@ -75,7 +74,7 @@ struct Logits {
   }
 };
 
-__device__ __forceinline__ int tiles(int64_t rows) { return static_cast<int>((rows + kTile - 1) / kTile); }
+__device__ __forceinline__ int tiles(int64_t rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
 
 // (largest, sum of e^(value - largest)) of two sets
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
@@ -86,34 +85,34 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 }
 
 // Statistics of a tile: part[tile of classes][row], and the logit of each row's label.
-template <int SEGS>
-__global__ __launch_bounds__(ntgemm::kThreads, 1) void stats_kernel(Logits f, int64_t n, float2* part, int first_tile,
+template <class S, int SEGS>
+__global__ __launch_bounds__(S::kThreads, S::kGroups) void stats_kernel(Logits f, int64_t n, float2* part, int first_tile,
                                                                     float* chosen) {
-  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
   int ia, ib;
-  ntgemm::tile_of(blockIdx.x, tiles(f.w.rows), tiles(n), ia, ib);
-  f32x4 acc[kFragA][kFragB];
-  ntgemm::product<SEGS>(f.w, f.x, ia, ib, f.ksteps, lds, acc);
-  const Place at(ia, ib);
-  float2* red = reinterpret_cast<float2*>(lds);  // [2][kTile]
+  ntgemm::tile_of(blockIdx.x, tiles(f.w.rows, S::TA), tiles(n, S::TB), ia, ib);
+  f32x4 acc[S::FA][S::FB];
+  ntgemm::product<S, SEGS>(f.w, f.x, ia, ib, f.ksteps, lds, acc);
+  const Place<S> at(ia, ib);
+  float2* red = reinterpret_cast<float2*>(lds);  // [WA][TB]
   const int wave = threadIdx.x / kWave, l = lane_id();
-  const bool plain = !f.bias && (ia + 1) * kTile <= f.w.rows;  // no class masked or behind the last
-  float bias[kFragA][4];
+  const bool plain = !f.bias && (ia + 1) * S::TA <= f.w.rows;  // no class masked or behind the last
+  float bias[S::FA][4];
   if (!plain)
 #pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa)
+    for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         bias[fa][r] = at.a(fa) + r < f.w.rows ? f.bias_of(at.a(fa) + r) : -INFINITY;
 #pragma unroll
-  for (int fb = 0; fb < kFragB; ++fb) {
+  for (int fb = 0; fb < S::FB; ++fb) {
     const int64_t row = at.b(fb);
     // the label's place behind the lane's first class
     const int64_t in = (f.labels && row < n ? f.labels[row] : -1) - f.first;
-    const int want = in >= at.a0 && in < f.w.rows && in - at.a0 < 128 ? static_cast<int>(in - at.a0) : -1;
+    const int want = in >= at.a0 && in < f.w.rows && in - at.a0 < S::TA / S::WA ? static_cast<int>(in - at.a0) : -1;
     float m = -INFINITY;
 #pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa) {
+    for (int fa = 0; fa < S::FA; ++fa) {
       if (!plain)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -129,18 +128,18 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void stats_kernel(Logits f, in
     const float by = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa)
+    for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
       for (int r = 0; r < 4; ++r) s += exp_of(acc[fa][fb][r] - by);
     join(m, s, xor_shfl<16>(m), xor_shfl<16>(s));
     join(m, s, xor_shfl<32>(m), xor_shfl<32>(s));
-    if (l < 16) red[(wave & 1) * kTile + (wave >> 1) * 64 + fb * 16 + l] = make_float2(m, s);
+    if (l < 16) red[(wave % S::WA) * S::TB + (wave / S::WA) * (S::TB / S::WB) + fb * 16 + l] = make_float2(m, s);
   }
   __syncthreads();
-  const int64_t row = static_cast<int64_t>(ib) * kTile + threadIdx.x;
-  if (threadIdx.x < kTile && row < n) {
+  const int64_t row = static_cast<int64_t>(ib) * S::TB + threadIdx.x;
+  if (threadIdx.x < S::TB && row < n) {
     float2 a = red[threadIdx.x];
-    const float2 b = red[kTile + threadIdx.x];
+    const float2 b = red[S::TB + threadIdx.x];
     join(a.x, a.y, b.x, b.y);
     part[static_cast<int64_t>(first_tile + ia) * n + row] = a;
   }
@@ -420,12 +419,14 @@ __global__ __launch_bounds__(kBlock) void join_kernel(int64_t n, int V, int nt, 
   loss[row] = out;
 }
 
-// Rows with a gradient, in order: list[0..count), and each row's place in it or -1.
+// Rows with a gradient, in order: list[0..count), and each row's place in it or -1;
+// marks of the listed rows, their labels that are classes or -1, and rests of zero.
 // One workgroup, 8192 rows at a time: a vote a wavefront for each 64 rows, the votes'
 // counts added up in the rows' order.
 __global__ __launch_bounds__(1024) void rows_kernel(int64_t n, const int64_t* labels, int64_t ignore,
-                                                    const float* g_loss, const float* g_lse, int32_t* list,
-                                                    int32_t* place, int32_t* count) {
+                                                    const float* g_loss, const float* g_lse, int64_t V,
+                                                    int32_t* list, int32_t* place, int32_t* count, int32_t* mark,
+                                                    float* rest) {
   constexpr int kEach = 8, kWaves = 1024 / kWave;
   __shared__ int32_t sums[kEach * kWaves];
   int32_t base = 0;
@@ -465,7 +466,11 @@ __global__ __launch_bounds__(1024) void rows_kernel(int64_t n, const int64_t* la
       if (r < n) {
         const bool on = votes[i] >> lane_id() & 1;
         place[r] = on ? at : -1;
-        if (on) list[at] = static_cast<int32_t>(r);
+        if (on) {
+          list[at] = static_cast<int32_t>(r);
+          mark[at] = g_loss && y[i] != ignore && y[i] >= 0 && y[i] < V ? static_cast<int32_t>(y[i]) : -1;
+          rest[at] = 0.0f;
+        }
       }
     }
     base += all;
@@ -568,24 +573,27 @@ struct Grads {
   uint16_t* dzt;
   int64_t ldt, partt;
   float* bias_part;        // [tile of rows][class of the piece] or null
+  float* rest;             // what rounding to bf16 leaves of the label's entry, by row
 };
 
-// A tile of 256 x 256 16-bit values in LDS, rows of 512 bytes and 16 more, so that
+// A tile of 16-bit values in LDS, rows of 512 (256) bytes and 16 more, so that
 // neither a column's nor a row's accesses meet on few banks.
-constexpr int kStageRow = kTile * 2 + 16;
-static_assert(kTile * kStageRow <= ntgemm::kLdsBytes, "a tile of results fits the operands' LDS");
+template <class S>
+constexpr int kStageRow = S::TA * 2 + 16;
+static_assert(Large::TB * kStageRow<Large> <= Large::kLdsBytes && Small::TB * kStageRow<Small> <= Small::kLdsBytes,
+              "a tile of results fits the operands' LDS");
 
-// Writes the staged tile to global rows `ld` values apart, 16 bytes a lane, 512 a
-// row: rows below `rows`, values below `cols` (of the tile), chunks whole where cols
+// Writes the staged tile to global rows `ld` values apart, 16 bytes a lane: rows below `rows`, values below `cols` (of the tile), chunks whole where cols
 // is a multiple of 8, value by value at a ragged end.
-template <bool RAGGED>
+template <class S, bool RAGGED>
 __device__ __forceinline__ void store_tile(const char* lds, uint16_t* out, int64_t ld, int rows, int cols) {
   typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));
-  const int c = (threadIdx.x & 31) * 8;
+  constexpr int kLanes = S::TA / 8;
+  const int c = (threadIdx.x % kLanes) * 8;
 #pragma unroll 4
-  for (int r = threadIdx.x >> 5; r < kTile; r += ntgemm::kThreads / 32) {
+  for (int r = threadIdx.x / kLanes; r < S::TB; r += S::kThreads / kLanes) {
     if (r >= rows || c >= cols) continue;
-    const U32x4 v = *reinterpret_cast<const U32x4*>(lds + r * kStageRow + c * 2);
+    const U32x4 v = *reinterpret_cast<const U32x4*>(lds + r * kStageRow<S> + c * 2);
     uint16_t* to = out + r * ld + c;
     if (!RAGGED) {
       *reinterpret_cast<U32x4*>(to) = v;
@@ -600,48 +608,50 @@ __device__ __forceinline__ void store_tile(const char* lds, uint16_t* out, int64
 }
 
 // Stages four consecutive rows of A by one of B a lane: [row of B][row of A].
+template <class S>
 __device__ __forceinline__ void stage(char* lds, int fa, int fb, uint32_t first, uint32_t second) {
   const int w = threadIdx.x / kWave, l = lane_id();
-  *reinterpret_cast<uint2*>(lds + ((w >> 1) * 64 + fb * 16 + (l & 15)) * kStageRow +
-                            ((w & 1) * 128 + fa * 16 + (l >> 4) * 4) * 2) = make_uint2(first, second);
+  *reinterpret_cast<uint2*>(lds + ((w / S::WA) * (S::TB / S::WB) + fb * 16 + (l & 15)) * kStageRow<S> +
+                            ((w % S::WA) * (S::TA / S::WA) + fa * 16 + (l >> 4) * 4) * 2) = make_uint2(first, second);
 }
 
 // The same transposed, [row of A][row of B]: two neighbouring lanes exchange two of
 // their values, so that each has two rows of A for both of its rows of B.
+template <class S>
 __device__ __forceinline__ void stage_t(char* lds, int fa, int fb, uint32_t first, uint32_t second) {
   const int w = threadIdx.x / kWave, l = lane_id();
   const bool odd = l & 1;
   const uint32_t give = odd ? first : second, keep = odd ? second : first;
   const uint32_t got = __float_as_uint(dpp<0xB1>(__uint_as_float(give)));  // of the lane beside
   const uint32_t even_lane = odd ? got : keep, odd_lane = odd ? keep : got;
-  char* to = lds + ((w & 1) * 128 + fa * 16 + (l >> 4) * 4 + 2 * odd) * kStageRow +
-             ((w >> 1) * 64 + fb * 16 + (l & 14)) * 2;
+  char* to = lds + ((w % S::WA) * (S::TA / S::WA) + fa * 16 + (l >> 4) * 4 + 2 * odd) * kStageRow<S> +
+             ((w / S::WA) * (S::TB / S::WB) + fb * 16 + (l & 14)) * 2;
   *reinterpret_cast<uint32_t*>(to) = (even_lane & 0xffff) | (odd_lane << 16);
-  *reinterpret_cast<uint32_t*>(to + kStageRow) = (even_lane >> 16) | (odd_lane & 0xffff0000u);
+  *reinterpret_cast<uint32_t*>(to + kStageRow<S>) = (even_lane >> 16) | (odd_lane & 0xffff0000u);
 }
 
-template <int SEGS>
-__global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Grads g) {
+template <class S, int SEGS>
+__global__ __launch_bounds__(S::kThreads, S::kGroups) void grad_kernel(Logits f, Grads g) {
   constexpr int PARTS = SEGS > 1 ? 3 : 1;
-  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
   const int64_t n = *f.count;
-  const int ta = tiles(f.w.rows), tb = tiles(n);
+  const int ta = tiles(f.w.rows, S::TA), tb = tiles(n, S::TB);
   if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(ta) * tb) return;
   int ia, ib;
   ntgemm::tile_of(blockIdx.x, ta, tb, ia, ib);
-  f32x4 acc[kFragA][kFragB];
+  f32x4 acc[S::FA][S::FB];
   Operand x = f.x;
   x.rows = n;
-  ntgemm::product<SEGS>(f.w, x, ia, ib, f.ksteps, lds, acc);
-  const Place at(ia, ib);
+  ntgemm::product<S, SEGS>(f.w, x, ia, ib, f.ksteps, lds, acc);
+  const Place<S> at(ia, ib);
   const int wave = threadIdx.x / kWave, l = lane_id();
-  const int rows = static_cast<int>(min(static_cast<int64_t>(kTile), n - static_cast<int64_t>(ib) * kTile));
-  const int classes = static_cast<int>(min(static_cast<int64_t>(kTile), f.w.rows - static_cast<int64_t>(ia) * kTile));
-  const int a0 = (wave & 1) * 128 + (l >> 4) * 4;  // the lane's first class in the tile
-  float own[kFragB], all[kFragB], shift[kFragB];
-  int want[kFragB];  // the label's place behind the lane's first class
+  const int rows = static_cast<int>(min(static_cast<int64_t>(S::TB), n - static_cast<int64_t>(ib) * S::TB));
+  const int classes = static_cast<int>(min(static_cast<int64_t>(S::TA), f.w.rows - static_cast<int64_t>(ia) * S::TA));
+  const int a0 = (wave % S::WA) * (S::TA / S::WA) + (l >> 4) * 4;  // the lane's first class in the tile
+  float own[S::FB], all[S::FB], shift[S::FB];
+  int want[S::FB];  // the label's place behind the lane's first class
 #pragma unroll
-  for (int fb = 0; fb < kFragB; ++fb) {
+  for (int fb = 0; fb < S::FB; ++fb) {
     const int64_t row = at.b(fb);
     own[fb] = all[fb] = 0.0f;
     shift[fb] = INFINITY;  // e^(z - inf) = 0
@@ -657,16 +667,16 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
       const float lse = g.lse[src];
       if (lse != -INFINITY) {  // a class is left
         shift[fb] = lse;
-        const int64_t in = y - f.first - static_cast<int64_t>(ia) * kTile;
+        const int64_t in = y - f.first - static_cast<int64_t>(ia) * S::TA;
         if (in >= 0 && in < classes) want[fb] = static_cast<int>(in) - a0;
       }
     }
   }
-  float* red = reinterpret_cast<float*>(lds);  // [4][kTile]
+  float* red = reinterpret_cast<float*>(lds);  // [WB][TA]
   // PLAIN: a whole tile without bias, where nothing is masked
   const auto gradients = [&](auto PLAIN) {
 #pragma unroll
-    for (int fa = 0; fa < kFragA; ++fa) {
+    for (int fa = 0; fa < S::FA; ++fa) {
       float bias[4], sum[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -674,7 +684,7 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
         if (!PLAIN) bias[r] = a0 + fa * 16 + r < classes ? f.bias_of(at.a(fa) + r) : -INFINITY;
       }
 #pragma unroll
-      for (int fb = 0; fb < kFragB; ++fb) {
+      for (int fb = 0; fb < S::FB; ++fb) {
         float d[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -689,7 +699,10 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
         if ((want[fb] >> 4) == fa) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if ((want[fb] & 15) == r) d[r] -= own[fb];
+            if ((want[fb] & 15) == r) {
+              d[r] -= own[fb];
+              if (PARTS == 1) g.rest[at.b(fb)] = d[r] - __uint_as_float(rowvec::pack_bf16(d[r], 0.0f) << 16);
+            }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -704,20 +717,23 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
           sum[r] += xor_shfl<2>(sum[r]);
           sum[r] += xor_shfl<4>(sum[r]);
           sum[r] += xor_shfl<8>(sum[r]);
-          if ((l & 15) == 0) red[(wave >> 1) * kTile + a0 + fa * 16 + r] = sum[r];
+          if ((l & 15) == 0) red[(wave / S::WA) * S::TA + a0 + fa * 16 + r] = sum[r];
         }
       }
     }
   };
-  if (!f.bias && rows == kTile && classes == kTile) {
+  if (!f.bias && rows == S::TB && classes == S::TA) {
     gradients(std::true_type());
   } else {
     gradients(std::false_type());
     if (g.bias_part) {
       __syncthreads();
-      if (static_cast<int>(threadIdx.x) < classes)
-        g.bias_part[static_cast<int64_t>(ib) * f.w.rows + static_cast<int64_t>(ia) * kTile + threadIdx.x] =
-            (red[threadIdx.x] + red[kTile + threadIdx.x]) + (red[2 * kTile + threadIdx.x] + red[3 * kTile + threadIdx.x]);
+      if (static_cast<int>(threadIdx.x) < classes) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < S::WB; ++k) sum += red[k * S::TA + threadIdx.x];
+        g.bias_part[static_cast<int64_t>(ib) * f.w.rows + static_cast<int64_t>(ia) * S::TA + threadIdx.x] = sum;
+      }
       __syncthreads();
     }
   }
@@ -734,32 +750,147 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
     };
     if (g.dz) {
 #pragma unroll
-      for (int fa = 0; fa < kFragA; ++fa)
+      for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
-        for (int fb = 0; fb < kFragB; ++fb) {
+        for (int fb = 0; fb < S::FB; ++fb) {
           uint32_t first, second;
           part(acc[fa][fb], first, second);
-          stage(lds, fa, fb, first, second);
+          stage<S>(lds, fa, fb, first, second);
         }
       __syncthreads();
-      store_tile<false>(lds, g.dz + q * g.part + static_cast<int64_t>(ib) * kTile * g.ld + static_cast<int64_t>(ia) * kTile,
+      store_tile<S, false>(lds, g.dz + q * g.part + static_cast<int64_t>(ib) * S::TB * g.ld + static_cast<int64_t>(ia) * S::TA,
                         g.ld, rows, (classes + kStep - 1) / kStep * kStep);
       __syncthreads();
     }
     if (g.dzt) {
 #pragma unroll
-      for (int fa = 0; fa < kFragA; ++fa)
+      for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
-        for (int fb = 0; fb < kFragB; ++fb) {
+        for (int fb = 0; fb < S::FB; ++fb) {
           uint32_t first, second;
           part(acc[fa][fb], first, second);
-          stage_t(lds, fa, fb, first, second);
+          stage_t<S>(lds, fa, fb, first, second);
         }
       __syncthreads();
-      store_tile<false>(lds, g.dzt + q * g.partt + static_cast<int64_t>(ia) * kTile * g.ldt + static_cast<int64_t>(ib) * kTile,
+      store_tile<S, false>(lds, g.dzt + q * g.partt + static_cast<int64_t>(ia) * S::TA * g.ldt + static_cast<int64_t>(ib) * S::TB,
                         g.ldt, classes, (rows + kStep - 1) / kStep * kStep);
       __syncthreads();
     }
+  }
+}
+
+// What is added to the weight's gradient for the labels' entries of the logits'
+// gradient, the only large ones of their rows: what their rounding to bf16 left, to 8
+// bits, times the rows (the gradient's error is then its own rounding, 1.7e-3, where it
+// was that and the entries', 2.4e-3). x: the listed rows, x_width values of each.
+struct Rests {
+  const int32_t* mark;  // null: none
+  const float* rest;
+  int64_t first;        // first class of the piece
+  const uint16_t* x;
+  int64_t ld;
+};
+
+// A workgroup's classes are b0 .. b0 + S::TB of the piece, its columns a0 ..: the rows
+// whose label is among them are listed in their order (eight marks a thread at a
+// time), their columns gathered into LDS, 64 rows at a time, and 32 are a product's
+// step, the entries' rests one operand and the rows the other.
+template <class S>
+__device__ __forceinline__ void add_rests(const Rests& f, int64_t n, int64_t a0, int64_t b0, int64_t classes, char* lds,
+                                          f32x4 (&acc)[S::FA][S::FB]) {
+  constexpr int kWaves = S::kThreads / kWave, kEach = 8, kBatch = kEach * S::kThreads;
+  constexpr int kList = kBatch + 4 * S::kThreads;  // entries
+  constexpr int kGather = 64, kRow = S::TA * 2 + 16;
+  int32_t* token = reinterpret_cast<int32_t*>(lds);
+  int32_t* what = token + kList;  // its class in the tile
+  float* rest = reinterpret_cast<float*>(what + kList);
+  int32_t* votes = reinterpret_cast<int32_t*>(rest + kList);  // [kEach][kWaves]
+  char* gathered = reinterpret_cast<char*>(votes + kEach * kWaves);
+  static_assert(kList * 12 + kEach * kWaves * 4 + kGather * kRow <= S::kLdsBytes, "lists and rows in LDS");
+  const int w = threadIdx.x / kWave, l = lane_id();
+  const int col = (w % S::WA) * (S::TA / S::WA) + (l & 15), row = (w / S::WA) * (S::TB / S::WB) + (l & 15);
+  int held = 0;
+  for (int64_t r0 = 0; r0 < n; r0 += kBatch) {
+    int in[kEach];
+    uint64_t vote[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      in[i] = f.mark[min(r0 + i * S::kThreads + threadIdx.x, n - 1)] - static_cast<int>(f.first + b0);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      vote[i] = __ballot(r0 + i * S::kThreads + threadIdx.x < n && in[i] >= 0 && in[i] < classes);
+      if (l == 0) votes[i * kWaves + w] = __popcll(vote[i]);
+    }
+    __syncthreads();
+    int at = held;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      for (int k = 0; k < kWaves; ++k) {
+        if (k == w && (vote[i] >> l & 1)) {
+          const int64_t r = r0 + i * S::kThreads + threadIdx.x;
+          const int to = at + __popcll(vote[i] & ((1ull << l) - 1));
+          token[to] = static_cast<int32_t>(r);
+          what[to] = in[i];
+          rest[to] = f.rest[r];
+        }
+        at += votes[i * kWaves + k];
+      }
+    }
+    held = at;
+    __syncthreads();
+    // on to the next marks while there is room for them
+    if (held == 0 || (held <= kList - kBatch && r0 + kBatch < n)) continue;
+    for (int i = held + threadIdx.x; i < (held + 31) / 32 * 32; i += S::kThreads) {
+      token[i] = 0;
+      what[i] = -1;
+      rest[i] = 0.0f;
+    }
+    __syncthreads();
+    for (int first = 0; first < held; first += kGather) {
+      const int some = min(kGather, (held - first + 31) / 32 * 32);
+      constexpr int kLanes = S::TA / 8;
+#pragma unroll
+      for (int j = 0; j < kGather * kLanes / S::kThreads; ++j) {
+        const int i = j * S::kThreads + threadIdx.x, c = i % kLanes * 8;
+        if (i / kLanes >= some) continue;
+        U32x4 v{0, 0, 0, 0};
+        if (a0 + c < f.ld) v = *reinterpret_cast<const U32x4*>(f.x + token[first + i / kLanes] * f.ld + a0 + c);
+        *reinterpret_cast<U32x4*>(gathered + i / kLanes * kRow + c * 2) = v;
+      }
+      __syncthreads();
+      for (int i = 0; i < some; i += 32) {
+        const int k0 = i + (l >> 4) * 8;
+        bf16x8 b[S::FB];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int4 c = *reinterpret_cast<const int4*>(what + first + k0 + 4 * h);
+          const float4 e = *reinterpret_cast<const float4*>(rest + first + k0 + 4 * h);
+          const int cs[4] = {c.x, c.y, c.z, c.w};
+          const float es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int fb = 0; fb < S::FB; ++fb)
+              b[fb][4 * h + k] = static_cast<__bf16>(cs[k] == row + fb * 16 ? es[k] : 0.0f);
+        }
+        // sixteen lanes' 8 bytes of four rows come back as four rows of one column a lane
+        const char* from = gathered + (k0 + ((l & 15) >> 2)) * kRow + ((col & ~15) + (l & 3) * 4) * 2;
+#pragma unroll
+        for (int fa = 0; fa < S::FA; ++fa) {
+          typedef short s16x4 __attribute__((ext_vector_type(4)));
+          typedef short s16x8 __attribute__((ext_vector_type(8)));
+          typedef __attribute__((address_space(3))) s16x4* Turned;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Turned)(from + fa * 32));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Turned)(from + 4 * kRow + fa * 32));
+          const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int fb = 0; fb < S::FB; ++fb)
+            acc[fa][fb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b[fb], acc[fa][fb], 0, 0, 0);
+        }
+      }
+      __syncthreads();
+    }
+    held = 0;
   }
 }
 
@@ -767,11 +898,11 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void grad_kernel(Logits f, Gra
 // sums of a run of the K steps, blockIdx.y's, added to what earlier pieces left
 // (accumulate); else rounded to T. The rows at work are the gradient's rows of B
 // (rows_of_b) or the K axis.
-template <typename T, int SEGS, bool SLOT>
-__global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Operand b, int ksteps, bool rows_of_b,
+template <class S, typename T, int SEGS, bool SLOT>
+__global__ __launch_bounds__(S::kThreads, S::kGroups) void out_kernel(Operand a, Operand b, int ksteps, bool rows_of_b,
                                                                   const int32_t* count, T* out, int64_t ldo,
-                                                                  int64_t slot, int accumulate) {
-  __shared__ __attribute__((aligned(1024))) char lds[ntgemm::kLdsBytes];
+                                                                  int64_t slot, int accumulate, Rests rests) {
+  __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
   if (rows_of_b) b.rows = *count;
   else ksteps = (*count + kStep - 1) / kStep;
   if (SLOT) {
@@ -781,33 +912,37 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Ope
     b.p += static_cast<int64_t>(from) * kStep;
     out += blockIdx.y * slot;
   }
-  const int ta = tiles(a.rows), tb = tiles(b.rows);
+  const int ta = tiles(a.rows, S::TA), tb = tiles(b.rows, S::TB);
   if (static_cast<int64_t>(blockIdx.x) >= static_cast<int64_t>(ta) * tb) return;
   int ia, ib;
   ntgemm::tile_of(blockIdx.x, ta, tb, ia, ib);
-  f32x4 acc[kFragA][kFragB];
-  ntgemm::product<SEGS>(a, b, ia, ib, ksteps, lds, acc);
-  const Place at(ia, ib);
+  f32x4 acc[S::FA][S::FB];
+  ntgemm::product<S, SEGS>(a, b, ia, ib, ksteps, lds, acc);
+  if constexpr (SEGS == 1)
+    if (rests.mark && (!SLOT || blockIdx.y == 0))
+      add_rests<S>(rests, *count, static_cast<int64_t>(ia) * S::TA, static_cast<int64_t>(ib) * S::TB,
+                   min(static_cast<int64_t>(S::TB), b.rows - static_cast<int64_t>(ib) * S::TB), lds, acc);
+  const Place<S> at(ia, ib);
   if constexpr (std::is_same_v<T, bf16>) {
 #pragma unroll
-    for (int fb = 0; fb < kFragB; ++fb)
+    for (int fb = 0; fb < S::FB; ++fb)
 #pragma unroll
-      for (int fa = 0; fa < kFragA; ++fa) {
+      for (int fa = 0; fa < S::FA; ++fa) {
         const f32x4 v = acc[fa][fb];
-        stage(lds, fa, fb, rowvec::pack_bf16(v[0], v[1]), rowvec::pack_bf16(v[2], v[3]));
+        stage<S>(lds, fa, fb, rowvec::pack_bf16(v[0], v[1]), rowvec::pack_bf16(v[2], v[3]));
       }
     __syncthreads();
-    uint16_t* to = reinterpret_cast<uint16_t*>(out) + static_cast<int64_t>(ib) * kTile * ldo + static_cast<int64_t>(ia) * kTile;
-    store_tile<true>(lds, to, ldo, static_cast<int>(min(static_cast<int64_t>(kTile), b.rows - static_cast<int64_t>(ib) * kTile)),
-                     static_cast<int>(min(static_cast<int64_t>(kTile), a.rows - static_cast<int64_t>(ia) * kTile)));
+    uint16_t* to = reinterpret_cast<uint16_t*>(out) + static_cast<int64_t>(ib) * S::TB * ldo + static_cast<int64_t>(ia) * S::TA;
+    store_tile<S, true>(lds, to, ldo, static_cast<int>(min(static_cast<int64_t>(S::TB), b.rows - static_cast<int64_t>(ib) * S::TB)),
+                     static_cast<int>(min(static_cast<int64_t>(S::TA), a.rows - static_cast<int64_t>(ia) * S::TA)));
   } else {
     typedef float Any __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
-    for (int fb = 0; fb < kFragB; ++fb) {
+    for (int fb = 0; fb < S::FB; ++fb) {
       if (at.b(fb) >= b.rows) continue;
       T* row = out + at.b(fb) * ldo;
 #pragma unroll
-      for (int fa = 0; fa < kFragA; ++fa) {
+      for (int fa = 0; fa < S::FA; ++fa) {
         const int64_t i = at.a(fa);
         if (SLOT) {  // rows of a multiple of four floats
           f32x4* to = reinterpret_cast<f32x4*>(row + i);
@@ -828,7 +963,9 @@ __global__ __launch_bounds__(ntgemm::kThreads, 1) void out_kernel(Operand a, Ope
 // with a gradient, by their places (zeros elsewhere), or without places.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, const int32_t* place, const float* slots,
-                                                          int ns, int64_t slot, int Dp, T* gx) {
+                                                          int ns, int64_t slot, int Dp, T* gx, const int32_t* mark,
+                                                          const float* rest, const T* w, int64_t ldw, const void* bias,
+                                                          int bias_f32) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
   const int per = Dp / 4;
   const int64_t r = i / per;
@@ -838,21 +975,31 @@ __global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, cons
   f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
   if (p >= 0)
     for (int s = 0; s < ns; ++s) v += *reinterpret_cast<const f32x4*>(slots + s * slot + p * Dp + c);
+  if (mark && p >= 0) {
+    // what rounding left of the label's entry (Rests); a masked label's weight is not read
+    const int y = mark[p];
+    if (y >= 0 && !(bias && bias_at(bias, bias_f32, y) == -INFINITY)) {
+      const T* row = w + y * ldw + c;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < D) v[k] = fmaf(rest[p], to_f32(row[k]), v[k]);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (c + k < D) gx[r * D + c + k] = from_f32<T>(v[k]);
 }
 
-// grad_b of a piece from the tiles' sums: 32 classes a workgroup, eight slices of the
+// grad_b of a piece from the sums of tiles of `tile` rows: 32 classes a workgroup, eight slices of the
 // tiles, then the slices in order.
 constexpr int kBiasCols = 32;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void bias_kernel(const int32_t* count, int64_t V, const float* part, T* gb) {
+__global__ __launch_bounds__(kBlock) void bias_kernel(const int32_t* count, int tile, int64_t V, const float* part, T* gb) {
   constexpr int kSlices = kBlock / kBiasCols;
   __shared__ float red[kSlices][kBiasCols];
   const int c = threadIdx.x % kBiasCols, k = threadIdx.x / kBiasCols;
   const int64_t v = static_cast<int64_t>(blockIdx.x) * kBiasCols + c;
-  const int nt = tiles(*count);
+  const int nt = tiles(*count, tile);
   float s = 0.0f;
   if (v < V)
     for (int t = k; t < nt; t += kSlices) s += part[t * V + v];
@@ -880,17 +1027,64 @@ bool in_place(int dtype, int D, const void* p, int64_t ld) {
   return dtype == kBF16 && D % kStep == 0 && rows_aligned(p, ld, 2) && ld <= (1 << 24);
 }
 
+// Tiles of a product of A's and B's rows, with tiles of 256 or 128 rows.
+int64_t tile_count(int64_t a, int64_t b, bool small) {
+  const int64_t t = small ? Small::TA : Large::TA;
+  return ((a + t - 1) / t) * ((b + t - 1) / t);
+}
+
+// Rounds of tiles over the card, in those of large ones: 256 at a time, or 512 small
+// ones, two a CU, in 0.8 of that time for half of the products (up to 256 in 0.6;
+// measured 0.76 to 0.89, and 0.55 to 0.61).
+constexpr int kCus = 256;
+double rounds(int64_t count, bool small) {
+  if (!small) return static_cast<double>((count + kCus - 1) / kCus);
+  return count <= kCus ? 0.6 : 0.8 * static_cast<double>((count + 2 * kCus - 1) / (2 * kCus));
+}
+
+// Whether the logits of a classes and b rows are formed in small tiles: where large
+// ones leave CUs without work (412 rows against 10,093 classes of 3404 float32: 80
+// large tiles 405 us, 316 small ones SMALLUS).
+bool small_tiles(int64_t a, int64_t b) {
+  return rounds(tile_count(a, b, true), true) < rounds(tile_count(a, b, false), false);
+}
+
+// A product whose K steps may be cut into slots.
+struct Out {
+  bool small;
+  int splits;
+};
+
+// Few tiles: their K steps cut into slots, so that every CU has work, as long as a slot
+// keeps eight steps; the tile by the rounds that takes, a slot's sums counted as two
+// steps.
+Out out_of(int64_t a, int64_t b, int64_t steps) {
+  Out best{false, 1};
+  double least = 0.0;
+  for (int small = 0; small < 2; ++small) {
+    const int64_t t = tile_count(a, b, small), room = small ? 2 * kCus : kCus;
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({room / std::max<int64_t>(1, t), steps / 8, 32}));
+    const double time = rounds(t * splits, small) * static_cast<double>((steps + splits - 1) / splits) + 2.0 * splits;
+    if (!small || time < least) {
+      best = Out{small != 0, static_cast<int>(splits)};
+      least = time;
+    }
+  }
+  return best;
+}
+
+constexpr int kTile = Large::TA;  // pieces are a multiple of it
+
 struct Cut {
   int parts, Kp;
-  int64_t fwd_piece;         // classes packed at a time by the forward
-  int64_t piece;             // classes of a piece of the backward
-  int64_t rows_p;            // rows to the next multiple of kStep
-  int splits;                // slots of the rows' gradient
-  int wsplits;               // slots of the weight's gradient, 1: none
+  int64_t fwd_piece;  // classes packed at a time by the forward
+  int64_t piece;      // classes of a piece of the backward
+  int64_t rows_p;     // rows to the next multiple of kStep
+  bool stats_small, grad_small;
+  Out dx, dw;         // the rows' gradient, in slots that the pieces add to; the weight's
   int Dp;
 };
 
-constexpr int kCus = 256;
 constexpr int64_t kPieceValues = 64ll << 20;   // of dz in a piece
 constexpr int64_t kPackValues = 256ll << 20;   // of packed classes in a piece of the forward
 
@@ -908,14 +1102,11 @@ Cut cut(int dtype, int64_t n, int64_t V, int D) {
   c.piece = even(std::min<int64_t>(kPieceValues / std::max<int64_t>(kStep, c.rows_p),
                                    kPackValues / (c.parts * static_cast<int64_t>(c.Kp))));
   c.Dp = static_cast<int>(up(D, 4));
-  // Few tiles: their K steps cut into slots, so that all 256 CUs have a workgroup, as
-  // long as a slot keeps eight steps.
-  const auto slots = [](int64_t tiles, int64_t steps) {
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kCus / std::max<int64_t>(1, tiles), steps / 8, 32})));
-  };
-  const int64_t cols = (D + kTile - 1) / kTile, most = std::min(c.piece, V);
-  c.splits = slots((n + kTile - 1) / kTile * cols, up(most, kStep) / kStep);
-  c.wsplits = slots((most + kTile - 1) / kTile * cols, c.rows_p / kStep);
+  const int64_t most = std::min(c.piece, V);
+  c.stats_small = small_tiles(std::min(c.fwd_piece, V), n);
+  c.grad_small = small_tiles(most, n);
+  c.dx = out_of(D, n, up(most, kStep) / kStep);
+  c.dw = out_of(D, most, c.rows_p / kStep);
   return c;
 }
 
@@ -933,8 +1124,8 @@ struct Regions {
 };
 
 // Sets of classes whose statistics are joined.
-int64_t stat_tiles(int64_t n, int64_t V) {
-  const int64_t classes = n <= kFewRows ? kFewClasses : kTile;
+int64_t stat_tiles(const Cut& c, int64_t n, int64_t V) {
+  const int64_t classes = n <= kFewRows ? kFewClasses : c.stats_small ? Small::TA : Large::TA;
   return (V + classes - 1) / classes;
 }
 
@@ -948,7 +1139,7 @@ struct FwdSpace {
 int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void* p, FwdSpace* s) {
   Regions r(p);
   FwdSpace f;
-  f.part = r.take<float2>(n * stat_tiles(n, V));
+  f.part = r.take<float2>(n * stat_tiles(c, n, V));
   f.chosen = r.take<float>(n);
   f.x = f.w = nullptr;
   if (n > kFewRows) {
@@ -960,7 +1151,8 @@ int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void
 }
 
 struct BwdSpace {
-  int32_t *list, *place, *count;
+  int32_t *list, *place, *count, *mark;
+  float* rest;
   uint16_t *x, *xt, *w, *wt, *dz, *dzt;
   float *slots, *wslots, *bias;
 };
@@ -972,19 +1164,21 @@ int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, 
   b.list = r.take<int32_t>(n);
   b.place = r.take<int32_t>(n);
   b.count = r.take<int32_t>(1);
+  b.mark = r.take<int32_t>(n);
+  b.rest = r.take<float>(n);
   b.x = r.take<uint16_t>(c.parts * n * c.Kp);
   if (!w_in) b.w = r.take<uint16_t>(c.parts * vc * c.Kp);
   if (of & 1) {
     b.wt = r.take<uint16_t>(c.parts * vc * D);
     b.dz = r.take<uint16_t>(c.parts * n * vc);
-    b.slots = r.take<float>(c.splits * n * c.Dp);
+    b.slots = r.take<float>(c.dx.splits * n * c.Dp);
   }
   if (of & 2) {
     b.xt = r.take<uint16_t>(c.parts * c.rows_p * D);
     b.dzt = r.take<uint16_t>(c.parts * c.rows_p * vc);
-    if (c.wsplits > 1) b.wslots = r.take<float>(c.wsplits * vc * c.Dp);
+    if (c.dw.splits > 1) b.wslots = r.take<float>(c.dw.splits * vc * c.Dp);
   }
-  if (of & 4) b.bias = r.take<float>(((n + kTile - 1) / kTile) * vc);
+  if (of & 4) b.bias = r.take<float>(((n + Small::TB - 1) / Small::TB) * vc);
   if (s) *s = b;
   return r.total;
 }
@@ -1020,8 +1214,12 @@ const void* bias_of(const void* bias, int f32, int64_t v) {
   return bias ? static_cast<const char*>(bias) + v * (f32 ? 4 : 2) : nullptr;
 }
 
-uint32_t tile_count(int64_t a, int64_t b) {
-  return static_cast<uint32_t>(((a + kTile - 1) / kTile) * ((b + kTile - 1) / kTile));
+// f(Large()) or f(Small()), and the grid of its tiles.
+template <class F>
+void with_tiles(bool small, int64_t a, int64_t b, int splits, F&& f) {
+  const dim3 grid(static_cast<uint32_t>(tile_count(a, b, small)), splits);
+  if (small) f(Small(), grid);
+  else f(Large(), grid);
 }
 
 template <typename T>
@@ -1033,7 +1231,7 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
   const bool xin = in_place(dtype, D, x, ldx), win = in_place(dtype, D, w, ldw);
   FwdSpace s;
   fwd_space(c, n, V, xin, win, ws, &s);
-  const int nt = static_cast<int>(stat_tiles(n, V));
+  const int nt = static_cast<int>(stat_tiles(c, n, V));
   if (n <= kFewRows) {
     const bool stream = rows_aligned(x, ldx, sizeof(T)) && rows_aligned(w, ldw, sizeof(T)) && D % (128 / sizeof(T)) == 0;
     const auto launch = [&](auto TC) {
@@ -1064,8 +1262,11 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
         if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, w + v * ldw, ldw, s.w, c.Kp, wo.part)) return rc;
       }
       const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, nullptr, labels};
-      hipLaunchKernelGGL((stats_kernel<SEGS>), dim3(tile_count(vn, n)), dim3(ntgemm::kThreads), 0, st, f, n, s.part,
-                         static_cast<int>(v / kTile), s.chosen);
+      with_tiles(c.stats_small, vn, n, 1, [&](auto shape, dim3 grid) {
+        using S = decltype(shape);
+        hipLaunchKernelGGL((stats_kernel<S, SEGS>), grid, dim3(S::kThreads), 0, st, f, n, s.part,
+                           static_cast<int>(v / S::TA), s.chosen);
+      });
       if (const int rc = check_launch("cign_linear_xent_fwd")) return rc;
     }
   }
@@ -1092,8 +1293,8 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
   const int of = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
   BwdSpace s;
   bwd_space(c, n, V, D, win, of, ws, &s);
-  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, n, labels, ignore, g_loss, g_lse, s.list, s.place,
-                     s.count);
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, n, labels, ignore, g_loss, g_lse,
+                     static_cast<int64_t>(V), s.list, s.place, s.count, s.mark, s.rest);
   if (const int rc = check_launch(who)) return rc;
   const Operand xo{s.x, n, c.Kp, n * c.Kp};
   if (const int rc = pack<T, PARTS>(st, n, s.count, s.list, D, x, ldx, s.x, c.Kp, xo.part)) return rc;
@@ -1110,8 +1311,11 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
     }
     const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, s.count, labels};
     const Grads g{s.list, lse,   g_loss, g_lse,    ignore,     V,    s.dz, vp,
-                  n * vp, s.dzt, c.rows_p, c.rows_p * vn, s.bias};
-    hipLaunchKernelGGL((grad_kernel<SEGS>), dim3(tile_count(vn, n)), dim3(ntgemm::kThreads), 0, st, f, g);
+                  n * vp, s.dzt, c.rows_p, c.rows_p * vn, s.bias, s.rest};
+    with_tiles(c.grad_small, vn, n, 1, [&](auto shape, dim3 grid) {
+      using S = decltype(shape);
+      hipLaunchKernelGGL((grad_kernel<S, SEGS>), grid, dim3(S::kThreads), 0, st, f, g);
+    });
     if (const int rc = check_launch(who)) return rc;
     if (gx) {
       const Operand wt{s.wt, D, vp, vp * D};
@@ -1119,39 +1323,51 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
                                             vp, wt.part))
         return rc;
       const Operand dz{s.dz, n, vp, n * vp};
-      hipLaunchKernelGGL((out_kernel<float, SEGS, true>), dim3(tile_count(D, n), c.splits), dim3(ntgemm::kThreads), 0, st,
-                         wt, dz, static_cast<int>(vp / kStep), true, s.count, s.slots, static_cast<int64_t>(c.Dp),
-                         n * c.Dp, v > 0);
+      with_tiles(c.dx.small, D, n, c.dx.splits, [&](auto shape, dim3 grid) {
+        using S = decltype(shape);
+        hipLaunchKernelGGL((out_kernel<S, float, SEGS, true>), grid, dim3(S::kThreads), 0, st, wt, dz,
+                           static_cast<int>(vp / kStep), true, s.count, s.slots, static_cast<int64_t>(c.Dp), n * c.Dp,
+                           v > 0, Rests{});
+      });
       if (const int rc = check_launch(who)) return rc;
     }
     if (gw) {
       const Operand dzt{s.dzt, vn, c.rows_p, c.rows_p * vn};
-      if (c.wsplits > 1) {
-        hipLaunchKernelGGL((out_kernel<float, SEGS, true>), dim3(tile_count(D, vn), c.wsplits), dim3(ntgemm::kThreads), 0,
-                           st, xt, dzt, 0, false, s.count, s.wslots, static_cast<int64_t>(c.Dp), vn * c.Dp, 0);
+      const Rests rests{PARTS == 1 ? s.mark : nullptr, s.rest, v, s.x, c.Kp};
+      with_tiles(c.dw.small, D, vn, c.dw.splits, [&](auto shape, dim3 grid) {
+        using S = decltype(shape);
+        if (c.dw.splits > 1)
+          hipLaunchKernelGGL((out_kernel<S, float, SEGS, true>), grid, dim3(S::kThreads), 0, st, xt, dzt, 0, false, s.count,
+                             s.wslots, static_cast<int64_t>(c.Dp), vn * c.Dp, 0, rests);
+        else
+          hipLaunchKernelGGL((out_kernel<S, T, SEGS, false>), grid, dim3(S::kThreads), 0, st, xt, dzt, 0, false, s.count,
+                             gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0, rests);
+      });
+      if (c.dw.splits > 1) {
         if (const int rc = check_launch(who)) return rc;
         hipLaunchKernelGGL((rows_out_kernel<T>), grid_of(vn * (c.Dp / 4)), dim3(kBlock), 0, st, vn, D,
-                           static_cast<const int32_t*>(nullptr), s.wslots, c.wsplits, vn * c.Dp, c.Dp, gw + v * D);
-      } else {
-        hipLaunchKernelGGL((out_kernel<T, SEGS, false>), dim3(tile_count(D, vn)), dim3(ntgemm::kThreads), 0, st, xt, dzt, 0,
-                           false, s.count, gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0);
+                           static_cast<const int32_t*>(nullptr), s.wslots, c.dw.splits, vn * c.Dp, c.Dp, gw + v * D,
+                           static_cast<const int32_t*>(nullptr), static_cast<const float*>(nullptr),
+                           static_cast<const T*>(nullptr), static_cast<int64_t>(0), static_cast<const void*>(nullptr), 0);
       }
       if (const int rc = check_launch(who)) return rc;
     }
     if (gb) {
       const dim3 bias_grid(static_cast<uint32_t>((vn + kBiasCols - 1) / kBiasCols));
       if (bias_f32)
-        hipLaunchKernelGGL((bias_kernel<float>), bias_grid, dim3(kBlock), 0, st, s.count, vn, s.bias,
+        hipLaunchKernelGGL((bias_kernel<float>), bias_grid, dim3(kBlock), 0, st, s.count, c.grad_small ? Small::TB : Large::TB, vn,
+                           s.bias,
                            static_cast<float*>(gb) + v);
       else
-        hipLaunchKernelGGL((bias_kernel<bf16>), bias_grid, dim3(kBlock), 0, st, s.count, vn, s.bias,
+        hipLaunchKernelGGL((bias_kernel<bf16>), bias_grid, dim3(kBlock), 0, st, s.count, c.grad_small ? Small::TB : Large::TB, vn,
+                           s.bias,
                            static_cast<bf16*>(gb) + v);
       if (const int rc = check_launch(who)) return rc;
     }
   }
   if (gx) {
     hipLaunchKernelGGL((rows_out_kernel<T>), grid_of(n * (c.Dp / 4)), dim3(kBlock), 0, st, n, D, s.place, s.slots,
-                       c.splits, n * c.Dp, c.Dp, gx);
+                       c.dx.splits, n * c.Dp, c.Dp, gx, PARTS == 1 ? s.mark : nullptr, s.rest, w, ldw, bias, bias_f32);
     return check_launch(who);
   }
   return kOk;
