@@ -4,14 +4,28 @@
 //   dz_v = (g_loss + g_lse) e^(z_v - lse) - g_loss [v = label],
 //   grad_x = dz W, grad_W = dz^T x, grad_b = sum over rows of dz.
 //
-// Forward: tiles of 256 rows by 256 classes (nt_gemm.h), whose largest logit and
-// sum of exponentials a row leave the tile; join_kernel brings them together. Few
-// rows (up to 64) stream W through the matrix units instead (few_kernel).
-// Backward: a piece's logits are formed again, and their gradient is stored in
-// bf16 as it stands and transposed, so that every product is one of rows that run
-// along the summed axis. float32 operands are held as three bf16 parts of 8 bits
-// each and multiplied in six products, the smallest first: the dropped ones lie
-// below 2^-26 of a product, so the sums are float32's own.
+// Forward: tiles of 256 rows by 256 classes (nt_gemm.h), or 128 by 128 where those
+// leave CUs idle, whose largest logit and sum of exponentials a row leave the tile;
+// join_kernel brings them together. Up to 64 rows take no tiles: the classes stream
+// through a wavefront's registers once (stream_kernel; few_kernel where rows do not
+// start 16-byte aligned).
+// Backward: the rows whose gradient is not zero are listed, a piece's logits are formed
+// again, their gradient is stored in bf16 parts, and both products read it: the weight's
+// with the rows as the summed axis, through LDS reads that turn 4 x 16 values.
+//
+// float32 operands are held as three bf16 parts of 8 bits each and multiplied in six
+// products, the smallest first: the dropped ones lie below 2^-26 of a product, so the
+// sums are float32's own. bfloat16 gradients of logits are rounded once, to bf16; the
+// entry of a row's label, which holds most of its row's sum, has what that rounding
+// dropped added back to the weight's gradient (Rests) and to the rows' (rows_out_kernel).
+//
+// What bounds it: the four products, 8 n V D operations, and beside them little. Forward
+// and backward of 8192 rows, 32,000 classes, 4096 wide, a tenth of the rows without a
+// label, 6.4 ms in bf16 (1,280 TFLOP/s over the four), of which 1.55 stats_kernel,
+// 4 x 0.40 each of grad_kernel and the two out_kernels, 0.1 the rest; 4096 rows, 131,072
+// classes, 2048 wide 7.2 ms. 24,492 rows, 2000 classes, 1280 wide, half of them without
+// a label, float32: 1.7 ms (six products each: 1,300 TFLOP/s of bf16 inside the tiles).
+// One row of 131,072 classes, 4096 wide, bf16: 185 us, 5.8 TB/s.
 #include <algorithm>
 
 #include "nt_gemm.h"
@@ -29,7 +43,7 @@ using ntgemm::Small;
 
 constexpr int kMaxClasses = 1 << 20;
 constexpr int kMaxWidth = 1 << 16;
-constexpr int kMaxRows = 1 << 23;  // 32-bit offsets in a tile of the transposed gradient
+constexpr int kMaxRows = 1 << 23;  // launches of n D / 8 threads stay in 32 bits of workgroups
 constexpr int kFewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -479,23 +493,26 @@ __global__ __launch_bounds__(1024) void rows_kernel(int64_t n, const int64_t* la
   if (threadIdx.x == 0) *count = base;
 }
 
-// Rows of D values of T as bf16 parts, Kp values apart with zeros behind the
-// row's own; rows of a list where there is one.
+// Rows of D values of T as bf16 parts, Kp values apart with zeros behind the row's
+// own, rows of a list where there is one; zeros for classes that a bias of -inf masks
+// (their logits' gradients are zero, which a NaN would not stay).
 template <typename T, int PARTS>
 __global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* count, const int32_t* list, int D,
-                                                      const T* src, int64_t ld, uint16_t* dst, int Kp, int64_t part) {
+                                                      const T* src, int64_t ld, const void* bias, int bias_f32,
+                                                      uint16_t* dst, int Kp, int64_t part) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
   const int per = Kp / 8;
   const int64_t r = i / per;
   const int c = static_cast<int>(i - r * per) * 8;
   if (r >= (count ? *count : n)) return;
   const T* row = src + (list ? list[r] : r) * ld;
+  const bool on = !(bias && bias_at(bias, bias_f32, r) == -INFINITY);
   float v[8];
-  if (c + 8 <= D) {
+  if (on && c + 8 <= D) {
     rowvec::RowChunk<T, 8>::unpack(rowvec::RowChunk<T, 8>::load(row + c), v);
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < D ? to_f32(row[c + k]) : 0.0f;
+    for (int k = 0; k < 8; ++k) v[k] = on && c + k < D ? to_f32(row[c + k]) : 0.0f;
   }
   U32x4 o[PARTS];
 #pragma unroll
@@ -509,58 +526,8 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* 
   for (int q = 0; q < PARTS; ++q) *reinterpret_cast<U32x4*>(dst + q * part + r * Kp + c) = o[q];
 }
 
-// The same transposed: dst[c][r], rows of dst Rp values apart, zeros for rows
-// from the last one to the next multiple of kStep, and for classes that a bias of
-// -inf masks (whose gradients are zero, which a NaN would not stay). 64 x 64 values a workgroup.
-template <typename T, int PARTS>
-__global__ __launch_bounds__(kBlock) void pack_t_kernel(int64_t n, const int32_t* count, const int32_t* list, int D,
-                                                        const T* src, int64_t ld, const void* bias, int bias_f32,
-                                                        uint16_t* dst, int64_t Rp, int64_t part) {
-  __shared__ float tile[64][65];
-  const int64_t rows = count ? *count : n;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
-  const int c0 = blockIdx.y * 64;
-  if (r0 >= rows) return;
-  const int a = threadIdx.x >> 2, b = (threadIdx.x & 3) * 16;
-  {
-    const int64_t r = r0 + a;
-    const bool on = r < rows && !(bias && bias_at(bias, bias_f32, r) == -INFINITY);
-    const T* row = src + (on ? (list ? list[r] : r) : 0) * ld;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + b + 8 * h;
-      float v[8];
-      if (on && c + 8 <= D) {
-        rowvec::RowChunk<T, 8>::unpack(rowvec::RowChunk<T, 8>::load(row + c), v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = on && c + k < D ? to_f32(row[c + k]) : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) tile[a][b + 8 * h + k] = v[k];
-    }
-  }
-  __syncthreads();
-  if (c0 + a >= D) return;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    U32x4 o[PARTS];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t p[PARTS];
-      split<PARTS>(tile[b + 8 * h + 2 * k][a], tile[b + 8 * h + 2 * k + 1][a], p);
-#pragma unroll
-      for (int q = 0; q < PARTS; ++q) o[q][k] = p[q];
-    }
-#pragma unroll
-    for (int q = 0; q < PARTS; ++q)
-      *reinterpret_cast<U32x4*>(dst + q * part + static_cast<int64_t>(c0 + a) * Rp + r0 + b + 8 * h) = o[q];
-  }
-}
-
-// The gradient of a piece's logits, in bf16 parts: dz[row][class] and
-// dzt[class][row], zeros up to the next multiple of kStep of each axis; and the
-// tile's sums over its rows, for the bias.
+// The gradient of a piece's logits, in bf16 parts: dz[row][class], zeros up to the next
+// multiple of kStep of each axis; and the tile's sums over its rows, for the bias.
 struct Grads {
   const int32_t* list;
   const float* lse;
@@ -570,8 +537,6 @@ struct Grads {
   int64_t V;
   uint16_t* dz;
   int64_t ld, part;
-  uint16_t* dzt;
-  int64_t ldt, partt;
   float* bias_part;        // [tile of rows][class of the piece] or null
   float* rest;             // what rounding to bf16 leaves of the label's entry, by row
 };
@@ -613,21 +578,6 @@ __device__ __forceinline__ void stage(char* lds, int fa, int fb, uint32_t first,
   const int w = threadIdx.x / kWave, l = lane_id();
   *reinterpret_cast<uint2*>(lds + ((w / S::WA) * (S::TB / S::WB) + fb * 16 + (l & 15)) * kStageRow<S> +
                             ((w % S::WA) * (S::TA / S::WA) + fa * 16 + (l >> 4) * 4) * 2) = make_uint2(first, second);
-}
-
-// The same transposed, [row of A][row of B]: two neighbouring lanes exchange two of
-// their values, so that each has two rows of A for both of its rows of B.
-template <class S>
-__device__ __forceinline__ void stage_t(char* lds, int fa, int fb, uint32_t first, uint32_t second) {
-  const int w = threadIdx.x / kWave, l = lane_id();
-  const bool odd = l & 1;
-  const uint32_t give = odd ? first : second, keep = odd ? second : first;
-  const uint32_t got = __float_as_uint(dpp<0xB1>(__uint_as_float(give)));  // of the lane beside
-  const uint32_t even_lane = odd ? got : keep, odd_lane = odd ? keep : got;
-  char* to = lds + ((w % S::WA) * (S::TA / S::WA) + fa * 16 + (l >> 4) * 4 + 2 * odd) * kStageRow<S> +
-             ((w / S::WA) * (S::TB / S::WB) + fb * 16 + (l & 14)) * 2;
-  *reinterpret_cast<uint32_t*>(to) = (even_lane & 0xffff) | (odd_lane << 16);
-  *reinterpret_cast<uint32_t*>(to + kStageRow<S>) = (even_lane >> 16) | (odd_lane & 0xffff0000u);
 }
 
 template <class S, int SEGS>
@@ -737,45 +687,23 @@ __global__ __launch_bounds__(S::kThreads, S::kGroups) void grad_kernel(Logits f,
       __syncthreads();
     }
   }
-  // each part as it stands, then transposed, through LDS; zeros up to the next
-  // multiple of kStep of either axis
+  if (!g.dz) return;
+  // each part through LDS; zeros up to the next multiple of kStep of either axis
 #pragma unroll
   for (int q = 0; q < PARTS; ++q) {
-    const auto part = [&](const f32x4& d, uint32_t& first, uint32_t& second) {
-      uint32_t lo[PARTS], hi[PARTS];
-      split<PARTS>(d[0], d[1], lo);
-      split<PARTS>(d[2], d[3], hi);
-      first = lo[q];
-      second = hi[q];
-    };
-    if (g.dz) {
 #pragma unroll
-      for (int fa = 0; fa < S::FA; ++fa)
+    for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
-        for (int fb = 0; fb < S::FB; ++fb) {
-          uint32_t first, second;
-          part(acc[fa][fb], first, second);
-          stage<S>(lds, fa, fb, first, second);
-        }
-      __syncthreads();
-      store_tile<S, false>(lds, g.dz + q * g.part + static_cast<int64_t>(ib) * S::TB * g.ld + static_cast<int64_t>(ia) * S::TA,
-                        g.ld, rows, (classes + kStep - 1) / kStep * kStep);
-      __syncthreads();
-    }
-    if (g.dzt) {
-#pragma unroll
-      for (int fa = 0; fa < S::FA; ++fa)
-#pragma unroll
-        for (int fb = 0; fb < S::FB; ++fb) {
-          uint32_t first, second;
-          part(acc[fa][fb], first, second);
-          stage_t<S>(lds, fa, fb, first, second);
-        }
-      __syncthreads();
-      store_tile<S, false>(lds, g.dzt + q * g.partt + static_cast<int64_t>(ia) * S::TA * g.ldt + static_cast<int64_t>(ib) * S::TB,
-                        g.ldt, classes, (rows + kStep - 1) / kStep * kStep);
-      __syncthreads();
-    }
+      for (int fb = 0; fb < S::FB; ++fb) {
+        uint32_t lo[PARTS], hi[PARTS];
+        split<PARTS>(acc[fa][fb][0], acc[fa][fb][1], lo);
+        split<PARTS>(acc[fa][fb][2], acc[fa][fb][3], hi);
+        stage<S>(lds, fa, fb, lo[q], hi[q]);
+      }
+    __syncthreads();
+    store_tile<S, false>(lds, g.dz + q * g.part + static_cast<int64_t>(ib) * S::TB * g.ld + static_cast<int64_t>(ia) * S::TA,
+                         g.ld, (rows + kStep - 1) / kStep * kStep, (classes + kStep - 1) / kStep * kStep);
+    __syncthreads();
   }
 }
 
@@ -784,7 +712,7 @@ __global__ __launch_bounds__(S::kThreads, S::kGroups) void grad_kernel(Logits f,
 // bits, times the rows (the gradient's error is then its own rounding, 1.7e-3, where it
 // was that and the entries', 2.4e-3). x: the listed rows, x_width values of each.
 struct Rests {
-  const int32_t* mark;  // null: none
+  const int32_t* mark;  // a listed row's label, or -1
   const float* rest;
   int64_t first;        // first class of the piece
   const uint16_t* x;
@@ -896,20 +824,27 @@ __device__ __forceinline__ void add_rests(const Rests& f, int64_t n, int64_t a0,
 
 // out[b][a] = sum_k A[a][k] B[b][k], rows of out `ldo` values apart. SLOT: float32
 // sums of a run of the K steps, blockIdx.y's, added to what earlier pieces left
-// (accumulate); else rounded to T. The rows at work are the gradient's rows of B
-// (rows_of_b) or the K axis.
-template <class S, typename T, int SEGS, bool SLOT>
-__global__ __launch_bounds__(S::kThreads, S::kGroups) void out_kernel(Operand a, Operand b, int ksteps, bool rows_of_b,
+// (accumulate); else rounded to T. The rows' gradient (ROWS): B's rows are those at
+// work, A is the weight, turned; the weight's: they are the K axis, both are turned.
+template <class S, typename T, int SEGS, bool SLOT, bool ROWS>
+__global__ __launch_bounds__(S::kThreads, S::kGroups) void out_kernel(Operand a, Operand b, int ksteps,
                                                                   const int32_t* count, T* out, int64_t ldo,
                                                                   int64_t slot, int accumulate, Rests rests) {
   __shared__ __attribute__((aligned(1024))) char lds[S::kLdsBytes];
-  if (rows_of_b) b.rows = *count;
-  else ksteps = (*count + kStep - 1) / kStep;
+  if (ROWS) {
+    b.rows = *count;
+  } else {
+    ksteps = (*count + kStep - 1) / kStep;
+    a.depth = *count;
+    b.depth = static_cast<int64_t>(ksteps) * kStep;
+  }
   if (SLOT) {
     const int each = (ksteps + gridDim.y - 1) / gridDim.y, from = blockIdx.y * each;
     ksteps = max(0, min(each, ksteps - from));
-    a.p += static_cast<int64_t>(from) * kStep;
-    b.p += static_cast<int64_t>(from) * kStep;
+    a.p += static_cast<int64_t>(from) * kStep * a.ld;
+    a.depth -= static_cast<int64_t>(from) * kStep;
+    b.p += static_cast<int64_t>(from) * kStep * (ROWS ? 1 : b.ld);
+    b.depth -= static_cast<int64_t>(from) * kStep;
     out += blockIdx.y * slot;
   }
   const int ta = tiles(a.rows, S::TA), tb = tiles(b.rows, S::TB);
@@ -917,9 +852,9 @@ __global__ __launch_bounds__(S::kThreads, S::kGroups) void out_kernel(Operand a,
   int ia, ib;
   ntgemm::tile_of(blockIdx.x, ta, tb, ia, ib);
   f32x4 acc[S::FA][S::FB];
-  ntgemm::product<S, SEGS>(a, b, ia, ib, ksteps, lds, acc);
-  if constexpr (SEGS == 1)
-    if (rests.mark && (!SLOT || blockIdx.y == 0))
+  ntgemm::product<S, SEGS, true, !ROWS>(a, b, ia, ib, ksteps, lds, acc);
+  if constexpr (SEGS == 1 && !ROWS)
+    if (!SLOT || blockIdx.y == 0)
       add_rests<S>(rests, *count, static_cast<int64_t>(ia) * S::TA, static_cast<int64_t>(ib) * S::TB,
                    min(static_cast<int64_t>(S::TB), b.rows - static_cast<int64_t>(ib) * S::TB), lds, acc);
   const Place<S> at(ia, ib);
@@ -1044,7 +979,7 @@ double rounds(int64_t count, bool small) {
 
 // Whether the logits of a classes and b rows are formed in small tiles: where large
 // ones leave CUs without work (412 rows against 10,093 classes of 3404 float32: 80
-// large tiles 405 us, 316 small ones SMALLUS).
+// large tiles 405 us, 316 small ones 308 us).
 bool small_tiles(int64_t a, int64_t b) {
   return rounds(tile_count(a, b, true), true) < rounds(tile_count(a, b, false), false);
 }
@@ -1153,11 +1088,11 @@ int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void
 struct BwdSpace {
   int32_t *list, *place, *count, *mark;
   float* rest;
-  uint16_t *x, *xt, *w, *wt, *dz, *dzt;
+  uint16_t *x, *w, *dz;
   float *slots, *wslots, *bias;
 };
 
-int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, void* p, BwdSpace* s) {
+int64_t bwd_space(const Cut& c, int64_t n, int64_t V, bool w_in, int of, void* p, BwdSpace* s) {
   Regions r(p);
   BwdSpace b{};
   const int64_t vc = std::min(c.piece, up(V, kStep));
@@ -1168,16 +1103,9 @@ int64_t bwd_space(const Cut& c, int64_t n, int64_t V, int D, bool w_in, int of, 
   b.rest = r.take<float>(n);
   b.x = r.take<uint16_t>(c.parts * n * c.Kp);
   if (!w_in) b.w = r.take<uint16_t>(c.parts * vc * c.Kp);
-  if (of & 1) {
-    b.wt = r.take<uint16_t>(c.parts * vc * D);
-    b.dz = r.take<uint16_t>(c.parts * n * vc);
-    b.slots = r.take<float>(c.dx.splits * n * c.Dp);
-  }
-  if (of & 2) {
-    b.xt = r.take<uint16_t>(c.parts * c.rows_p * D);
-    b.dzt = r.take<uint16_t>(c.parts * c.rows_p * vc);
-    if (c.dw.splits > 1) b.wslots = r.take<float>(c.dw.splits * vc * c.Dp);
-  }
+  if (of & 3) b.dz = r.take<uint16_t>(c.parts * c.rows_p * vc);
+  if (of & 1) b.slots = r.take<float>(c.dx.splits * n * c.Dp);
+  if ((of & 2) && c.dw.splits > 1) b.wslots = r.take<float>(c.dw.splits * vc * c.Dp);
   if (of & 4) b.bias = r.take<float>(((n + Small::TB - 1) / Small::TB) * vc);
   if (s) *s = b;
   return r.total;
@@ -1196,18 +1124,10 @@ dim3 grid_of(int64_t threads) { return dim3(static_cast<uint32_t>((threads + kBl
 
 template <typename T, int PARTS>
 int pack(hipStream_t st, int64_t n, const int32_t* count, const int32_t* list, int D, const T* src, int64_t ld,
-         uint16_t* dst, int Kp, int64_t part) {
+         const void* bias, int bias_f32, uint16_t* dst, int Kp, int64_t part) {
   hipLaunchKernelGGL((pack_kernel<T, PARTS>), grid_of(n * (Kp / 8)), dim3(kBlock), 0, st, n, count, list, D, src, ld,
-                     dst, Kp, part);
+                     bias, bias_f32, dst, Kp, part);
   return check_launch("cign_linear_xent (pack)");
-}
-
-template <typename T, int PARTS>
-int pack_t(hipStream_t st, int64_t n, const int32_t* count, const int32_t* list, int D, const T* src, int64_t ld,
-           const void* bias, int bias_f32, uint16_t* dst, int64_t Rp, int64_t part) {
-  hipLaunchKernelGGL((pack_t_kernel<T, PARTS>), dim3(static_cast<uint32_t>((n + 63) / 64), (D + 63) / 64), dim3(kBlock),
-                     0, st, n, count, list, D, src, ld, bias, bias_f32, dst, Rp, part);
-  return check_launch("cign_linear_xent (transpose)");
 }
 
 const void* bias_of(const void* bias, int f32, int64_t v) {
@@ -1251,7 +1171,7 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
     Operand xo{reinterpret_cast<const uint16_t*>(x), n, ldx, 0};
     if (!xin) {
       xo = Operand{s.x, n, c.Kp, n * c.Kp};
-      if (const int rc = pack<T, PARTS>(st, n, nullptr, nullptr, D, x, ldx, s.x, c.Kp, xo.part)) return rc;
+      if (const int rc = pack<T, PARTS>(st, n, nullptr, nullptr, D, x, ldx, nullptr, 0, s.x, c.Kp, xo.part)) return rc;
     }
     const int64_t piece = win ? V : c.fwd_piece;
     for (int64_t v = 0; v < V; v += piece) {
@@ -1259,7 +1179,8 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
       Operand wo{reinterpret_cast<const uint16_t*>(w + v * ldw), vn, ldw, 0};
       if (!win) {
         wo = Operand{s.w, vn, c.Kp, vn * c.Kp};
-        if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, w + v * ldw, ldw, s.w, c.Kp, wo.part)) return rc;
+        if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, w + v * ldw, ldw, nullptr, 0, s.w, c.Kp, wo.part))
+          return rc;
       }
       const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, nullptr, labels};
       with_tiles(c.stats_small, vn, n, 1, [&](auto shape, dim3 grid) {
@@ -1289,58 +1210,55 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
   constexpr int PARTS = dtype == kF32 ? 3 : 1, SEGS = PARTS == 3 ? 6 : 1;
   const char* who = "cign_linear_xent_bwd";
   const Cut c = cut(dtype, n, V, D);
-  const bool win = in_place(dtype, D, w, ldw);
   const int of = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
+  const bool win = in_place(dtype, D, w, ldw) && !(bias && gx);  // masked classes are packed as zeros
   BwdSpace s;
-  bwd_space(c, n, V, D, win, of, ws, &s);
+  bwd_space(c, n, V, win, of, ws, &s);
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, n, labels, ignore, g_loss, g_lse,
                      static_cast<int64_t>(V), s.list, s.place, s.count, s.mark, s.rest);
   if (const int rc = check_launch(who)) return rc;
   const Operand xo{s.x, n, c.Kp, n * c.Kp};
-  if (const int rc = pack<T, PARTS>(st, n, s.count, s.list, D, x, ldx, s.x, c.Kp, xo.part)) return rc;
-  const Operand xt{s.xt, D, c.rows_p, c.rows_p * D};
-  if (gw)
-    if (const int rc = pack_t<T, PARTS>(st, n, s.count, s.list, D, x, ldx, nullptr, 0, s.xt, xt.ld, xt.part)) return rc;
+  if (const int rc = pack<T, PARTS>(st, n, s.count, s.list, D, x, ldx, nullptr, 0, s.x, c.Kp, xo.part)) return rc;
+  const Operand xt{s.x, D, c.Kp, n * c.Kp, c.Kp, 0};
   for (int64_t v = 0; v < V; v += c.piece) {
     const int64_t vn = std::min<int64_t>(c.piece, V - v), vp = up(vn, kStep);
     const T* wv = w + v * ldw;
     Operand wo{reinterpret_cast<const uint16_t*>(wv), vn, ldw, 0};
     if (!win) {
       wo = Operand{s.w, vn, c.Kp, vn * c.Kp};
-      if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, wv, ldw, s.w, c.Kp, wo.part)) return rc;
+      if (const int rc = pack<T, PARTS>(st, vn, nullptr, nullptr, D, wv, ldw, bias_of(bias, bias_f32, v), bias_f32, s.w,
+                                            c.Kp, wo.part))
+        return rc;
     }
     const Logits f{wo, xo, c.Kp / kStep, bias, bias_f32, v, s.count, labels};
-    const Grads g{s.list, lse,   g_loss, g_lse,    ignore,     V,    s.dz, vp,
-                  n * vp, s.dzt, c.rows_p, c.rows_p * vn, s.bias, s.rest};
+    const int64_t dz_part = c.rows_p * vp;
+    const Grads g{s.list, lse, g_loss, g_lse, ignore, V, s.dz, vp, dz_part, s.bias, s.rest};
     with_tiles(c.grad_small, vn, n, 1, [&](auto shape, dim3 grid) {
       using S = decltype(shape);
       hipLaunchKernelGGL((grad_kernel<S, SEGS>), grid, dim3(S::kThreads), 0, st, f, g);
     });
     if (const int rc = check_launch(who)) return rc;
     if (gx) {
-      const Operand wt{s.wt, D, vp, vp * D};
-      if (const int rc = pack_t<T, PARTS>(st, vn, nullptr, nullptr, D, wv, ldw, bias_of(bias, bias_f32, v), bias_f32, s.wt,
-                                            vp, wt.part))
-        return rc;
-      const Operand dz{s.dz, n, vp, n * vp};
+      const Operand wt{wo.p, D, wo.ld, wo.part, c.Kp, vn};
+      const Operand dz{s.dz, n, vp, dz_part};
       with_tiles(c.dx.small, D, n, c.dx.splits, [&](auto shape, dim3 grid) {
         using S = decltype(shape);
-        hipLaunchKernelGGL((out_kernel<S, float, SEGS, true>), grid, dim3(S::kThreads), 0, st, wt, dz,
-                           static_cast<int>(vp / kStep), true, s.count, s.slots, static_cast<int64_t>(c.Dp), n * c.Dp,
+        hipLaunchKernelGGL((out_kernel<S, float, SEGS, true, true>), grid, dim3(S::kThreads), 0, st, wt, dz,
+                           static_cast<int>(vp / kStep), s.count, s.slots, static_cast<int64_t>(c.Dp), n * c.Dp,
                            v > 0, Rests{});
       });
       if (const int rc = check_launch(who)) return rc;
     }
     if (gw) {
-      const Operand dzt{s.dzt, vn, c.rows_p, c.rows_p * vn};
+      const Operand dz{s.dz, vn, vp, dz_part, vp, 0};
       const Rests rests{PARTS == 1 ? s.mark : nullptr, s.rest, v, s.x, c.Kp};
       with_tiles(c.dw.small, D, vn, c.dw.splits, [&](auto shape, dim3 grid) {
         using S = decltype(shape);
         if (c.dw.splits > 1)
-          hipLaunchKernelGGL((out_kernel<S, float, SEGS, true>), grid, dim3(S::kThreads), 0, st, xt, dzt, 0, false, s.count,
+          hipLaunchKernelGGL((out_kernel<S, float, SEGS, true, false>), grid, dim3(S::kThreads), 0, st, xt, dz, 0, s.count,
                              s.wslots, static_cast<int64_t>(c.Dp), vn * c.Dp, 0, rests);
         else
-          hipLaunchKernelGGL((out_kernel<S, T, SEGS, false>), grid, dim3(S::kThreads), 0, st, xt, dzt, 0, false, s.count,
+          hipLaunchKernelGGL((out_kernel<S, T, SEGS, false, false>), grid, dim3(S::kThreads), 0, st, xt, dz, 0, s.count,
                              gw + v * D, static_cast<int64_t>(D), static_cast<int64_t>(0), 0, rests);
       });
       if (c.dw.splits > 1) {
@@ -1386,7 +1304,7 @@ int64_t cign_linear_xent_workspace_bytes(int32_t dtype, int64_t n, int32_t V, in
   if (check_args("cign_linear_xent_workspace_bytes", dtype, n, V, D) || of < 0 || of > 7 || n == 0) return 0;
   const Cut c = cut(dtype, n, V, D);
   const bool xin = in_place(dtype, D, x, x_stride), win = in_place(dtype, D, weight, weight_stride);
-  return of ? bwd_space(c, n, V, D, win, of, nullptr, nullptr) : fwd_space(c, n, V, xin, win, nullptr, nullptr);
+  return of ? bwd_space(c, n, V, win && !(of & 1), of, nullptr, nullptr) : fwd_space(c, n, V, xin, win, nullptr, nullptr);
 }
 
 int cign_linear_xent_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,

@@ -185,6 +185,36 @@ def test_masks(n, dtype):
     assert bool((r.loss == math.inf).all()) and all(g.isfinite().all() for g in torch.autograd.grad(r.loss, q, gl))
 
 
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("n,D,V", [(3000, 700, 5000), (2100, 1984, 2500)])
+def test_turned_operands_at_odd_edges(n, D, V, dtype):
+    """Products along the rows and along the classes whose last lines and columns end inside a tile."""
+    x, w, labels, b, gl, gs = _inputs(n, D, V, dtype, bias=D == 700, seed=12)
+    _check(x, w, labels, b, gl, gs)
+
+
+def test_masked_classes_that_are_read_where_they_lie():
+    """bfloat16 rows of a multiple of 64 values, in a wider storage of NaN; the masked classes NaN too, the last ones
+    among them. The weight's gradient alone reads them where they lie, the rows' packs them."""
+    from cign_amd.linear_cross_entropy import linear_cross_entropy
+
+    x, w, labels, b, gl, _ = _inputs(300, 128, 1000, B, seed=13)
+    off = torch.zeros(1000, dtype=torch.bool, device="cuda")
+    off[64:130] = off[700:] = True
+    b[off] = -math.inf
+    labels[(labels >= 64) & (labels < 130) | (labels >= 700)] = 5
+    _, clean = _check(x, w, labels, b, gl, None)
+    wide = torch.full((1000, 192), math.nan, dtype=B, device="cuda")
+    wide[:, :128] = w
+    wide[off] = math.nan
+    for pick in (1, 2, 3):
+        xs, ws = x.detach().requires_grad_(bool(pick & 1)), wide[:, :128].detach().requires_grad_(bool(pick & 2))
+        r = linear_cross_entropy(xs, ws, labels, bias=b)
+        got = torch.autograd.grad(r.loss, [t for t in (xs, ws) if t.requires_grad], gl)
+        for g, name in zip(got, ("x",) * (pick & 1) + ("weight",)):
+            assert torch.equal(g, clean[name])
+
+
 @pytest.mark.parametrize("n", [10, 200])
 def test_labels_out_of_range_and_nonfinite_rows(n):
     from cign_amd.linear_cross_entropy import linear_cross_entropy
