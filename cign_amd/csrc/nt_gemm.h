@@ -397,41 +397,53 @@ __device__ __forceinline__ void product(const Operand& A, const Operand& B, int 
   else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   barrier();
   if (second) barrier();
-  uint32_t ua = 0, ub = kUnitBytes;  // units of this step
-  for (int t = 0; t < total; ++t) {
-    const bool more = t + 2 < total;
+  const auto steps = [&](auto on) {
+    using ON = decltype(on);
+    uint32_t ua = 0, ub = kUnitBytes;  // units of this step
+    for (int t = 0; t < total; ++t) {
+      const bool more = t + 2 < total;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8 a[S::FA], b[S::FB];
-      if (h == 0) load_b();
-      else load_a();
-      static_assert(TURN_A || !TURN_B, "a turned B beside a turned A only");
-      if constexpr (!TURN_A) read_both(at_a[h] + ua, at_b[h] + ub, a, b);
-      else if constexpr (TURN_B) read_turned<4 * kLineBytes>(at_a[h] + ua, at_b[h] + ub, a, b);
-      else read_turned_a<4 * kLineBytes>(at_a[h] + ua, at_b[h] + ub, a, b);
-      if (h == 1 && second) {
-        if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      if (S::kPaired) {
-        barrier();
-        __builtin_amdgcn_s_setprio(1);
-      }
+      for (int h = 0; h < 2; ++h) {
+        bf16x8 a[S::FA], b[S::FB];
+        if (h == 0) load_b();
+        else load_a();
+        static_assert(TURN_A || !TURN_B, "a turned B beside a turned A only");
+        if constexpr (ON::value) {
+          if constexpr (!TURN_A) read_both(at_a[h] + ua, at_b[h] + ub, a, b);
+          else if constexpr (TURN_B) read_turned<4 * kLineBytes>(at_a[h] + ua, at_b[h] + ub, a, b);
+          else read_turned_a<4 * kLineBytes>(at_a[h] + ua, at_b[h] + ub, a, b);
+        }
+        if (h == 1 && second) {
+          if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+          else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (S::kPaired) {
+          barrier();
+          __builtin_amdgcn_s_setprio(1);
+        }
+        if constexpr (ON::value) {
 #pragma unroll
-      for (int fa = 0; fa < S::FA; ++fa)
+          for (int fa = 0; fa < S::FA; ++fa)
 #pragma unroll
-        for (int fb = 0; fb < S::FB; ++fb)
-          acc[fa][fb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[fa], b[fb], acc[fa][fb], 0, 0, 0);
-      if (S::kPaired) __builtin_amdgcn_s_setprio(0);
-      if (h == 1 && !second) {
-        if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            for (int fb = 0; fb < S::FB; ++fb)
+              acc[fa][fb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[fa], b[fb], acc[fa][fb], 0, 0, 0);
+        }
+        if (S::kPaired) __builtin_amdgcn_s_setprio(0);
+        if (h == 1 && !second) {
+          if (more) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+          else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (S::kPaired || h == 1) barrier();
       }
-      if (S::kPaired || h == 1) barrier();
+      ua = ua >= 3 * kUnitBytes ? ua - 3 * kUnitBytes : ua + 2 * kUnitBytes;
+      ub = ub >= 3 * kUnitBytes ? ub - 3 * kUnitBytes : ub + 2 * kUnitBytes;
     }
-    ua = ua >= 3 * kUnitBytes ? ua - 3 * kUnitBytes : ua + 2 * kUnitBytes;
-    ub = ub >= 3 * kUnitBytes ? ub - 3 * kUnitBytes : ub + 2 * kUnitBytes;
-  }
+  };
+  // A wavefront whose results lie behind the last row of A or B only brings its part of
+  // the units and keeps the barriers: a tile of up to half its rows takes 0.75 of a full
+  // one's time (777 rows against 50,001 classes of 1001 float32, forward: 605 -> 570 us).
+  if (a0 + first_a < A.rows && b0 + first_b < B.rows) steps(std::true_type());
+  else steps(std::false_type());
   if (S::kPaired && !second) barrier();
   __syncthreads();
 }
