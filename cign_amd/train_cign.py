@@ -21,7 +21,8 @@ to go from a dataset on disk to timed training steps.
     (train_cign.py:1820-1821, 2103-2155);
   * predict_nodes, teacher_targets, distill_one_epoch: what a node's logits say
     (prediction, confidence, entropy), and training a model on another one's top
-    classes (no counterpart in the reference).
+    classes (no counterpart in the reference); train_one_epoch's fused_loss
+    (the classifier's loss without its logits) and max_grad_norm (nor these).
 
 The model itself runs on libcign_amd's HIP kernels; nothing here computes
 on the host beyond the one-time graph preparation and the metrics.
