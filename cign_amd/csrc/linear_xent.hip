@@ -43,7 +43,7 @@ using ntgemm::Small;
 
 constexpr int kMaxClasses = 1 << 20;
 constexpr int kMaxWidth = 1 << 16;
-constexpr int kMaxRows = 1 << 23;  // launches of n D / 8 threads stay in 32 bits of workgroups
+constexpr int kMaxRows = 1 << 23;
 constexpr int kFewRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -87,6 +87,10 @@ struct Logits {
     return bias ? bias_at(bias, bias_f32, first + v) : 0.0f;
   }
 };
+
+__device__ __forceinline__ int64_t thread_of() {
+  return (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kBlock + threadIdx.x;
+}
 
 __device__ __forceinline__ int tiles(int64_t rows, int tile) { return static_cast<int>((rows + tile - 1) / tile); }
 
@@ -500,7 +504,7 @@ template <typename T, int PARTS>
 __global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* count, const int32_t* list, int D,
                                                       const T* src, int64_t ld, const void* bias, int bias_f32,
                                                       uint16_t* dst, int Kp, int64_t part) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  const int64_t i = thread_of();
   const int per = Kp / 8;
   const int64_t r = i / per;
   const int c = static_cast<int>(i - r * per) * 8;
@@ -901,7 +905,7 @@ __global__ __launch_bounds__(kBlock) void rows_out_kernel(int64_t n, int D, cons
                                                           int ns, int64_t slot, int Dp, T* gx, const int32_t* mark,
                                                           const float* rest, const T* w, int64_t ldw, const void* bias,
                                                           int bias_f32) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+  const int64_t i = thread_of();
   const int per = Dp / 4;
   const int64_t r = i / per;
   const int c = static_cast<int>(i - r * per) * 4;
@@ -1012,7 +1016,8 @@ constexpr int kTile = Large::TA;  // pieces are a multiple of it
 
 struct Cut {
   int parts, Kp;
-  int64_t fwd_piece;  // classes packed at a time by the forward
+  int64_t fwd_most;   // classes of a launch of the forward
+  int64_t fwd_piece;  // classes packed at a time by it
   int64_t piece;      // classes of a piece of the backward
   int64_t rows_p;     // rows to the next multiple of kStep
   bool stats_small, grad_small;
@@ -1022,6 +1027,7 @@ struct Cut {
 
 constexpr int64_t kPieceValues = 64ll << 20;   // of dz in a piece
 constexpr int64_t kPackValues = 256ll << 20;   // of packed classes in a piece of the forward
+constexpr int64_t kMostTiles = 1 << 22;        // of a launch of the forward: 512 threads each, 32 bits of them
 
 Cut cut(int dtype, int64_t n, int64_t V, int D) {
   Cut c;
@@ -1032,7 +1038,8 @@ Cut cut(int dtype, int64_t n, int64_t V, int D) {
     const int64_t pieces = (V + most - 1) / most;
     return up((V + pieces - 1) / pieces, kTile);
   };
-  c.fwd_piece = even(kPackValues / (c.parts * static_cast<int64_t>(c.Kp)));
+  c.fwd_most = kMostTiles / ((n + kTile - 1) / kTile + 1) * kTile;
+  c.fwd_piece = even(std::min<int64_t>(kPackValues / (c.parts * static_cast<int64_t>(c.Kp)), c.fwd_most));
   c.rows_p = up(n, kStep);
   c.piece = even(std::min<int64_t>(kPieceValues / std::max<int64_t>(kStep, c.rows_p),
                                    kPackValues / (c.parts * static_cast<int64_t>(c.Kp))));
@@ -1120,7 +1127,12 @@ int check_args(const char* who, int dtype, int64_t n, int64_t V, int64_t D) {
   return kOk;
 }
 
-dim3 grid_of(int64_t threads) { return dim3(static_cast<uint32_t>((threads + kBlock - 1) / kBlock)); }
+// Workgroups for so many threads (thread_of), at most 2^23 along x: a launch's threads
+// along an axis are 32 bits.
+dim3 grid_of(int64_t threads) {
+  const int64_t groups = (threads + kBlock - 1) / kBlock, x = std::min<int64_t>(groups, 1 << 23);
+  return dim3(static_cast<uint32_t>(x), static_cast<uint32_t>((groups + x - 1) / x));
+}
 
 template <typename T, int PARTS>
 int pack(hipStream_t st, int64_t n, const int32_t* count, const int32_t* list, int D, const T* src, int64_t ld,
@@ -1173,7 +1185,7 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
       xo = Operand{s.x, n, c.Kp, n * c.Kp};
       if (const int rc = pack<T, PARTS>(st, n, nullptr, nullptr, D, x, ldx, nullptr, 0, s.x, c.Kp, xo.part)) return rc;
     }
-    const int64_t piece = win ? V : c.fwd_piece;
+    const int64_t piece = win ? c.fwd_most : c.fwd_piece;
     for (int64_t v = 0; v < V; v += piece) {
       const int64_t vn = std::min<int64_t>(piece, V - v);
       Operand wo{reinterpret_cast<const uint16_t*>(w + v * ldw), vn, ldw, 0};

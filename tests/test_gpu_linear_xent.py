@@ -234,6 +234,60 @@ def test_labels_out_of_range_and_nonfinite_rows(n):
     assert gx[[1, 2, 3, 5, 6]].isnan().all() and gx[keep].isfinite().all()
 
 
+@pytest.mark.parametrize("n", [30, 180])
+@pytest.mark.parametrize("dtype", [F, B])
+def test_masks_of_the_lowest_value(n, dtype):
+    """Biases of the type's lowest value: of some classes, which then have no part in anything; of all of them, whose
+    logits are that value (a step of it is 2e31), so that logsumexp is too and the loss log 500."""
+    from cign_amd.linear_cross_entropy import linear_cross_entropy
+
+    x, w, labels, b, gl, gs = _inputs(n, 64, 500, dtype, seed=14, ignored=0.0)
+    low = torch.finfo(dtype).min
+    labels = labels % 100
+    b[200:350] = low
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    r = linear_cross_entropy(leaves[0], leaves[1], labels, bias=leaves[2])
+    got = torch.autograd.grad((r.loss, r.logsumexp), leaves, (gl, gs))
+    assert not got[1][200:350].any() and not got[2][200:350].any()
+    b2 = b.clone()
+    b2[200:350] = -math.inf
+    others = [t.detach().requires_grad_() for t in (x, w, b2)]
+    q = linear_cross_entropy(others[0], others[1], labels, bias=others[2])
+    assert torch.equal(q.loss, r.loss) and torch.equal(q.logsumexp, r.logsumexp)
+    assert all(torch.equal(s, t) for s, t in zip(got, torch.autograd.grad((q.loss, q.logsumexp), others, (gl, gs))))
+    r = linear_cross_entropy(x, w, labels, bias=torch.full_like(b, low))
+    assert bool((r.logsumexp == low).all()) and bool(((r.loss - math.log(500)).abs() <= 4 * U * math.log(500)).all())
+
+
+def test_launches_beyond_32_bits_of_threads():
+    """Rows so many that a launch of all their tiles, or of a thread for each eight of their values, would pass 2^32
+    threads: 2^23 rows against 70,000 classes, read where they lie; 2^23 rows of 2050 values, one row throughout, packed."""
+    from cign_amd.linear_cross_entropy import linear_cross_entropy
+
+    n = 1 << 23
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    x = torch.randn(n, 64, generator=gen, device="cuda", dtype=B)
+    w = torch.randn(70000, 64, generator=gen, device="cuda", dtype=B)
+    labels = torch.randint(0, 70000, (n,), generator=gen, device="cuda")
+    with torch.no_grad():
+        r = linear_cross_entropy(x, w, labels)
+    some = torch.cat([torch.randint(0, n, (300,), generator=gen, device="cuda"), torch.arange(n - 3, n, device="cuda")])
+    ref, _ = _bounds(x[some], w, labels[some], None, None, None, B)
+    for name, v in (("loss", r.loss[some]), ("lse", r.logsumexp[some])):
+        val, tol = ref[name]
+        assert bool(((v.double() - val).abs() <= tol + U * val.abs()).all()), name
+    assert bool(r.loss.isfinite().all())
+    del x, w, r, ref
+    row, w = torch.randn(1, 2050, generator=gen, device="cuda", dtype=B), torch.randn(2, 2050, generator=gen, device="cuda", dtype=B)
+    with torch.no_grad():
+        few = linear_cross_entropy(row.expand(200, 2050), w, labels[:200] % 2)
+        r = linear_cross_entropy(row.expand(n, 2050), w, labels % 2)
+    assert bool((r.logsumexp == few.logsumexp[0]).all())
+    one = (labels % 2).bool()
+    ref = [linear_cross_entropy(row.expand(200, 2050), w, torch.full((200,), k, device="cuda")).loss[0] for k in (0, 1)]
+    assert bool((r.loss == torch.where(one, ref[1], ref[0])).all())
+
+
 def test_large_logits():
     """Differences of a thousand: one class has all the mass, others none."""
     x, w, labels, b, gl, gs = _inputs(150, 64, 400, F, seed=9)
