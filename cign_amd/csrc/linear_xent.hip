@@ -6,9 +6,10 @@
 //
 // Forward: tiles of 256 rows by 256 classes (nt_gemm.h), or 128 by 128 where those
 // leave CUs idle, whose largest logit and sum of exponentials a row leave the tile;
-// join_kernel brings them together. Up to 64 rows take no tiles: the classes stream
-// through a wavefront's registers once (stream_kernel; few_kernel where rows do not
-// start 16-byte aligned).
+// join_kernel brings them together. Up to 64 rows, and more of float32 where that is
+// faster, take no tiles: 64 classes a wavefront stream through LDS once for each 64 rows
+// (stream_kernel, cut into runs of the summed axis where classes are few; few_kernel
+// where rows do not start 16-byte aligned).
 // Backward: the rows whose gradient is not zero are listed, a piece's logits are formed
 // again, their gradient is stored in bf16 parts, and both products read it: the weight's
 // with the rows as the summed axis, through LDS reads that turn 4 x 16 values.
@@ -203,10 +204,11 @@ __device__ __forceinline__ typename Few<T>::Raw few_tail(const T* p, int left) {
 
 constexpr int kFewClasses = 64;  // of a wavefront
 
-// Statistics of a wavefront's classes from their products.
+// Statistics of a wavefront's classes from their products with n rows; part's sets of
+// classes are `ldp` rows apart.
 template <int TOKENS>
 __device__ __forceinline__ void few_stats(f32x4 (&acc)[4][TOKENS / 16], int c0, int64_t n, int V, const void* bias,
-                                          int bias_f32, const int64_t* labels, float2* part, float* chosen) {
+                                          int bias_f32, const int64_t* labels, float2* part, int64_t ldp, float* chosen) {
   constexpr int TA = 4, TB = TOKENS / 16;
   const int l = lane_id();
 #pragma unroll
@@ -236,7 +238,7 @@ __device__ __forceinline__ void few_stats(f32x4 (&acc)[4][TOKENS / 16], int c0, 
       for (int r = 0; r < 4; ++r) s += exp_of(acc[a][b][r] - by);
     join(m, s, xor_shfl<16>(m), xor_shfl<16>(s));
     join(m, s, xor_shfl<32>(m), xor_shfl<32>(s));
-    if (l < 16 && row < n) part[static_cast<int64_t>(c0 / kFewClasses) * n + row] = make_float2(m, s);
+    if (l < 16 && row < n) part[static_cast<int64_t>(c0 / kFewClasses) * ldp + row] = make_float2(m, s);
   }
 }
 
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(kBlock) void few_kernel(int64_t n, int V, int D, co
 #pragma unroll
       for (int j = 0; j < TB; ++j) acc[i][j] = F::mul(a[i], b[j], acc[i][j]);
   }
-  few_stats<TOKENS>(acc, c0, n, V, bias, bias_f32, labels, part, chosen);
+  few_stats<TOKENS>(acc, c0, n, V, bias, bias_f32, labels, part, n, chosen);
 }
 
 // Four 16-byte reads of LDS, 2048 bytes apart, and one, waited for in the same statement.
@@ -315,6 +317,12 @@ __device__ __forceinline__ U32x4 read_one(uint32_t at) {
   return v;
 }
 
+// A slot of the products of stream_kernel's workgroup x, run y of the steps.
+template <int TOKENS>
+__device__ __forceinline__ int64_t slot_of(int y, int x) {
+  return (static_cast<int64_t>(y) * gridDim.x + x) * (4 * (TOKENS / 16) * kWave);
+}
+
 // Rows that start 16-byte aligned and are a multiple of 128 bytes wide: a workgroup is
 // one wavefront; steps of 128 bytes of its 64 classes and of the rows of x go to LDS
 // without passing registers, in a ring of steps. Nothing waits for another wavefront,
@@ -325,11 +333,14 @@ __device__ __forceinline__ U32x4 read_one(uint32_t at) {
 // enough for the memory (three 195 us, four 188). float32 rows beyond 16 are bounded
 // by the matrix units, whose SIMDs have to have as many wavefronts each: rings, or
 // room kept free, of 36 to 40 KB, four wavefronts a CU (40 rows: 640 us; five
-// wavefronts a CU 1,010).
+// wavefronts a CU 1,010). More rows than TOKENS come in `groups`, workgroups `wide`
+// apart (8: on one XCD) for the same classes. Few classes: the steps are cut into gridDim.y runs,
+// whose products go to slots (slot_of), and few_join_kernel adds them up.
 template <typename T, int TOKENS>
 __global__ __launch_bounds__(kWave) void stream_kernel(int64_t n, int V, int D, const T* x, int64_t ldx, const T* w,
                                                        int64_t ldw, const void* bias, int bias_f32,
-                                                       const int64_t* labels, float2* part, float* chosen) {
+                                                       const int64_t* labels, float2* part, float* chosen, int groups, int wide,
+                                                       f32x4* slots) {
   using F = Few<T>;
   constexpr int TB = TOKENS / 16;
   constexpr int kWide = 128 / sizeof(T);                    // values of a step
@@ -341,18 +352,21 @@ __global__ __launch_bounds__(kWave) void stream_kernel(int64_t n, int V, int D, 
   static_assert(kLoads * (RING - 1) < 63, "vmcnt");
   __shared__ __attribute__((aligned(1024))) char mine[kKept];
   const int l = lane_id();
-  const int c0 = blockIdx.x * kFewClasses;
+  const int k = blockIdx.x / wide, set = k / groups * wide + blockIdx.x % wide, c0 = set * kFewClasses;
+  if (c0 >= V) return;
+  const int64_t first = static_cast<int64_t>(k % groups) * TOKENS, rows = min(static_cast<int64_t>(TOKENS), n - first);
   const int r8 = l >> 3, chunk = ((l & 7) ^ r8) * (16 / static_cast<int>(sizeof(T)));
   const T *wp[8], *xp[2 * TB];
 #pragma unroll
   for (int j = 0; j < 8; ++j) wp[j] = w + static_cast<int64_t>(min(c0 + j * 8 + r8, V - 1)) * ldw + chunk;
 #pragma unroll
-  for (int j = 0; j < 2 * TB; ++j) xp[j] = x + min(static_cast<int64_t>(j * 8 + r8), n - 1) * ldx + chunk;
-  const int total = D / kWide;
-  const int skew = blockIdx.x * 13 % total;
+  for (int j = 0; j < 2 * TB; ++j) xp[j] = x + (first + min(static_cast<int64_t>(j * 8 + r8), rows - 1)) * ldx + chunk;
+  const int each = (D / kWide + gridDim.y - 1) / gridDim.y, begin = blockIdx.y * each;
+  const int total = min(each, D / kWide - begin);  // one at least
+  const int skew = set * 13 % total;
   const auto load = [&](int step) {
     char* to = mine + (step % RING) * kStepBytes;
-    const int t = step + skew < total ? step + skew : step + skew - total;
+    const int t = begin + (step + skew < total ? step + skew : step + skew - total);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       __builtin_amdgcn_global_load_lds((ntgemm::GlobalPtr)(wp[j] + t * kWide), (ntgemm::LdsPtr)(to + j * 1024), 16, 0, 0);
@@ -392,7 +406,40 @@ __global__ __launch_bounds__(kWave) void stream_kernel(int64_t n, int V, int D, 
       }
     }
   }
-  few_stats<TOKENS>(acc, c0, n, V, bias, bias_f32, labels, part, chosen);
+  if (slots) {
+    f32x4* to = slots + slot_of<TOKENS>(blockIdx.y, blockIdx.x) + l;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < TB; ++b) to[(a * TB + b) * kWave] = acc[a][b];
+    return;
+  }
+  few_stats<TOKENS>(acc, c0, rows, V, bias, bias_f32, labels ? labels + first : nullptr, part + first, n, chosen + first);
+}
+
+// Statistics of stream_kernel's slots, summed in their order.
+template <int TOKENS>
+__global__ __launch_bounds__(kWave) void few_join_kernel(int64_t n, int V, const void* bias, int bias_f32,
+                                                         const int64_t* labels, float2* part, float* chosen, int groups, int wide,
+                                                         const f32x4* slots, int splits) {
+  constexpr int TB = TOKENS / 16;
+  const int k = blockIdx.x / wide, c0 = (k / groups * wide + blockIdx.x % wide) * kFewClasses;
+  if (c0 >= V) return;
+  const int64_t first = static_cast<int64_t>(k % groups) * TOKENS, rows = min(static_cast<int64_t>(TOKENS), n - first);
+  f32x4 acc[4][TB];
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+  for (int y = 0; y < splits; ++y) {
+    const f32x4* from = slots + slot_of<TOKENS>(y, blockIdx.x) + lane_id();
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < TB; ++b) acc[a][b] += from[(a * TB + b) * kWave];
+  }
+  few_stats<TOKENS>(acc, c0, rows, V, bias, bias_f32, labels ? labels + first : nullptr, part + first, n, chosen + first);
 }
 
 // loss and lse of ROWS rows a workgroup, 256 / ROWS threads a row over its nt tiles;
@@ -528,6 +575,20 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(int64_t n, const int32_t* 
   }
 #pragma unroll
   for (int q = 0; q < PARTS; ++q) *reinterpret_cast<U32x4*>(dst + q * part + r * Kp + c) = o[q];
+}
+
+// Rows of D float32 values, `wide` apart with zeros behind their own.
+__global__ __launch_bounds__(kBlock) void copy_kernel(int64_t n, int D, const float* src, int64_t ld, float* dst, int wide) {
+  const int64_t i = thread_of();
+  const int per = wide / 4;
+  const int64_t r = i / per;
+  const int c = static_cast<int>(i - r * per) * 4;
+  if (r >= n) return;
+  const float* row = src + r * ld;
+  f32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = c + k < D ? row[c + k] : 0.0f;
+  *reinterpret_cast<f32x4*>(dst + r * wide + c) = v;
 }
 
 // The gradient of a piece's logits, in bf16 parts: dz[row][class], zeros up to the next
@@ -810,7 +871,6 @@ __device__ __forceinline__ void add_rests(const Rests& f, int64_t n, int64_t a0,
 #pragma unroll
         for (int fa = 0; fa < S::FA; ++fa) {
           typedef short s16x4 __attribute__((ext_vector_type(4)));
-          typedef short s16x8 __attribute__((ext_vector_type(8)));
           typedef __attribute__((address_space(3))) s16x4* Turned;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Turned)(from + fa * 32));
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Turned)(from + 4 * kRow + fa * 32));
@@ -1020,6 +1080,9 @@ struct Cut {
   int64_t fwd_piece;  // classes packed at a time by it
   int64_t piece;      // classes of a piece of the backward
   int64_t rows_p;     // rows to the next multiple of kStep
+  bool few, stream;   // the forward streams the classes, by stream_kernel,
+  bool copied;        // which reads copies
+  int tokens, groups, wide, few_grid, few_splits;
   bool stats_small, grad_small;
   Out dx, dw;         // the rows' gradient, in slots that the pieces add to; the weight's
   int Dp;
@@ -1027,9 +1090,16 @@ struct Cut {
 
 constexpr int64_t kPieceValues = 64ll << 20;   // of dz in a piece
 constexpr int64_t kPackValues = 256ll << 20;   // of packed classes in a piece of the forward
+constexpr int kFewSteps = 8;                   // of stream_kernel's run, at least
 constexpr int64_t kMostTiles = 1 << 22;        // of a launch of the forward: 512 threads each, 32 bits of them
 
-Cut cut(int dtype, int64_t n, int64_t V, int D) {
+// Whether stream_kernel takes these.
+bool streams(int dtype, int D, const void* x, int64_t ldx, const void* w, int64_t ldw) {
+  const int64_t size = dtype == kF32 ? 4 : 2;
+  return rows_aligned(x, ldx, size) && rows_aligned(w, ldw, size) && D * size % 128 == 0;
+}
+
+Cut cut(int dtype, int64_t n, int64_t V, int D, const void* x, int64_t ldx, const void* w, int64_t ldw) {
   Cut c;
   c.parts = dtype == kF32 ? 3 : 1;
   c.Kp = static_cast<int>(up(D, kStep));
@@ -1045,7 +1115,40 @@ Cut cut(int dtype, int64_t n, int64_t V, int D) {
                                    kPackValues / (c.parts * static_cast<int64_t>(c.Kp))));
   c.Dp = static_cast<int>(up(D, 4));
   const int64_t most = std::min(c.piece, V);
-  c.stats_small = small_tiles(std::min(c.fwd_piece, V), n);
+  const int64_t some = std::min(c.fwd_piece, V);
+  c.stats_small = small_tiles(some, n);
+  const int64_t sets = (V + kFewClasses - 1) / kFewClasses, groups = (n + kFewRows - 1) / kFewRows;
+  c.tokens = n <= 16 ? 16 : n <= 32 ? 32 : kFewRows;
+  c.groups = static_cast<int>(groups);
+  // Few wavefronts: runs of eight steps and more, where that gives a CU more of them, up
+  // to four (1000 classes of 4096 float32: one row 93 -> 16 us, 64 rows 279 -> 40; two
+  // runs gain nothing: 30,000 classes of 2048 bf16, one row, 25 -> 29).
+  const int64_t steps = up(D, dtype == kF32 ? 32 : 64) / (dtype == kF32 ? 32 : 64), waves = sets * groups;
+  const int64_t most_runs = std::min<int64_t>({4 * kCus / waves, steps / kFewSteps, 32});
+  const int64_t each = most_runs > 2 ? (steps + most_runs - 1) / most_runs : std::max<int64_t>(1, steps);
+  c.few_splits = static_cast<int>(std::max<int64_t>(1, (steps + each - 1) / each));
+  // More rows of float32: by float32 products, 64 at a time, or packed for the tiles'
+  // six of bf16. Microseconds of either, fitted to 131,072 x 4096 (128 rows 1.23 ms
+  // streamed, 2.96 in tiles; 256 rows 2.31 and 3.30), 126,733 x 1184 (125 rows 0.38 and
+  // 0.57; 192 rows 0.54 and 0.59), 1000 x 4096 (300 rows 60 us and 245), 10,000 x 512
+  // (192 rows 48 and 58), 50,000 x 256 (192 rows 83 and 69), copied: 3000 x 4097 (200
+  // rows 111 and 256), 50,001 x 1001 (100 rows 229 and 205).
+  const double turns = waves <= 4 * kCus ? 1.0 : static_cast<double>(waves) / (4 * kCus) + 0.3;
+  const double packs = 1.7e-6 * static_cast<double>(V + n) * D;  // or copies, where rows do not fill steps
+  const double streamed = turns * (0.0754 * D / c.few_splits + 8.0) + (c.few_splits > 1 ? 10.0 : 0.0) +
+                          (D % 32 ? packs : 0.0);
+  const double tiled = packs + 15.0 + (c.stats_small ? 0.10 : 0.13) * c.Kp *
+                       static_cast<double>((V + some - 1) / some) * rounds(tile_count(some, n, c.stats_small), c.stats_small);
+  // Rows that stream_kernel cannot read are copied for it (up to 1 GB of them), so that
+  // which of the two it is, and with it the result, hangs on the sizes alone.
+  const bool aligned = streams(dtype, D, x, ldx, w, ldw);
+  const bool more = n > kFewRows && dtype == kF32 && streamed < tiled && (aligned || V * up(D, 32) <= kPackValues);
+  c.few = n <= kFewRows || more;
+  c.copied = more && !aligned;
+  c.stream = aligned || more;
+  if (!c.few || !c.stream) c.few_splits = 1;
+  c.wide = sets >= 64 ? 8 : 1;
+  c.few_grid = c.few ? static_cast<int>(up(sets, c.wide) * groups) : 0;
   c.grad_small = small_tiles(most, n);
   c.dx = out_of(D, n, up(most, kStep) / kStep);
   c.dw = out_of(D, most, c.rows_p / kStep);
@@ -1067,24 +1170,29 @@ struct Regions {
 
 // Sets of classes whose statistics are joined.
 int64_t stat_tiles(const Cut& c, int64_t n, int64_t V) {
-  const int64_t classes = n <= kFewRows ? kFewClasses : c.stats_small ? Small::TA : Large::TA;
+  const int64_t classes = c.few ? kFewClasses : c.stats_small ? Small::TA : Large::TA;
   return (V + classes - 1) / classes;
 }
 
 struct FwdSpace {
   float2* part;
   float* chosen;
+  f32x4* slots;
+  float *copied_x, *copied_w;
   uint16_t *x, *w;
 };
 
 // x_in, w_in: read in place
-int64_t fwd_space(const Cut& c, int64_t n, int64_t V, bool x_in, bool w_in, void* p, FwdSpace* s) {
+int64_t fwd_space(const Cut& c, int64_t n, int64_t V, int D, bool x_in, bool w_in, void* p, FwdSpace* s) {
   Regions r(p);
   FwdSpace f;
   f.part = r.take<float2>(n * stat_tiles(c, n, V));
   f.chosen = r.take<float>(n);
   f.x = f.w = nullptr;
-  if (n > kFewRows) {
+  f.slots = c.few_splits > 1 ? r.take<f32x4>(static_cast<int64_t>(c.few_splits) * c.few_grid * (c.tokens / 4) * kWave) : nullptr;
+  f.copied_x = c.copied ? r.take<float>(n * up(D, 32)) : nullptr;
+  f.copied_w = c.copied ? r.take<float>(V * up(D, 32)) : nullptr;
+  if (!c.few) {
     if (!x_in) f.x = r.take<uint16_t>(c.parts * n * c.Kp);
     if (!w_in) f.w = r.take<uint16_t>(c.parts * std::min(c.fwd_piece, V) * c.Kp);
   }
@@ -1159,24 +1267,36 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
             int bias_f32, const int64_t* labels, int64_t ignore, float* loss, float* lse, void* ws) {
   constexpr int dtype = std::is_same_v<T, float> ? kF32 : kBF16;
   constexpr int PARTS = dtype == kF32 ? 3 : 1, SEGS = PARTS == 3 ? 6 : 1;
-  const Cut c = cut(dtype, n, V, D);
+  const Cut c = cut(dtype, n, V, D, x, ldx, w, ldw);
   const bool xin = in_place(dtype, D, x, ldx), win = in_place(dtype, D, w, ldw);
   FwdSpace s;
-  fwd_space(c, n, V, xin, win, ws, &s);
+  fwd_space(c, n, V, D, xin, win, ws, &s);
   const int nt = static_cast<int>(stat_tiles(c, n, V));
-  if (n <= kFewRows) {
-    const bool stream = rows_aligned(x, ldx, sizeof(T)) && rows_aligned(w, ldw, sizeof(T)) && D % (128 / sizeof(T)) == 0;
+  if (c.few) {
+    if constexpr (std::is_same_v<T, float>)
+      if (c.copied) {
+        const int wide = static_cast<int>(up(D, 32));
+        hipLaunchKernelGGL(copy_kernel, grid_of(n * (wide / 4)), dim3(kBlock), 0, st, n, D, x, ldx, s.copied_x, wide);
+        hipLaunchKernelGGL(copy_kernel, grid_of(int64_t{V} * (wide / 4)), dim3(kBlock), 0, st, int64_t{V}, D, w, ldw,
+                           s.copied_w, wide);
+        x = s.copied_x;
+        w = s.copied_w;
+        ldx = ldw = D = wide;
+      }
     const auto launch = [&](auto TC) {
       constexpr int TOKENS = decltype(TC)::value;
-      if (stream)
-        hipLaunchKernelGGL((stream_kernel<T, TOKENS>), dim3(nt), dim3(kWave), 0, st, n, V, D, x, ldx, w, ldw, bias,
-                           bias_f32, labels, s.part, s.chosen);
+      if (c.stream)
+        hipLaunchKernelGGL((stream_kernel<T, TOKENS>), dim3(c.few_grid, c.few_splits), dim3(kWave), 0, st, n, V, D, x,
+                           ldx, w, ldw, bias, bias_f32, labels, s.part, s.chosen, c.groups, c.wide, s.slots);
       else
-        hipLaunchKernelGGL((few_kernel<T, TOKENS>), dim3((nt + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlock), 0, st, n, V, D, x, ldx, w, ldw, bias, bias_f32,
-                           labels, s.part, s.chosen);
+        hipLaunchKernelGGL((few_kernel<T, TOKENS>), dim3((nt + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlock), 0, st,
+                           n, V, D, x, ldx, w, ldw, bias, bias_f32, labels, s.part, s.chosen);
+      if (s.slots)
+        hipLaunchKernelGGL((few_join_kernel<TOKENS>), dim3(c.few_grid), dim3(kWave), 0, st, n, V, bias, bias_f32, labels,
+                           s.part, s.chosen, c.groups, c.wide, s.slots, c.few_splits);
     };
-    if (n <= 16) launch(IC<16>());
-    else if (n <= 32) launch(IC<32>());
+    if (c.tokens == 16) launch(IC<16>());
+    else if (c.tokens == 32) launch(IC<32>());
     else launch(IC<64>());
     if (const int rc = check_launch("cign_linear_xent_fwd")) return rc;
   } else {
@@ -1209,7 +1329,7 @@ int forward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, co
     hipLaunchKernelGGL((join_kernel<ROWS>), dim3(static_cast<uint32_t>((n + ROWS - 1) / ROWS)), dim3(kBlock), 0, st, n, V,
                        nt, s.part, labels, ignore, s.chosen, loss, lse);
   };
-  if (n <= kFewRows) joined(IC<1>());
+  if (c.few && n <= 512) joined(IC<1>());
   else joined(IC<8>());
   return check_launch("cign_linear_xent_fwd");
 }
@@ -1221,7 +1341,7 @@ int backward(hipStream_t st, int64_t n, int V, int D, const T* x, int64_t ldx, c
   constexpr int dtype = std::is_same_v<T, float> ? kF32 : kBF16;
   constexpr int PARTS = dtype == kF32 ? 3 : 1, SEGS = PARTS == 3 ? 6 : 1;
   const char* who = "cign_linear_xent_bwd";
-  const Cut c = cut(dtype, n, V, D);
+  const Cut c = cut(dtype, n, V, D, x, ldx, w, ldw);
   const int of = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0);
   const bool win = in_place(dtype, D, w, ldw) && !(bias && gx);  // masked classes are packed as zeros
   BwdSpace s;
@@ -1314,9 +1434,9 @@ extern "C" {
 int64_t cign_linear_xent_workspace_bytes(int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x,
                                          int64_t x_stride, const void* weight, int64_t weight_stride, int32_t of) {
   if (check_args("cign_linear_xent_workspace_bytes", dtype, n, V, D) || of < 0 || of > 7 || n == 0) return 0;
-  const Cut c = cut(dtype, n, V, D);
+  const Cut c = cut(dtype, n, V, D, x, x_stride, weight, weight_stride);
   const bool xin = in_place(dtype, D, x, x_stride), win = in_place(dtype, D, weight, weight_stride);
-  return of ? bwd_space(c, n, V, win && !(of & 1), of, nullptr, nullptr) : fwd_space(c, n, V, xin, win, nullptr, nullptr);
+  return of ? bwd_space(c, n, V, win && !(of & 1), of, nullptr, nullptr) : fwd_space(c, n, V, D, xin, win, nullptr, nullptr);
 }
 
 int cign_linear_xent_fwd(void* stream, int32_t dtype, int64_t n, int32_t V, int32_t D, const void* x, int64_t x_stride,

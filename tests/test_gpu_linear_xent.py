@@ -99,7 +99,8 @@ def _check(x, w, labels, b, gl, gs, want=None):
 
 SHAPES = [(1, 1, 1), (1, 64, 300), (3, 7, 2), (16, 33, 257), (17, 128, 1000), (33, 100, 70), (64, 64, 4097),
           (65, 64, 255), (130, 65, 511), (255, 192, 256), (257, 1, 600), (300, 1001, 777), (513, 320, 2049),
-          (1000, 64, 33)]
+          (1000, 64, 33), (66, 32, 65), (100, 96, 1000), (128, 160, 4100), (129, 96, 700),
+          (1, 1024, 300), (40, 2048, 129), (200, 1024, 200), (70, 1056, 1100), (150, 288, 5000), (2000, 64, 5)]
 
 
 @pytest.mark.parametrize("n,D,V", SHAPES)
